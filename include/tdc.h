@@ -402,6 +402,80 @@ int tdc_model_set_constants(const double *values, int32_t count);
 int tdc_set_autotune(int32_t classes);
 int tdc_get_autotune(void);
 
+/* ---- channels-last operators -----------------------------------------------------------------------------------
+ * Group norm with an activation (forward, gradient), numbers in microscaled 4-bit floating point, and the product of
+ * two such operands: what stands around a 1x1 factor convolution once its tensors are [image][pixel][channel] and the
+ * factor is a matrix product.  (No counterpart in the reference, whose networks carry batch norm folded into the
+ * convolutions.)  Unlike the convolutions above these take 32- and 16-bit numbers, and EVERY pointer is a device
+ * pointer.  Strides are in elements, 0 = dense; a channel's neighbours are always adjacent.  No operator keeps state
+ * between calls: a call's scratch is the `ws` it is handed (at least the bytes the *_workspace function names for the
+ * same descriptor, 16-byte aligned, not shared by calls that can overlap on the device).  Nothing is allocated, nothing is
+ * waited for, results are the same on every run, and calls may be captured into a HIP graph.  Outputs must not overlap
+ * inputs.  Sizes of zero are legal and launch nothing. */
+typedef enum tdc_dtype { TDC_F32 = 0, TDC_F16 = 1, TDC_BF16 = 2, TDC_MX4 = 3 } tdc_dtype;
+typedef enum tdc_act { TDC_ACT_NONE = 0, TDC_ACT_RELU = 1, TDC_ACT_SILU = 2 } tdc_act;
+
+/* y[b,s,c] = act(gamma[c] * (x[b,s,c] - mean[b,g]) * rstd[b,g] + beta[c]),  g = c / (C / groups),
+ * mean and rstd = 1/sqrt(variance + eps) over the pixels and channels of one image and group.  ReLU keeps a NaN. */
+typedef struct tdc_group_norm_desc {
+    int32_t batch;
+    int32_t C;
+    int32_t groups;          /* divides C                                                    */
+    int32_t act;             /* tdc_act                                                      */
+    int32_t dtype;           /* of x, y, dy, dx: TDC_F32, TDC_F16, TDC_BF16                   */
+    int32_t param_dtype;     /* of gamma, beta: TDC_F32 or `dtype`                            */
+    float eps;
+    int32_t reserved;        /* 0                                                            */
+    int64_t pixels;          /* H * W, below 2^31                                            */
+    int64_t x_pixel_stride, x_image_stride;   /* 0 or at least C; forward and backward       */
+    int64_t y_pixel_stride, y_image_stride;   /* of y (forward) and dy (backward); dx is dense */
+} tdc_group_norm_desc;
+
+int tdc_group_norm_workspace(const tdc_group_norm_desc *desc, size_t *forward_bytes, size_t *backward_bytes);
+/* gamma, beta: [C] or NULL (1, 0).  mean, rstd: [batch][groups] fp32 or NULL. */
+int tdc_group_norm_forward(const tdc_group_norm_desc *desc, const void *x, const void *gamma, const void *beta, void *y,
+                           float *mean, float *rstd, void *ws, size_t ws_bytes, void *stream);
+/* dx [batch][pixels][C] in `dtype`, dgamma and dbeta [C] in fp32; any of the three may be NULL.  mean and rstd are the
+ * forward's.  The gradient of ReLU at 0 is 0. */
+int tdc_group_norm_backward(const tdc_group_norm_desc *desc, const void *x, const void *dy, const void *gamma, const void *beta,
+                            const float *mean, const float *rstd, void *dx, float *dgamma, float *dbeta, void *ws,
+                            size_t ws_bytes, void *stream);
+/* The forward with its result in 4 bits instead of y (batch * pixels rows of C numbers, quantised from the 32-bit values;
+ * y strides are ignored). */
+int tdc_group_norm_forward_mx4(const tdc_group_norm_desc *desc, const void *x, const void *gamma, const void *beta, void *codes,
+                               void *scales, void *ws, size_t ws_bytes, void *stream);
+int tdc_group_norm_mx4_workspace(const tdc_group_norm_desc *desc, size_t *bytes);
+
+/* Microscaled 4-bit numbers (the MXFP4 format of the OCP Microscaling specification): `rows` rows of K numbers, each an
+ * E2M1 value (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times the power of two of its block of 32 along K.  The scale of a
+ * block is 2^(floor(log2 max|x|) - 2), kept as the byte exponent + 127 (0 at least); numbers are rounded to nearest,
+ * halfway cases to the even code, and saturate at 6.  A block that holds an infinity or a NaN gets the scale 255 and
+ * stands for NaNs; a block of zeros gets the scale 0.  Layout, with Kp = K rounded up to 128:
+ *   codes   [rows][Kp / 2] bytes, the number of even place in the low half; zeros from K on
+ *   scales  [Kp / 128][rows][4] bytes: the four blocks of 128 numbers of a row together, so that the scales of
+ *           neighbouring rows are neighbouring words */
+int tdc_mx4_sizes(int64_t rows, int64_t K, size_t *code_bytes, size_t *scale_bytes);
+int tdc_mx4_quantize(const void *x, int32_t dtype, int64_t rows, int64_t K, int64_t row_stride, void *codes, void *scales,
+                     void *stream);
+int tdc_mx4_dequantize(const void *codes, const void *scales, int64_t rows, int64_t K, void *y, int32_t dtype,
+                       int64_t row_stride, void *stream);
+
+/* y[m,n] = act(sum_k x[m,k] * w[n,k] + bias[n] + residual[m,n]), x and w in 4 bits, products and sums in fp32. */
+typedef struct tdc_mx4_linear_desc {
+    int64_t M, N, K;
+    int32_t x_dtype;         /* TDC_MX4: x is given in codes and scales; else x is quantised on the way */
+    int32_t y_dtype;         /* of y and residual: TDC_F32, TDC_F16, TDC_BF16                */
+    int32_t bias_dtype;      /* TDC_F32 or y_dtype                                           */
+    int32_t act;             /* tdc_act                                                      */
+    int64_t x_stride, y_stride, residual_stride;   /* between rows, 0 = dense (x_stride: numbers only) */
+} tdc_mx4_linear_desc;
+
+int tdc_mx4_linear_workspace(const tdc_mx4_linear_desc *desc, size_t *bytes);
+/* x_scales: of x when it is TDC_MX4, else NULL.  bias, residual: or NULL. */
+int tdc_mx4_linear(const tdc_mx4_linear_desc *desc, const void *x, const void *x_scales, const void *w_codes,
+                   const void *w_scales, const void *bias, const void *residual, void *y, void *ws, size_t ws_bytes,
+                   void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,77 @@
+"""The channels-last operators in 64 bits, from their definitions (numpy; test infrastructure)."""
+import numpy as np
+
+GRID = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def act(z, name):
+    if name == "relu":
+        return np.where(z < 0, 0.0, z)
+    if name == "silu":
+        with np.errstate(over="ignore"):
+            return z / (1 + np.exp(-z))
+    return z
+
+
+def act_slope(z, name):
+    if name == "relu":
+        return (z > 0).astype(np.float64)
+    if name == "silu":
+        s = 1 / (1 + np.exp(-z))
+        return s * (1 + z * (1 - s))
+    return np.ones_like(z)
+
+
+def norm_parts(x, groups, gamma, beta, eps):
+    """x [B, S, C]: (x hat, z, mean, rstd), the last two [B, 1, C]."""
+    B, S, C = x.shape
+    g = x.reshape(B, S, groups, C // groups)
+    mean = g.mean(axis=(1, 3), keepdims=True)
+    var = ((g - mean) ** 2).mean(axis=(1, 3), keepdims=True)
+    wide = lambda v: np.repeat(v.reshape(B, 1, groups), C // groups, axis=2)  # noqa: E731
+    mean, rstd = wide(mean), wide(1 / np.sqrt(var + eps))
+    xh = (x - mean) * rstd
+    return xh, xh * gamma + beta, mean, rstd
+
+
+def norm_grads(x, dy, groups, gamma, beta, eps, name):
+    """(dx, dgamma, dbeta) of [B, S, C]."""
+    B, S, C = x.shape
+    xh, z, _, rstd = norm_parts(x, groups, gamma, beta, eps)
+    dz = dy * act_slope(z, name)
+    group_mean = lambda v: np.repeat(v.reshape(B, S, groups, -1).mean(axis=(1, 3)).reshape(B, 1, groups), C // groups, axis=2)  # noqa: E731
+    dx = rstd * (gamma * dz - group_mean(gamma * dz) - xh * group_mean(gamma * dz * xh))
+    return dx, (dz * xh).sum(axis=(0, 1)), dz.sum(axis=(0, 1))
+
+
+def mx4(x):
+    """(codes [rows, K], scale bytes [rows, blocks], values [rows, K]) of x [rows, K]."""
+    x = np.asarray(x, np.float64)
+    rows, K = x.shape
+    blocks = -(-K // 32)
+    v = np.zeros((rows, blocks * 32))
+    v[:, :K] = x
+    v = v.reshape(rows, blocks, 32)
+    top = np.abs(v).max(axis=2) if rows else np.zeros((0, blocks))
+    special = ~np.isfinite(v).all(axis=2)
+    _, e = np.frexp(np.where(special | (top == 0), 1.0, top))      # top = m 2^e, m in [0.5, 1)
+    byte = np.maximum(e - 3 + 127, 0)
+    byte = np.where(top == 0, 0, byte)
+    byte = np.where(special, 255, byte)
+    scale = np.ldexp(1.0, byte - 127)[:, :, None]
+    size = np.abs(np.where(special[:, :, None], 0.0, v)) / scale
+    away = np.abs(size[..., None] - GRID)
+    best = away.min(axis=-1, keepdims=True)
+    # nearest; of two as near, the even place
+    place = np.where(away == best, np.arange(8) + 8 * (np.arange(8) % 2), 99).argmin(axis=-1)
+    values = np.where(special[:, :, None], np.nan, np.copysign(GRID[place] * scale, v))
+    codes = place + 8 * np.signbit(v)
+    return codes.reshape(rows, blocks * 32)[:, :K], byte, values.reshape(rows, blocks * 32)[:, :K]
+
+
+def mx4_unpack(codes, scales, K):
+    """The library's bytes as (codes [rows, K], scale bytes [rows, blocks], what pads the codes)."""
+    rows = codes.shape[0]
+    nib = np.stack([codes & 15, codes >> 4], axis=2).reshape(rows, 2 * codes.shape[1])
+    byte = scales.transpose(1, 0, 2).reshape(rows, 4 * scales.shape[0])
+    return nib[:, :K], byte[:, :-(-K // 32)], nib[:, K:]

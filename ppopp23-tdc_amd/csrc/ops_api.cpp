@@ -1,0 +1,355 @@
+// C entry points of the channels-last operators: argument checks, plans, workspaces.
+#include <hip/hip_runtime_api.h>
+
+#include <algorithm>
+#include <cmath>
+#include <numeric>
+#include <string>
+
+#include "ops_internal.hpp"
+#include "tdc_internal.hpp"
+
+namespace tdc {
+namespace {
+
+int invalid(const std::string &what) { return api_fail(TDC_ERR_INVALID, what); }
+int launched(const char *what, int err) {
+    return err ? api_fail(TDC_ERR_HIP, std::string(what) + ": " + hipGetErrorString((hipError_t)err)) : (int)TDC_OK;
+}
+bool number(int dtype) { return dtype == TDC_F32 || dtype == TDC_F16 || dtype == TDC_BF16; }
+bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (unsigned)(bytes - 1)) == 0; }
+
+// ---- group norm ----
+
+constexpr int kNormThreads = 256;
+
+// `quantised`: tiles end at multiples of 32 channels, the blocks of the result.
+NormPlan norm_plan(const tdc_group_norm_desc &d, int vec, bool quantised) {
+    NormPlan n{};
+    n.vec = vec;
+    const int Cg = d.C / d.groups;
+    const long long widest = (long long)kNormThreads * vec;
+    const long long whole = std::lcm((long long)Cg, std::lcm((long long)vec, quantised ? 32ll : 1ll));
+    if (d.C <= widest) n.unit = d.C;
+    else if (whole <= widest) n.unit = (int)(widest / whole * whole);
+    else n.unit = (int)widest;
+    n.tiles = (d.C + n.unit - 1) / n.unit;
+    n.tiles_per_group = n.unit % Cg == 0 ? 1 : std::min(n.tiles, (Cg + n.unit - 2) / n.unit + 1);
+    // Workgroups: eight to a compute unit, as long as each thread has four pixels to move.
+    const int rows = kNormThreads / (n.unit / vec);
+    const long long across = (long long)n.tiles * std::max(d.batch, 1);
+    const long long want = (2048 + across - 1) / across;
+    const long long most = (d.pixels + 4 * rows - 1) / (4 * rows);
+    const long long chunks = std::max(1ll, std::min({want, most, 256ll}));
+    n.chunk_rows = (int)round_up(std::max(1ll, ((long long)d.pixels + chunks - 1) / chunks), rows);
+    n.chunks = (int)((d.pixels + n.chunk_rows - 1) / n.chunk_rows);
+    n.slots = n.chunks * n.tiles_per_group;
+    return n;
+}
+size_t stat_bytes(const tdc_group_norm_desc &d, const NormPlan &n) { return sizeof(NormStat) * d.batch * d.groups * n.slots; }
+size_t part_bytes(const tdc_group_norm_desc &d, const NormPlan &n) {
+    return (size_t)round_up((long long)sizeof(float2) * d.batch * d.groups * n.slots, 16);
+}
+size_t chan_bytes(const tdc_group_norm_desc &d, const NormPlan &n) { return (size_t)8 * d.batch * n.chunks * d.C; }
+
+int widest_vec(int dtype) { return dtype == TDC_F32 ? 4 : 8; }
+
+// Normalised copy of the descriptor with every stride filled in; an error code if it makes no sense.
+int norm_check(const tdc_group_norm_desc *desc, tdc_group_norm_desc &d) {
+    if (!desc) return invalid("group norm: null descriptor");
+    d = *desc;
+    if (d.batch < 0 || d.pixels < 0 || d.C < 1) return invalid("group norm: batch, pixels and C have to be 0, 0 and 1 at least");
+    if (d.pixels >= (1ll << 31) || d.C >= (1 << 24)) return invalid("group norm: pixels has to be below 2^31, C below 2^24");
+    if (d.groups < 1 || d.C % d.groups)
+        return invalid("group norm: " + std::to_string(d.groups) + " groups do not divide " + std::to_string(d.C) + " channels");
+    if (!number(d.dtype)) return invalid("group norm: dtype has to be TDC_F32, TDC_F16 or TDC_BF16");
+    if (d.param_dtype != TDC_F32 && d.param_dtype != d.dtype) return invalid("group norm: param_dtype has to be TDC_F32 or dtype");
+    if (d.act < TDC_ACT_NONE || d.act > TDC_ACT_SILU) return invalid("group norm: unknown activation");
+    if (!(d.eps >= 0.0f) || !std::isfinite(d.eps)) return invalid("group norm: eps has to be finite and not negative");
+    if (d.reserved) return invalid("group norm: reserved has to be 0");
+    for (auto pair : {std::make_pair(&d.x_pixel_stride, &d.x_image_stride), std::make_pair(&d.y_pixel_stride, &d.y_image_stride)}) {
+        if (*pair.first == 0) *pair.first = d.C;
+        if (*pair.first < d.C) return invalid("group norm: a pixel stride below C");
+        const long long image = d.pixels ? (d.pixels - 1) * *pair.first + d.C : 0;
+        if (*pair.second == 0) *pair.second = d.pixels * *pair.first;
+        if (d.batch > 1 && *pair.second < image) return invalid("group norm: an image stride below one image");
+    }
+    const NormPlan n = norm_plan(d, 1, false);
+    if ((long long)d.batch * n.tiles * n.chunks > (1ll << 30)) return invalid("group norm: batch too large");
+    return TDC_OK;
+}
+
+// The widest vector that C, the strides and the addresses allow.
+int norm_vec(const tdc_group_norm_desc &d, const void *x, bool with_y, std::initializer_list<const void *> dense) {
+    for (int vec : {widest_vec(d.dtype), 2}) {
+        const int bytes = vec * dtype_bytes(d.dtype);
+        bool ok = d.C % vec == 0 && d.x_pixel_stride % vec == 0 && (d.batch < 2 || d.x_image_stride % vec == 0) && aligned(x, bytes);
+        if (with_y) ok = ok && d.y_pixel_stride % vec == 0 && (d.batch < 2 || d.y_image_stride % vec == 0);
+        for (const void *p : dense) ok = ok && aligned(p, bytes);
+        if (ok) return vec;
+    }
+    return 1;
+}
+// Scratch for whichever vector the addresses will allow.
+void norm_workspace(const tdc_group_norm_desc &d, size_t &fwd, size_t &bwd, size_t &mx4) {
+    fwd = bwd = mx4 = 0;
+    for (int vec : {widest_vec(d.dtype), 2, 1}) {
+        if (d.C % vec) continue;
+        const NormPlan n = norm_plan(d, vec, false);
+        fwd = std::max(fwd, stat_bytes(d, n));
+        bwd = std::max(bwd, part_bytes(d, n) + chan_bytes(d, n));
+        mx4 = std::max(mx4, stat_bytes(d, norm_plan(d, vec, true)));
+    }
+}
+NormArgs norm_args(const tdc_group_norm_desc &d, const void *x, const void *gamma, const void *beta) {
+    NormArgs a{};
+    a.x = x;
+    a.gamma = gamma;
+    a.beta = beta;
+    a.x_ps = d.x_pixel_stride;
+    a.x_is = d.x_image_stride;
+    a.rows = d.batch * d.pixels;
+    a.batch = d.batch;
+    a.pixels = (int)d.pixels;
+    a.C = d.C;
+    a.groups = d.groups;
+    a.Cg = d.C / d.groups;
+    a.act = d.act;
+    a.param_dtype = d.param_dtype;
+    a.eps = d.eps;
+    return a;
+}
+int ws_check(const char *what, const void *ws, size_t have, size_t need) {
+    if (!need) return TDC_OK;
+    if (!ws || have < need)
+        return invalid(std::string(what) + ": the workspace has " + std::to_string(ws ? have : 0) + " bytes, needs " + std::to_string(need));
+    if (!aligned(ws, 16)) return invalid(std::string(what) + ": the workspace is not 16-byte aligned");
+    return TDC_OK;
+}
+
+// ---- 4-bit numbers ----
+
+int mx4_range(const char *what, long long rows, long long K) {
+    if (rows < 0 || K < 1) return invalid(std::string(what) + ": rows has to be 0 and K 1 at least");
+    if (K > (1ll << 30) || rows > (1ll << 35) / mx4_padded(K) * 32) return invalid(std::string(what) + ": more numbers than 2^40");
+    return TDC_OK;
+}
+int mx4_check(const char *what, long long rows, long long K, const void *codes, const void *scales) {
+    if (int st = mx4_range(what, rows, K)) return st;
+    if (rows && (!codes || !scales)) return invalid(std::string(what) + ": null codes or scales");
+    if (rows && (!aligned(codes, 16) || !aligned(scales, 4)))
+        return invalid(std::string(what) + ": codes have to be 16-byte and scales 4-byte aligned");
+    return TDC_OK;
+}
+
+// ---- product ----
+
+int linear_check(const tdc_mx4_linear_desc *desc, tdc_mx4_linear_desc &d) {
+    if (!desc) return invalid("4-bit product: null descriptor");
+    d = *desc;
+    if (d.M < 0 || d.N < 0 || d.K < 1) return invalid("4-bit product: M, N and K have to be 0, 0 and 1 at least");
+    if (d.K > (1ll << 30) || d.M > (1ll << 34) || d.N > (1ll << 34) || d.M * d.N > (1ll << 40))
+        return invalid("4-bit product: too large");
+    if (d.x_dtype != TDC_MX4 && !number(d.x_dtype)) return invalid("4-bit product: unknown x_dtype");
+    if (!number(d.y_dtype)) return invalid("4-bit product: y_dtype has to be TDC_F32, TDC_F16 or TDC_BF16");
+    if (d.bias_dtype != TDC_F32 && d.bias_dtype != d.y_dtype) return invalid("4-bit product: bias_dtype has to be TDC_F32 or y_dtype");
+    if (d.act < TDC_ACT_NONE || d.act > TDC_ACT_SILU) return invalid("4-bit product: unknown activation");
+    if (!d.x_stride) d.x_stride = d.K;
+    if (!d.y_stride) d.y_stride = d.N;
+    if (!d.residual_stride) d.residual_stride = d.N;
+    if (d.x_dtype != TDC_MX4 && d.M > 1 && d.x_stride < d.K) return invalid("4-bit product: a row stride of x below K");
+    if (d.M > 1 && (d.y_stride < d.N || d.residual_stride < d.N)) return invalid("4-bit product: a row stride below N");
+    return TDC_OK;
+}
+size_t linear_codes(const tdc_mx4_linear_desc &d) { return (size_t)(d.M * mx4_padded(d.K) / 2); }
+size_t linear_ws(const tdc_mx4_linear_desc &d) {
+    return d.x_dtype == TDC_MX4 ? 0 : linear_codes(d) + (size_t)(d.M * mx4_padded(d.K) / 32);
+}
+
+}  // namespace
+}  // namespace tdc
+
+using namespace tdc;
+
+// (an error message is the only thing here that allocates: no exception leaves a C entry)
+#define TDC_ENTRY try
+#define TDC_ENTRY_END                 \
+    catch (...) {                     \
+        return (int)TDC_ERR_NOMEM;    \
+    }
+
+extern "C" {
+
+int tdc_group_norm_workspace(const tdc_group_norm_desc *desc, size_t *forward_bytes, size_t *backward_bytes) TDC_ENTRY {
+    tdc_group_norm_desc d;
+    if (int st = norm_check(desc, d)) return st;
+    size_t fwd, bwd, mx4;
+    norm_workspace(d, fwd, bwd, mx4);
+    if (forward_bytes) *forward_bytes = fwd;
+    if (backward_bytes) *backward_bytes = bwd;
+    return TDC_OK;
+}
+TDC_ENTRY_END
+
+int tdc_group_norm_mx4_workspace(const tdc_group_norm_desc *desc, size_t *bytes) TDC_ENTRY {
+    tdc_group_norm_desc d;
+    if (int st = norm_check(desc, d)) return st;
+    if (!bytes) return invalid("group norm: null argument");
+    size_t fwd, bwd;
+    norm_workspace(d, fwd, bwd, *bytes);
+    return TDC_OK;
+}
+TDC_ENTRY_END
+
+int tdc_group_norm_forward(const tdc_group_norm_desc *desc, const void *x, const void *gamma, const void *beta, void *y,
+                           float *mean, float *rstd, void *ws, size_t ws_bytes, void *stream) TDC_ENTRY {
+    tdc_group_norm_desc d;
+    if (int st = norm_check(desc, d)) return st;
+    if (!d.batch || !d.pixels) return TDC_OK;
+    if (!x || !y) return invalid("group norm: null x or y");
+    size_t fwd, bwd, mx4;
+    norm_workspace(d, fwd, bwd, mx4);
+    if (int st = ws_check("group norm", ws, ws_bytes, fwd)) return st;
+    NormArgs a = norm_args(d, x, gamma, beta);
+    a.out = y;
+    a.o_ps = d.y_pixel_stride;
+    a.o_is = d.y_image_stride;
+    a.mean = mean;
+    a.rstd = rstd;
+    a.stat = (NormStat *)ws;
+    a.plan = norm_plan(d, norm_vec(d, x, true, {y}), false);
+    return launched("group norm", launch_norm_forward(a, d.dtype, stream));
+}
+TDC_ENTRY_END
+
+int tdc_group_norm_forward_mx4(const tdc_group_norm_desc *desc, const void *x, const void *gamma, const void *beta, void *codes,
+                               void *scales, void *ws, size_t ws_bytes, void *stream) TDC_ENTRY {
+    tdc_group_norm_desc d;
+    if (int st = norm_check(desc, d)) return st;
+    if (!d.batch || !d.pixels) return TDC_OK;
+    if (!x) return invalid("group norm: null x");
+    if (int st = mx4_check("group norm", d.batch * d.pixels, d.C, codes, scales)) return st;
+    size_t fwd, bwd, mx4;
+    norm_workspace(d, fwd, bwd, mx4);
+    if (int st = ws_check("group norm", ws, ws_bytes, mx4)) return st;
+    NormArgs a = norm_args(d, x, gamma, beta);
+    a.codes = (unsigned char *)codes;
+    a.scales = (unsigned char *)scales;
+    a.stat = (NormStat *)ws;
+    a.plan = norm_plan(d, norm_vec(d, x, false, {}), true);
+    return launched("group norm", launch_norm_forward(a, d.dtype, stream));
+}
+TDC_ENTRY_END
+
+int tdc_group_norm_backward(const tdc_group_norm_desc *desc, const void *x, const void *dy, const void *gamma, const void *beta,
+                            const float *mean, const float *rstd, void *dx, float *dgamma, float *dbeta, void *ws,
+                            size_t ws_bytes, void *stream) TDC_ENTRY {
+    tdc_group_norm_desc d;
+    if (int st = norm_check(desc, d)) return st;
+    if (!dx && !dgamma && !dbeta) return TDC_OK;
+    if (!d.batch || !d.pixels) {
+        // no numbers: the parameters' gradients are sums of nothing
+        if (dgamma)
+            if (int e = launch_zero_words((unsigned *)dgamma, d.C, stream)) return launched("group norm", e);
+        if (dbeta)
+            if (int e = launch_zero_words((unsigned *)dbeta, d.C, stream)) return launched("group norm", e);
+        return TDC_OK;
+    }
+    if (!x || !dy || !mean || !rstd) return invalid("group norm: null x, dy, mean or rstd");
+    size_t fwd, bwd, mx4;
+    norm_workspace(d, fwd, bwd, mx4);
+    if (int st = ws_check("group norm", ws, ws_bytes, bwd)) return st;
+    NormArgs a = norm_args(d, x, gamma, beta);
+    a.dy = dy;
+    a.d_ps = d.y_pixel_stride;
+    a.d_is = d.y_image_stride;
+    a.out = dx;
+    a.o_ps = d.C;
+    a.o_is = d.pixels * d.C;
+    a.mean = const_cast<float *>(mean);
+    a.rstd = const_cast<float *>(rstd);
+    a.dgamma = dgamma;
+    a.dbeta = dbeta;
+    a.plan = norm_plan(d, norm_vec(d, x, true, {dy, dx}), false);
+    a.part = (float2 *)ws;
+    a.chan = (float *)((char *)ws + part_bytes(d, a.plan));
+    return launched("group norm", launch_norm_backward(a, d.dtype, stream));
+}
+TDC_ENTRY_END
+
+int tdc_mx4_sizes(int64_t rows, int64_t K, size_t *code_bytes, size_t *scale_bytes) TDC_ENTRY {
+    if (int st = mx4_range("4-bit numbers", rows, K)) return st;
+    if (code_bytes) *code_bytes = (size_t)(rows * mx4_padded(K) / 2);
+    if (scale_bytes) *scale_bytes = (size_t)(rows * mx4_padded(K) / 32);
+    return TDC_OK;
+}
+TDC_ENTRY_END
+
+int tdc_mx4_quantize(const void *x, int32_t dtype, int64_t rows, int64_t K, int64_t row_stride, void *codes, void *scales, void *stream) TDC_ENTRY {
+    if (!number(dtype)) return invalid("4-bit numbers: dtype has to be TDC_F32, TDC_F16 or TDC_BF16");
+    if (int st = mx4_check("4-bit numbers", rows, K, codes, scales)) return st;
+    if (!rows) return TDC_OK;
+    if (!x) return invalid("4-bit numbers: null x");
+    if (!row_stride) row_stride = K;
+    if (rows > 1 && row_stride < K) return invalid("4-bit numbers: a row stride below K");
+    return launched("4-bit numbers", launch_mx4_quantize(x, dtype, rows, K, row_stride, codes, scales, stream));
+}
+TDC_ENTRY_END
+
+int tdc_mx4_dequantize(const void *codes, const void *scales, int64_t rows, int64_t K, void *y, int32_t dtype, int64_t row_stride,
+                       void *stream) TDC_ENTRY {
+    if (!number(dtype)) return invalid("4-bit numbers: dtype has to be TDC_F32, TDC_F16 or TDC_BF16");
+    if (int st = mx4_check("4-bit numbers", rows, K, codes, scales)) return st;
+    if (!rows) return TDC_OK;
+    if (!y) return invalid("4-bit numbers: null y");
+    if (!row_stride) row_stride = K;
+    if (rows > 1 && row_stride < K) return invalid("4-bit numbers: a row stride below K");
+    return launched("4-bit numbers", launch_mx4_dequantize(codes, scales, rows, K, y, dtype, row_stride, stream));
+}
+TDC_ENTRY_END
+
+int tdc_mx4_linear_workspace(const tdc_mx4_linear_desc *desc, size_t *bytes) TDC_ENTRY {
+    tdc_mx4_linear_desc d;
+    if (int st = linear_check(desc, d)) return st;
+    if (!bytes) return invalid("4-bit product: null argument");
+    *bytes = linear_ws(d);
+    return TDC_OK;
+}
+TDC_ENTRY_END
+
+int tdc_mx4_linear(const tdc_mx4_linear_desc *desc, const void *x, const void *x_scales, const void *w_codes, const void *w_scales,
+                   const void *bias, const void *residual, void *y, void *ws, size_t ws_bytes, void *stream) TDC_ENTRY {
+    tdc_mx4_linear_desc d;
+    if (int st = linear_check(desc, d)) return st;
+    if (!d.M || !d.N) return TDC_OK;
+    if (!x || !y) return invalid("4-bit product: null x or y");
+    if (int st = mx4_check("4-bit product", d.N, d.K, w_codes, w_scales)) return st;
+    ProductArgs a{};
+    if (d.x_dtype == TDC_MX4) {
+        if (int st = mx4_check("4-bit product", d.M, d.K, x, x_scales)) return st;
+        a.x_codes = (const unsigned char *)x;
+        a.x_scales = (const unsigned char *)x_scales;
+    } else {
+        if (int st = ws_check("4-bit product", ws, ws_bytes, linear_ws(d))) return st;
+        a.x_codes = (const unsigned char *)ws;
+        a.x_scales = a.x_codes + linear_codes(d);
+        if (int e = launch_mx4_quantize(x, d.x_dtype, d.M, d.K, d.x_stride, ws, (char *)ws + linear_codes(d), stream))
+            return launched("4-bit product", e);
+    }
+    a.w_codes = (const unsigned char *)w_codes;
+    a.w_scales = (const unsigned char *)w_scales;
+    a.bias = bias;
+    a.residual = residual;
+    a.y = y;
+    a.M = d.M;
+    a.N = d.N;
+    a.y_stride = d.y_stride;
+    a.r_stride = d.residual_stride;
+    a.ksteps = (int)(mx4_padded(d.K) / 128);
+    a.bias_dtype = d.bias_dtype;
+    a.act = d.act;
+    return launched("4-bit product", launch_mx4_product(a, d.y_dtype, stream));
+}
+TDC_ENTRY_END
+
+}  // extern "C"

@@ -1,0 +1,72 @@
+// Declarations shared by the channels-last operators' kernels (group_norm.hip, mx4.hip, mx4_product.hip) and their C entry
+// points (ops_api.cpp).  Nothing here is exported.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+
+#include <hip/hip_vector_types.h>
+
+#include "tdc.h"
+
+namespace tdc {
+
+inline int dtype_bytes(int dtype) { return dtype == TDC_F32 ? 4 : 2; }
+inline long long round_up(long long v, long long to) { return (v + to - 1) / to * to; }
+
+// Numbers of a row in 4 bits, rounded up to the 128 of one matrix instruction.
+inline long long mx4_padded(long long K) { return round_up(K, 128); }
+
+// How a norm's work is dealt out.  A workgroup owns `unit` channels (unit / vec vectors, a thread each) of `chunk_rows`
+// pixels of one image; `slots` partial results per image and group meet in the second launch.
+struct NormPlan {
+    int vec;            // channels a thread moves at once
+    int unit;           // channels of a workgroup
+    int tiles;          // workgroups across the channels
+    int tiles_per_group;// at most so many of them share a group (1 unless a group is wider than a workgroup)
+    int chunks;         // workgroups along the pixels of an image
+    int chunk_rows;
+    int slots;          // chunks * tiles_per_group
+};
+
+// Partial statistics of one group: the sum, and the squared deviations from its mean.
+struct NormStat {
+    double sum;
+    float m2, unused;
+};
+
+struct NormArgs {
+    const void *x, *dy, *gamma, *beta;
+    void *out;                      // y or dx
+    float *mean, *rstd;
+    float *dgamma, *dbeta;
+    NormStat *stat;                 // forward: [image][group][slot]
+    float2 *part;                   // backward: the same places, sums of gamma dz and gamma dz xh
+    float *chan;                    // backward: [image][chunk][2][C]
+    unsigned char *codes, *scales;  // forward in 4 bits
+    long long x_ps, x_is, o_ps, o_is, d_ps, d_is;
+    long long rows;                 // batch * pixels
+    int batch, pixels, C, groups, Cg, act, param_dtype;
+    float eps;
+    NormPlan plan;
+};
+
+// All return a hipError_t as int.
+int launch_norm_forward(const NormArgs &a, int dtype, void *stream);
+int launch_norm_backward(const NormArgs &a, int dtype, void *stream);
+
+int launch_mx4_quantize(const void *x, int dtype, long long rows, long long K, long long stride, void *codes, void *scales, void *stream);
+int launch_mx4_dequantize(const void *codes, const void *scales, long long rows, long long K, void *y, int dtype, long long stride,
+                          void *stream);
+
+struct ProductArgs {
+    const unsigned char *x_codes, *x_scales, *w_codes, *w_scales;
+    const void *bias, *residual;
+    void *y;
+    long long M, N, y_stride, r_stride;
+    int ksteps;                     // padded K / 128
+    int bias_dtype, act;
+};
+int launch_mx4_product(const ProductArgs &a, int y_dtype, void *stream);
+
+}  // namespace tdc

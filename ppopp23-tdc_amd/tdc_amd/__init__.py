@@ -3,7 +3,8 @@ from ._lib import (LIB_PATH, ConvDesc, TdcError, Tile, TileInfo, conv_desc, lib,
                    model_select, set_autotune)
 
 __all__ = ["LIB_PATH", "ConvDesc", "TdcError", "Tile", "TileInfo", "conv_desc", "lib", "model_enumerate",
-           "model_evaluate", "model_select", "set_autotune", "Conv2dPlan", "TKConvOp", "TKConv2dC", "ranks_dict", "partial_tucker2"]
+           "model_evaluate", "model_select", "set_autotune", "Conv2dPlan", "TKConvOp", "TKConv2dC", "ranks_dict", "partial_tucker2",
+           "group_norm_act", "group_norm_act_mx4", "mx4_quantize", "mx4_linear", "mx4_conv1x1", "Mx4Tensor"]
 
 
 def __getattr__(name):
@@ -14,4 +15,7 @@ def __getattr__(name):
     if name in ("TKConv2dC", "ranks_dict", "partial_tucker2"):
         from . import TKConv
         return getattr(TKConv, name)
+    if name in ("group_norm_act", "group_norm_act_mx4", "mx4_quantize", "mx4_linear", "mx4_conv1x1", "Mx4Tensor"):
+        from . import channels_last
+        return getattr(channels_last, name)
     raise AttributeError(name)

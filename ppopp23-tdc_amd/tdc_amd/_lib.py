@@ -30,6 +30,9 @@ EXPORTS = (
     "tdc_net_create", "tdc_net_tensor", "tdc_net_view", "tdc_net_affine", "tdc_net_affine_conv", "tdc_net_conv", "tdc_net_conv_tail", "tdc_net_set_input_affine", "tdc_net_tkconv", "tdc_net_pool", "tdc_net_global_avgpool", "tdc_net_concat",
     "tdc_net_tensor_shape", "tdc_net_num_kernels", "tdc_net_finalize", "tdc_net_forward", "tdc_net_time",
     "tdc_net_read_tensor", "tdc_net_destroy",
+    "tdc_group_norm_workspace", "tdc_group_norm_forward", "tdc_group_norm_backward", "tdc_group_norm_forward_mx4",
+    "tdc_group_norm_mx4_workspace", "tdc_mx4_sizes", "tdc_mx4_quantize", "tdc_mx4_dequantize", "tdc_mx4_linear_workspace",
+    "tdc_mx4_linear",
 )
 
 
@@ -80,6 +83,17 @@ class KernelOccupancy(Structure):
 class TKConvDesc(Structure):
     _fields_ = [(n, c_int32) for n in ("batch", "C", "R1", "R2", "N", "H", "W", "K", "stride", "pad", "dilation",
                                        "has_bias", "relu")]
+
+
+class GroupNormDesc(Structure):
+    _fields_ = [(n, c_int32) for n in ("batch", "C", "groups", "act", "dtype", "param_dtype")] + [
+        ("eps", ctypes.c_float), ("reserved", c_int32)] + [(n, ctypes.c_int64) for n in (
+            "pixels", "x_pixel_stride", "x_image_stride", "y_pixel_stride", "y_image_stride")]
+
+
+class Mx4LinearDesc(Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("M", "N", "K")] + [(n, c_int32) for n in (
+        "x_dtype", "y_dtype", "bias_dtype", "act")] + [(n, ctypes.c_int64) for n in ("x_stride", "y_stride", "residual_stride")]
 
 
 _lib = None
@@ -150,6 +164,17 @@ def lib():
     L.tdc_net_destroy.restype = None
     L.tdc_set_autotune.argtypes = [i32]
     L.tdc_get_autotune.argtypes = []
+    sz, szp, norm, linear = ctypes.c_size_t, POINTER(ctypes.c_size_t), POINTER(GroupNormDesc), POINTER(Mx4LinearDesc)
+    L.tdc_group_norm_workspace.argtypes = [norm, szp, szp]
+    L.tdc_group_norm_mx4_workspace.argtypes = [norm, szp]
+    L.tdc_group_norm_forward.argtypes = [norm] + [c_void_p] * 7 + [sz, c_void_p]
+    L.tdc_group_norm_forward_mx4.argtypes = [norm] + [c_void_p] * 6 + [sz, c_void_p]
+    L.tdc_group_norm_backward.argtypes = [norm] + [c_void_p] * 10 + [sz, c_void_p]
+    L.tdc_mx4_sizes.argtypes = [i64, i64, szp, szp]
+    L.tdc_mx4_quantize.argtypes = [c_void_p, i32, i64, i64, i64, c_void_p, c_void_p, c_void_p]
+    L.tdc_mx4_dequantize.argtypes = [c_void_p, c_void_p, i64, i64, c_void_p, i32, i64, c_void_p]
+    L.tdc_mx4_linear_workspace.argtypes = [linear, szp]
+    L.tdc_mx4_linear.argtypes = [linear] + [c_void_p] * 8 + [sz, c_void_p]
     for name in EXPORTS:
         fn = getattr(L, name)
         if fn.restype is c_int:  # default restype: status code

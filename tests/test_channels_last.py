@@ -1,0 +1,147 @@
+"""What the channels-last operators refuse (no GPU needed), and their 64-bit oracle against hand-worked numbers."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import tdc_amd
+from oracle import channels_last_ref as ref
+from tdc_amd import _lib
+from tdc_amd.channels_last import _dense_strides, _pixel_strides
+
+INVALID = _lib.TDC_ERR_INVALID
+
+
+def norm(**kw):
+    d = dict(batch=2, C=8, groups=2, act=0, dtype=0, param_dtype=0, eps=1e-5, reserved=0, pixels=9, x_pixel_stride=0, x_image_stride=0,
+             y_pixel_stride=0, y_image_stride=0)
+    d.update(kw)
+    return _lib.GroupNormDesc(*[d[n] for n, _ in _lib.GroupNormDesc._fields_])
+
+
+def linear(**kw):
+    d = dict(M=4, N=5, K=40, x_dtype=0, y_dtype=0, bias_dtype=0, act=0, x_stride=0, y_stride=0, residual_stride=0)
+    d.update(kw)
+    return _lib.Mx4LinearDesc(*[d[n] for n, _ in _lib.Mx4LinearDesc._fields_])
+
+
+def error():
+    return tdc_amd.lib().tdc_last_error_string().decode()
+
+
+def test_struct_layouts():
+    assert ctypes.sizeof(_lib.GroupNormDesc) == 8 * 4 + 5 * 8
+    assert ctypes.sizeof(_lib.Mx4LinearDesc) == 3 * 8 + 4 * 4 + 3 * 8
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(C=0), "C"), (dict(groups=3), "divide"), (dict(groups=0), "divide"), (dict(batch=-1), "batch"), (dict(pixels=-1), "pixels"),
+    (dict(pixels=1 << 31), "2^31"), (dict(dtype=3), "dtype"), (dict(dtype=1, param_dtype=2), "param_dtype"), (dict(act=3), "activation"),
+    (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(x_pixel_stride=7), "pixel stride"), (dict(x_image_stride=71), "image stride"),
+    (dict(y_pixel_stride=-8), "pixel stride"), (dict(y_image_stride=8), "image stride"), (dict(reserved=1), "reserved")])
+def test_norm_descriptors_are_refused(bad, word):
+    L, d, a, b = tdc_amd.lib(), norm(**bad), ctypes.c_size_t(), ctypes.c_size_t()
+    assert L.tdc_group_norm_workspace(ctypes.byref(d), ctypes.byref(a), ctypes.byref(b)) == INVALID and word in error()
+    assert L.tdc_group_norm_forward(ctypes.byref(d), 16, None, None, 16, None, None, 16, 1 << 20, None) == INVALID
+    assert L.tdc_group_norm_backward(ctypes.byref(d), 16, 16, None, None, 16, 16, 16, None, None, 16, 1 << 20, None) == INVALID
+    assert L.tdc_group_norm_forward_mx4(ctypes.byref(d), 16, None, None, 16, 16, 16, 1 << 20, None) == INVALID
+
+
+def test_norm_arguments_are_refused():
+    L, d, a, b = tdc_amd.lib(), norm(), ctypes.c_size_t(), ctypes.c_size_t()
+    assert L.tdc_group_norm_workspace(None, ctypes.byref(a), ctypes.byref(b)) == INVALID
+    assert L.tdc_group_norm_workspace(ctypes.byref(d), ctypes.byref(a), ctypes.byref(b)) == 0 and 0 < a.value < b.value
+    p = ctypes.byref(d)
+    assert L.tdc_group_norm_forward(p, None, None, None, 16, None, None, 16, a, None) == INVALID
+    assert L.tdc_group_norm_forward(p, 16, None, None, None, None, None, 16, a, None) == INVALID
+    assert L.tdc_group_norm_forward(p, 16, None, None, 16, None, None, None, a, None) == INVALID
+    assert L.tdc_group_norm_forward(p, 16, None, None, 16, None, None, 16, a.value - 1, None) == INVALID and "workspace" in error()
+    assert L.tdc_group_norm_forward(p, 16, None, None, 16, None, None, 8, a, None) == INVALID and "aligned" in error()
+    assert L.tdc_group_norm_backward(p, 16, 16, None, None, None, 16, 16, None, None, 16, b, None) == INVALID
+    assert L.tdc_group_norm_forward_mx4(p, 16, None, None, 8, 16, 16, b, None) == INVALID and "aligned" in error()
+    # nothing to do is no error, whatever the pointers
+    assert L.tdc_group_norm_forward(ctypes.byref(norm(batch=0)), None, None, None, None, None, None, None, 0, None) == 0
+    assert L.tdc_group_norm_backward(p, None, None, None, None, None, None, None, None, None, None, 0, None) == 0
+
+
+def test_4_bit_arguments_are_refused():
+    L, c, s = tdc_amd.lib(), ctypes.c_size_t(), ctypes.c_size_t()
+    assert L.tdc_mx4_sizes(3, 130, ctypes.byref(c), ctypes.byref(s)) == 0 and (c.value, s.value) == (3 * 128, 3 * 8)
+    for rows, K in ((-1, 4), (2, 0), (1 << 36, 64), (2, 1 << 31)):
+        assert L.tdc_mx4_sizes(rows, K, ctypes.byref(c), ctypes.byref(s)) == INVALID
+    assert L.tdc_mx4_quantize(16, 3, 2, 32, 0, 16, 16, None) == INVALID and "dtype" in error()
+    assert L.tdc_mx4_quantize(16, 0, 2, 32, 31, 16, 16, None) == INVALID and "stride" in error()
+    assert L.tdc_mx4_quantize(None, 0, 2, 32, 0, 16, 16, None) == INVALID
+    assert L.tdc_mx4_quantize(16, 0, 2, 32, 0, 24, 16, None) == INVALID and "aligned" in error()
+    assert L.tdc_mx4_quantize(16, 0, 2, 32, 0, 16, 18, None) == INVALID
+    assert L.tdc_mx4_dequantize(16, 16, 2, 32, None, 0, 0, None) == INVALID
+    assert L.tdc_mx4_dequantize(16, None, 2, 32, 16, 0, 0, None) == INVALID
+    assert L.tdc_mx4_quantize(None, 0, 0, 32, 0, None, None, None) == 0
+
+
+@pytest.mark.parametrize("bad", [dict(M=-1), dict(N=-1), dict(K=0), dict(x_dtype=4), dict(y_dtype=3), dict(y_dtype=1, bias_dtype=2), dict(act=-1),
+                                 dict(x_stride=39), dict(y_stride=4), dict(residual_stride=-5), dict(M=1 << 30, N=1 << 30)])
+def test_product_descriptors_are_refused(bad):
+    L, n, d = tdc_amd.lib(), ctypes.c_size_t(), linear(**bad)
+    assert L.tdc_mx4_linear_workspace(ctypes.byref(d), ctypes.byref(n)) == INVALID and len(error()) > 15
+    assert L.tdc_mx4_linear(ctypes.byref(d), 16, None, 16, 16, None, None, 16, 16, 1 << 20, None) == INVALID
+
+
+def test_product_arguments_are_refused():
+    L, n, d = tdc_amd.lib(), ctypes.c_size_t(), linear()
+    assert L.tdc_mx4_linear_workspace(ctypes.byref(d), ctypes.byref(n)) == 0
+    assert L.tdc_mx4_linear(ctypes.byref(d), None, None, 16, 16, None, None, 16, 16, n, None) == INVALID
+    assert L.tdc_mx4_linear(ctypes.byref(d), 16, None, 16, 16, None, None, None, 16, n, None) == INVALID
+    assert L.tdc_mx4_linear(ctypes.byref(d), 16, None, 16, None, None, None, 16, 16, n, None) == INVALID
+    if n.value:
+        assert L.tdc_mx4_linear(ctypes.byref(d), 16, None, 16, 16, None, None, 16, None, 0, None) == INVALID
+    q = linear(x_dtype=3)
+    assert L.tdc_mx4_linear(ctypes.byref(q), 16, None, 16, 16, None, None, 16, None, 0, None) == INVALID
+    assert L.tdc_mx4_linear(ctypes.byref(linear(M=0)), None, None, None, None, None, None, None, None, 0, None) == 0
+
+
+def test_python_refusals_without_a_device():
+    x = torch.zeros(2, 8, 3, 3).contiguous(memory_format=torch.channels_last)
+    with pytest.raises(ValueError, match="device tensor"):
+        tdc_amd.group_norm_act(x, 2)
+    with pytest.raises(TypeError, match="float32, float16 or bfloat16"):
+        tdc_amd.group_norm_act(x.double(), 2)
+    with pytest.raises(ValueError, match="device tensor"):
+        tdc_amd.mx4_quantize(x)
+    with pytest.raises(TypeError, match="has to be a tensor"):
+        tdc_amd.mx4_quantize([1.0])
+    with pytest.raises(TypeError, match="Mx4Tensor"):
+        tdc_amd.mx4_linear(x, torch.zeros(4, 3))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        tdc_amd.group_norm_act_mx4(x.requires_grad_(), 2)
+    with pytest.raises(ValueError, match="uint8 device tensor"):
+        tdc_amd.Mx4Tensor(torch.zeros(2, 64, dtype=torch.uint8), torch.zeros(1, 2, 4, dtype=torch.uint8), (2, 128))
+
+
+def test_channels_last_is_recognised():
+    def of(t):
+        return _pixel_strides(tuple(t.shape), t.stride())
+    t = torch.zeros(2, 5, 6, 8)
+    assert of(t.permute(0, 3, 1, 2)) == (30, 8, 240)
+    assert of(t) is None
+    assert of(t.permute(0, 3, 1, 2)[:, 2:6]) == (30, 8, 240)
+    assert of(t.permute(0, 3, 1, 2)[:, :, ::2]) is None                       # rows skipped
+    assert of(t.permute(0, 3, 1, 2)[:, :, :, ::2]) == (15, 16, 240)           # columns skipped: still evenly spaced
+    assert of(torch.zeros(4, 7, 1, 1)) == (1, 7, 7)
+    assert of(torch.zeros(4, 1, 3, 5)) == (15, 1, 15)
+    assert of(torch.zeros(1, 8, 1, 1).expand(4, 8, 3, 3)) is None
+    assert of(torch.zeros(1, 3, 3, 8).permute(0, 3, 1, 2).expand(4, 8, 3, 3)) is None
+    assert _dense_strides((2, 8, 5, 6)) == (240, 1, 48, 8)
+    assert _dense_strides((3, 4)) == (4, 1)
+
+
+def test_oracle_of_4_bit_numbers():
+    x = np.zeros((1, 40))
+    x[0, :10] = [6, 5, 3.5, 2.5, 1.75, 0.75, 0.25, -0.25, -5.1, 7.9]
+    x[0, 32:35] = [0.1, -0.05, 0.0]
+    codes, byte, values = ref.mx4(x)
+    assert byte.tolist() == [[127, 127 - 6]]
+    assert values[0, :10].tolist() == [6, 4, 4, 2, 2, 1, 0, 0, -6, 6]
+    assert codes[0, :10].tolist() == [7, 6, 6, 4, 4, 2, 0, 8, 15, 7]
+    assert values[0, 32:35].tolist() == [6 / 64, -3 / 64, 0]      # 0.1 * 64 = 6.4, 0.05 * 64 = 3.2
