@@ -1,72 +1,119 @@
 // Numbers into microscaled 4-bit floating point and back (format and layout: include/tdc.h).
 //
-// Memory traffic: x in, 17/32 byte a number out.  A thread takes one block of 32 numbers.
+// Memory traffic: x on one side, 17/32 byte a number on the other.  Sixteen lanes take 128 numbers of a row, eight each: one request of
+// 16 bytes (two in 32 bits), a block's largest magnitude from four neighbouring lanes, one word of codes a lane and
+// one word of scales from the sixteen.  The sixteen rows of a workgroup keep their scale words together in memory.
+// Requests need no alignment beyond the number's own; only the last one of a row may end early.
 #include "ops_device.hpp"
 
 namespace tdc {
 
+static constexpr int kRows = 16;      // of a workgroup of 256
+static constexpr int kSteps = 4;      // runs of 128 numbers a thread has in flight
+
 template <int DT>
-__global__ void __launch_bounds__(256) tdc_mx4_quantize_kernel(const void *x, long long rows, long long K, long long stride, long long blocks,
-                                                           unsigned char *codes, unsigned char *scales) {
+__global__ void __launch_bounds__(256) tdc_mx4_quantize_kernel(const void *x, long long rows, long long K, long long stride, int groups,
+                                                               int runs, unsigned *codes, unsigned *scales) {
     using T = typename Num<DT>::type;
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (idx >= rows * blocks) return;
-    const long long row = idx / blocks, kb = idx - row * blocks;
-    const T *src = reinterpret_cast<const T *>(x) + row * stride + kb * 32;
-    const int n = (int)max(0ll, min(32ll, K - kb * 32));
-    float v[32], top = 0.0f;
+    typedef T vec_t __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    const long long rb = blockIdx.x / (unsigned)runs;
+    const int g0 = (blockIdx.x - (unsigned)rb * runs) * kSteps, lane = threadIdx.x & 15;
+    const long long row = rb * kRows + (threadIdx.x >> 4);
+    if (row >= rows) return;
+    const T *const src = reinterpret_cast<const T *>(x) + row * stride + lane * 8;
+    vec_t p[kSteps];
+    if ((long long)(g0 + kSteps) * 128 <= K) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        v[i] = i < n ? Num<DT>::up(src[i]) : 0.0f;
-        top = larger(top, v[i]);
+        for (int s = 0; s < kSteps; ++s) p[s] = *reinterpret_cast<const vec_t *>(src + (g0 + s) * 128ll);
+    } else {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            p[s] = vec_t{};
+            if ((g0 + s) * 128ll + lane * 8 + 8 <= K) p[s] = *reinterpret_cast<const vec_t *>(src + (g0 + s) * 128ll);
+        }
+        // (the numbers of a row's last request, where it ends early)
+        if (K & 7) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const int n = (int)(K - (g0 + s) * 128ll) - lane * 8;
+                if (n > 0 && n < 8) {
+#pragma unroll
+                    for (int i = 0; i < 7; ++i)
+                        if (i < n) p[s][i] = src[(g0 + s) * 128ll + i];
+                }
+            }
+        }
     }
-    const int byte = mx4_scale_byte(top);
-    const float scale = mx4_divisor(byte);
-    *reinterpret_cast<uint4 *>(codes + idx * 16) =
-        make_uint4(mx4_codes(v, scale), mx4_codes(v + 8, scale), mx4_codes(v + 16, scale), mx4_codes(v + 24, scale));
-    scales[((kb >> 2) * rows + row) * 4 + (kb & 3)] = (unsigned char)byte;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        if (g0 + s >= groups) continue;
+        float v[8], top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[i] = Num<DT>::up(p[s][i]);
+            top = larger(top, v[i]);
+        }
+        const int byte = mx4_scale_byte(quad_larger(top));
+        codes[(row * groups + g0 + s) * 16 + lane] = mx4_codes(v, mx4_divisor(byte));
+        const unsigned word = mx4_scale_word(byte);
+        if (lane == 0) scales[(long long)(g0 + s) * rows + row] = word;
+    }
 }
 
 template <int DT>
-__global__ void __launch_bounds__(256) tdc_mx4_dequantize_kernel(const unsigned char *codes, const unsigned char *scales, long long rows,
-                                                             long long K, long long blocks, void *y, long long stride) {
+__global__ void __launch_bounds__(256) tdc_mx4_dequantize_kernel(const unsigned *codes, const unsigned *scales, long long rows, long long K,
+                                                                 int groups, int runs, void *y, long long stride) {
     using T = typename Num<DT>::type;
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (idx >= rows * blocks) return;
-    const long long row = idx / blocks, kb = idx - row * blocks;
-    const int n = (int)max(0ll, min(32ll, K - kb * 32));
-    T *dst = reinterpret_cast<T *>(y) + row * stride + kb * 32;
-    const float scale = mx4_scale(scales[((kb >> 2) * rows + row) * 4 + (kb & 3)]);
-    const uint4 c = *reinterpret_cast<const uint4 *>(codes + idx * 16);
-    const unsigned w[4] = {c.x, c.y, c.z, c.w};
-    constexpr float value[8] = {0.0f, 0.5f, 1.0f, 1.5f, 2.0f, 3.0f, 4.0f, 6.0f};
-    for (int i = 0; i < n; ++i) {
-        const unsigned code = w[i >> 3] >> (4 * (i & 7));
-        const float v = value[code & 7] * scale;
-        dst[i] = Num<DT>::down(code & 8 ? -v : v);
+    typedef T vec_t __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    const long long rb = blockIdx.x / (unsigned)runs;
+    const int g0 = (blockIdx.x - (unsigned)rb * runs) * kSteps, lane = threadIdx.x & 15;
+    const long long row = rb * kRows + (threadIdx.x >> 4);
+    if (row >= rows) return;
+    T *const dst = reinterpret_cast<T *>(y) + row * stride + lane * 8;
+    unsigned code[kSteps], word[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int g = min(g0 + s, groups - 1);
+        code[s] = codes[(row * groups + g) * 16 + lane];
+        word[s] = scales[(long long)g * rows + row];
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const long long k = (long long)(g0 + s) * 128 + lane * 8;
+        if (k >= K) continue;
+        const int byte = (word[s] >> (lane >> 2) * 8) & 255;
+        float v[8];
+        mx4_values(code[s], mx4_divisor(byte), v);
+        vec_t p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = Num<DT>::down(byte == 255 ? __builtin_nanf("") : v[i]);
+        if (k + 8 <= K) *reinterpret_cast<vec_t *>(dst + k - lane * 8) = p;
+        else
+            for (int i = 0; i < 8; ++i)
+                if (k + i < K) dst[k - lane * 8 + i] = p[i];
     }
 }
 
 int launch_mx4_quantize(const void *x, int dtype, long long rows, long long K, long long stride, void *codes, void *scales, void *stream) {
-    const long long blocks = mx4_padded(K) / 32;
-    const unsigned grid = (unsigned)((rows * blocks + 255) / 256);
+    const int groups = (int)(mx4_padded(K) / 128), runs = (groups + kSteps - 1) / kSteps;
+    const unsigned grid = (unsigned)((rows + kRows - 1) / kRows * runs);
     const hipStream_t s = (hipStream_t)stream;
-    auto *c = (unsigned char *)codes, *e = (unsigned char *)scales;
-    if (dtype == TDC_F32) tdc_mx4_quantize_kernel<TDC_F32><<<grid, 256, 0, s>>>(x, rows, K, stride, blocks, c, e);
-    else if (dtype == TDC_F16) tdc_mx4_quantize_kernel<TDC_F16><<<grid, 256, 0, s>>>(x, rows, K, stride, blocks, c, e);
-    else tdc_mx4_quantize_kernel<TDC_BF16><<<grid, 256, 0, s>>>(x, rows, K, stride, blocks, c, e);
+    auto *c = (unsigned *)codes, *e = (unsigned *)scales;
+    if (dtype == TDC_F32) tdc_mx4_quantize_kernel<TDC_F32><<<grid, 256, 0, s>>>(x, rows, K, stride, groups, runs, c, e);
+    else if (dtype == TDC_F16) tdc_mx4_quantize_kernel<TDC_F16><<<grid, 256, 0, s>>>(x, rows, K, stride, groups, runs, c, e);
+    else tdc_mx4_quantize_kernel<TDC_BF16><<<grid, 256, 0, s>>>(x, rows, K, stride, groups, runs, c, e);
     return (int)hipGetLastError();
 }
 
 int launch_mx4_dequantize(const void *codes, const void *scales, long long rows, long long K, void *y, int dtype, long long stride,
                           void *stream) {
-    const long long blocks = mx4_padded(K) / 32;
-    const unsigned grid = (unsigned)((rows * blocks + 255) / 256);
+    const int groups = (int)(mx4_padded(K) / 128), runs = (groups + kSteps - 1) / kSteps;
+    const unsigned grid = (unsigned)((rows + kRows - 1) / kRows * runs);
     const hipStream_t s = (hipStream_t)stream;
-    auto *c = (const unsigned char *)codes, *e = (const unsigned char *)scales;
-    if (dtype == TDC_F32) tdc_mx4_dequantize_kernel<TDC_F32><<<grid, 256, 0, s>>>(c, e, rows, K, blocks, y, stride);
-    else if (dtype == TDC_F16) tdc_mx4_dequantize_kernel<TDC_F16><<<grid, 256, 0, s>>>(c, e, rows, K, blocks, y, stride);
-    else tdc_mx4_dequantize_kernel<TDC_BF16><<<grid, 256, 0, s>>>(c, e, rows, K, blocks, y, stride);
+    auto *c = (const unsigned *)codes, *e = (const unsigned *)scales;
+    if (dtype == TDC_F32) tdc_mx4_dequantize_kernel<TDC_F32><<<grid, 256, 0, s>>>(c, e, rows, K, groups, runs, y, stride);
+    else if (dtype == TDC_F16) tdc_mx4_dequantize_kernel<TDC_F16><<<grid, 256, 0, s>>>(c, e, rows, K, groups, runs, y, stride);
+    else tdc_mx4_dequantize_kernel<TDC_BF16><<<grid, 256, 0, s>>>(c, e, rows, K, groups, runs, y, stride);
     return (int)hipGetLastError();
 }
 

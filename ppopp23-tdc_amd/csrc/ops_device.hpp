@@ -115,5 +115,22 @@ __device__ __forceinline__ unsigned mx4_codes(const float *v, float divisor) {
     r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], divisor, 2);
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], divisor, 3);
 }
+// What eight codes stand for.
+__device__ __forceinline__ void mx4_values(unsigned codes, float scale, float (&v)[8]) {
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 1);
+    const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 3);
+    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = c[0], v[5] = c[1], v[6] = d[0], v[7] = d[1];
+}
+// The largest magnitude of four neighbouring lanes (quad_perm: each lane's neighbour, then the other pair).
+__device__ __forceinline__ float quad_larger(float top) {
+    top = larger(top, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, top), 0xB1, 0xf, 0xf, true)));
+    return larger(top, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, top), 0x4E, 0xf, 0xf, true)));
+}
+// The scale bytes of the four quads of sixteen lanes as one word, in lane 0 of them (row_shl: the value n lanes up).
+__device__ __forceinline__ unsigned mx4_scale_word(int byte) {
+    const unsigned b1 = __builtin_amdgcn_mov_dpp(byte, 0x104, 0xf, 0xf, true), b2 = __builtin_amdgcn_mov_dpp(byte, 0x108, 0xf, 0xf, true),
+                   b3 = __builtin_amdgcn_mov_dpp(byte, 0x10C, 0xf, 0xf, true);
+    return (unsigned)byte | b1 << 8 | b2 << 16 | b3 << 24;
+}
 
 }  // namespace tdc
