@@ -245,7 +245,16 @@ __global__ void __launch_bounds__(kThreads) tdc_norm_apply_mx4_kernel(const Norm
         const float divisor = mx4_divisor(byte);
         *reinterpret_cast<uint4 *>(a.codes + row * (padded / 2) + block * 16) =
             make_uint4(mx4_codes(v, divisor), mx4_codes(v + 8, divisor), mx4_codes(v + 16, divisor), mx4_codes(v + 24, divisor));
-        a.scales[((block >> 2) * a.rows + row) * 4 + (block & 3)] = (unsigned char)byte;
+        a.scales[((block >> 4) * a.rows + row) * 16 + (block & 3) * 4 + (block >> 2 & 3)] = (unsigned char)byte;
+    }
+    // (the scale bytes past a row's last block)
+    if (p.c0 + p.width == a.C) {
+        const int past = (a.C + 511) / 512 * 16 - padded / 32;
+        for (int i = threadIdx.x; i < p.rows * past; i += kThreads) {
+            const int r = i / past, block = padded / 32 + i - r * past;
+            const long long row = (long long)p.image * a.pixels + p.row0 + r;
+            a.scales[((block >> 4) * a.rows + row) * 16 + (block & 3) * 4 + (block >> 2 & 3)] = 0;
+        }
     }
 }
 

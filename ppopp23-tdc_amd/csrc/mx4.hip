@@ -1,15 +1,15 @@
 // Numbers into microscaled 4-bit floating point and back (format and layout: include/tdc.h).
 //
 // Memory traffic: x on one side, 17/32 byte a number on the other.  Sixteen lanes take 128 numbers of a row, eight each: one request of
-// 16 bytes (two in 32 bits), a block's largest magnitude from four neighbouring lanes, one word of codes a lane and
-// one word of scales from the sixteen.  The sixteen rows of a workgroup keep their scale words together in memory.
+// 16 bytes (two in 32 bits), a block's largest magnitude from four neighbouring lanes, one word of codes a lane.  A thread goes
+// on for 512 numbers, so that a quad of lanes ends up with one word of scales.
 // Requests need no alignment beyond the number's own; only the last one of a row may end early.
 #include "ops_device.hpp"
 
 namespace tdc {
 
 static constexpr int kRows = 16;      // of a workgroup of 256
-static constexpr int kSteps = 4;      // runs of 128 numbers a thread has in flight
+static constexpr int kSteps = 4;      // runs of 128 numbers a thread has in flight: those of a word of scales
 
 template <int DT>
 __global__ void __launch_bounds__(256) tdc_mx4_quantize_kernel(const void *x, long long rows, long long K, long long stride, int groups,
@@ -44,6 +44,7 @@ __global__ void __launch_bounds__(256) tdc_mx4_quantize_kernel(const void *x, lo
             }
         }
     }
+    unsigned word = 0;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
         if (g0 + s >= groups) continue;
@@ -55,9 +56,9 @@ __global__ void __launch_bounds__(256) tdc_mx4_quantize_kernel(const void *x, lo
         }
         const int byte = mx4_scale_byte(quad_larger(top));
         codes[(row * groups + g0 + s) * 16 + lane] = mx4_codes(v, mx4_divisor(byte));
-        const unsigned word = mx4_scale_word(byte);
-        if (lane == 0) scales[(long long)(g0 + s) * rows + row] = word;
+        word |= (unsigned)byte << 8 * s;
     }
+    if ((lane & 3) == 0) scales[((g0 >> 2) * rows + row) * 4 + (lane >> 2)] = word;
 }
 
 template <int DT>
@@ -70,18 +71,18 @@ __global__ void __launch_bounds__(256) tdc_mx4_dequantize_kernel(const unsigned 
     const long long row = rb * kRows + (threadIdx.x >> 4);
     if (row >= rows) return;
     T *const dst = reinterpret_cast<T *>(y) + row * stride + lane * 8;
-    unsigned code[kSteps], word[kSteps];
+    unsigned code[kSteps];
+    const unsigned word = scales[((g0 >> 2) * rows + row) * 4 + (lane >> 2)];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
         const int g = min(g0 + s, groups - 1);
         code[s] = codes[(row * groups + g) * 16 + lane];
-        word[s] = scales[(long long)g * rows + row];
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
         const long long k = (long long)(g0 + s) * 128 + lane * 8;
         if (k >= K) continue;
-        const int byte = (word[s] >> (lane >> 2) * 8) & 255;
+        const int byte = (word >> 8 * s) & 255;
         float v[8];
         mx4_values(code[s], mx4_divisor(byte), v);
         vec_t p;

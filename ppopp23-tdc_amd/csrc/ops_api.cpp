@@ -137,8 +137,8 @@ int mx4_range(const char *what, long long rows, long long K) {
 int mx4_check(const char *what, long long rows, long long K, const void *codes, const void *scales) {
     if (int st = mx4_range(what, rows, K)) return st;
     if (rows && (!codes || !scales)) return invalid(std::string(what) + ": null codes or scales");
-    if (rows && (!aligned(codes, 16) || !aligned(scales, 4)))
-        return invalid(std::string(what) + ": codes have to be 16-byte and scales 4-byte aligned");
+    if (rows && (!aligned(codes, 16) || !aligned(scales, 16)))
+        return invalid(std::string(what) + ": codes and scales have to be 16-byte aligned");
     return TDC_OK;
 }
 
@@ -148,8 +148,8 @@ int linear_check(const tdc_mx4_linear_desc *desc, tdc_mx4_linear_desc &d) {
     if (!desc) return invalid("4-bit product: null descriptor");
     d = *desc;
     if (d.M < 0 || d.N < 0 || d.K < 1) return invalid("4-bit product: M, N and K have to be 0, 0 and 1 at least");
-    if (d.K > (1ll << 30) || d.M > (1ll << 34) || d.N > (1ll << 34) || d.M * d.N > (1ll << 40))
-        return invalid("4-bit product: too large");
+    if (d.K > (1ll << 24) || d.M > (1ll << 34) || d.N > (1ll << 34) || d.M * d.N > (1ll << 40))
+        return invalid("4-bit product: K above 2^24 or M * N above 2^40");
     if (d.x_dtype != TDC_MX4 && !number(d.x_dtype)) return invalid("4-bit product: unknown x_dtype");
     if (!number(d.y_dtype)) return invalid("4-bit product: y_dtype has to be TDC_F32, TDC_F16 or TDC_BF16");
     if (d.bias_dtype != TDC_F32 && d.bias_dtype != d.y_dtype) return invalid("4-bit product: bias_dtype has to be TDC_F32 or y_dtype");
@@ -163,7 +163,7 @@ int linear_check(const tdc_mx4_linear_desc *desc, tdc_mx4_linear_desc &d) {
 }
 size_t linear_codes(const tdc_mx4_linear_desc &d) { return (size_t)(d.M * mx4_padded(d.K) / 2); }
 size_t linear_ws(const tdc_mx4_linear_desc &d) {
-    return d.x_dtype == TDC_MX4 ? 0 : linear_codes(d) + (size_t)(d.M * mx4_padded(d.K) / 32);
+    return d.x_dtype == TDC_MX4 ? 0 : linear_codes(d) + (size_t)(d.M * mx4_scale_bytes(d.K));
 }
 
 }  // namespace
@@ -280,7 +280,7 @@ TDC_ENTRY_END
 int tdc_mx4_sizes(int64_t rows, int64_t K, size_t *code_bytes, size_t *scale_bytes) TDC_ENTRY {
     if (int st = mx4_range("4-bit numbers", rows, K)) return st;
     if (code_bytes) *code_bytes = (size_t)(rows * mx4_padded(K) / 2);
-    if (scale_bytes) *scale_bytes = (size_t)(rows * mx4_padded(K) / 32);
+    if (scale_bytes) *scale_bytes = (size_t)(rows * mx4_scale_bytes(K));
     return TDC_OK;
 }
 TDC_ENTRY_END

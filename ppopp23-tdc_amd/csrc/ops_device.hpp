@@ -126,11 +126,5 @@ __device__ __forceinline__ float quad_larger(float top) {
     top = larger(top, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, top), 0xB1, 0xf, 0xf, true)));
     return larger(top, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, top), 0x4E, 0xf, 0xf, true)));
 }
-// The scale bytes of the four quads of sixteen lanes as one word, in lane 0 of them (row_shl: the value n lanes up).
-__device__ __forceinline__ unsigned mx4_scale_word(int byte) {
-    const unsigned b1 = __builtin_amdgcn_mov_dpp(byte, 0x104, 0xf, 0xf, true), b2 = __builtin_amdgcn_mov_dpp(byte, 0x108, 0xf, 0xf, true),
-                   b3 = __builtin_amdgcn_mov_dpp(byte, 0x10C, 0xf, 0xf, true);
-    return (unsigned)byte | b1 << 8 | b2 << 16 | b3 << 24;
-}
 
 }  // namespace tdc

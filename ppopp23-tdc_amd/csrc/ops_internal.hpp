@@ -16,6 +16,8 @@ inline long long round_up(long long v, long long to) { return (v + to - 1) / to 
 
 // Numbers of a row in 4 bits, rounded up to the 128 of one matrix instruction.
 inline long long mx4_padded(long long K) { return round_up(K, 128); }
+// Scale bytes of a row.
+inline long long mx4_scale_bytes(long long K) { return round_up(K, 512) / 32; }
 
 // How a norm's work is dealt out.  A workgroup owns `unit` channels (unit / vec vectors, a thread each) of `chunk_rows`
 // pixels of one image; `slots` partial results per image and group meet in the second launch.

@@ -304,6 +304,14 @@ def test_product(M, N, K, dtype):
     check_product(tdc_amd.mx4_linear(xd, wq, out_dtype=other), xv, wv, None, None, "none", "another type out")
 
 
+@pytest.mark.parametrize("dtype,M,N,K", [(F32, 3333, 3850, 420), (F16, 4100, 3590, 128), (BF16, 3328, 4096, 1700)])
+def test_product_of_many_tiles(dtype, M, N, K):
+    x, w = numbers(16, M, K).to(dtype), numbers(17, N, K) / math.sqrt(K)
+    bias, residual = numbers(18, N), numbers(19, M, N).to(dtype)
+    y = tdc_amd.mx4_linear(x.cuda(), tdc_amd.mx4_quantize(w.cuda()), bias.cuda(), residual.cuda(), act="relu")
+    check_product(y, ref.mx4(x.double().numpy())[2], ref.mx4(w.double().numpy())[2], bias, residual, "relu")
+
+
 def test_product_of_whole_numbers_is_exact():
     g = seeded(21)
     values = torch.tensor([0.0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.5, -1, -1.5, -2, -3, -4, -6])
