@@ -116,7 +116,7 @@ def test_python_refusals_without_a_device():
     with pytest.raises(RuntimeError, match="no gradient"):
         tdc_amd.group_norm_act_mx4(x.requires_grad_(), 2)
     with pytest.raises(ValueError, match="uint8 device tensor"):
-        tdc_amd.Mx4Tensor(torch.zeros(2, 64, dtype=torch.uint8), torch.zeros(1, 2, 16, dtype=torch.uint8), (2, 128))
+        tdc_amd.Mx4Tensor(torch.zeros(1, 2, 64, dtype=torch.uint8), torch.zeros(1, 2, 16, dtype=torch.uint8), (2, 128))
 
 
 def test_channels_last_is_recognised():

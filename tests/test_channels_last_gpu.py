@@ -108,7 +108,7 @@ def test_norm_of_nothing_and_of_constants():
         x.requires_grad_()
         dx, dw, db = torch.autograd.grad(tdc_amd.group_norm_act(x, 2, w, b).sum(), (x, w, b))
         assert dx.shape == shape and not dw.any() and not db.any()
-        assert tdc_amd.group_norm_act_mx4(x.detach(), 2).codes.shape[0] == 0
+        assert tdc_amd.group_norm_act_mx4(x.detach(), 2).rows == 0
     x = torch.full((2, 8, 5, 5), 3.25, device="cuda").contiguous(memory_format=torch.channels_last)
     beta = torch.arange(8.0, device="cuda") - 3
     y = tdc_amd.group_norm_act(x, 2, bias=beta, act="relu")
