@@ -451,8 +451,9 @@ int tdc_group_norm_mx4_workspace(const tdc_group_norm_desc *desc, size_t *bytes)
  * block is 2^(floor(log2 max|x|) - 2), kept as the byte exponent + 127 (0 at least); numbers are rounded to nearest,
  * halfway cases to the even code, and saturate at 6.  A block that holds an infinity or a NaN gets the scale 255 and
  * stands for NaNs; a block of zeros gets the scale 0.  Layout, with Kp = K rounded up to 128:
- *   codes   [Kp / 128][rows][64] bytes, the number of even place in the low half; zeros from K on.  (The same 128
- *           numbers of neighbouring rows are neighbours: a matrix product reads a block of rows 128 numbers at a time.)
+ *   codes   [Kp / 128][ceil(rows / 32)][4][32][16] bytes: of 128 numbers and 32 rows the first blocks of 32 numbers row by
+ *           row, the second, the third, the fourth, as the matrix instruction's lanes take them; the number of even
+ *           place in the low half of a byte, zeros from K on, nothing in particular from `rows` on
  *   scales  [ceil(K / 512)][rows][16] bytes, block b of the sixteen of 512 numbers at byte 4 (b mod 4) + b / 4 (zeros
  *           past the last block): the word a lane of the matrix instruction wants for four of them in a row */
 int tdc_mx4_sizes(int64_t rows, int64_t K, size_t *code_bytes, size_t *scale_bytes);

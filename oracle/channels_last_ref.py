@@ -71,8 +71,8 @@ def mx4(x):
 
 def mx4_unpack(codes, scales, K):
     """The library's bytes as (codes [rows, K], scale bytes [rows, blocks], what pads the codes)."""
-    rows = codes.shape[1]
-    codes = codes.transpose(1, 0, 2).reshape(rows, 64 * codes.shape[0])
+    rows = scales.shape[1]
+    codes = codes.transpose(1, 3, 0, 2, 4).reshape(32 * codes.shape[1], 64 * codes.shape[0])[:rows]
     nib = np.stack([codes & 15, codes >> 4], axis=2).reshape(rows, 2 * codes.shape[1])
     byte = scales.transpose(1, 0, 2).reshape(rows, scales.shape[0], 4, 4).transpose(0, 1, 3, 2).reshape(rows, 16 * scales.shape[0])
     assert not byte[:, 4 * (codes.shape[1] // 64):].any()

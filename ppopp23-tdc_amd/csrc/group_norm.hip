@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads) tdc_norm_apply_mx4_kernel(const Norm
         }
         const int byte = mx4_scale_byte(top);
         const float divisor = mx4_divisor(byte);
-        *reinterpret_cast<uint4 *>(a.codes + ((block >> 2) * a.rows + row) * 64 + (block & 3) * 16) =
+        *reinterpret_cast<uint4 *>(a.codes + mx4_block_at(a.rows, row, block)) =
             make_uint4(mx4_codes(v, divisor), mx4_codes(v + 8, divisor), mx4_codes(v + 16, divisor), mx4_codes(v + 24, divisor));
         a.scales[((block >> 4) * a.rows + row) * 16 + (block & 3) * 4 + (block >> 2 & 3)] = (unsigned char)byte;
     }

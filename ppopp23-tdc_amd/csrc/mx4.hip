@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(256) tdc_mx4_quantize_kernel(const void *x, lo
             top = larger(top, v[i]);
         }
         const int byte = mx4_scale_byte(quad_larger(top));
-        codes[((g0 + s) * rows + row) * 16 + lane] = mx4_codes(v, mx4_divisor(byte));
+        codes[(mx4_block_at(rows, row, (g0 + s) * 4 + (lane >> 2)) >> 2) + (lane & 3)] = mx4_codes(v, mx4_divisor(byte));
         word |= (unsigned)byte << 8 * s;
     }
     if ((lane & 3) == 0) scales[((g0 >> 2) * rows + row) * 4 + (lane >> 2)] = word;
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(256) tdc_mx4_dequantize_kernel(const unsigned 
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
         const int g = min(g0 + s, groups - 1);
-        code[s] = codes[(g * rows + row) * 16 + lane];
+        code[s] = codes[(mx4_block_at(rows, row, g * 4 + (lane >> 2)) >> 2) + (lane & 3)];
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {

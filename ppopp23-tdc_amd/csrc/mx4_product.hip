@@ -58,13 +58,12 @@ static __device__ __forceinline__ void bias8(const ProductArgs &a, long long n, 
 // ---- tiles ----
 //
 // A workgroup of four waves owns 64 MB rows of x and 64 NB of w, a wave a quarter of it: MB x NB blocks of 32 x 32.  A step is
-// 128 numbers of each row.  Codes go from global memory through registers into LDS buffers, a step each: asked for four steps
-// ahead of their use, stored two ahead; scales do so for four steps at a time.  A wave's step has a part for each two blocks of
-// weights; each part starts the LDS reads of the next part's weights and of the next step's x, stores what global memory has
-// brought, and asks for more, so that one wave to a SIMD keeps the matrix unit fed across its one barrier a step.
+// 128 numbers of each row.  Codes go straight from global memory into one of four LDS buffers, a step each, 1 KiB a request:
+// asked for three steps ahead of their use, waited for one ahead; scales do so for four steps at a time.  A wave's step has a
+// part for each two blocks of weights; each part starts the LDS reads of the next part's weights and of the next step's x, so
+// that one wave to a SIMD keeps the matrix unit fed across its one barrier a step.  LDS holds the codes as they lie in
+// memory: a block's read is 1 KiB in a row, which meets no bank twice.
 //
-// LDS holds 32 rows by their places: place p of row i, 16 bytes, at 512 p + 16 (i ^ 4 p).  Reads take a place of 32 rows, 512 bytes in
-// a row; stores take four places of sixteen rows, and the twist spreads them over the banks.
 // The row of w that is row r of a block: bits 2 and 3 change places, which makes a lane's outputs 8 i .. 8 i + 7 neighbours.
 static __device__ __forceinline__ int weight_row(int r) { return (r & 19) | (r & 4) << 1 | (r & 8) >> 1; }
 
@@ -74,7 +73,8 @@ struct Tile {
     static constexpr int kBuffer = (M + N) * 64;              // bytes of a step's codes: x, then w
     static constexpr int kScales = (M + N) * 16;              // bytes of four steps' scales
     static constexpr int kLds = 4 * kBuffer + 2 * kScales;
-    static constexpr int kX = MB, kChunks = MB + NB;          // requests of 16 bytes a thread and step: of x, in all
+    static constexpr int kX = MB, kChunks = MB + NB;          // requests of a wave and step: of x, in all
+    static constexpr int kScaleRequests = (M + N) / 256;      // of a wave and four steps
     static constexpr int kParts = NB / 2;
 };
 
@@ -92,49 +92,45 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
     const int group = id / (8 * tiles_n), rest = id - group * 8 * tiles_n, high = min(8, tiles_m - group * 8);
     const long long m0 = (long long)(group * 8 + rest % high) * L::M, n0 = (long long)(rest / high) * L::N;
 
-    const int last = a.ksteps - 1, last_m = (int)min((long long)L::M, a.M - m0) - 1, last_n = (int)min((long long)L::N, a.N - n0) - 1;
-    const unsigned char *const xc = a.x_codes + m0 * 64, *const wc = a.w_codes + n0 * 64;
-    const int place = t & 3;
-    unsigned from[L::kChunks];          // (rows past the last repeat it: their products go nowhere)
+    // Requests straight into LDS: 16 bytes a lane, in the order of the lanes, at a wave's own place.
+    auto bring = [&](const unsigned char *base, int offset, unsigned char *to) {
+        const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(base), 0, 0x7fffffff, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)to, 16, lane * 16, offset, 0, 0);
+    };
+    // Codes: request i of a wave is half a block of 32 rows.  (Blocks past the last repeat it: their products go nowhere.)
+    const long long x_blocks = (a.M + 31) >> 5, w_blocks = (a.N + 31) >> 5;
+    int from[L::kChunks];
 #pragma unroll
     for (int i = 0; i < L::kChunks; ++i) {
-        const int row = (i < L::kX ? i : i - L::kX) * 64 + (t >> 2);
-        from[i] = min(row, i < L::kX ? last_m : last_n) * 64 + place * 16;
+        const int c = (i < L::kX ? i : i - L::kX) * 4 + wave;
+        from[i] = (int)min((long long)(c / 2), (i < L::kX ? x_blocks - (m0 >> 5) : w_blocks - (n0 >> 5)) - 1) * 2048 + c % 2 * 1024;
     }
-    i4_t chunk[2][L::kChunks];
-    auto fetch = [&](int set, int i, int step) {
-        const long long k = min(step, last);
-        chunk[set][i] = *reinterpret_cast<const i4_t *>((i < L::kX ? xc + k * a.M * 64 : wc + k * a.N * 64) + from[i]);
+    auto fetch = [&](int i, int step) {
+        const long long k = min(step, a.ksteps - 1);
+        const unsigned char *const base = i < L::kX ? a.x_codes + (k * x_blocks + (m0 >> 5)) * 2048 : a.w_codes + (k * w_blocks + (n0 >> 5)) * 2048;
+        bring(base, from[i], lds + (step & 3) * L::kBuffer + (i * 4 + wave) * 1024);
     };
-    const int to = (t >> 7) * 2048 + place * 512 + ((t >> 2 & 31) ^ 4 * place) * 16;
-    auto park = [&](int set, int i, int buffer) { *reinterpret_cast<i4_t *>(lds + buffer + i * 4096 + to) = chunk[set][i]; };
-
-    // Scales of four steps: thread t brings row t of x and row t of w.
-    i4_t sx_in, sw_in;
-    const int groups = (a.ksteps + 3) / 4;
+    // Scales of four steps: rows of x, then of w, a row a thread.
+    const int groups = (a.ksteps + 3) / 4, last_m = (int)min((long long)L::M, a.M - m0) - 1, last_n = (int)min((long long)L::N, a.N - n0) - 1;
+    unsigned char *const lds_scales = lds + 4 * L::kBuffer;
     auto fetch_scales = [&](int g) {
         const long long at = min(g, groups - 1);
-        sx_in = *reinterpret_cast<const i4_t *>(a.x_scales + (at * a.M + m0 + min(t, last_m)) * 16);
-        sw_in = *reinterpret_cast<const i4_t *>(a.w_scales + (at * a.N + n0 + min(t, last_n)) * 16);
-    };
-    unsigned char *const lds_scales = lds + 4 * L::kBuffer;
-    auto park_scales = [&](int g) {
-        unsigned char *const to = lds_scales + (g & 1) * L::kScales + t * 16;
-        if (L::M == 256 || t < L::M) *reinterpret_cast<i4_t *>(to) = sx_in;
-        if (L::N == 256 || t < L::N) *reinterpret_cast<i4_t *>(to + L::M * 16) = sw_in;
+        unsigned char *const to = lds_scales + (g & 1) * L::kScales + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < L::kScaleRequests; ++i) {
+            const bool of_x = i * 256 + wave * 64 < L::M;
+            const unsigned char *const base = of_x ? a.x_scales + (at * a.M + m0) * 16 : a.w_scales + (at * a.N + n0) * 16;
+            const int row = i * 256 + t, in = of_x ? min(row, last_m) : min(row - L::M, last_n);
+            const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(base), 0, 0x7fffffff, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)(to + i * 4096), 16, in * 16, 0, 0, 0);
+        }
     };
 
-    // Places q and 2 + q (`half`) of row r of a block.
+    // Row r of a block; its places q and 2 + q for the two halves of a step.
     const int x_row = wm * 32 * MB + r, w_row = wn * 32 * NB + weight_row(r);
-    const int x_at = wm * MB * 2048 + q * 512, w_at = L::M * 64 + wn * NB * 2048 + q * 512;
-    int x_in[2], w_in[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        x_in[h] = x_at + h * 1024 + (r ^ 4 * (2 * h + q)) * 16;
-        w_in[h] = w_at + h * 1024 + (weight_row(r) ^ 4 * (2 * h + q)) * 16;
-    }
-    auto x_frag = [&](int i, int half, int buffer) { return *reinterpret_cast<const i4_t *>(lds + buffer + x_in[half] + i * 2048); };
-    auto w_frag = [&](int j, int half, int buffer) { return *reinterpret_cast<const i4_t *>(lds + buffer + w_in[half] + j * 2048); };
+    const int x_at = wm * MB * 2048 + q * 512 + r * 16, w_at = L::M * 64 + wn * NB * 2048 + q * 512 + weight_row(r) * 16;
+    auto x_frag = [&](int i, int half, int buffer) { return *reinterpret_cast<const i4_t *>(lds + buffer + x_at + i * 2048 + half * 1024); };
+    auto w_frag = [&](int j, int half, int buffer) { return *reinterpret_cast<const i4_t *>(lds + buffer + w_at + j * 2048 + half * 1024); };
     auto read_scales = [&](int g, int (&sx)[MB][2], int (&sw)[NB][2]) {
         const unsigned char *const at = lds_scales + (g & 1) * L::kScales + q * 4;
 #pragma unroll
@@ -145,11 +141,17 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
             for (int j = 0; j < NB; ++j) sw[j][h] = *reinterpret_cast<const int *>(at + (L::M + w_row + j * 32) * 16 + h * 8);
         }
     };
-    auto meet = [&]() {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    // Waits until all but the wave's newest `left` requests have come and its LDS reads are done, then for the other waves.  (A fence
+    // in place of the waits would wait for every request.)
+    auto meet = [&](auto left) {
+        constexpr int n = decltype(left)::value;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 7 << 4);
         __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        asm volatile("" ::: "memory");
     };
+    using None = std::integral_constant<int, 0>;
+    using Codes = std::integral_constant<int, L::kChunks>;
 
     f16_t acc[NB][MB];
 #pragma unroll
@@ -159,27 +161,14 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.0f;
 
-    // (each set's requests in order: the waits of the loop count them)
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-        for (int i = 0; i < L::kChunks; ++i) fetch(s, i, s);
-        __builtin_amdgcn_sched_barrier(0);
-    }
+    // (an odd number of steps is rounded up: the scales past the last are zero, and so is what that step adds)
+    const int steps = (a.ksteps + 1) / 2 * 2;
     fetch_scales(0);
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 3; ++s)
 #pragma unroll
-        for (int i = 0; i < L::kChunks; ++i) {
-            park(s, i, s * L::kBuffer);
-            fetch(s, i, 2 + s);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    park_scales(0);
-    fetch_scales(1);
-    meet();
+        for (int i = 0; i < L::kChunks; ++i) fetch(i, s);
+    meet(Codes{});
     i4_t x[2][MB][2], w[2][2][2];
     int sx[MB][2], sw[NB][2];
 #pragma unroll
@@ -194,7 +183,7 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
     // Step `step`, of which S = step mod 2.
     auto run = [&](auto parity, int step) {
         constexpr int S = decltype(parity)::value, P = L::kParts;
-        const int now = (step & 3) * L::kBuffer, next = (step + 1 & 3) * L::kBuffer, fill = (step + 2 & 3) * L::kBuffer;
+        const int now = (step & 3) * L::kBuffer, next = (step + 1 & 3) * L::kBuffer;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const int set = P == 1 ? S : p & 1;
@@ -207,10 +196,7 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
                 constexpr int kSlots = 2 * P;
                 const int slot = 2 * p + h;
 #pragma unroll
-                for (int i = slot * L::kChunks / kSlots; i < (slot + 1) * L::kChunks / kSlots; ++i) {
-                    park(S, i, fill);
-                    fetch(S, i, step + 4);
-                }
+                for (int i = slot * L::kChunks / kSlots; i < (slot + 1) * L::kChunks / kSlots; ++i) fetch(i, step + 3);
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -226,21 +212,21 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
 #pragma unroll
             for (int j = 0; j < NB; ++j) sw[j][h] = (int)((unsigned)sw[j][h] >> 8);
         }
-        meet();
+        meet(Codes{});      // (the codes of the step after the next have to be there: all requests but this step's)
     };
-    // (an odd number of steps is rounded up: the scales past the last are zero, and so is what that step adds)
+    // (no branch stands between a step's requests and its matrix instructions, or the compiler moves these behind the barrier; the
+    // last three steps bring codes that no one needs)
     int step = 0;
-    const int steps = (a.ksteps + 1) / 2 * 2;
     for (int g = 0; g < groups; ++g) {
-        // Four steps: their scales are in registers; those of the next four are stored here and read when these are done.
-        park_scales(g + 1);
-        fetch_scales(g + 2);
+        // Four steps: their scales are in registers, those of the next four are asked for here and read when these are done.
+        fetch_scales(g + 1);
         for (const int end = min(step + 4, steps); step < end; step += 2) {
             run(std::integral_constant<int, 0>{}, step);
             run(std::integral_constant<int, 1>{}, step + 1);
         }
         read_scales(g + 1, sx, sw);
     }
+    meet(None{});       // (nothing may still be on its way into LDS when the workgroup ends)
 
     // A lane's outputs of a block: row r of x, and of w 16 u + 8 q .. 16 u + 8 q + 7, u = 0, 1.
     auto finish = [&](auto act) {

@@ -1,6 +1,4 @@
 // C entry points of the channels-last operators: argument checks, plans, workspaces.
-#include <hip/hip_runtime_api.h>
-
 #include <algorithm>
 #include <cmath>
 #include <numeric>
@@ -161,7 +159,7 @@ int linear_check(const tdc_mx4_linear_desc *desc, tdc_mx4_linear_desc &d) {
     if (d.M > 1 && (d.y_stride < d.N || d.residual_stride < d.N)) return invalid("4-bit product: a row stride below N");
     return TDC_OK;
 }
-size_t linear_codes(const tdc_mx4_linear_desc &d) { return (size_t)(d.M * mx4_padded(d.K) / 2); }
+size_t linear_codes(const tdc_mx4_linear_desc &d) { return (size_t)mx4_code_bytes(d.M, d.K); }
 size_t linear_ws(const tdc_mx4_linear_desc &d) {
     return d.x_dtype == TDC_MX4 ? 0 : linear_codes(d) + (size_t)(d.M * mx4_scale_bytes(d.K));
 }
@@ -279,7 +277,7 @@ TDC_ENTRY_END
 
 int tdc_mx4_sizes(int64_t rows, int64_t K, size_t *code_bytes, size_t *scale_bytes) TDC_ENTRY {
     if (int st = mx4_range("4-bit numbers", rows, K)) return st;
-    if (code_bytes) *code_bytes = (size_t)(rows * mx4_padded(K) / 2);
+    if (code_bytes) *code_bytes = (size_t)mx4_code_bytes(rows, K);
     if (scale_bytes) *scale_bytes = (size_t)(rows * mx4_scale_bytes(K));
     return TDC_OK;
 }

@@ -5,7 +5,7 @@
 #include <cstddef>
 #include <cstdint>
 
-#include <hip/hip_vector_types.h>
+#include <hip/hip_runtime.h>
 
 #include "tdc.h"
 
@@ -16,6 +16,11 @@ inline long long round_up(long long v, long long to) { return (v + to - 1) / to 
 
 // Numbers of a row in 4 bits, rounded up to the 128 of one matrix instruction.
 inline long long mx4_padded(long long K) { return round_up(K, 128); }
+// Code bytes of `rows` rows, and the place of block b (of 32 numbers) of a row.
+inline long long mx4_code_bytes(long long rows, long long K) { return round_up(rows, 32) * mx4_padded(K) / 2; }
+__host__ __device__ inline long long mx4_block_at(long long rows, long long row, long long b) {
+    return ((b >> 2) * ((rows + 31) >> 5) + (row >> 5)) * 2048 + (b & 3) * 512 + (row & 31) * 16;
+}
 // Scale bytes of a row.
 inline long long mx4_scale_bytes(long long K) { return round_up(K, 512) / 32; }
 

@@ -232,7 +232,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
 class Mx4Tensor:
     """Numbers in microscaled 4-bit floating point, in blocks of 32 along the last axis.
 
-    ``shape`` is that of the numbers, ``codes`` [ceil(K / 128), rows, 64] and ``scales``
+    ``shape`` is that of the numbers, ``codes`` [ceil(K / 128), ceil(rows / 32), 4, 32, 16] and ``scales``
     [ceil(K / 512), rows, 16] are bytes (the layout is that of include/tdc.h)."""
     __slots__ = ("codes", "scales", "shape", "rows", "K")
 
@@ -244,7 +244,7 @@ class Mx4Tensor:
         self.rows = 1
         for n in shape[:-1]:
             self.rows *= n
-        for t, want, what in ((codes, ((self.K + 127) // 128, self.rows, 64), "codes"), (scales, ((self.K + 511) // 512, self.rows, 16), "scales")):
+        for t, want, what in ((codes, ((self.K + 127) // 128, (self.rows + 31) // 32, 4, 32, 16), "codes"), (scales, ((self.K + 511) // 512, self.rows, 16), "scales")):
             if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous() or not t.is_cuda:
                 raise ValueError(f"{what} has to be a contiguous uint8 device tensor of shape {want}")
         if codes.device != scales.device:
@@ -254,7 +254,7 @@ class Mx4Tensor:
     @classmethod
     def _new(cls, rows, K, shape, device):
         t = cls.__new__(cls)
-        t.codes = _empty(((K + 127) // 128, rows, 64), dtype=torch.uint8, device=device)
+        t.codes = _empty(((K + 127) // 128, (rows + 31) // 32, 4, 32, 16), dtype=torch.uint8, device=device)
         t.scales = _empty(((K + 511) // 512, rows, 16), dtype=torch.uint8, device=device)
         t.shape, t.rows, t.K = shape, rows, K
         return t

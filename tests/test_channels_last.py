@@ -67,7 +67,7 @@ def test_norm_arguments_are_refused():
 
 def test_4_bit_arguments_are_refused():
     L, c, s = tdc_amd.lib(), ctypes.c_size_t(), ctypes.c_size_t()
-    assert L.tdc_mx4_sizes(3, 130, ctypes.byref(c), ctypes.byref(s)) == 0 and (c.value, s.value) == (3 * 128, 3 * 16)
+    assert L.tdc_mx4_sizes(3, 130, ctypes.byref(c), ctypes.byref(s)) == 0 and (c.value, s.value) == (32 * 128, 3 * 16)
     for rows, K in ((-1, 4), (2, 0), (1 << 36, 64), (2, 1 << 31)):
         assert L.tdc_mx4_sizes(rows, K, ctypes.byref(c), ctypes.byref(s)) == INVALID
     assert L.tdc_mx4_quantize(16, 3, 2, 32, 0, 16, 16, None) == INVALID and "dtype" in error()
@@ -116,7 +116,7 @@ def test_python_refusals_without_a_device():
     with pytest.raises(RuntimeError, match="no gradient"):
         tdc_amd.group_norm_act_mx4(x.requires_grad_(), 2)
     with pytest.raises(ValueError, match="uint8 device tensor"):
-        tdc_amd.Mx4Tensor(torch.zeros(1, 2, 64, dtype=torch.uint8), torch.zeros(1, 2, 16, dtype=torch.uint8), (2, 128))
+        tdc_amd.Mx4Tensor(torch.zeros(1, 1, 4, 32, 16, dtype=torch.uint8), torch.zeros(1, 2, 16, dtype=torch.uint8), (2, 128))
 
 
 def test_channels_last_is_recognised():
