@@ -1,0 +1,190 @@
+// Gradient of the group norm with an activation over channels-last tensors.
+//
+//   dz = dy act'(gamma_c xh + beta_c),  xh = (x - mean) rstd,  dbeta_c = sum dz,  dgamma_c = sum dz xh,
+//   dx = rstd (gamma_c dz - mean_g(gamma dz) - xh mean_g(gamma dz xh))
+//
+// Memory traffic, dealt out like the forward's: x and dy of a workgroup's channels and pixels sit in its registers, read once
+// where the pixels of an image fit (up to 128 KiB of each a workgroup), else twice, in two launches.  The sums over pixels are
+// kept per channel: weighted by gamma and added over a group they are the two group means, and added over workgroups the
+// parameters' gradients (by the launch's first workgroups if there is a second one, in a launch of their own if not).  No atomics, the
+// same order on every run.
+#include "norm_device.hpp"
+
+namespace tdc {
+
+enum { kWhole, kSums, kApply };
+
+// dz and xh of a thread's channels of one pixel.
+template <int DT, int V, int ACT>
+static __device__ __forceinline__ void slopes(const typename Pack<DT, V>::type &x, const typename Pack<DT, V>::type &dy, const float (&mean)[V],
+                                              const float (&rstd)[V], const float (&gamma)[V], const float (&beta)[V], float (&dz)[V],
+                                              float (&xh)[V]) {
+    Pack<DT, V>::up(x, xh);
+    Pack<DT, V>::up(dy, dz);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        xh[j] = (xh[j] - mean[j]) * rstd[j];
+        dz[j] *= act_slope<ACT>(fmaf(xh[j], gamma[j], beta[j]));
+    }
+}
+
+template <int DT, int V, int NV, int MODE, int ACT>
+__global__ void __launch_bounds__(512) tdc_norm_grad_kernel(const NormArgs a) {
+    using P = Pack<DT, V>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const Part p = part_of(a, V, blockIdx.x, gridDim.x);
+    const int n = rows_of(p, p.tr), c = p.c0 + p.tc * V;
+    typename P::type x[NV], dy[NV];
+    hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, n, x);
+    hold<DT, V, NV>(a.dy, a.d_is, a.d_ps, p, n, dy);
+    float mean[V], rstd[V], gamma[V], beta[V];
+    if (n > 0) {
+        params<DT, V>(a, c, gamma, beta);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const long long g = (long long)p.image * a.groups + (c + j) / a.Cg;
+            mean[j] = a.mean[g];
+            rstd[j] = a.rstd[g];
+        }
+    }
+    float2 *const cell = reinterpret_cast<float2 *>(lds), *const stat = cell + (MODE == kApply ? 0 : a.plan.threads * V);
+    const float inv = 1.0f / ((float)a.pixels * a.Cg);
+    const Team t = team_of(a.plan.threads, p.ng);
+    if constexpr (MODE != kApply) {
+        if (n > 0) {
+            float sz[V], sx[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) sz[j] = sx[j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (i < n) {
+                    float dz[V], xh[V];
+                    slopes<DT, V, ACT>(x[i], dy[i], mean, rstd, gamma, beta, dz, xh);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        sz[j] += dz[j];
+                        sx[j] = fmaf(dz[j], xh[j], sx[j]);
+                    }
+                }
+#pragma unroll
+            for (int j = 0; j < V; ++j) cell[p.tr * p.width + p.tc * V + j] = make_float2(sz[j], sx[j]);
+        }
+        __syncthreads();
+        float *const chan = a.chan + ((long long)p.image * a.plan.chunks + p.chunk) * 2 * a.C + p.c0;
+        const int used = min(p.R, p.rows);
+        for (int ch = threadIdx.x; ch < p.width; ch += a.plan.threads) {
+            float2 s = cell[ch];
+            for (int r = 1; r < used; ++r) {
+                const float2 e = cell[r * p.width + ch];
+                s.x += e.x;
+                s.y += e.y;
+            }
+            chan[ch] = s.x;
+            chan[a.C + ch] = s.y;
+            const float w = a.gamma ? param<DT>(a.gamma, p.c0 + ch, a.param_dtype) : 1.0f;
+            cell[ch] = make_float2(w * s.x, w * s.y);
+        }
+        __syncthreads();
+        for (int i = t.first; i < p.ng; i += t.step) {
+            const int g = p.g0 + i, lo = max(g * a.Cg, p.c0) - p.c0, channels = shared_channels(a, g, p.tile);
+            float s = 0.0f, u = 0.0f;
+            for (int e = t.at; e < channels; e += t.lanes) {
+                s += cell[lo + e].x;
+                u += cell[lo + e].y;
+            }
+            s = team_sum(s, t.lanes);
+            u = team_sum(u, t.lanes);
+            if (t.at == 0) {
+                if (MODE == kSums) a.part[slot_of(a, p, g)] = make_float2(s, u);
+                else stat[i] = make_float2(s * inv, u * inv);
+            }
+        }
+        if (MODE == kSums) return;
+    } else {
+        const NormPlan &m = a.plan;
+        for (int i = t.first; i < p.ng; i += t.step) {
+            const int g = p.g0 + i, tiles = ((g + 1) * a.Cg - 1) / m.unit - g * a.Cg / m.unit + 1;
+            const float2 *part = a.part + ((long long)p.image * a.groups + g) * m.slots;
+            float s = 0.0f, u = 0.0f;
+            for (int k = 0; k < tiles; ++k)
+                for (int e = t.at; e < m.chunks; e += t.lanes) {
+                    const float2 v = part[e * m.tiles_per_group + k];
+                    s += v.x;
+                    u += v.y;
+                }
+            s = team_sum(s, t.lanes) * inv;
+            u = team_sum(u, t.lanes) * inv;
+            if (t.at == 0) stat[i] = make_float2(s, u);
+        }
+    }
+    __syncthreads();
+    if (n == 0 || !a.out) return;
+    float s1[V], s2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float2 st = stat[(c + j) / a.Cg - p.g0];
+        s1[j] = st.x;
+        s2[j] = st.y;
+    }
+    const long long out = p.image * a.o_is + (long long)(p.row0 + p.tr) * a.o_ps + c, step = p.R * a.o_ps;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (i < n) {
+            float dz[V], xh[V];
+            slopes<DT, V, ACT>(x[i], dy[i], mean, rstd, gamma, beta, dz, xh);
+#pragma unroll
+            for (int j = 0; j < V; ++j) dz[j] = rstd[j] * (fmaf(gamma[j], dz[j], -s1[j]) - xh[j] * s2[j]);
+            P::store(a.out, out + i * step, P::down(dz));
+        }
+}
+
+// The parameters' gradients: a workgroup adds up 16 of the 2 C columns of the per-channel sums.
+static __global__ void __launch_bounds__(256) tdc_norm_param_grad_kernel(const NormArgs a) {
+    __shared__ float sum[256];
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4, rows = a.batch * a.plan.chunks;
+    float s = 0.0f;
+    if (col < 2 * a.C) {
+#pragma unroll 8
+        for (int r = lane; r < rows; r += 16) s += a.chan[(long long)r * 2 * a.C + col];
+    }
+    sum[threadIdx.x] = s;
+    __syncthreads();
+    if (lane == 0 && col < 2 * a.C) {
+        for (int r = 1; r < 16; ++r) s += sum[r * 16 + threadIdx.x];
+        float *const to = col < a.C ? a.dbeta : a.dgamma;
+        if (to) to[col < a.C ? col : col - a.C] = s;
+    }
+}
+
+template <int DT, int V, int NV, int ACT>
+static int run(const NormArgs &a, hipStream_t s) {
+    const unsigned grid = (unsigned)a.plan.chunks * a.plan.tiles * a.batch, threads = a.plan.threads;
+    if (a.plan.whole) tdc_norm_grad_kernel<DT, V, NV, kWhole, ACT><<<grid, threads, a.plan.lds, s>>>(a);
+    else {
+        tdc_norm_grad_kernel<DT, V, NV, kSums, ACT><<<grid, threads, a.plan.lds, s>>>(a);
+        if (a.out) tdc_norm_grad_kernel<DT, V, NV, kApply, ACT><<<grid, threads, a.plan.lds, s>>>(a);
+    }
+    if (a.dgamma || a.dbeta) tdc_norm_param_grad_kernel<<<(2 * a.C + 15) / 16, 256, 0, s>>>(a);
+    return (int)hipGetLastError();
+}
+template <int DT, int ACT>
+static int by_shape(const NormArgs &a, hipStream_t s) {
+    constexpr int VM = DT == TDC_F32 ? 4 : 8;
+    if (a.plan.vec == VM) return a.plan.held == 4 ? run<DT, VM, 4, ACT>(a, s) : run<DT, VM, 16, ACT>(a, s);
+    return a.plan.vec == 2 ? run<DT, 2, 16, ACT>(a, s) : run<DT, 1, 16, ACT>(a, s);
+}
+template <int DT>
+static int by_act(const NormArgs &a, hipStream_t s) {
+    if (a.act == TDC_ACT_RELU) return by_shape<DT, TDC_ACT_RELU>(a, s);
+    if (a.act == TDC_ACT_SILU) return by_shape<DT, TDC_ACT_SILU>(a, s);
+    return by_shape<DT, TDC_ACT_NONE>(a, s);
+}
+
+int launch_norm_backward(const NormArgs &a, int dtype, void *stream) {
+    const hipStream_t s = (hipStream_t)stream;
+    if (dtype == TDC_F32) return by_act<TDC_F32>(a, s);
+    if (dtype == TDC_F16) return by_act<TDC_F16>(a, s);
+    return by_act<TDC_BF16>(a, s);
+}
+
+}  // namespace tdc

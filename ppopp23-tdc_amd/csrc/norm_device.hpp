@@ -1,0 +1,104 @@
+// Device-side pieces shared by the group norm kernels: what a workgroup owns, its pixels in registers, sums over groups.
+#pragma once
+#include "ops_device.hpp"
+
+namespace tdc {
+
+// What a workgroup owns.
+struct Part {
+    int image, tile, chunk;
+    int c0, width, vecs;     // its channels, in all and as vectors
+    int tr, tc, R;           // this thread's pixel row and vector, rows at a time (threads past them idle: tr >= R)
+    int row0, rows;          // its pixels
+    int g0, ng;              // its groups
+};
+
+// Workgroups are dealt to the dies round robin: each die gets a run of neighbouring tiles, which share cache lines.
+static __device__ __forceinline__ Part part_of(const NormArgs &a, int vec, unsigned block, unsigned blocks) {
+    Part p;
+    const NormPlan &n = a.plan;
+    const unsigned die = block & 7, longer = blocks & 7;
+    unsigned idx = die * (blocks >> 3) + min(die, longer) + (block >> 3);
+    p.tile = idx % n.tiles;
+    idx /= n.tiles;
+    p.chunk = idx % n.chunks;
+    p.image = idx / n.chunks;
+    p.c0 = p.tile * n.unit;
+    p.width = min(n.unit, a.C - p.c0);
+    p.vecs = p.width / vec;
+    p.R = n.threads / p.vecs;
+    p.tr = threadIdx.x / p.vecs;
+    p.tc = threadIdx.x - p.tr * p.vecs;
+    p.row0 = p.chunk * n.chunk_rows;
+    p.rows = min(n.chunk_rows, a.pixels - p.row0);
+    p.g0 = p.c0 / a.Cg;
+    p.ng = (p.c0 + p.width - 1) / a.Cg - p.g0 + 1;
+    return p;
+}
+// Pixels of thread row r.
+static __device__ __forceinline__ int rows_of(const Part &p, int r) { return r < p.rows && r < p.R ? (p.rows - r + p.R - 1) / p.R : 0; }
+
+// This thread's vectors of a tensor, all requested at once.
+template <int DT, int V, int NV>
+static __device__ __forceinline__ void hold(const void *base, long long image_stride, long long pixel_stride, const Part &p, int n,
+                                            typename Pack<DT, V>::type (&v)[NV]) {
+    const long long at = p.image * image_stride + (long long)(p.row0 + p.tr) * pixel_stride + p.c0 + p.tc * V, step = p.R * pixel_stride;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        v[i] = typename Pack<DT, V>::type{};
+        if (i < n) v[i] = Pack<DT, V>::load(base, at + i * step);
+    }
+}
+
+// Makes a thread's vectors new to the compiler, which would else keep all of them unpacked from one use to the next.
+template <typename T, int NV>
+static __device__ __forceinline__ void pack_again(T (&v)[NV]) {
+    if constexpr (sizeof(T) == 16) {
+        typedef int i4_t __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            i4_t w = __builtin_bit_cast(i4_t, v[i]);
+            asm volatile("" : "+v"(w));
+            v[i] = __builtin_bit_cast(T, w);
+        }
+    }
+}
+
+// So many lanes work on one group (a power of two, at most a wave), and this thread's place among them.
+struct Team {
+    int lanes, at, first, step;
+};
+static __device__ __forceinline__ Team team_of(int threads, int ng) {
+    Team t;
+    t.lanes = 64;
+    while (t.lanes > 1 && ng * t.lanes > threads) t.lanes >>= 1;
+    t.at = threadIdx.x & (t.lanes - 1);
+    t.first = threadIdx.x / t.lanes;
+    t.step = threads / t.lanes;
+    return t;
+}
+template <typename T>
+static __device__ __forceinline__ T team_sum(T v, int lanes) {
+    for (int m = 1; m < lanes; m <<= 1) v += __shfl_xor(v, m, 64);
+    return v;
+}
+// Channels that a group and a workgroup's tile share.
+static __device__ __forceinline__ int shared_channels(const NormArgs &a, int g, int tile) {
+    const int lo = max(g * a.Cg, tile * a.plan.unit), hi = min((g + 1) * a.Cg, min(a.C, (tile + 1) * a.plan.unit));
+    return hi - lo;
+}
+static __device__ __forceinline__ long long slot_of(const NormArgs &a, const Part &p, int g) {
+    return ((long long)p.image * a.groups + g) * a.plan.slots + p.chunk * a.plan.tiles_per_group + (p.tile - g * a.Cg / a.plan.unit);
+}
+
+// Parameters of a thread's channels.
+template <int DT, int V>
+static __device__ __forceinline__ void params(const NormArgs &a, int c, float (&gamma)[V], float (&beta)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        gamma[j] = a.gamma ? param<DT>(a.gamma, c + j, a.param_dtype) : 1.0f;
+        beta[j] = a.beta ? param<DT>(a.beta, c + j, a.param_dtype) : 0.0f;
+    }
+}
+
+}  // namespace tdc

@@ -19,29 +19,52 @@ bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (unsigned)(bytes
 
 // ---- group norm ----
 
-constexpr int kNormThreads = 256;
-
-// `quantised`: tiles end at multiples of 32 channels, the blocks of the result.
-NormPlan norm_plan(const tdc_group_norm_desc &d, int vec, bool quantised) {
+// `quantised`: tiles end at multiples of 32 channels, the blocks of the result.  `grad`: x and dy are held side by side.
+NormPlan norm_plan(const tdc_group_norm_desc &d, bool quantised, bool grad) {
     NormPlan n{};
-    n.vec = vec;
-    const int Cg = d.C / d.groups;
-    const long long widest = (long long)kNormThreads * vec;
-    const long long whole = std::lcm((long long)Cg, std::lcm((long long)vec, quantised ? 32ll : 1ll));
-    if (d.C <= widest) n.unit = d.C;
-    else if (whole <= widest) n.unit = (int)(widest / whole * whole);
-    else n.unit = (int)widest;
+    const int Cg = d.C / d.groups, size = dtype_bytes(d.dtype), widest = 16 / size;
+    const long long pixels = std::max<long long>(d.pixels, 1), batch = std::max(d.batch, 1);
+    n.vec = d.C % widest == 0 ? widest : d.C % 2 == 0 ? 2 : 1;
+    n.places = n.vec / std::gcd(n.vec, Cg);
+    // Threads: the kernels' launch bounds, and at most 2048 sums in LDS.
+    const int most = std::min(grad ? 512 : 1024, 2048 / (grad ? 1 : n.places));
+    const int whole = (int)std::min((long long)d.C, std::lcm((long long)Cg, std::lcm((long long)n.vec, quantised ? 32ll : 1ll)));
+    // A tile of whole groups and vectors, of some `bytes` a pixel; groups that are too wide are shared.
+    auto tile = [&](int bytes) {
+        if (whole > most * n.vec) return most * n.vec;
+        const int unit = std::max(1, (bytes / size + whole - 1) / whole) * whole;
+        return std::min(std::min(unit, most * n.vec / whole * whole), d.C);
+    };
+    auto fits = [&](int unit) { return unit % Cg == 0 && pixels <= (long long)(most / (unit / n.vec)) * 16; };
+    // Whole cache lines where that leaves a workgroup for every compute unit, half ones else: their neighbours come to the same die.
+    n.unit = tile(128);
+    n.whole = fits(n.unit) && batch * ((d.C + n.unit - 1) / n.unit) >= 256;
+    if (!n.whole && fits(tile(64))) {
+        n.unit = tile(64);
+        n.whole = true;
+    }
     n.tiles = (d.C + n.unit - 1) / n.unit;
     n.tiles_per_group = n.unit % Cg == 0 ? 1 : std::min(n.tiles, (Cg + n.unit - 2) / n.unit + 1);
-    // Workgroups: eight to a compute unit, as long as each thread has four pixels to move.
-    const int rows = kNormThreads / (n.unit / vec);
-    const long long across = (long long)n.tiles * std::max(d.batch, 1);
-    const long long want = (2048 + across - 1) / across;
-    const long long most = (d.pixels + 4 * rows - 1) / (4 * rows);
-    const long long chunks = std::max(1ll, std::min({want, most, 256ll}));
-    n.chunk_rows = (int)round_up(std::max(1ll, ((long long)d.pixels + chunks - 1) / chunks), rows);
-    n.chunks = (int)((d.pixels + n.chunk_rows - 1) / n.chunk_rows);
+    const int vecs = n.unit / n.vec;
+    const long long across = n.tiles * batch;
+    n.threads = most;
+    if (n.whole) {
+        // Few workgroups: many threads with few requests each.  Many: few threads, so that several workgroups share a compute unit.
+        const int held = across >= 512 ? 16 : 4;
+        while (n.threads > 64 && n.threads / 2 >= vecs && (long long)(n.threads / 2 / vecs) * held >= pixels) n.threads /= 2;
+        n.chunk_rows = (int)pixels;
+    } else {
+        while (n.threads > 512 && n.threads / 2 >= vecs) n.threads /= 2;
+        // Workgroups: four to a compute unit, as long as each thread has two pixels to move.
+        const int rows = n.threads / vecs;
+        const long long want = (1024 + across - 1) / across, held = std::min(16ll, std::max(2ll, (pixels + rows * want - 1) / (rows * want)));
+        n.chunk_rows = (int)std::min(round_up(pixels, rows), rows * held);
+    }
+    n.chunks = (int)((pixels + n.chunk_rows - 1) / n.chunk_rows);
+    n.held = n.vec == widest && (n.chunk_rows + n.threads / vecs - 1) / (n.threads / vecs) <= 4 ? 4 : 16;
     n.slots = n.chunks * n.tiles_per_group;
+    const int groups = std::min(n.unit, (n.unit - 1) / Cg + 2);
+    n.lds = grad ? 8 * (n.threads * n.vec + groups) : 12 * n.threads * n.places + 8 * groups;
     return n;
 }
 size_t stat_bytes(const tdc_group_norm_desc &d, const NormPlan &n) { return sizeof(NormStat) * d.batch * d.groups * n.slots; }
@@ -49,8 +72,6 @@ size_t part_bytes(const tdc_group_norm_desc &d, const NormPlan &n) {
     return (size_t)round_up((long long)sizeof(float2) * d.batch * d.groups * n.slots, 16);
 }
 size_t chan_bytes(const tdc_group_norm_desc &d, const NormPlan &n) { return (size_t)8 * d.batch * n.chunks * d.C; }
-
-int widest_vec(int dtype) { return dtype == TDC_F32 ? 4 : 8; }
 
 // Normalised copy of the descriptor with every stride filled in; an error code if it makes no sense.
 int norm_check(const tdc_group_norm_desc *desc, tdc_group_norm_desc &d) {
@@ -72,32 +93,20 @@ int norm_check(const tdc_group_norm_desc *desc, tdc_group_norm_desc &d) {
         if (*pair.second == 0) *pair.second = d.pixels * *pair.first;
         if (d.batch > 1 && *pair.second < image) return invalid("group norm: an image stride below one image");
     }
-    const NormPlan n = norm_plan(d, 1, false);
-    if ((long long)d.batch * n.tiles * n.chunks > (1ll << 30)) return invalid("group norm: batch too large");
+    for (bool grad : {false, true}) {
+        const NormPlan n = norm_plan(d, false, grad);
+        if ((long long)d.batch * n.tiles * n.chunks > (1ll << 30) || n.slots > (1 << 24)) return invalid("group norm: too large");
+    }
     return TDC_OK;
 }
 
-// The widest vector that C, the strides and the addresses allow.
-int norm_vec(const tdc_group_norm_desc &d, const void *x, bool with_y, std::initializer_list<const void *> dense) {
-    for (int vec : {widest_vec(d.dtype), 2}) {
-        const int bytes = vec * dtype_bytes(d.dtype);
-        bool ok = d.C % vec == 0 && d.x_pixel_stride % vec == 0 && (d.batch < 2 || d.x_image_stride % vec == 0) && aligned(x, bytes);
-        if (with_y) ok = ok && d.y_pixel_stride % vec == 0 && (d.batch < 2 || d.y_image_stride % vec == 0);
-        for (const void *p : dense) ok = ok && aligned(p, bytes);
-        if (ok) return vec;
-    }
-    return 1;
-}
-// Scratch for whichever vector the addresses will allow.
-void norm_workspace(const tdc_group_norm_desc &d, size_t &fwd, size_t &bwd, size_t &mx4) {
-    fwd = bwd = mx4 = 0;
-    for (int vec : {widest_vec(d.dtype), 2, 1}) {
-        if (d.C % vec) continue;
-        const NormPlan n = norm_plan(d, vec, false);
-        fwd = std::max(fwd, stat_bytes(d, n));
-        bwd = std::max(bwd, part_bytes(d, n) + chan_bytes(d, n));
-        mx4 = std::max(mx4, stat_bytes(d, norm_plan(d, vec, true)));
-    }
+size_t forward_ws(const tdc_group_norm_desc &d, const NormPlan &n) { return n.whole ? 0 : stat_bytes(d, n); }
+size_t backward_ws(const tdc_group_norm_desc &d, const NormPlan &n) { return part_bytes(d, n) + chan_bytes(d, n); }
+// The plan of the result in 4 bits: in one launch only where its blocks fit the vectors.
+NormPlan mx4_plan(const tdc_group_norm_desc &d) {
+    NormPlan n = norm_plan(d, true, false);
+    if (d.C % 32) n.whole = false;
+    return n;
 }
 NormArgs norm_args(const tdc_group_norm_desc &d, const void *x, const void *gamma, const void *beta) {
     NormArgs a{};
@@ -181,10 +190,8 @@ extern "C" {
 int tdc_group_norm_workspace(const tdc_group_norm_desc *desc, size_t *forward_bytes, size_t *backward_bytes) TDC_ENTRY {
     tdc_group_norm_desc d;
     if (int st = norm_check(desc, d)) return st;
-    size_t fwd, bwd, mx4;
-    norm_workspace(d, fwd, bwd, mx4);
-    if (forward_bytes) *forward_bytes = fwd;
-    if (backward_bytes) *backward_bytes = bwd;
+    if (forward_bytes) *forward_bytes = forward_ws(d, norm_plan(d, false, false));
+    if (backward_bytes) *backward_bytes = backward_ws(d, norm_plan(d, false, true));
     return TDC_OK;
 }
 TDC_ENTRY_END
@@ -193,8 +200,7 @@ int tdc_group_norm_mx4_workspace(const tdc_group_norm_desc *desc, size_t *bytes)
     tdc_group_norm_desc d;
     if (int st = norm_check(desc, d)) return st;
     if (!bytes) return invalid("group norm: null argument");
-    size_t fwd, bwd;
-    norm_workspace(d, fwd, bwd, *bytes);
+    *bytes = forward_ws(d, mx4_plan(d));
     return TDC_OK;
 }
 TDC_ENTRY_END
@@ -205,9 +211,8 @@ int tdc_group_norm_forward(const tdc_group_norm_desc *desc, const void *x, const
     if (int st = norm_check(desc, d)) return st;
     if (!d.batch || !d.pixels) return TDC_OK;
     if (!x || !y) return invalid("group norm: null x or y");
-    size_t fwd, bwd, mx4;
-    norm_workspace(d, fwd, bwd, mx4);
-    if (int st = ws_check("group norm", ws, ws_bytes, fwd)) return st;
+    const NormPlan plan = norm_plan(d, false, false);
+    if (int st = ws_check("group norm", ws, ws_bytes, forward_ws(d, plan))) return st;
     NormArgs a = norm_args(d, x, gamma, beta);
     a.out = y;
     a.o_ps = d.y_pixel_stride;
@@ -215,7 +220,7 @@ int tdc_group_norm_forward(const tdc_group_norm_desc *desc, const void *x, const
     a.mean = mean;
     a.rstd = rstd;
     a.stat = (NormStat *)ws;
-    a.plan = norm_plan(d, norm_vec(d, x, true, {y}), false);
+    a.plan = plan;
     return launched("group norm", launch_norm_forward(a, d.dtype, stream));
 }
 TDC_ENTRY_END
@@ -227,14 +232,13 @@ int tdc_group_norm_forward_mx4(const tdc_group_norm_desc *desc, const void *x, c
     if (!d.batch || !d.pixels) return TDC_OK;
     if (!x) return invalid("group norm: null x");
     if (int st = mx4_check("group norm", d.batch * d.pixels, d.C, codes, scales)) return st;
-    size_t fwd, bwd, mx4;
-    norm_workspace(d, fwd, bwd, mx4);
-    if (int st = ws_check("group norm", ws, ws_bytes, mx4)) return st;
+    const NormPlan plan = mx4_plan(d);
+    if (int st = ws_check("group norm", ws, ws_bytes, forward_ws(d, plan))) return st;
     NormArgs a = norm_args(d, x, gamma, beta);
     a.codes = (unsigned char *)codes;
     a.scales = (unsigned char *)scales;
     a.stat = (NormStat *)ws;
-    a.plan = norm_plan(d, norm_vec(d, x, false, {}), true);
+    a.plan = plan;
     return launched("group norm", launch_norm_forward(a, d.dtype, stream));
 }
 TDC_ENTRY_END
@@ -254,9 +258,8 @@ int tdc_group_norm_backward(const tdc_group_norm_desc *desc, const void *x, cons
         return TDC_OK;
     }
     if (!x || !dy || !mean || !rstd) return invalid("group norm: null x, dy, mean or rstd");
-    size_t fwd, bwd, mx4;
-    norm_workspace(d, fwd, bwd, mx4);
-    if (int st = ws_check("group norm", ws, ws_bytes, bwd)) return st;
+    const NormPlan plan = norm_plan(d, false, true);
+    if (int st = ws_check("group norm", ws, ws_bytes, backward_ws(d, plan))) return st;
     NormArgs a = norm_args(d, x, gamma, beta);
     a.dy = dy;
     a.d_ps = d.y_pixel_stride;
@@ -268,7 +271,7 @@ int tdc_group_norm_backward(const tdc_group_norm_desc *desc, const void *x, cons
     a.rstd = const_cast<float *>(rstd);
     a.dgamma = dgamma;
     a.dbeta = dbeta;
-    a.plan = norm_plan(d, norm_vec(d, x, true, {dy, dx}), false);
+    a.plan = plan;
     a.part = (float2 *)ws;
     a.chan = (float *)((char *)ws + part_bytes(d, a.plan));
     return launched("group norm", launch_norm_backward(a, d.dtype, stream));

@@ -27,11 +27,12 @@ struct Num<TDC_BF16> {
     static __device__ __forceinline__ __bf16 down(float v) { return (__bf16)v; }
 };
 
-// V neighbouring numbers as one request.
+// V neighbouring numbers as one request, which needs the alignment of one of them.
 template <int DT, int V>
 struct Pack {
     using T = typename Num<DT>::type;
     typedef T type __attribute__((ext_vector_type(V)));
+    typedef T mem_t __attribute__((ext_vector_type(V), aligned(sizeof(T))));
     static __device__ __forceinline__ void up(const type &p, float (&v)[V]) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = Num<DT>::up(p[i]);
@@ -43,10 +44,10 @@ struct Pack {
         return p;
     }
     static __device__ __forceinline__ type load(const void *base, long long at) {
-        return *reinterpret_cast<const type *>(reinterpret_cast<const T *>(base) + at);
+        return *reinterpret_cast<const mem_t *>(reinterpret_cast<const T *>(base) + at);
     }
     static __device__ __forceinline__ void store(void *base, long long at, const type &p) {
-        *reinterpret_cast<type *>(reinterpret_cast<T *>(base) + at) = p;
+        *reinterpret_cast<mem_t *>(reinterpret_cast<T *>(base) + at) = p;
     }
 };
 // (a vector of one number is the number)

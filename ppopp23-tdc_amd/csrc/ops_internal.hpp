@@ -24,16 +24,22 @@ __host__ __device__ inline long long mx4_block_at(long long rows, long long row,
 // Scale bytes of a row.
 inline long long mx4_scale_bytes(long long K) { return round_up(K, 512) / 32; }
 
-// How a norm's work is dealt out.  A workgroup owns `unit` channels (unit / vec vectors, a thread each) of `chunk_rows`
-// pixels of one image; `slots` partial results per image and group meet in the second launch.
+// How a norm's work is dealt out.  A workgroup of `threads` owns `unit` channels (unit / vec vectors, a thread each) of `chunk_rows`
+// pixels of one image, at most `held` pixels a thread, which it keeps in registers.  Where one workgroup holds all pixels
+// (chunks = 1) a norm is one launch; else `slots` partial results per image and group meet in a second one.
 struct NormPlan {
     int vec;            // channels a thread moves at once
     int unit;           // channels of a workgroup
     int tiles;          // workgroups across the channels
     int tiles_per_group;// at most so many of them share a group (1 unless a group is wider than a workgroup)
+    int threads;
+    int held;           // the kernel's registers: pixels a thread (of x, and of dy)
     int chunks;         // workgroups along the pixels of an image
     int chunk_rows;
     int slots;          // chunks * tiles_per_group
+    int places;         // sums a thread keeps apart: its vector may span groups
+    int lds;            // bytes
+    bool whole;         // one workgroup has all pixels and channels of its groups
 };
 
 // Partial statistics of one group: the sum, and the squared deviations from its mean.

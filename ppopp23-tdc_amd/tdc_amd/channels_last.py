@@ -158,12 +158,12 @@ def _norm_forward(x, groups, weight, bias, eps, act, stats):
     plan = _norm_for(x, groups, weight, bias, eps, act)
     dev = x.device
     y = torch.empty_strided(x.shape, plan.y_strides, dtype=x.dtype, device=dev)
-    ws = _empty(plan.forward_ws, dtype=torch.uint8, device=dev)
+    ws = _empty(plan.forward_ws, dtype=torch.uint8, device=dev) if plan.forward_ws else None
     kept = _empty(plan.stats_shape, dtype=torch.float32, device=dev) if stats else None
     mean = kept.data_ptr() if stats else None
     status = lib().tdc_group_norm_forward(plan.ref, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean,
                                           mean + 4 * plan.stats_shape[1] * plan.stats_shape[2] if stats and mean else None,
-                                          ws.data_ptr(), plan.forward_ws, _raw_stream(x.get_device()))
+                                          _ptr(ws), plan.forward_ws, _raw_stream(x.get_device()))
     if status:
         check(status)
     return y, kept
@@ -325,9 +325,9 @@ def _norm_mx4(x, groups, weight, bias, eps, act):
     plan = _norm_for(x, groups, weight, bias, eps, act)
     d = plan.desc
     q = Mx4Tensor._new(d.batch * d.pixels, d.C, (x.shape[0], *x.shape[2:], d.C), x.device)
-    ws = _empty(plan.mx4_ws, dtype=torch.uint8, device=x.device)
+    ws = _empty(plan.mx4_ws, dtype=torch.uint8, device=x.device) if plan.mx4_ws else None
     status = lib().tdc_group_norm_forward_mx4(plan.ref, x.data_ptr(), _ptr(weight), _ptr(bias), q.codes.data_ptr(), q.scales.data_ptr(),
-                                              ws.data_ptr(), plan.mx4_ws, _raw_stream(x.get_device()))
+                                              _ptr(ws), plan.mx4_ws, _raw_stream(x.get_device()))
     if status:
         check(status)
     return q

@@ -44,12 +44,12 @@ def test_norm_descriptors_are_refused(bad, word):
     L, d, a, b = tdc_amd.lib(), norm(**bad), ctypes.c_size_t(), ctypes.c_size_t()
     assert L.tdc_group_norm_workspace(ctypes.byref(d), ctypes.byref(a), ctypes.byref(b)) == INVALID and word in error()
     assert L.tdc_group_norm_forward(ctypes.byref(d), 16, None, None, 16, None, None, 16, 1 << 20, None) == INVALID
-    assert L.tdc_group_norm_backward(ctypes.byref(d), 16, 16, None, None, 16, 16, 16, None, None, 16, 1 << 20, None) == INVALID
-    assert L.tdc_group_norm_forward_mx4(ctypes.byref(d), 16, None, None, 16, 16, 16, 1 << 20, None) == INVALID
+    assert L.tdc_group_norm_backward(ctypes.byref(d), 16, 16, None, None, 16, 16, 16, None, None, 16, 1 << 30, None) == INVALID
+    assert L.tdc_group_norm_forward_mx4(ctypes.byref(d), 16, None, None, 16, 16, 16, 1 << 30, None) == INVALID
 
 
 def test_norm_arguments_are_refused():
-    L, d, a, b = tdc_amd.lib(), norm(), ctypes.c_size_t(), ctypes.c_size_t()
+    L, d, a, b = tdc_amd.lib(), norm(pixels=1 << 20), ctypes.c_size_t(), ctypes.c_size_t()
     assert L.tdc_group_norm_workspace(None, ctypes.byref(a), ctypes.byref(b)) == INVALID
     assert L.tdc_group_norm_workspace(ctypes.byref(d), ctypes.byref(a), ctypes.byref(b)) == 0 and 0 < a.value < b.value
     p = ctypes.byref(d)
