@@ -6,73 +6,45 @@
 // pixels, and holds them in registers: a thread asks for `vec` channels of every R-th pixel, all requests at once.  Where the
 // pixels of an image fit (up to 256 KiB a workgroup) that is all: x is read once, the statistics meet in LDS, y is written.
 // Else one launch leaves partial statistics, and a second reads x again and joins, while it comes, the partial results of its own
-// groups: no atomics, no third launch, the same order on every run.
+// groups: no atomics, no third launch, the same order on every run.  These two are made of many small workgroups whose threads have
+// four requests on their way while they work on four.
 //
 // Mean: summed in 64 bits (an add of which costs the vector unit what one in 32 does), so that it is off by the rounding of its
-// last conversion alone, however the numbers cancel.  Variance: a thread sums the squared deviations from its own mean, and
-// those of threads and workgroups are joined by M2 = sum M2_i + n_i (mean_i - mean)^2: an offset common to a group cancels
-// before it is squared.  Everything else between load and store is fp32.
+// last conversion alone, however the numbers cancel.  Variance: a thread sums the squared deviations from its own mean (or its first
+// number), and those of threads and workgroups are joined by M2 = sum M2_i + n_i (mean_i - mean)^2: an offset common to a group
+// cancels before it is squared.  Everything else between load and store is fp32.
 #include "norm_device.hpp"
 
 namespace tdc {
 
-// The statistics of this workgroup's part of its groups, from the vectors its threads hold: `done(i, sum, m2)` for the group i of
-// them, in the team's first lane.  `run`: so many of a thread's channels are of one group and share a place in LDS.
-template <int DT, int V, int NV, typename Done>
-static __device__ __forceinline__ void part_stats(const NormArgs &a, const Part &p, int n, typename Pack<DT, V>::type (&x)[NV], int run,
-                                                  double *sums, float *devs, Done done) {
+// Neighbouring channels of a thread that share a place (`run` of them, a power of two): all of them end up with its sum.
+template <typename T, int V>
+static __device__ __forceinline__ void join_run(T (&s)[V], int run) {
+#pragma unroll
+    for (int w = 1; w < V; w *= 2)
+        if (run > w) {
+#pragma unroll
+            for (int j = 0; j < V; j += 2 * w) {
+                const T both = s[j] + s[j + w];
+#pragma unroll
+                for (int k = 0; k < 2 * w; ++k) s[j + k] = both;
+            }
+        }
+}
+
+// The statistics of this workgroup's part of its groups: `done(i, sum, m2)` for the group i of them, in the team's first lane, from
+// the threads' sums s and squared deviations q about the means of their places.
+template <int V, typename Done>
+static __device__ __forceinline__ void join_threads(const NormArgs &a, const Part &p, int n, const double (&s)[V], const float (&q)[V], int run,
+                                                    double *sums, float *devs, Done done) {
     const int places = p.vecs * (V / run);      // of a thread row
     if (n > 0) {
-        double s[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = 0.0;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (i < n) {
-                float v[V];
-                Pack<DT, V>::up(x[i], v);
-#pragma unroll
-                for (int j = 0; j < V; ++j) s[j] += v[j];
-            }
-        // (neighbours that share a place: all of them end up with its sum)
-#pragma unroll
-        for (int w = 1; w < V; w *= 2)
-            if (run > w) {
-#pragma unroll
-                for (int j = 0; j < V; j += 2 * w) {
-                    const double both = s[j] + s[j + w];
-#pragma unroll
-                    for (int k = 0; k < 2 * w; ++k) s[j + k] = both;
-                }
-            }
-        pack_again(x);
-        float mean[V], m2[V];
-        const double inv = 1.0 / ((double)n * run);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            mean[j] = (float)(s[j] * inv);
-            m2[j] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (i < n) {
-                float v[V];
-                Pack<DT, V>::up(x[i], v);
-#pragma unroll
-                for (int j = 0; j < V; ++j) m2[j] = fmaf(v[j] - mean[j], v[j] - mean[j], m2[j]);
-            }
-#pragma unroll
-        for (int w = 1; w < V; w *= 2)
-            if (run > w) {
-#pragma unroll
-                for (int j = 0; j < V; j += 2 * w) m2[j] += m2[j + w];
-            }
         const int at = p.tr * places + p.tc * (V / run);
 #pragma unroll
         for (int j = 0; j < V; ++j)
             if (j % run == 0) {
                 sums[at + j / run] = s[j];
-                devs[at + j / run] = m2[j];
+                devs[at + j / run] = q[j];
             }
     }
     __syncthreads();
@@ -96,6 +68,83 @@ static __device__ __forceinline__ void part_stats(const NormArgs &a, const Part 
         m2 = team_sum(m2, t.lanes);
         if (t.at == 0) done(i, sum, m2);
     }
+}
+
+// Of vectors that stay in registers: the deviations from the mean of the place itself.
+template <int DT, int V, int NV>
+static __device__ __forceinline__ void held_sums(int n, typename Pack<DT, V>::type (&x)[NV], int run, double (&s)[V], float (&q)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        s[j] = 0.0;
+        q[j] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (i < n) {
+            float v[V];
+            Pack<DT, V>::up(x[i], v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] += v[j];
+        }
+    join_run(s, run);
+    pack_again(x);
+    float mean[V];
+    const double inv = 1.0 / ((double)max(n, 1) * run);
+#pragma unroll
+    for (int j = 0; j < V; ++j) mean[j] = (float)(s[j] * inv);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (i < n) {
+            float v[V];
+            Pack<DT, V>::up(x[i], v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) q[j] = fmaf(v[j] - mean[j], v[j] - mean[j], q[j]);
+        }
+    join_run(q, run);
+}
+
+// Of any number of pixels, NV of them on their way while NV are added up: the deviations from a channel's first number, an error of
+// which is one part in n of the deviations that this number itself has, then moved to the mean of the place.
+template <int DT, int V, int NV>
+static __device__ __forceinline__ void passing_sums(const NormArgs &a, const Part &p, int n, int run, double (&s)[V], float (&q)[V]) {
+    using P = Pack<DT, V>;
+    float first[V];
+    typename P::type next[NV];
+    hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, 0, n, next);
+    P::up(next[0], first);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        s[j] = 0.0;
+        q[j] = 0.0f;
+    }
+    for (int at = 0; at < n; at += NV) {
+        typename P::type x[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) x[i] = next[i];
+        hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, at + NV, n, next);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at + i < n) {
+                float v[V];
+                P::up(x[i], v);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    s[j] += v[j];
+                    q[j] = fmaf(v[j] - first[j], v[j] - first[j], q[j]);
+                }
+            }
+    }
+    double own[V];
+    const double inv = 1.0 / max(n, 1);
+#pragma unroll
+    for (int j = 0; j < V; ++j) own[j] = s[j] * inv;
+    join_run(s, run);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float d = (float)(own[j] - first[j]), e = (float)(own[j] - s[j] * inv / run);
+        q[j] = fmaxf(q[j] - n * d * d, 0.0f) + n * e * e;
+    }
+    join_run(q, run);
 }
 
 // One group's (mean, rstd); the first workgroup that has it keeps them for the caller.
@@ -168,24 +217,29 @@ static __device__ __forceinline__ void store_mx4_padding(const NormArgs &a, cons
 enum { kWhole, kStats, kApply };
 
 template <int DT, int V, int NV, int MODE, int ACT, bool MX4>
-__global__ void __launch_bounds__(1024) tdc_norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(const NormArgs a) {
     using P = Pack<DT, V>;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const Part p = part_of(a, V, blockIdx.x, gridDim.x);
     const int n = rows_of(p, p.tr);
+    const int run = V / a.plan.places, most = a.plan.threads * a.plan.places;
+    double *const sums = reinterpret_cast<double *>(lds);
+    float *const devs = reinterpret_cast<float *>(sums + most);
+    float2 *const stat = MODE == kApply ? reinterpret_cast<float2 *>(lds) : reinterpret_cast<float2 *>(devs + most);
+    double s[V];
+    float q[V];
+    if constexpr (MODE == kStats) {
+        passing_sums<DT, V, NV>(a, p, n, run, s, q);
+        join_threads(a, p, n, s, q, run, sums, devs, [&](int i, double sum, float m2) { a.stat[slot_of(a, p, p.g0 + i)] = NormStat{sum, m2}; });
+        return;
+    }
     typename P::type x[NV];
-    hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, n, x);
-    float2 *stat = reinterpret_cast<float2 *>(lds);
-    if constexpr (MODE != kApply) {
-        const int run = V / a.plan.places, most = a.plan.threads * a.plan.places;
-        double *const sums = reinterpret_cast<double *>(lds);
-        float *const devs = reinterpret_cast<float *>(sums + most);
-        stat = reinterpret_cast<float2 *>(devs + most);
-        part_stats<DT, V, NV>(a, p, n, x, run, sums, devs, [&](int i, double sum, float m2) {
-            if (MODE == kStats) a.stat[slot_of(a, p, p.g0 + i)] = NormStat{sum, m2};
-            else stat[i] = finish_stats(a, p, p.g0 + i, sum / ((double)a.pixels * a.Cg), m2, true);
+    hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, 0, n, x);
+    if constexpr (MODE == kWhole) {
+        held_sums<DT, V, NV>(n, x, run, s, q);
+        join_threads(a, p, n, s, q, run, sums, devs, [&](int i, double sum, float m2) {
+            stat[i] = finish_stats(a, p, p.g0 + i, sum / ((double)a.pixels * a.Cg), m2, true);
         });
-        if (MODE == kStats) return;
     } else join_stats(a, p, stat);
     __syncthreads();
     const int c = p.c0 + p.tc * V;
@@ -199,23 +253,31 @@ __global__ void __launch_bounds__(1024) tdc_norm_kernel(const NormArgs a) {
             scale[j] *= st.y;
         }
         const long long row = p.row0 + p.tr, out = p.image * a.o_is + row * a.o_ps + c, step = p.R * a.o_ps;
+        for (int at = 0; at < (MODE == kWhole ? 1 : n); at += NV) {
+            typename P::type next[NV];
+            if constexpr (MODE != kWhole) hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, at + NV, n, next);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (i < n) {
-                float v[V];
-                P::up(x[i], v);
+            for (int i = 0; i < NV; ++i)
+                if (at + i < n) {
+                    float v[V];
+                    P::up(x[i], v);
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = act_of<ACT>(fmaf(v[j] - mean[j], scale[j], shift[j]));
-                if constexpr (MX4) store_mx4<V>(a, (long long)p.image * a.pixels + row + (long long)i * p.R, c, v);
-                else P::store(a.out, out + i * step, P::down(v));
+                    for (int j = 0; j < V; ++j) v[j] = act_of<ACT>(fmaf(v[j] - mean[j], scale[j], shift[j]));
+                    if constexpr (MX4) store_mx4<V>(a, (long long)p.image * a.pixels + row + (long long)(at + i) * p.R, c, v);
+                    else P::store(a.out, out + (at + i) * step, P::down(v));
+                }
+            if constexpr (MODE != kWhole) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) x[i] = next[i];
             }
+        }
     }
     if (MX4 && p.c0 + p.width == a.C) store_mx4_padding(a, p);
 }
 
 // The second half into 4 bits where a row's blocks and vectors do not fit together: a thread takes a block of 32 channels of a pixel.
 template <int DT, int ACT>
-__global__ void __launch_bounds__(1024) tdc_norm_blocks_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(256) tdc_norm_blocks_kernel(const NormArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     using T = typename Num<DT>::type;
     const Part p = part_of(a, a.plan.vec, blockIdx.x, gridDim.x);
@@ -253,15 +315,15 @@ static int run(const NormArgs &a, hipStream_t s) {
     const unsigned grid = (unsigned)a.plan.chunks * a.plan.tiles * a.batch, threads = a.plan.threads;
     if (a.plan.whole) tdc_norm_kernel<DT, V, NV, kWhole, ACT, MX4><<<grid, threads, a.plan.lds, s>>>(a);
     else {
-        tdc_norm_kernel<DT, V, NV, kStats, TDC_ACT_NONE, false><<<grid, threads, a.plan.lds, s>>>(a);
-        tdc_norm_kernel<DT, V, NV, kApply, ACT, MX4><<<grid, threads, a.plan.lds, s>>>(a);
+        tdc_norm_kernel<DT, V, 4, kStats, TDC_ACT_NONE, false><<<grid, threads, a.plan.lds, s>>>(a);
+        tdc_norm_kernel<DT, V, 4, kApply, ACT, MX4><<<grid, threads, a.plan.lds, s>>>(a);
     }
     return (int)hipGetLastError();
 }
-template <int DT, int V, int NV, int ACT>
+template <int DT, int V, int ACT>
 static int run_blocks(const NormArgs &a, hipStream_t s) {
     const unsigned grid = (unsigned)a.plan.chunks * a.plan.tiles * a.batch, threads = a.plan.threads;
-    tdc_norm_kernel<DT, V, NV, kStats, TDC_ACT_NONE, false><<<grid, threads, a.plan.lds, s>>>(a);
+    tdc_norm_kernel<DT, V, 4, kStats, TDC_ACT_NONE, false><<<grid, threads, a.plan.lds, s>>>(a);
     tdc_norm_blocks_kernel<DT, ACT><<<grid, threads, a.plan.lds, s>>>(a);
     return (int)hipGetLastError();
 }
@@ -270,8 +332,8 @@ static int by_shape(const NormArgs &a, hipStream_t s) {
     constexpr int VM = DT == TDC_F32 ? 4 : 8;
     const NormPlan &n = a.plan;
     if (a.codes && (a.C % 32 || n.vec != VM)) {
-        if (n.vec == VM) return run_blocks<DT, VM, 16, ACT>(a, s);
-        return n.vec == 2 ? run_blocks<DT, 2, 16, ACT>(a, s) : run_blocks<DT, 1, 16, ACT>(a, s);
+        if (n.vec == VM) return run_blocks<DT, VM, ACT>(a, s);
+        return n.vec == 2 ? run_blocks<DT, 2, ACT>(a, s) : run_blocks<DT, 1, ACT>(a, s);
     }
     if (a.codes) return n.held == 4 ? run<DT, VM, 4, ACT, true>(a, s) : run<DT, VM, 16, ACT, true>(a, s);
     if (n.vec == VM) return n.held == 4 ? run<DT, VM, 4, ACT, false>(a, s) : run<DT, VM, 16, ACT, false>(a, s);

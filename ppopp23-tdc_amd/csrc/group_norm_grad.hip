@@ -4,9 +4,10 @@
 //   dx = rstd (gamma_c dz - mean_g(gamma dz) - xh mean_g(gamma dz xh))
 //
 // Memory traffic, dealt out like the forward's: x and dy of a workgroup's channels and pixels sit in its registers, read once
-// where the pixels of an image fit (up to 128 KiB of each a workgroup), else twice, in two launches.  The sums over pixels are
+// where the pixels of an image fit (up to 128 KiB of each a workgroup), else twice, in two launches of many small workgroups whose
+// threads have two pixels on their way while they work on two.  The sums over pixels are
 // kept per channel: weighted by gamma and added over a group they are the two group means, and added over workgroups the
-// parameters' gradients (by the launch's first workgroups if there is a second one, in a launch of their own if not).  No atomics, the
+// parameters' gradients (by the first workgroups of the second launch, or in a launch of their own).  No atomics, the
 // same order on every run.
 #include "norm_device.hpp"
 
@@ -28,15 +29,44 @@ static __device__ __forceinline__ void slopes(const typename Pack<DT, V>::type &
     }
 }
 
+// The parameters' gradients: a workgroup of 256 adds up 4 of the 2 C columns of the per-channel sums.
+static __device__ __forceinline__ void add_params(const NormArgs &a, unsigned block, float *sum) {
+    const int col = block * 4 + (threadIdx.x & 3), lane = threadIdx.x >> 2, rows = a.batch * a.plan.chunks;
+    float s = 0.0f;
+    if (col < 2 * a.C) {
+#pragma unroll 8
+        for (int r = lane; r < rows; r += 64) s += a.chan[(long long)r * 2 * a.C + col];
+    }
+    sum[threadIdx.x] = s;
+    __syncthreads();
+    for (int half = 32; half; half /= 2) {
+        if (lane < half) sum[threadIdx.x] += sum[threadIdx.x + 4 * half];
+        __syncthreads();
+    }
+    if (lane == 0 && col < 2 * a.C) {
+        float *const to = col < a.C ? a.dbeta : a.dgamma;
+        if (to) to[col < a.C ? col : col - a.C] = sum[threadIdx.x];
+    }
+}
+static __global__ void __launch_bounds__(256) tdc_norm_param_grad_kernel(const NormArgs a) {
+    __shared__ float sum[256];
+    add_params(a, blockIdx.x, sum);
+}
+
+// (of the second launch, the first `param_blocks` workgroups do the parameters)
 template <int DT, int V, int NV, int MODE, int ACT>
-__global__ void __launch_bounds__(512) tdc_norm_grad_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kernel(const NormArgs a, unsigned param_blocks) {
     using P = Pack<DT, V>;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    const Part p = part_of(a, V, blockIdx.x, gridDim.x);
+    if (MODE == kApply && blockIdx.x < param_blocks) {
+        add_params(a, blockIdx.x, reinterpret_cast<float *>(lds));
+        return;
+    }
+    const Part p = part_of(a, V, blockIdx.x - param_blocks, gridDim.x - param_blocks);
     const int n = rows_of(p, p.tr), c = p.c0 + p.tc * V;
     typename P::type x[NV], dy[NV];
-    hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, n, x);
-    hold<DT, V, NV>(a.dy, a.d_is, a.d_ps, p, n, dy);
+    hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, 0, n, x);
+    hold<DT, V, NV>(a.dy, a.d_is, a.d_ps, p, 0, n, dy);
     float mean[V], rstd[V], gamma[V], beta[V];
     if (n > 0) {
         params<DT, V>(a, c, gamma, beta);
@@ -55,17 +85,31 @@ __global__ void __launch_bounds__(512) tdc_norm_grad_kernel(const NormArgs a) {
             float sz[V], sx[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) sz[j] = sx[j] = 0.0f;
+            for (int at = 0; at < (MODE == kWhole ? 1 : n); at += NV) {
+                typename P::type next_x[NV], next_dy[NV];
+                if constexpr (MODE != kWhole) {
+                    hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, at + NV, n, next_x);
+                    hold<DT, V, NV>(a.dy, a.d_is, a.d_ps, p, at + NV, n, next_dy);
+                }
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (i < n) {
-                    float dz[V], xh[V];
-                    slopes<DT, V, ACT>(x[i], dy[i], mean, rstd, gamma, beta, dz, xh);
+                for (int i = 0; i < NV; ++i)
+                    if (at + i < n) {
+                        float dz[V], xh[V];
+                        slopes<DT, V, ACT>(x[i], dy[i], mean, rstd, gamma, beta, dz, xh);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        sz[j] += dz[j];
-                        sx[j] = fmaf(dz[j], xh[j], sx[j]);
+                        for (int j = 0; j < V; ++j) {
+                            sz[j] += dz[j];
+                            sx[j] = fmaf(dz[j], xh[j], sx[j]);
+                        }
+                    }
+                if constexpr (MODE != kWhole) {
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        x[i] = next_x[i];
+                        dy[i] = next_dy[i];
                     }
                 }
+            }
 #pragma unroll
             for (int j = 0; j < V; ++j) cell[p.tr * p.width + p.tc * V + j] = make_float2(sz[j], sx[j]);
         }
@@ -127,44 +171,41 @@ __global__ void __launch_bounds__(512) tdc_norm_grad_kernel(const NormArgs a) {
         s2[j] = st.y;
     }
     const long long out = p.image * a.o_is + (long long)(p.row0 + p.tr) * a.o_ps + c, step = p.R * a.o_ps;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (i < n) {
-            float dz[V], xh[V];
-            slopes<DT, V, ACT>(x[i], dy[i], mean, rstd, gamma, beta, dz, xh);
-#pragma unroll
-            for (int j = 0; j < V; ++j) dz[j] = rstd[j] * (fmaf(gamma[j], dz[j], -s1[j]) - xh[j] * s2[j]);
-            P::store(a.out, out + i * step, P::down(dz));
+    if constexpr (MODE == kWhole) pack_again(x);
+    for (int at = 0; at < (MODE == kWhole ? 1 : n); at += NV) {
+        typename P::type next_x[NV], next_dy[NV];
+        if constexpr (MODE != kWhole) {
+            hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, at + NV, n, next_x);
+            hold<DT, V, NV>(a.dy, a.d_is, a.d_ps, p, at + NV, n, next_dy);
         }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at + i < n) {
+                float dz[V], xh[V];
+                slopes<DT, V, ACT>(x[i], dy[i], mean, rstd, gamma, beta, dz, xh);
+#pragma unroll
+                for (int j = 0; j < V; ++j) dz[j] = rstd[j] * (fmaf(gamma[j], dz[j], -s1[j]) - xh[j] * s2[j]);
+                P::store(a.out, out + (at + i) * step, P::down(dz));
+            }
+        if constexpr (MODE != kWhole) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                x[i] = next_x[i];
+                dy[i] = next_dy[i];
+            }
+        }
+    }
 }
 
-// The parameters' gradients: a workgroup adds up 16 of the 2 C columns of the per-channel sums.
-static __global__ void __launch_bounds__(256) tdc_norm_param_grad_kernel(const NormArgs a) {
-    __shared__ float sum[256];
-    const int col = blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4, rows = a.batch * a.plan.chunks;
-    float s = 0.0f;
-    if (col < 2 * a.C) {
-#pragma unroll 8
-        for (int r = lane; r < rows; r += 16) s += a.chan[(long long)r * 2 * a.C + col];
-    }
-    sum[threadIdx.x] = s;
-    __syncthreads();
-    if (lane == 0 && col < 2 * a.C) {
-        for (int r = 1; r < 16; ++r) s += sum[r * 16 + threadIdx.x];
-        float *const to = col < a.C ? a.dbeta : a.dgamma;
-        if (to) to[col < a.C ? col : col - a.C] = s;
-    }
-}
 
 template <int DT, int V, int NV, int ACT>
 static int run(const NormArgs &a, hipStream_t s) {
     const unsigned grid = (unsigned)a.plan.chunks * a.plan.tiles * a.batch, threads = a.plan.threads;
-    if (a.plan.whole) tdc_norm_grad_kernel<DT, V, NV, kWhole, ACT><<<grid, threads, a.plan.lds, s>>>(a);
-    else {
-        tdc_norm_grad_kernel<DT, V, NV, kSums, ACT><<<grid, threads, a.plan.lds, s>>>(a);
-        if (a.out) tdc_norm_grad_kernel<DT, V, NV, kApply, ACT><<<grid, threads, a.plan.lds, s>>>(a);
-    }
-    if (a.dgamma || a.dbeta) tdc_norm_param_grad_kernel<<<(2 * a.C + 15) / 16, 256, 0, s>>>(a);
+    const unsigned param_blocks = a.dgamma || a.dbeta ? (unsigned)(2 * a.C + 3) / 4 : 0;
+    if (a.plan.whole) tdc_norm_grad_kernel<DT, V, NV, kWhole, ACT><<<grid, threads, a.plan.lds, s>>>(a, 0);
+    else tdc_norm_grad_kernel<DT, V, 2, kSums, ACT><<<grid, threads, a.plan.lds, s>>>(a, 0);
+    if (!a.plan.whole && a.out) tdc_norm_grad_kernel<DT, V, 2, kApply, ACT><<<param_blocks + grid, threads, a.plan.lds, s>>>(a, param_blocks);
+    else if (param_blocks) tdc_norm_param_grad_kernel<<<param_blocks, 256, 0, s>>>(a);
     return (int)hipGetLastError();
 }
 template <int DT, int ACT>

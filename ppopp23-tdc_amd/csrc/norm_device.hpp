@@ -38,15 +38,15 @@ static __device__ __forceinline__ Part part_of(const NormArgs &a, int vec, unsig
 // Pixels of thread row r.
 static __device__ __forceinline__ int rows_of(const Part &p, int r) { return r < p.rows && r < p.R ? (p.rows - r + p.R - 1) / p.R : 0; }
 
-// This thread's vectors of a tensor, all requested at once.
+// This thread's vectors of a tensor from its pixel `first` on, all requested at once.
 template <int DT, int V, int NV>
-static __device__ __forceinline__ void hold(const void *base, long long image_stride, long long pixel_stride, const Part &p, int n,
+static __device__ __forceinline__ void hold(const void *base, long long image_stride, long long pixel_stride, const Part &p, int first, int n,
                                             typename Pack<DT, V>::type (&v)[NV]) {
     const long long at = p.image * image_stride + (long long)(p.row0 + p.tr) * pixel_stride + p.c0 + p.tc * V, step = p.R * pixel_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         v[i] = typename Pack<DT, V>::type{};
-        if (i < n) v[i] = Pack<DT, V>::load(base, at + i * step);
+        if (first + i < n) v[i] = Pack<DT, V>::load(base, at + (first + i) * step);
     }
 }
 

@@ -19,23 +19,26 @@ bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (unsigned)(bytes
 
 // ---- group norm ----
 
-// `quantised`: tiles end at multiples of 32 channels, the blocks of the result.  `grad`: x and dy are held side by side.
+// `quantised`: tiles end at multiples of 32 channels, the blocks of the result, which is written in one launch only where rows end
+// there too.  `grad`: x and dy are held side by side.
 NormPlan norm_plan(const tdc_group_norm_desc &d, bool quantised, bool grad) {
     NormPlan n{};
     const int Cg = d.C / d.groups, size = dtype_bytes(d.dtype), widest = 16 / size;
     const long long pixels = std::max<long long>(d.pixels, 1), batch = std::max(d.batch, 1);
     n.vec = d.C % widest == 0 ? widest : d.C % 2 == 0 ? 2 : 1;
     n.places = n.vec / std::gcd(n.vec, Cg);
-    // Threads: the kernels' launch bounds, and at most 2048 sums in LDS.
+    // Threads: the kernels' launch bounds (256 where a workgroup does not have all pixels), and at most 2048 sums in LDS.
+    const int across = 256;      // vectors of a pixel
     const int most = std::min(grad ? 512 : 1024, 2048 / (grad ? 1 : n.places));
     const int whole = (int)std::min((long long)d.C, std::lcm((long long)Cg, std::lcm((long long)n.vec, quantised ? 32ll : 1ll)));
     // A tile of whole groups and vectors, of some `bytes` a pixel; groups that are too wide are shared.
     auto tile = [&](int bytes) {
-        if (whole > most * n.vec) return most * n.vec;
+        if (whole > across * n.vec) return across * n.vec;
         const int unit = std::max(1, (bytes / size + whole - 1) / whole) * whole;
-        return std::min(std::min(unit, most * n.vec / whole * whole), d.C);
+        return std::min(std::min(unit, across * n.vec / whole * whole), d.C);
     };
-    auto fits = [&](int unit) { return unit % Cg == 0 && pixels <= (long long)(most / (unit / n.vec)) * 16; };
+    const bool blocks = quantised && d.C % 32 != 0;
+    auto fits = [&](int unit) { return !blocks && unit % Cg == 0 && pixels <= (long long)(most / (unit / n.vec)) * 16; };
     // Whole cache lines where that leaves a workgroup for every compute unit, half ones else: their neighbours come to the same die.
     n.unit = tile(128);
     n.whole = fits(n.unit) && batch * ((d.C + n.unit - 1) / n.unit) >= 256;
@@ -46,19 +49,20 @@ NormPlan norm_plan(const tdc_group_norm_desc &d, bool quantised, bool grad) {
     n.tiles = (d.C + n.unit - 1) / n.unit;
     n.tiles_per_group = n.unit % Cg == 0 ? 1 : std::min(n.tiles, (Cg + n.unit - 2) / n.unit + 1);
     const int vecs = n.unit / n.vec;
-    const long long across = n.tiles * batch;
+    const long long dealt = n.tiles * batch;
     n.threads = most;
     if (n.whole) {
         // Few workgroups: many threads with few requests each.  Many: few threads, so that several workgroups share a compute unit.
-        const int held = across >= 512 ? 16 : 4;
+        const int held = dealt >= 512 ? 16 : 4;
         while (n.threads > 64 && n.threads / 2 >= vecs && (long long)(n.threads / 2 / vecs) * held >= pixels) n.threads /= 2;
         n.chunk_rows = (int)pixels;
     } else {
-        while (n.threads > 512 && n.threads / 2 >= vecs) n.threads /= 2;
-        // Workgroups: four to a compute unit, as long as each thread has two pixels to move.
+        // Workgroups of 256: four to a compute unit, which all kernels have the registers for, as long as each thread has four
+        // pixels to move.
+        n.threads = std::min(most, 256);
         const int rows = n.threads / vecs;
-        const long long want = (1024 + across - 1) / across, held = std::min(16ll, std::max(2ll, (pixels + rows * want - 1) / (rows * want)));
-        n.chunk_rows = (int)std::min(round_up(pixels, rows), rows * held);
+        const long long want = std::max(1ll, 1024 / dealt);
+        n.chunk_rows = (int)std::min(round_up(pixels, rows), round_up(std::max(4ll * rows, (pixels + want - 1) / want), rows));
     }
     n.chunks = (int)((pixels + n.chunk_rows - 1) / n.chunk_rows);
     n.held = n.vec == widest && (n.chunk_rows + n.threads / vecs - 1) / (n.threads / vecs) <= 4 ? 4 : 16;
@@ -102,12 +106,6 @@ int norm_check(const tdc_group_norm_desc *desc, tdc_group_norm_desc &d) {
 
 size_t forward_ws(const tdc_group_norm_desc &d, const NormPlan &n) { return n.whole ? 0 : stat_bytes(d, n); }
 size_t backward_ws(const tdc_group_norm_desc &d, const NormPlan &n) { return part_bytes(d, n) + chan_bytes(d, n); }
-// The plan of the result in 4 bits: in one launch only where its blocks fit the vectors.
-NormPlan mx4_plan(const tdc_group_norm_desc &d) {
-    NormPlan n = norm_plan(d, true, false);
-    if (d.C % 32) n.whole = false;
-    return n;
-}
 NormArgs norm_args(const tdc_group_norm_desc &d, const void *x, const void *gamma, const void *beta) {
     NormArgs a{};
     a.x = x;
@@ -200,7 +198,7 @@ int tdc_group_norm_mx4_workspace(const tdc_group_norm_desc *desc, size_t *bytes)
     tdc_group_norm_desc d;
     if (int st = norm_check(desc, d)) return st;
     if (!bytes) return invalid("group norm: null argument");
-    *bytes = forward_ws(d, mx4_plan(d));
+    *bytes = forward_ws(d, norm_plan(d, true, false));
     return TDC_OK;
 }
 TDC_ENTRY_END
@@ -232,7 +230,7 @@ int tdc_group_norm_forward_mx4(const tdc_group_norm_desc *desc, const void *x, c
     if (!d.batch || !d.pixels) return TDC_OK;
     if (!x) return invalid("group norm: null x");
     if (int st = mx4_check("group norm", d.batch * d.pixels, d.C, codes, scales)) return st;
-    const NormPlan plan = mx4_plan(d);
+    const NormPlan plan = norm_plan(d, true, false);
     if (int st = ws_check("group norm", ws, ws_bytes, forward_ws(d, plan))) return st;
     NormArgs a = norm_args(d, x, gamma, beta);
     a.codes = (unsigned char *)codes;
