@@ -4,6 +4,7 @@
 // (lane / 32), with that block's scale; products and sums are fp32.  The weights are the first operand, so that a lane ends up with
 // neighbouring outputs of one row.  (16x16x128 does as much per instruction but takes the matrix unit 35 cycles where 32x32x64, with
 // twice the work, takes 36: registers only, one wave a SIMD, 4.6 against 8.9 PFLOP/s, 6.4 on random numbers for their power.)
+#include <algorithm>
 #include <type_traits>
 
 #include "ops_device.hpp"
@@ -255,6 +256,132 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
     else finish(std::integral_constant<int, TDC_ACT_NONE>{});
 }
 
+// ---- few rows of x ----
+//
+// Bound by the weights' bytes, or by latency.  A workgroup owns 32 rows of w and 32 MB of x; its waves share K, 512 numbers at a
+// time, with their codes straight in registers: a block of 32 rows by 64 numbers is one request of 1 KiB.  The waves' sums meet
+// in LDS, in the order of the waves.  XS: x in 4 bits (TDC_MX4), or numbers of that type, which a workgroup makes into 4 bits in LDS
+// by itself: for few rows that costs less than a launch.
+// Eight numbers a thread into codes in LDS: block b of row m at (b M + m) 16, its scale byte behind all codes, words of four steps.
+template <int XS>
+static __device__ __forceinline__ void take_numbers(const ProductArgs &a, unsigned char *codes, unsigned char *scales) {
+    using P = Pack<XS, 8>;
+    const int M = (int)a.M, octets = a.ksteps * 16;
+    for (int i = threadIdx.x; i < M * octets; i += blockDim.x) {
+        const int m = i / octets, o = i - m * octets, n = (int)min(8ll, a.K - (long long)o * 8);
+        float v[8];
+        if (n == 8) P::up(P::load(a.x, m * a.x_stride + o * 8), v);
+        else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j < n ? Num<XS>::up(reinterpret_cast<const typename Num<XS>::type *>(a.x)[m * a.x_stride + o * 8 + j]) : 0.0f;
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = larger(top, v[j]);
+        const int byte = mx4_scale_byte(quad_larger(top)), b = o >> 2;
+        *reinterpret_cast<unsigned *>(codes + (b * M + m) * 16 + (o & 3) * 4) = mx4_codes(v, mx4_divisor(byte));
+        if ((o & 3) == 0) scales[(b >> 4) * M * 16 + m * 16 + (b & 3) * 4 + (b >> 2 & 3)] = (unsigned char)byte;
+    }
+}
+
+template <int DT, int XS, int MB>
+__global__ void __launch_bounds__(1024) tdc_mx4_product_few_kernel(const ProductArgs a, int blocks_m) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), waves = blockDim.x >> 6, r = lane & 31, q = lane >> 5;
+    const long long n0 = (long long)(blockIdx.x / (unsigned)blocks_m) * 32, m0 = (long long)(blockIdx.x % (unsigned)blocks_m) * 32 * MB;
+    const long long x_blocks = (a.M + 31) >> 5, w_blocks = (a.N + 31) >> 5;
+    const int groups = (a.ksteps + 3) / 4, M = (int)min(a.M, 32ll);
+    const long long w_row = min(n0 + r, a.N - 1);
+
+    i4_t w[4][2], x[MB][4][2];
+    int sw[2], sx[MB][2];
+    // (steps past the last repeat it, their scales are zero)
+    auto ask = [&](int g) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const long long k = min(g * 4 + s, a.ksteps - 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                w[s][h] = *reinterpret_cast<const i4_t *>(a.w_codes + (k * w_blocks + (n0 >> 5)) * 2048 + h * 1024 + lane * 16);
+                if constexpr (XS == TDC_MX4) {
+#pragma unroll
+                    for (int i = 0; i < MB; ++i)
+                        x[i][s][h] = *reinterpret_cast<const i4_t *>(a.x_codes + (k * x_blocks + min((m0 >> 5) + i, x_blocks - 1)) * 2048 + h * 1024 + lane * 16);
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            sw[h] = *reinterpret_cast<const int *>(a.w_scales + ((long long)g * a.N + w_row) * 16 + q * 4 + h * 8);
+            if constexpr (XS == TDC_MX4) {
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+                    sx[i][h] = *reinterpret_cast<const int *>(a.x_scales + ((long long)g * a.M + min(m0 + i * 32 + r, a.M - 1)) * 16 + q * 4 + h * 8);
+            }
+        }
+    };
+    unsigned char *const x_lds = lds, *const sx_lds = lds + a.ksteps * 64 * M;
+    if (wave < groups) ask(wave);
+    if constexpr (XS != TDC_MX4) {
+        // (the scale bytes past a row's last block)
+        for (int i = t; i < M * 16; i += blockDim.x) sx_lds[(groups - 1) * M * 16 + i] = 0;
+        __syncthreads();
+        take_numbers<XS>(a, x_lds, sx_lds);
+        __syncthreads();
+    }
+    f16_t acc[MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
+    for (int g = wave; g < groups; g += waves) {
+        if constexpr (XS != TDC_MX4) {
+            const int m = min(r, M - 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const int k = min(g * 4 + s, a.ksteps - 1);
+                    x[0][s][h] = *reinterpret_cast<const i4_t *>(x_lds + ((k * 4 + 2 * h + q) * M + m) * 16);
+                }
+                sx[0][h] = *reinterpret_cast<const int *>(sx_lds + (g * M + m) * 16 + q * 4 + h * 8);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+                    acc[i] = mfma4(w[s][h], x[i][s][h], acc[i], (int)((unsigned)sw[h] >> 8 * s), (int)((unsigned)sx[i][h] >> 8 * s));
+        if (g + waves < groups) ask(g + waves);
+    }
+    // Sums of the waves: output e of a lane, row 8 (e / 4) + 4 q + e mod 4 of w and r of x.
+    if constexpr (XS != TDC_MX4) __syncthreads();
+    float *const part = reinterpret_cast<float *>(lds);
+    using T = typename Num<DT>::type;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        if (i) __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) part[(wave * 16 + e) * 64 + lane] = acc[i][e];
+        __syncthreads();
+        const int rows = (int)min(32ll, a.M - m0 - i * 32);
+        for (int o = t; o < 32 * rows; o += blockDim.x) {
+            const int n = o & 31, m = o >> 5, at = ((n >> 3) * 4 + (n & 3)) * 64 + (n >> 2 & 1) * 32 + m;
+            if (n0 + n >= a.N) continue;
+            float v = a.bias ? param<DT>(a.bias, n0 + n, a.bias_dtype) : 0.0f;
+            float sum = 0.0f;
+            for (int k = 0; k < waves; ++k) sum += part[k * 1024 + at];
+            v += sum;
+            const long long row = m0 + i * 32 + m;
+            if (a.residual) v += Num<DT>::up(reinterpret_cast<const T *>(a.residual)[row * a.r_stride + n0 + n]);
+            v = a.act == TDC_ACT_RELU ? act_of<TDC_ACT_RELU>(v) : a.act == TDC_ACT_SILU ? act_of<TDC_ACT_SILU>(v) : v;
+            reinterpret_cast<T *>(a.y)[row * a.y_stride + n0 + n] = Num<DT>::down(v);
+        }
+    }
+}
+
 // Lets a kernel have more than 64 KiB of LDS; once per kernel and device.
 static int allow_lds(const void *fn, int bytes, unsigned long long &done) {
     int device = 0;
@@ -277,12 +404,30 @@ static int launch_tile(const ProductArgs &a, hipStream_t s) {
     fn<<<grid, 256, L::kLds, s>>>(a, tm, tn);
     return (int)hipGetLastError();
 }
+template <int DT, int XS, int MB>
+static int launch_few(const ProductArgs &a, hipStream_t s) {
+    // A wave for every 512 numbers of K, four to sixteen of them.
+    const int groups = (a.ksteps + 3) / 4, waves = groups <= 4 ? 4 : groups <= 8 ? 8 : 16;
+    const int x_bytes = XS == TDC_MX4 ? 0 : (int)a.M * (a.ksteps * 64 + groups * 16), lds = std::max(waves * 4096, x_bytes);
+    const unsigned bm = (unsigned)((a.M + 32 * MB - 1) / (32 * MB)), bn = (unsigned)((a.N + 31) / 32);
+    tdc_mx4_product_few_kernel<DT, XS, MB><<<bm * bn, waves * 64, lds, s>>>(a, (int)bm);
+    return (int)hipGetLastError();
+}
 template <int DT>
 static int launch_product(const ProductArgs &a, hipStream_t s) {
+    if (a.x) {
+        if (a.x_dtype == TDC_F32) return launch_few<DT, TDC_F32, 1>(a, s);
+        return a.x_dtype == TDC_F16 ? launch_few<DT, TDC_F16, 1>(a, s) : launch_few<DT, TDC_BF16, 1>(a, s);
+    }
+    if (a.M <= 32) return launch_few<DT, TDC_MX4, 1>(a, s);
+    if (a.M <= 64) return launch_few<DT, TDC_MX4, 2>(a, s);
     const long long big = ((a.M + 255) / 256) * ((a.N + 255) / 256);
     if (big >= 192) return launch_tile<DT, 4, 4>(a, s);
     return launch_tile<DT, 2, 2>(a, s);
 }
+
+// x as it comes, without a launch of its own: eight rows and 64 Ki numbers at most (34 KiB of LDS), as each workgroup repeats the work.
+bool product_takes_numbers(long long M, long long K) { return M <= 8 && M * mx4_padded(K) <= 65536; }
 
 int launch_mx4_product(const ProductArgs &a, int y_dtype, void *stream) {
     const hipStream_t s = (hipStream_t)stream;

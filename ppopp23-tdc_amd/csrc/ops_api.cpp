@@ -168,7 +168,7 @@ int linear_check(const tdc_mx4_linear_desc *desc, tdc_mx4_linear_desc &d) {
 }
 size_t linear_codes(const tdc_mx4_linear_desc &d) { return (size_t)mx4_code_bytes(d.M, d.K); }
 size_t linear_ws(const tdc_mx4_linear_desc &d) {
-    return d.x_dtype == TDC_MX4 ? 0 : linear_codes(d) + (size_t)(d.M * mx4_scale_bytes(d.K));
+    return d.x_dtype == TDC_MX4 || product_takes_numbers(d.M, d.K) ? 0 : linear_codes(d) + (size_t)(d.M * mx4_scale_bytes(d.K));
 }
 
 }  // namespace
@@ -328,6 +328,10 @@ int tdc_mx4_linear(const tdc_mx4_linear_desc *desc, const void *x, const void *x
         if (int st = mx4_check("4-bit product", d.M, d.K, x, x_scales)) return st;
         a.x_codes = (const unsigned char *)x;
         a.x_scales = (const unsigned char *)x_scales;
+    } else if (product_takes_numbers(d.M, d.K)) {
+        a.x = x;
+        a.x_dtype = d.x_dtype;
+        a.x_stride = d.x_stride;
     } else {
         if (int st = ws_check("4-bit product", ws, ws_bytes, linear_ws(d))) return st;
         a.x_codes = (const unsigned char *)ws;
@@ -342,6 +346,7 @@ int tdc_mx4_linear(const tdc_mx4_linear_desc *desc, const void *x, const void *x
     a.y = y;
     a.M = d.M;
     a.N = d.N;
+    a.K = d.K;
     a.y_stride = d.y_stride;
     a.r_stride = d.residual_stride;
     a.ksteps = (int)(mx4_padded(d.K) / 128);

@@ -74,12 +74,16 @@ int launch_mx4_dequantize(const void *codes, const void *scales, long long rows,
 
 struct ProductArgs {
     const unsigned char *x_codes, *x_scales, *w_codes, *w_scales;
+    const void *x;                  // numbers in place of codes (see product_takes_numbers), or null
+    long long K, x_stride;
+    int x_dtype;
     const void *bias, *residual;
     void *y;
     long long M, N, y_stride, r_stride;
     int ksteps;                     // padded K / 128
     int bias_dtype, act;
 };
+bool product_takes_numbers(long long M, long long K);
 int launch_mx4_product(const ProductArgs &a, int y_dtype, void *stream);
 
 }  // namespace tdc
