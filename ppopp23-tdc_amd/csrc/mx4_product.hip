@@ -256,9 +256,9 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
     else finish(std::integral_constant<int, TDC_ACT_NONE>{});
 }
 
-// ---- few rows of x ----
+// ---- few outputs ----
 //
-// Bound by the weights' bytes, or by latency.  A workgroup owns 32 rows of w and 32 MB of x; its waves share K, 512 numbers at a
+// Bound by the weights' bytes, or by latency.  A workgroup owns 32 rows of w and 32 of x; its waves share K, 512 numbers at a
 // time, with their codes straight in registers: a block of 32 rows by 64 numbers is one request of 1 KiB.  The waves' sums meet
 // in LDS, in the order of the waves.  XS: x in 4 bits (TDC_MX4), or numbers of that type, which a workgroup makes into 4 bits in LDS
 // by itself: for few rows that costs less than a launch.
@@ -284,17 +284,17 @@ static __device__ __forceinline__ void take_numbers(const ProductArgs &a, unsign
     }
 }
 
-template <int DT, int XS, int MB>
+template <int DT, int XS>
 __global__ void __launch_bounds__(1024) tdc_mx4_product_few_kernel(const ProductArgs a, int blocks_m) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), waves = blockDim.x >> 6, r = lane & 31, q = lane >> 5;
-    const long long n0 = (long long)(blockIdx.x / (unsigned)blocks_m) * 32, m0 = (long long)(blockIdx.x % (unsigned)blocks_m) * 32 * MB;
+    const long long n0 = (long long)(blockIdx.x / (unsigned)blocks_m) * 32, m0 = (long long)(blockIdx.x % (unsigned)blocks_m) * 32;
     const long long x_blocks = (a.M + 31) >> 5, w_blocks = (a.N + 31) >> 5;
     const int groups = (a.ksteps + 3) / 4, M = (int)min(a.M, 32ll);
-    const long long w_row = min(n0 + r, a.N - 1);
+    const long long w_row = min(n0 + r, a.N - 1), x_row = min(m0 + r, a.M - 1);
 
-    i4_t w[4][2], x[MB][4][2];
-    int sw[2], sx[MB][2];
+    i4_t w[4][2], x[4][2];
+    int sw[2], sx[2];
     // (steps past the last repeat it, their scales are zero)
     auto ask = [&](int g) {
 #pragma unroll
@@ -303,21 +303,14 @@ __global__ void __launch_bounds__(1024) tdc_mx4_product_few_kernel(const Product
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 w[s][h] = *reinterpret_cast<const i4_t *>(a.w_codes + (k * w_blocks + (n0 >> 5)) * 2048 + h * 1024 + lane * 16);
-                if constexpr (XS == TDC_MX4) {
-#pragma unroll
-                    for (int i = 0; i < MB; ++i)
-                        x[i][s][h] = *reinterpret_cast<const i4_t *>(a.x_codes + (k * x_blocks + min((m0 >> 5) + i, x_blocks - 1)) * 2048 + h * 1024 + lane * 16);
-                }
+                if constexpr (XS == TDC_MX4)
+                    x[s][h] = *reinterpret_cast<const i4_t *>(a.x_codes + (k * x_blocks + (m0 >> 5)) * 2048 + h * 1024 + lane * 16);
             }
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             sw[h] = *reinterpret_cast<const int *>(a.w_scales + ((long long)g * a.N + w_row) * 16 + q * 4 + h * 8);
-            if constexpr (XS == TDC_MX4) {
-#pragma unroll
-                for (int i = 0; i < MB; ++i)
-                    sx[i][h] = *reinterpret_cast<const int *>(a.x_scales + ((long long)g * a.M + min(m0 + i * 32 + r, a.M - 1)) * 16 + q * 4 + h * 8);
-            }
+            if constexpr (XS == TDC_MX4) sx[h] = *reinterpret_cast<const int *>(a.x_scales + ((long long)g * a.M + x_row) * 16 + q * 4 + h * 8);
         }
     };
     unsigned char *const x_lds = lds, *const sx_lds = lds + a.ksteps * 64 * M;
@@ -329,11 +322,9 @@ __global__ void __launch_bounds__(1024) tdc_mx4_product_few_kernel(const Product
         take_numbers<XS>(a, x_lds, sx_lds);
         __syncthreads();
     }
-    f16_t acc[MB];
+    f16_t acc;
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
+    for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
     for (int g = wave; g < groups; g += waves) {
         if constexpr (XS != TDC_MX4) {
             const int m = min(r, M - 1);
@@ -342,18 +333,15 @@ __global__ void __launch_bounds__(1024) tdc_mx4_product_few_kernel(const Product
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     const int k = min(g * 4 + s, a.ksteps - 1);
-                    x[0][s][h] = *reinterpret_cast<const i4_t *>(x_lds + ((k * 4 + 2 * h + q) * M + m) * 16);
+                    x[s][h] = *reinterpret_cast<const i4_t *>(x_lds + ((k * 4 + 2 * h + q) * M + m) * 16);
                 }
-                sx[0][h] = *reinterpret_cast<const int *>(sx_lds + (g * M + m) * 16 + q * 4 + h * 8);
+                sx[h] = *reinterpret_cast<const int *>(sx_lds + (g * M + m) * 16 + q * 4 + h * 8);
             }
         }
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < MB; ++i)
-                    acc[i] = mfma4(w[s][h], x[i][s][h], acc[i], (int)((unsigned)sw[h] >> 8 * s), (int)((unsigned)sx[i][h] >> 8 * s));
+            for (int h = 0; h < 2; ++h) acc = mfma4(w[s][h], x[s][h], acc, (int)((unsigned)sw[h] >> 8 * s), (int)((unsigned)sx[h] >> 8 * s));
         if (g + waves < groups) ask(g + waves);
     }
     // Sums of the waves: output e of a lane, row 8 (e / 4) + 4 q + e mod 4 of w and r of x.
@@ -361,24 +349,18 @@ __global__ void __launch_bounds__(1024) tdc_mx4_product_few_kernel(const Product
     float *const part = reinterpret_cast<float *>(lds);
     using T = typename Num<DT>::type;
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
-        if (i) __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 16; ++e) part[(wave * 16 + e) * 64 + lane] = acc[i][e];
-        __syncthreads();
-        const int rows = (int)min(32ll, a.M - m0 - i * 32);
-        for (int o = t; o < 32 * rows; o += blockDim.x) {
-            const int n = o & 31, m = o >> 5, at = ((n >> 3) * 4 + (n & 3)) * 64 + (n >> 2 & 1) * 32 + m;
-            if (n0 + n >= a.N) continue;
-            float v = a.bias ? param<DT>(a.bias, n0 + n, a.bias_dtype) : 0.0f;
-            float sum = 0.0f;
-            for (int k = 0; k < waves; ++k) sum += part[k * 1024 + at];
-            v += sum;
-            const long long row = m0 + i * 32 + m;
-            if (a.residual) v += Num<DT>::up(reinterpret_cast<const T *>(a.residual)[row * a.r_stride + n0 + n]);
-            v = a.act == TDC_ACT_RELU ? act_of<TDC_ACT_RELU>(v) : a.act == TDC_ACT_SILU ? act_of<TDC_ACT_SILU>(v) : v;
-            reinterpret_cast<T *>(a.y)[row * a.y_stride + n0 + n] = Num<DT>::down(v);
-        }
+    for (int e = 0; e < 16; ++e) part[(wave * 16 + e) * 64 + lane] = acc[e];
+    __syncthreads();
+    const int rows = (int)min(32ll, a.M - m0);
+    for (int o = t; o < 32 * rows; o += blockDim.x) {
+        const int n = o & 31, m = o >> 5, at = ((n >> 3) * 4 + (n & 3)) * 64 + (n >> 2 & 1) * 32 + m;
+        if (n0 + n >= a.N) continue;
+        float v = 0.0f;
+        for (int k = 0; k < waves; ++k) v += part[k * 1024 + at];
+        if (a.bias) v += param<DT>(a.bias, n0 + n, a.bias_dtype);
+        if (a.residual) v += Num<DT>::up(reinterpret_cast<const T *>(a.residual)[(m0 + m) * a.r_stride + n0 + n]);
+        v = a.act == TDC_ACT_RELU ? act_of<TDC_ACT_RELU>(v) : a.act == TDC_ACT_SILU ? act_of<TDC_ACT_SILU>(v) : v;
+        reinterpret_cast<T *>(a.y)[(m0 + m) * a.y_stride + n0 + n] = Num<DT>::down(v);
     }
 }
 
@@ -404,25 +386,30 @@ static int launch_tile(const ProductArgs &a, hipStream_t s) {
     fn<<<grid, 256, L::kLds, s>>>(a, tm, tn);
     return (int)hipGetLastError();
 }
-template <int DT, int XS, int MB>
+template <int DT, int XS>
 static int launch_few(const ProductArgs &a, hipStream_t s) {
     // A wave for every 512 numbers of K, four to sixteen of them.
     const int groups = (a.ksteps + 3) / 4, waves = groups <= 4 ? 4 : groups <= 8 ? 8 : 16;
     const int x_bytes = XS == TDC_MX4 ? 0 : (int)a.M * (a.ksteps * 64 + groups * 16), lds = std::max(waves * 4096, x_bytes);
-    const unsigned bm = (unsigned)((a.M + 32 * MB - 1) / (32 * MB)), bn = (unsigned)((a.N + 31) / 32);
-    tdc_mx4_product_few_kernel<DT, XS, MB><<<bm * bn, waves * 64, lds, s>>>(a, (int)bm);
+    const unsigned bm = (unsigned)((a.M + 31) / 32), bn = (unsigned)((a.N + 31) / 32);
+    tdc_mx4_product_few_kernel<DT, XS><<<bm * bn, waves * 64, lds, s>>>(a, (int)bm);
     return (int)hipGetLastError();
 }
+
+// Timed in turn over M 16 .. 25088, N 64 .. 8192, K 128 .. 8192 (us):
+//   32 x 32 outputs a workgroup while there are 256 of them, or 512 of long sums: 512 x 512 x 2048 5.5 against 9.7 in tiles of 128,
+//   1024 x 512 x 2048 7.5 against 9.7, but 1024 x 512 x 512 6.7 against 6.6 and 1024 x 1024 x 2048 11.9 against 9.9;
+//   tiles of 256 for long sums that fill the compute units: 4096 x 8192 x 8192 155 against 171, 25088 x 512 x 8192 65 against 80, but
+//   8192 x 8192 x 2048 122 against 110 (a tile's first loads and its stores run alone) and 1024 x 8192 x 8192 60 against 44.
 template <int DT>
 static int launch_product(const ProductArgs &a, hipStream_t s) {
     if (a.x) {
-        if (a.x_dtype == TDC_F32) return launch_few<DT, TDC_F32, 1>(a, s);
-        return a.x_dtype == TDC_F16 ? launch_few<DT, TDC_F16, 1>(a, s) : launch_few<DT, TDC_BF16, 1>(a, s);
+        if (a.x_dtype == TDC_F32) return launch_few<DT, TDC_F32>(a, s);
+        return a.x_dtype == TDC_F16 ? launch_few<DT, TDC_F16>(a, s) : launch_few<DT, TDC_BF16>(a, s);
     }
-    if (a.M <= 32) return launch_few<DT, TDC_MX4, 1>(a, s);
-    if (a.M <= 64) return launch_few<DT, TDC_MX4, 2>(a, s);
-    const long long big = ((a.M + 255) / 256) * ((a.N + 255) / 256);
-    if (big >= 192) return launch_tile<DT, 4, 4>(a, s);
+    auto tiles = [&](long long edge) { return ((a.M + edge - 1) / edge) * ((a.N + edge - 1) / edge); };
+    if (tiles(32) <= (a.ksteps >= 8 ? 512 : 256)) return launch_few<DT, TDC_MX4>(a, s);
+    if (a.ksteps >= 32 && tiles(256) >= 192) return launch_tile<DT, 4, 4>(a, s);
     return launch_tile<DT, 2, 2>(a, s);
 }
 

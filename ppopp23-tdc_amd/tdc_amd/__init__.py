@@ -8,14 +8,14 @@ __all__ = ["LIB_PATH", "ConvDesc", "TdcError", "Tile", "TileInfo", "conv_desc", 
 
 
 def __getattr__(name):
-    # torch-dependent classes are imported lazily so the model API works without torch.
+    # torch-dependent classes are imported lazily so the model API works without torch; once loaded they are plain attributes.
     if name in ("Conv2dPlan", "TKConvOp"):
-        from . import conv
-        return getattr(conv, name)
-    if name in ("TKConv2dC", "ranks_dict", "partial_tucker2"):
-        from . import TKConv
-        return getattr(TKConv, name)
-    if name in ("group_norm_act", "group_norm_act_mx4", "mx4_quantize", "mx4_linear", "mx4_conv1x1", "Mx4Tensor"):
-        from . import channels_last
-        return getattr(channels_last, name)
-    raise AttributeError(name)
+        from . import conv as module
+    elif name in ("TKConv2dC", "ranks_dict", "partial_tucker2"):
+        from . import TKConv as module
+    elif name in ("group_norm_act", "group_norm_act_mx4", "mx4_quantize", "mx4_linear", "mx4_conv1x1", "Mx4Tensor"):
+        from . import channels_last as module
+    else:
+        raise AttributeError(name)
+    globals()[name] = value = getattr(module, name)
+    return value

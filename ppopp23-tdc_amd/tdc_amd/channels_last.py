@@ -23,7 +23,16 @@ from .conv import _device, _raw_stream
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _MX4 = 3
 _ACTS = {"none": 0, "relu": 1, "silu": 2}
-_empty = torch.empty
+_empty, _empty_strided, _u8, _f32 = torch.empty, torch.empty_strided, torch.uint8, torch.float32
+_calls = {}
+
+
+def _call(name):
+    """The library's entry point of that name (looked up once)."""
+    fn = _calls.get(name)
+    if fn is None:
+        fn = _calls[name] = getattr(lib(), name)
+    return fn
 
 
 def _act(name):
@@ -108,7 +117,7 @@ def _dense_strides(shape):
 
 class _Norm:
     """A norm's descriptor and sizes, for one shape of x (and of y or dy)."""
-    __slots__ = ("desc", "ref", "forward_ws", "backward_ws", "mx4_ws", "y_strides", "stats_shape", "dense")
+    __slots__ = ("desc", "ref", "forward_ws", "backward_ws", "mx4_ws", "y_strides", "stats_shape", "stats_bytes", "mx4_shape", "dense")
 
     def __init__(self, x_shape, x_stride, y_stride, dtype, param_dtype, groups, eps, act):
         x = _pixel_strides(x_shape, x_stride)
@@ -127,6 +136,8 @@ class _Norm:
         check(lib().tdc_group_norm_mx4_workspace(self.ref, byref(mx4)))
         self.forward_ws, self.backward_ws, self.mx4_ws = fwd.value, bwd.value, mx4.value
         self.stats_shape = (2, x_shape[0], groups)
+        self.stats_bytes = 4 * x_shape[0] * groups
+        self.mx4_shape = (x_shape[0], *x_shape[2:], x_shape[1])
 
 
 _norms = _Cache()
@@ -157,13 +168,16 @@ def _norm_for(x, groups, weight, bias, eps, act, y_stride=None):
 def _norm_forward(x, groups, weight, bias, eps, act, stats):
     plan = _norm_for(x, groups, weight, bias, eps, act)
     dev = x.device
-    y = torch.empty_strided(x.shape, plan.y_strides, dtype=x.dtype, device=dev)
-    ws = _empty(plan.forward_ws, dtype=torch.uint8, device=dev) if plan.forward_ws else None
-    kept = _empty(plan.stats_shape, dtype=torch.float32, device=dev) if stats else None
-    mean = kept.data_ptr() if stats else None
-    status = lib().tdc_group_norm_forward(plan.ref, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean,
-                                          mean + 4 * plan.stats_shape[1] * plan.stats_shape[2] if stats and mean else None,
-                                          _ptr(ws), plan.forward_ws, _raw_stream(x.get_device()))
+    y = _empty_strided(x.shape, plan.y_strides, dtype=x.dtype, device=dev)
+    need = plan.forward_ws
+    ws = _empty(need, dtype=_u8, device=dev) if need else None
+    kept = mean = rstd = None
+    if stats:
+        kept = _empty(plan.stats_shape, dtype=_f32, device=dev)
+        mean = kept.data_ptr()
+        rstd = mean + plan.stats_bytes if mean else None
+    status = _call("tdc_group_norm_forward")(plan.ref, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean, rstd, _ptr(ws), need,
+                                             _raw_stream(x.get_device()))
     if status:
         check(status)
     return y, kept
@@ -185,24 +199,21 @@ class _GroupNormAct(torch.autograd.Function):
         plan = _norm_for(x, groups, weight, bias, eps, act, dy.stride())
         dev, C = x.device, x.shape[1]
         if plan.dense:
-            dy = torch.empty_strided(x.shape, plan.y_strides, dtype=x.dtype, device=dev).copy_(dy)
+            dy = _empty_strided(x.shape, plan.y_strides, dtype=x.dtype, device=dev).copy_(dy)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty_strided(x.shape, plan.y_strides, dtype=x.dtype, device=dev) if need_x else None
-        dparam = _empty((2, C), dtype=torch.float32, device=dev) if need_w or need_b else None
-        at = _ptr(dparam)
-        ws = _empty(plan.backward_ws, dtype=torch.uint8, device=dev)
+        dx = _empty_strided(x.shape, plan.y_strides, dtype=x.dtype, device=dev) if need_x else None
+        dw = _empty(C, dtype=_f32, device=dev) if need_w else None
+        db = _empty(C, dtype=_f32, device=dev) if need_b else None
+        ws = _empty(plan.backward_ws, dtype=_u8, device=dev)
         mean = stats.data_ptr()
-        status = lib().tdc_group_norm_backward(
-            plan.ref, x.data_ptr(), dy.data_ptr(), _ptr(weight), _ptr(bias), mean, mean + 4 * plan.stats_shape[1] * plan.stats_shape[2],
-            _ptr(dx), at if need_w else None, at + 4 * C if need_b else None, ws.data_ptr(), plan.backward_ws,
-            _raw_stream(x.get_device()))
+        status = _call("tdc_group_norm_backward")(plan.ref, x.data_ptr(), dy.data_ptr(), _ptr(weight), _ptr(bias), mean,
+                                                  mean + plan.stats_bytes, _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(),
+                                                  plan.backward_ws, _raw_stream(x.get_device()))
         if status:
             check(status)
-        dw = dparam[0] if need_w else None
-        db = dparam[1] if need_b else None
-        if need_w and weight.dtype != torch.float32:
+        if need_w and weight.dtype != _f32:
             dw = dw.to(weight.dtype)
-        if need_b and bias.dtype != torch.float32:
+        if need_b and bias.dtype != _f32:
             db = db.to(bias.dtype)
         return dx, dw, db, None, None, None
 
@@ -234,51 +245,73 @@ class Mx4Tensor:
 
     ``shape`` is that of the numbers, ``codes`` [ceil(K / 128), ceil(rows / 32), 4, 32, 16] and ``scales``
     [ceil(K / 512), rows, 16] are bytes (the layout is that of include/tdc.h)."""
-    __slots__ = ("codes", "scales", "shape", "rows", "K")
+    __slots__ = ("shape", "rows", "K", "device", "index", "_held", "_codes_at", "_scales_at")
 
     def __init__(self, codes, scales, shape):
         shape = tuple(int(n) for n in shape)
         if not shape or shape[-1] < 1:
             raise ValueError(f"the last axis has to hold a number at least: got {shape}")
-        self.shape, self.K = shape, shape[-1]
-        self.rows = 1
-        for n in shape[:-1]:
-            self.rows *= n
-        for t, want, what in ((codes, ((self.K + 127) // 128, (self.rows + 31) // 32, 4, 32, 16), "codes"), (scales, ((self.K + 511) // 512, self.rows, 16), "scales")):
-            if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous() or not t.is_cuda:
+        self.shape, self.K, self.rows = shape, shape[-1], _product(shape[:-1])
+        for t, want, what in zip((codes, scales), self._byte_shapes(), ("codes", "scales")):
+            if t.dtype != _u8 or tuple(t.shape) != want or not t.is_contiguous() or not t.is_cuda:
                 raise ValueError(f"{what} has to be a contiguous uint8 device tensor of shape {want}")
         if codes.device != scales.device:
             raise ValueError("codes and scales must be on one device")
-        self.codes, self.scales = codes, scales
+        self.device, self.index, self._held = codes.device, codes.get_device(), (codes, scales)
+        self._codes_at, self._scales_at = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
-    def _new(cls, rows, K, shape, device):
+    def _new(cls, rows, K, shape, device, index):
         t = cls.__new__(cls)
-        t.codes = _empty(((K + 127) // 128, (rows + 31) // 32, 4, 32, 16), dtype=torch.uint8, device=device)
-        t.scales = _empty(((K + 511) // 512, rows, 16), dtype=torch.uint8, device=device)
-        t.shape, t.rows, t.K = shape, rows, K
+        codes = (K + 127) // 128 * ((rows + 31) // 32) * 2048
+        t._held = _empty(codes + (K + 511) // 512 * rows * 16, dtype=_u8, device=device)
+        t._codes_at = t._held.data_ptr()
+        t._scales_at = t._codes_at + codes
+        t.shape, t.rows, t.K, t.device, t.index = shape, rows, K, device, index
         return t
 
+    def _byte_shapes(self):
+        return ((self.K + 127) // 128, (self.rows + 31) // 32, 4, 32, 16), ((self.K + 511) // 512, self.rows, 16)
+
+    def _bytes(self, which):
+        if type(self._held) is tuple:
+            return self._held[which]
+        shapes = self._byte_shapes()
+        split = _product(shapes[0])
+        return (self._held[split:] if which else self._held[:split]).view(shapes[which])
+
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self):
+        return self._bytes(0)
+
+    @property
+    def scales(self):
+        return self._bytes(1)
 
     def dequantize(self, dtype=torch.float32):
         """The numbers that the codes and scales stand for (each is exact in float32 and bfloat16)."""
-        if dtype not in _DTYPES:
+        kind = _DTYPES.get(dtype)
+        if kind is None:
             raise TypeError(f"dtype has to be float32, float16 or bfloat16: got {dtype}")
-        return _on(self.codes, self._dequantize, dtype)
-
-    def _dequantize(self, dtype):
-        y = _empty(self.shape, dtype=dtype, device=self.codes.device)
-        status = lib().tdc_mx4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), self.rows, self.K, y.data_ptr(), _DTYPES[dtype],
-                                          self.K, _raw_stream(self.codes.get_device()))
+        if self.index != _device():
+            with torch.cuda.device(self.device):
+                return self.dequantize(dtype)
+        y = _empty(self.shape, dtype=dtype, device=self.device)
+        status = _call("tdc_mx4_dequantize")(self._codes_at, self._scales_at, self.rows, self.K, y.data_ptr(), kind, self.K,
+                                             _raw_stream(self.index))
         if status:
             check(status)
         return y
 
     def __repr__(self):
         return f"Mx4Tensor(shape={self.shape}, device={self.device})"
+
+
+def _product(shape):
+    n = 1
+    for k in shape:
+        n *= k
+    return n
 
 
 def _rows(t):
@@ -295,9 +328,9 @@ def _rows(t):
 
 def _quantize(x):
     flat, step = _rows(x)
-    q = Mx4Tensor._new(flat.shape[0], flat.shape[1], tuple(x.shape), x.device)
-    status = lib().tdc_mx4_quantize(flat.data_ptr(), _DTYPES[x.dtype], q.rows, q.K, step, q.codes.data_ptr(), q.scales.data_ptr(),
-                                    _raw_stream(x.get_device()))
+    index = x.get_device()
+    q = Mx4Tensor._new(flat.shape[0], flat.shape[1], tuple(x.shape), x.device, index)
+    status = _call("tdc_mx4_quantize")(flat.data_ptr(), _DTYPES[x.dtype], q.rows, q.K, step, q._codes_at, q._scales_at, _raw_stream(index))
     if status:
         check(status)
     return q
@@ -323,11 +356,11 @@ def group_norm_act_mx4(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
 
 def _norm_mx4(x, groups, weight, bias, eps, act):
     plan = _norm_for(x, groups, weight, bias, eps, act)
-    d = plan.desc
-    q = Mx4Tensor._new(d.batch * d.pixels, d.C, (x.shape[0], *x.shape[2:], d.C), x.device)
-    ws = _empty(plan.mx4_ws, dtype=torch.uint8, device=x.device) if plan.mx4_ws else None
-    status = lib().tdc_group_norm_forward_mx4(plan.ref, x.data_ptr(), _ptr(weight), _ptr(bias), q.codes.data_ptr(), q.scales.data_ptr(),
-                                              _ptr(ws), plan.mx4_ws, _raw_stream(x.get_device()))
+    d, index, need = plan.desc, x.get_device(), plan.mx4_ws
+    q = Mx4Tensor._new(d.batch * d.pixels, d.C, plan.mx4_shape, x.device, index)
+    ws = _empty(need, dtype=_u8, device=x.device) if need else None
+    status = _call("tdc_group_norm_forward_mx4")(plan.ref, x.data_ptr(), _ptr(weight), _ptr(bias), q._codes_at, q._scales_at, _ptr(ws), need,
+                                                 _raw_stream(index))
     if status:
         check(status)
     return q
@@ -338,56 +371,64 @@ def _norm_mx4(x, groups, weight, bias, eps, act):
 _linears = _Cache()
 
 
-def _linear(x, weight, bias, residual, act, out_dtype):
-    quantised = type(x) is Mx4Tensor
-    if quantised:
-        flat, x_step, dev, x_type = None, 0, x.codes.device, _MX4
-        M, lead, dtype = x.rows, x.shape[:-1], out_dtype or torch.bfloat16
-    else:
-        flat, x_step = _rows(x)
-        M, lead, dev, dtype, x_type = flat.shape[0], x.shape[:-1], x.device, out_dtype or x.dtype, _DTYPES[x.dtype]
-    r_step = 0
-    if residual is not None:
-        if residual.dtype != dtype or residual.device != dev or residual.shape != (*lead, weight.rows):
-            raise ValueError(f"residual has to be {dtype} of shape {(*lead, weight.rows)} on {dev}: got {residual.dtype} "
-                             f"{tuple(residual.shape)} on {residual.device}")
-        residual, r_step = _rows(residual)
-    _vector(bias, weight.rows, dtype, dev, "bias")
-    bias_type = bias.dtype if bias is not None else torch.float32
-    key = (M, weight.rows, weight.K, x_type, dtype, bias_type, act, x_step, r_step)
-    plan = _linears.get(key)
-    if plan is None:
-        if dtype not in _DTYPES:
-            raise TypeError(f"out_dtype has to be float32, float16 or bfloat16: got {dtype}")
-        desc = _lib.Mx4LinearDesc(M, weight.rows, weight.K, x_type, _DTYPES[dtype], _DTYPES[bias_type], _act(act), x_step, weight.rows, r_step)
-        need = ctypes.c_size_t()
-        check(lib().tdc_mx4_linear_workspace(byref(desc), byref(need)))
-        plan = _linears.keep(key, (byref(desc), need.value))
-    ref, need = plan
-    y = _empty((*lead, weight.rows), dtype=dtype, device=dev)
-    ws = _empty(need, dtype=torch.uint8, device=dev) if need else None
-    status = lib().tdc_mx4_linear(ref, x.codes.data_ptr() if quantised else flat.data_ptr(), x.scales.data_ptr() if quantised else None,
-                                  weight.codes.data_ptr(), weight.scales.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(),
-                                  _ptr(ws), need, _raw_stream(weight.codes.get_device()))
-    if status:
-        check(status)
-    return y
-
-
-def _linear_checked(x, weight, bias, residual, act, out_dtype):
+def _linear(x, weight, bias, residual, act, out_dtype, pixels):
+    """``pixels``: x [B, H, W, K] stands for a channels-last [B, K, H, W], as the result [B, N, H, W] does."""
     if type(weight) is not Mx4Tensor or len(weight.shape) != 2:
         raise TypeError("weight has to be an Mx4Tensor of shape [N, K]: mx4_quantize(weight)")
-    if type(x) is not Mx4Tensor:
+    index, dev, N = weight.index, weight.device, weight.rows
+    quantised = type(x) is Mx4Tensor
+    if not quantised:
         _number_tensor(x, "x")
         if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("the 4-bit product has no gradient: call it under torch.no_grad()")
         if x.dim() < 1:
             raise ValueError("expected x [..., K]")
-    if x.shape[-1] != weight.K:
-        raise ValueError(f"x has {x.shape[-1]} numbers a row, weight {weight.K}")
-    if x.device != weight.device:
-        raise ValueError(f"x is on {x.device}, weight on {weight.device}")
-    return _on(weight.codes, _linear, x, weight, bias, residual, act, out_dtype)
+    shape = x.shape
+    if shape[-1] != weight.K:
+        raise ValueError(f"x has {shape[-1]} numbers a row, weight {weight.K}")
+    if x.device != dev:
+        raise ValueError(f"x is on {x.device}, weight on {dev}")
+    if index != _device():
+        with torch.cuda.device(dev):
+            return _linear(x, weight, bias, residual, act, out_dtype, pixels)
+    if quantised:
+        M, dtype, x_type, x_step = x.rows, out_dtype or torch.bfloat16, _MX4, 0
+        x_at, x_scales = x._codes_at, x._scales_at
+    else:
+        flat, x_step = _rows(x)
+        M, dtype, x_type = flat.shape[0], out_dtype or x.dtype, _DTYPES[x.dtype]
+        x_at, x_scales = flat.data_ptr(), None
+    r_step, r_at, bias_type, b_at = 0, None, _f32, None
+    if residual is not None:
+        if residual.dtype != dtype or residual.device != dev or residual.shape != (*shape[:-1], N):
+            raise ValueError(f"residual has to be {dtype} of shape {(*shape[:-1], N)} on {dev}: got {residual.dtype} "
+                             f"{tuple(residual.shape)} on {residual.device}")
+        residual, r_step = _rows(residual)
+        r_at = residual.data_ptr()
+    if bias is not None:
+        _vector(bias, N, dtype, dev, "bias")
+        bias_type, b_at = bias.dtype, bias.data_ptr()
+    key = (M, N, weight.K, x_type, dtype, bias_type, act, x_step, r_step)
+    plan = _linears.get(key)
+    if plan is None:
+        if dtype not in _DTYPES:
+            raise TypeError(f"out_dtype has to be float32, float16 or bfloat16: got {dtype}")
+        desc = _lib.Mx4LinearDesc(M, N, weight.K, x_type, _DTYPES[dtype], _DTYPES[bias_type], _act(act), x_step, N, r_step)
+        need = ctypes.c_size_t()
+        check(lib().tdc_mx4_linear_workspace(byref(desc), byref(need)))
+        plan = _linears.keep(key, (byref(desc), need.value))
+    ref, need = plan
+    if pixels:
+        B, H, W = shape[:3]
+        y = _empty_strided((B, N, H, W), (H * W * N, 1, W * N, N), dtype=dtype, device=dev)
+    else:
+        y = _empty((*shape[:-1], N), dtype=dtype, device=dev)
+    ws = _empty(need, dtype=_u8, device=dev) if need else None
+    status = _call("tdc_mx4_linear")(ref, x_at, x_scales, weight._codes_at, weight._scales_at, b_at, r_at, y.data_ptr(), _ptr(ws), need,
+                                     _raw_stream(index))
+    if status:
+        check(status)
+    return y
 
 
 def mx4_linear(x, weight, bias=None, residual=None, act="none", out_dtype=None):
@@ -396,7 +437,7 @@ def mx4_linear(x, weight, bias=None, residual=None, act="none", out_dtype=None):
     ``weight`` is an ``Mx4Tensor`` [N, K]; ``x`` [..., K] is numbers (float32, float16, bfloat16), quantised on the way, or an
     ``Mx4Tensor``.  ``out_dtype`` is x's type unless given (bfloat16 for an Mx4Tensor); ``residual`` [..., N] is of that type,
     ``bias`` [N] of it or float32.  Has no gradient."""
-    return _linear_checked(x, weight, bias, residual, act, out_dtype)
+    return _linear(x, weight, bias, residual, act, out_dtype, False)
 
 
 def mx4_conv1x1(x, weight, bias=None, residual=None, act="none", out_dtype=None):
@@ -414,4 +455,4 @@ def mx4_conv1x1(x, weight, bias=None, residual=None, act="none", out_dtype=None)
         if residual.dim() != 4:
             raise ValueError(f"expected residual [batch, channels, height, width], got {tuple(residual.shape)}")
         residual = residual.permute(0, 2, 3, 1)
-    return _linear_checked(x, weight, bias, residual, act, out_dtype).permute(0, 3, 1, 2)
+    return _linear(x, weight, bias, residual, act, out_dtype, True)

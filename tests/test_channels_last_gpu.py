@@ -304,7 +304,7 @@ def test_product(M, N, K, dtype):
     check_product(tdc_amd.mx4_linear(xd, wq, out_dtype=other), xv, wv, None, None, "none", "another type out")
 
 
-@pytest.mark.parametrize("dtype,M,N,K", [(F32, 3333, 3850, 420), (F16, 4100, 3590, 128), (BF16, 3328, 4096, 1700)])
+@pytest.mark.parametrize("dtype,M,N,K", [(F32, 3333, 3850, 420), (F16, 4100, 3590, 128), (BF16, 3328, 4096, 1700), (BF16, 3333, 3850, 4100)])
 def test_product_of_many_tiles(dtype, M, N, K):
     x, w = numbers(16, M, K).to(dtype), numbers(17, N, K) / math.sqrt(K)
     bias, residual = numbers(18, N), numbers(19, M, N).to(dtype)
