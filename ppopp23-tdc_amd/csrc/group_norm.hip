@@ -17,6 +17,17 @@
 
 namespace tdc {
 
+// Number i of a channel (`last` of those at hand): four at a time are added in 32 bits where they have 16, which is exact unless one is
+// 2^11 times another, the others and the fours in 64.
+template <int DT>
+static __device__ __forceinline__ void add_up(int i, bool last, float v, float &four, double &sum) {
+    if constexpr (DT == TDC_F32) sum += v;
+    else {
+        four = i % 4 == 0 ? v : four + v;
+        if (last || i % 4 == 3) sum += four;
+    }
+}
+
 // Neighbouring channels of a thread that share a place (`run` of them, a power of two): all of them end up with its sum.
 template <typename T, int V>
 static __device__ __forceinline__ void join_run(T (&s)[V], int run) {
@@ -78,13 +89,14 @@ static __device__ __forceinline__ void held_sums(int n, typename Pack<DT, V>::ty
         s[j] = 0.0;
         q[j] = 0.0f;
     }
+    float four[V];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (i < n) {
             float v[V];
             Pack<DT, V>::up(x[i], v);
 #pragma unroll
-            for (int j = 0; j < V; ++j) s[j] += v[j];
+            for (int j = 0; j < V; ++j) add_up<DT>(i, i == n - 1, v[j], four[j], s[j]);
         }
     join_run(s, run);
     pack_again(x);
@@ -103,39 +115,37 @@ static __device__ __forceinline__ void held_sums(int n, typename Pack<DT, V>::ty
     join_run(q, run);
 }
 
-// Of any number of pixels, NV of them on their way while NV are added up: the deviations from a channel's first number, an error of
-// which is one part in n of the deviations that this number itself has, then moved to the mean of the place.
+// Of any number of pixels: the deviations from a channel's first number, an error of which is one part in n of the deviations that this
+// number itself has, then moved to the mean of the place.
 template <int DT, int V, int NV>
 static __device__ __forceinline__ void passing_sums(const NormArgs &a, const Part &p, int n, int run, double (&s)[V], float (&q)[V]) {
     using P = Pack<DT, V>;
+    if (n == 0) return;
+    const Walk<DT, V> in(a.x, a.x_is, a.x_ps, p, n);
     float first[V];
-    typename P::type next[NV];
-    hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, 0, n, next);
-    P::up(next[0], first);
+    P::up(P::load(in.base, in.at), first);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         s[j] = 0.0;
         q[j] = 0.0f;
     }
-    for (int at = 0; at < n; at += NV) {
-        typename P::type x[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) x[i] = next[i];
-        hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, at + NV, n, next);
+    typename P::type x[2][NV];
+    walk<NV>(n, p.rows / p.R, [&](int set, int at) { in.ask(at, x[set]); }, [&](int set, int, auto some) {
+        float four[V];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (at + i < n) {
+            if (i < some) {
                 float v[V];
-                P::up(x[i], v);
+                P::up(x[set][i], v);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    s[j] += v[j];
+                    add_up<DT>(i, i == some - 1, v[j], four[j], s[j]);
                     q[j] = fmaf(v[j] - first[j], v[j] - first[j], q[j]);
                 }
             }
-    }
+    });
     double own[V];
-    const double inv = 1.0 / max(n, 1);
+    const double inv = 1.0 / n;
 #pragma unroll
     for (int j = 0; j < V; ++j) own[j] = s[j] * inv;
     join_run(s, run);
@@ -233,18 +243,9 @@ __global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(c
         join_threads(a, p, n, s, q, run, sums, devs, [&](int i, double sum, float m2) { a.stat[slot_of(a, p, p.g0 + i)] = NormStat{sum, m2}; });
         return;
     }
-    typename P::type x[NV];
-    hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, 0, n, x);
-    if constexpr (MODE == kWhole) {
-        held_sums<DT, V, NV>(n, x, run, s, q);
-        join_threads(a, p, n, s, q, run, sums, devs, [&](int i, double sum, float m2) {
-            stat[i] = finish_stats(a, p, p.g0 + i, sum / ((double)a.pixels * a.Cg), m2, true);
-        });
-    } else join_stats(a, p, stat);
-    __syncthreads();
     const int c = p.c0 + p.tc * V;
-    if (n > 0) {
-        float mean[V], scale[V], shift[V];
+    float mean[V], scale[V], shift[V];
+    auto constants = [&]() {
         params<DT, V>(a, c, scale, shift);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -252,24 +253,42 @@ __global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(c
             mean[j] = st.x;
             scale[j] *= st.y;
         }
-        const long long row = p.row0 + p.tr, out = p.image * a.o_is + row * a.o_ps + c, step = p.R * a.o_ps;
-        for (int at = 0; at < (MODE == kWhole ? 1 : n); at += NV) {
-            typename P::type next[NV];
-            if constexpr (MODE != kWhole) hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, at + NV, n, next);
+    };
+    const long long row = p.row0 + p.tr, out = p.image * a.o_is + row * a.o_ps + c, step = p.R * a.o_ps;
+    auto finish = [&](const typename P::type &x, int i) {
+        float v[V];
+        P::up(x, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = act_of<ACT>(fmaf(v[j] - mean[j], scale[j], shift[j]));
+        if constexpr (MX4) store_mx4<V>(a, (long long)p.image * a.pixels + row + (long long)i * p.R, c, v);
+        else P::store(a.out, out + i * step, P::down(v));
+    };
+    if constexpr (MODE == kWhole) {
+        typename P::type x[NV];
+        hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, n, x);
+        held_sums<DT, V, NV>(n, x, run, s, q);
+        join_threads(a, p, n, s, q, run, sums, devs, [&](int i, double sum, float m2) {
+            stat[i] = finish_stats(a, p, p.g0 + i, sum / ((double)a.pixels * a.Cg), m2, true);
+        });
+        __syncthreads();
+        if (n > 0) {
+            constants();
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (at + i < n) {
-                    float v[V];
-                    P::up(x[i], v);
+                if (i < n) finish(x[i], i);
+        }
+    } else {
+        join_stats(a, p, stat);
+        __syncthreads();
+        if (n > 0) {
+            constants();
+            const Walk<DT, V> in(a.x, a.x_is, a.x_ps, p, n);
+            typename P::type x[2][NV];
+            walk<NV>(n, p.rows / p.R, [&](int set, int at) { in.ask(at, x[set]); }, [&](int set, int at, auto some) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) v[j] = act_of<ACT>(fmaf(v[j] - mean[j], scale[j], shift[j]));
-                    if constexpr (MX4) store_mx4<V>(a, (long long)p.image * a.pixels + row + (long long)(at + i) * p.R, c, v);
-                    else P::store(a.out, out + (at + i) * step, P::down(v));
-                }
-            if constexpr (MODE != kWhole) {
-#pragma unroll
-                for (int i = 0; i < NV; ++i) x[i] = next[i];
-            }
+                for (int i = 0; i < NV; ++i)
+                    if (i < some) finish(x[set][i], at + i);
+            });
         }
     }
     if (MX4 && p.c0 + p.width == a.C) store_mx4_padding(a, p);

@@ -64,9 +64,12 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
     }
     const Part p = part_of(a, V, blockIdx.x - param_blocks, gridDim.x - param_blocks);
     const int n = rows_of(p, p.tr), c = p.c0 + p.tc * V;
-    typename P::type x[NV], dy[NV];
-    hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, 0, n, x);
-    hold<DT, V, NV>(a.dy, a.d_is, a.d_ps, p, 0, n, dy);
+    constexpr bool whole = MODE == kWhole;
+    typename P::type x[whole ? 1 : 2][NV], dy[whole ? 1 : 2][NV];
+    if constexpr (whole) {
+        hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, n, x[0]);
+        hold<DT, V, NV>(a.dy, a.d_is, a.d_ps, p, n, dy[0]);
+    }
     float mean[V], rstd[V], gamma[V], beta[V];
     if (n > 0) {
         params<DT, V>(a, c, gamma, beta);
@@ -77,6 +80,24 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
             rstd[j] = a.rstd[g];
         }
     }
+    // All pixels of this thread, which has some.
+    auto each = [&](auto use) {
+        if constexpr (whole) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (i < n) use(0, i, i);
+        } else {
+            const Walk<DT, V> in(a.x, a.x_is, a.x_ps, p, n), din(a.dy, a.d_is, a.d_ps, p, n);
+            walk<NV>(n, p.rows / p.R, [&](int set, int at) {
+                in.ask(at, x[set]);
+                din.ask(at, dy[set]);
+            }, [&](int set, int at, auto some) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (i < some) use(set, i, at + i);
+            });
+        }
+    };
     float2 *const cell = reinterpret_cast<float2 *>(lds), *const stat = cell + (MODE == kApply ? 0 : a.plan.threads * V);
     const float inv = 1.0f / ((float)a.pixels * a.Cg);
     const Team t = team_of(a.plan.threads, p.ng);
@@ -85,31 +106,15 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
             float sz[V], sx[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) sz[j] = sx[j] = 0.0f;
-            for (int at = 0; at < (MODE == kWhole ? 1 : n); at += NV) {
-                typename P::type next_x[NV], next_dy[NV];
-                if constexpr (MODE != kWhole) {
-                    hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, at + NV, n, next_x);
-                    hold<DT, V, NV>(a.dy, a.d_is, a.d_ps, p, at + NV, n, next_dy);
+            each([&](int set, int i, int) {
+                float dz[V], xh[V];
+                slopes<DT, V, ACT>(x[set][i], dy[set][i], mean, rstd, gamma, beta, dz, xh);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    sz[j] += dz[j];
+                    sx[j] = fmaf(dz[j], xh[j], sx[j]);
                 }
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (at + i < n) {
-                        float dz[V], xh[V];
-                        slopes<DT, V, ACT>(x[i], dy[i], mean, rstd, gamma, beta, dz, xh);
-#pragma unroll
-                        for (int j = 0; j < V; ++j) {
-                            sz[j] += dz[j];
-                            sx[j] = fmaf(dz[j], xh[j], sx[j]);
-                        }
-                    }
-                if constexpr (MODE != kWhole) {
-#pragma unroll
-                    for (int i = 0; i < NV; ++i) {
-                        x[i] = next_x[i];
-                        dy[i] = next_dy[i];
-                    }
-                }
-            }
+            });
 #pragma unroll
             for (int j = 0; j < V; ++j) cell[p.tr * p.width + p.tc * V + j] = make_float2(sz[j], sx[j]);
         }
@@ -171,32 +176,15 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
         s2[j] = st.y;
     }
     const long long out = p.image * a.o_is + (long long)(p.row0 + p.tr) * a.o_ps + c, step = p.R * a.o_ps;
-    if constexpr (MODE == kWhole) pack_again(x);
-    for (int at = 0; at < (MODE == kWhole ? 1 : n); at += NV) {
-        typename P::type next_x[NV], next_dy[NV];
-        if constexpr (MODE != kWhole) {
-            hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, at + NV, n, next_x);
-            hold<DT, V, NV>(a.dy, a.d_is, a.d_ps, p, at + NV, n, next_dy);
-        }
+    if constexpr (whole) pack_again(x[0]);
+    each([&](int set, int i, int at) {
+        float dz[V], xh[V];
+        slopes<DT, V, ACT>(x[set][i], dy[set][i], mean, rstd, gamma, beta, dz, xh);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (at + i < n) {
-                float dz[V], xh[V];
-                slopes<DT, V, ACT>(x[i], dy[i], mean, rstd, gamma, beta, dz, xh);
-#pragma unroll
-                for (int j = 0; j < V; ++j) dz[j] = rstd[j] * (fmaf(gamma[j], dz[j], -s1[j]) - xh[j] * s2[j]);
-                P::store(a.out, out + (at + i) * step, P::down(dz));
-            }
-        if constexpr (MODE != kWhole) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                x[i] = next_x[i];
-                dy[i] = next_dy[i];
-            }
-        }
-    }
+        for (int j = 0; j < V; ++j) dz[j] = rstd[j] * (fmaf(gamma[j], dz[j], -s1[j]) - xh[j] * s2[j]);
+        P::store(a.out, out + at * step, P::down(dz));
+    });
 }
-
 
 template <int DT, int V, int NV, int ACT>
 static int run(const NormArgs &a, hipStream_t s) {

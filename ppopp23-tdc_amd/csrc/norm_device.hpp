@@ -1,5 +1,7 @@
 // Device-side pieces shared by the group norm kernels: what a workgroup owns, its pixels in registers, sums over groups.
 #pragma once
+#include <type_traits>
+
 #include "ops_device.hpp"
 
 namespace tdc {
@@ -38,15 +40,52 @@ static __device__ __forceinline__ Part part_of(const NormArgs &a, int vec, unsig
 // Pixels of thread row r.
 static __device__ __forceinline__ int rows_of(const Part &p, int r) { return r < p.rows && r < p.R ? (p.rows - r + p.R - 1) / p.R : 0; }
 
-// This thread's vectors of a tensor from its pixel `first` on, all requested at once.
+// This thread's vectors of a tensor, all requested at once.
 template <int DT, int V, int NV>
-static __device__ __forceinline__ void hold(const void *base, long long image_stride, long long pixel_stride, const Part &p, int first, int n,
+static __device__ __forceinline__ void hold(const void *base, long long image_stride, long long pixel_stride, const Part &p, int n,
                                             typename Pack<DT, V>::type (&v)[NV]) {
     const long long at = p.image * image_stride + (long long)(p.row0 + p.tr) * pixel_stride + p.c0 + p.tc * V, step = p.R * pixel_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         v[i] = typename Pack<DT, V>::type{};
-        if (first + i < n) v[i] = Pack<DT, V>::load(base, at + (first + i) * step);
+        if (i < n) v[i] = Pack<DT, V>::load(base, at + i * step);
+    }
+}
+
+// A thread's pixels of a tensor one after the other.
+template <int DT, int V>
+struct Walk {
+    const void *base;
+    long long at, step;
+    int last;
+    __device__ __forceinline__ Walk(const void *tensor, long long image_stride, long long pixel_stride, const Part &p, int n)
+        : base(tensor), at(p.image * image_stride + (long long)(p.row0 + p.tr) * pixel_stride + p.c0 + p.tc * V), step(p.R * pixel_stride), last(n - 1) {}
+    // (the pixels past the last repeat it: requests without a branch, so that the compiler can count them)
+    template <int NV>
+    __device__ __forceinline__ void ask(int first, typename Pack<DT, V>::type (&v)[NV]) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = Pack<DT, V>::load(base, at + min(first + i, last) * step);
+    }
+};
+// Pixels 0 .. n - 1 of a thread that has some: `ask(set, at)` requests those from `at` on into one of two sets of NV, `use(set, at, some)`
+// takes the first `some` of them.  While one set is worked on the other is on its way; in the rounds that all threads have (`all`
+// pixels) nothing is conditional, and `some` is a constant NV.
+template <int NV, typename Ask, typename Use>
+static __device__ __forceinline__ void walk(int n, int all, Ask ask, Use use) {
+    using All = std::integral_constant<int, NV>;
+    ask(0, 0);
+    int at = 0;
+    for (; at + 2 * NV <= all; at += 2 * NV) {
+        ask(1, at + NV);
+        use(0, at, All{});
+        ask(0, at + 2 * NV);
+        use(1, at + NV, All{});
+    }
+    for (; at < n; at += 2 * NV) {
+        ask(1, at + NV);
+        use(0, at, min(n - at, NV));
+        ask(0, at + 2 * NV);
+        if (at + NV < n) use(1, at + NV, min(n - at - NV, NV));
     }
 }
 
