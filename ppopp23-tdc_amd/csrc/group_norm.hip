@@ -43,11 +43,44 @@ static __device__ __forceinline__ void join_run(T (&s)[V], int run) {
         }
 }
 
-// The statistics of this workgroup's part of its groups: `done(i, sum, m2)` for the group i of them, in the team's first lane, from
-// the threads' sums s and squared deviations q about the means of their places.
+// A sum of `count` numbers and the squared deviations from their mean, over some lanes' places of one group.
+struct PartSum {
+    double sum;
+    float m2;
+    int count;
+};
+// `mine` places of each of `used` thread rows, from lane `at` on in steps of `step`; `lanes` of them add up.
+static __device__ __forceinline__ PartSum sum_places(const Part &p, const double *sums, const float *devs, int places, int lo, int mine, int used,
+                                                     int run, int at, int step, int lanes) {
+    // (a thread row has one pixel more or less: reciprocals of both counts; places by multiplication, exact for so few)
+    const int most = rows_of(p, 0), longer = p.rows - (most - 1) * p.R;
+    const float per = 1.0f / mine;
+    const double inv_most = 1.0 / (most * run), inv_less = most > 1 ? 1.0 / ((most - 1) * run) : 0.0;
+    PartSum r{0.0, 0.0f, 0};
+    for (int e = at; e < mine * used; e += step) {
+        const int row = (int)((e + 0.5f) * per);
+        r.sum += sums[row * places + lo + e - row * mine];
+        r.count += (row < longer ? most : most - 1) * run;
+    }
+    r.sum = team_sum(r.sum, lanes);
+    r.count = team_sum(r.count, lanes);
+    const double mean = r.sum / max(r.count, 1);
+    for (int e = at; e < mine * used; e += step) {
+        const int row = (int)((e + 0.5f) * per), i = row * places + lo + e - row * mine;
+        const bool full = row < longer;
+        const float d = (float)(sums[i] * (full ? inv_most : inv_less) - mean);
+        r.m2 += devs[i] + (full ? most : most - 1) * run * d * d;
+    }
+    r.m2 = team_sum(r.m2, lanes);
+    return r;
+}
+
+// The statistics of this workgroup's part of its groups: `done(i, sum, m2)` for the group i of them, in one lane, from the threads'
+// sums s and squared deviations q about the means of their places.  Few groups: several waves add up one, their results meet in
+// `waves`.
 template <int V, typename Done>
 static __device__ __forceinline__ void join_threads(const NormArgs &a, const Part &p, int n, const double (&s)[V], const float (&q)[V], int run,
-                                                    double *sums, float *devs, Done done) {
+                                                    double *sums, float *devs, PartSum *waves, Done done) {
     const int places = p.vecs * (V / run);      // of a thread row
     if (n > 0) {
         const int at = p.tr * places + p.tc * (V / run);
@@ -59,25 +92,38 @@ static __device__ __forceinline__ void join_threads(const NormArgs &a, const Par
             }
     }
     __syncthreads();
-    const Team t = team_of(a.plan.threads, p.ng);
-    const int used = min(p.R, p.rows);
-    for (int i = t.first; i < p.ng; i += t.step) {
-        const int g = p.g0 + i, lo = (max(g * a.Cg, p.c0) - p.c0) / run, channels = shared_channels(a, g, p.tile), mine = channels / run;
-        double sum = 0.0;
-        for (int e = t.at; e < mine * used; e += t.lanes) {
-            const int r = e / mine;
-            sum += sums[r * places + lo + e - r * mine];
+    const int used = min(p.R, p.rows), all = a.plan.threads >> 6, wave = threadIdx.x >> 6;
+    auto first = [&](int i) { return (max((p.g0 + i) * a.Cg, p.c0) - p.c0) / run; };
+    auto mine = [&](int i) { return shared_channels(a, p.g0 + i, p.tile) / run; };
+    if (p.ng < all) {
+        const int share = all / p.ng, i = wave / share, k = wave - i * share;
+        if (i < p.ng) {
+            const PartSum r = sum_places(p, sums, devs, places, first(i), mine(i), used, run, k * 64 + (threadIdx.x & 63), share * 64, 64);
+            if ((threadIdx.x & 63) == 0) waves[wave] = r;
         }
-        sum = team_sum(sum, t.lanes);
-        const double mean = sum / ((double)p.rows * channels);
-        float m2 = 0.0f;
-        for (int e = t.at; e < mine * used; e += t.lanes) {
-            const int r = e / mine, at = r * places + lo + e - r * mine;
-            const float count = (float)(rows_of(p, r) * run), d = (float)(sums[at] / count - mean);
-            m2 += devs[at] + count * d * d;
+        __syncthreads();
+        if ((int)threadIdx.x < p.ng) {
+            const PartSum *const w = waves + threadIdx.x * share;
+            double sum = 0.0;
+            int count = 0;
+            for (int k = 0; k < share; ++k) {
+                sum += w[k].sum;
+                count += w[k].count;
+            }
+            const double mean = sum / count;
+            float m2 = 0.0f;
+            for (int k = 0; k < share; ++k) {
+                const float d = (float)(w[k].sum / max(w[k].count, 1) - mean);
+                m2 += w[k].m2 + w[k].count * d * d;
+            }
+            done(threadIdx.x, sum, m2);
         }
-        m2 = team_sum(m2, t.lanes);
-        if (t.at == 0) done(i, sum, m2);
+    } else {
+        const Team t = team_of(a.plan.threads, p.ng);
+        for (int i = t.first; i < p.ng; i += t.step) {
+            const PartSum r = sum_places(p, sums, devs, places, first(i), mine(i), used, run, t.at, t.lanes, t.lanes);
+            if (t.at == 0) done(i, r.sum, r.m2);
+        }
     }
 }
 
@@ -192,26 +238,32 @@ static __device__ __forceinline__ void join_stats(const NormArgs &a, const Part 
     }
 }
 
-// A block's share of V numbers into 4 bits: 32 / V neighbouring lanes hold a block.
+// Where a thread's share of a block of 32 channels goes, and V numbers of a row into it: 32 / V neighbouring lanes hold a block.
 template <int V>
-static __device__ __forceinline__ void store_mx4(const NormArgs &a, long long row, int c, const float (&v)[V]) {
-    float top = 0.0f;
+struct Mx4Place {
+    unsigned char *codes, *scales;      // of row 0; of the scales only in a block's first lane
+    __device__ __forceinline__ Mx4Place(const NormArgs &a, int c)
+        : codes(a.codes + mx4_block_at(a.rows, 0, c >> 5) + (c & 31) / 2),
+          scales(c & 31 ? nullptr : a.scales + (long long)(c >> 9) * a.rows * 16 + (c >> 5 & 3) * 4 + (c >> 7 & 3)) {}
+    __device__ __forceinline__ void store(long long row, const float (&v)[V]) const {
+        unsigned top = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) top = larger(top, v[j]);
-    top = quad_larger(top);
-    if (V == 4) top = larger(top, __shfl_xor(top, 4, 64));
-    const int byte = mx4_scale_byte(top), block = c >> 5;
-    const float divisor = mx4_divisor(byte);
-    unsigned char *const to = a.codes + mx4_block_at(a.rows, row, block) + (c & 31) / 2;
-    if constexpr (V == 8) *reinterpret_cast<unsigned *>(to) = mx4_codes(v, divisor);
-    else {
-        unsigned r = 0;
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], divisor, 0);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], divisor, 1);
-        *reinterpret_cast<unsigned short *>(to) = (unsigned short)r;
+        for (int j = 0; j < V; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+        float most = quad_larger(__uint_as_float(top));
+        if (V == 4) most = larger(most, __shfl_xor(most, 4, 64));
+        const int byte = mx4_scale_byte(most);
+        const float divisor = mx4_divisor(byte);
+        unsigned char *const to = codes + ((row >> 5) * 2048 + (row & 31) * 16);
+        if constexpr (V == 8) *reinterpret_cast<unsigned *>(to) = mx4_codes(v, divisor);
+        else {
+            unsigned r = 0;
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], divisor, 0);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], divisor, 1);
+            *reinterpret_cast<unsigned short *>(to) = (unsigned short)r;
+        }
+        if (scales) scales[row * 16] = (unsigned char)byte;
     }
-    if ((c & 31) == 0) a.scales[((block >> 4) * a.rows + row) * 16 + (block & 3) * 4 + (block >> 2 & 3)] = (unsigned char)byte;
-}
+};
 // What pads a row: blocks up to a multiple of 128 numbers, scale bytes up to one of 512.
 static __device__ __forceinline__ void store_mx4_padding(const NormArgs &a, const Part &p) {
     const int from = (a.C + 31) / 32, blocks = (a.C + 127) / 128 * 4, past = (a.C + 511) / 512 * 16 - from;
@@ -235,18 +287,18 @@ __global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(c
     const int run = V / a.plan.places, most = a.plan.threads * a.plan.places;
     double *const sums = reinterpret_cast<double *>(lds);
     float *const devs = reinterpret_cast<float *>(sums + most);
-    float2 *const stat = MODE == kApply ? reinterpret_cast<float2 *>(lds) : reinterpret_cast<float2 *>(devs + most);
+    PartSum *const waves = reinterpret_cast<PartSum *>(devs + most);
+    float2 *const stat = MODE == kApply ? reinterpret_cast<float2 *>(lds) : reinterpret_cast<float2 *>(waves + a.plan.threads / 64);
     double s[V];
     float q[V];
     if constexpr (MODE == kStats) {
         passing_sums<DT, V, NV>(a, p, n, run, s, q);
-        join_threads(a, p, n, s, q, run, sums, devs, [&](int i, double sum, float m2) { a.stat[slot_of(a, p, p.g0 + i)] = NormStat{sum, m2}; });
+        join_threads(a, p, n, s, q, run, sums, devs, waves, [&](int i, double sum, float m2) { a.stat[slot_of(a, p, p.g0 + i)] = NormStat{sum, m2}; });
         return;
     }
     const int c = p.c0 + p.tc * V;
     float mean[V], scale[V], shift[V];
     auto constants = [&]() {
-        params<DT, V>(a, c, scale, shift);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float2 st = stat[(c + j) / a.Cg - p.g0];
@@ -254,40 +306,44 @@ __global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(c
             scale[j] *= st.y;
         }
     };
-    const long long row = p.row0 + p.tr, out = p.image * a.o_is + row * a.o_ps + c, step = p.R * a.o_ps;
-    auto finish = [&](const typename P::type &x, int i) {
+    const long long row = p.row0 + p.tr, out = p.image * a.o_is + row * a.o_ps + c, step = p.R * a.o_ps, first = p.image * (long long)a.pixels + row;
+    auto finish = [&](const Mx4Place<V> &place, const typename P::type &x, int i) {
         float v[V];
         P::up(x, v);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = act_of<ACT>(fmaf(v[j] - mean[j], scale[j], shift[j]));
-        if constexpr (MX4) store_mx4<V>(a, (long long)p.image * a.pixels + row + (long long)i * p.R, c, v);
+        if constexpr (MX4) place.store(first + i * p.R, v);
         else P::store(a.out, out + i * step, P::down(v));
     };
     if constexpr (MODE == kWhole) {
         typename P::type x[NV];
         hold<DT, V, NV>(a.x, a.x_is, a.x_ps, p, n, x);
         held_sums<DT, V, NV>(n, x, run, s, q);
-        join_threads(a, p, n, s, q, run, sums, devs, [&](int i, double sum, float m2) {
+        if (n > 0) params<DT, V>(a, c, scale, shift);
+        join_threads(a, p, n, s, q, run, sums, devs, waves, [&](int i, double sum, float m2) {
             stat[i] = finish_stats(a, p, p.g0 + i, sum / ((double)a.pixels * a.Cg), m2, true);
         });
         __syncthreads();
         if (n > 0) {
             constants();
+            const Mx4Place<V> place(a, c);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (i < n) finish(x[i], i);
+                if (i < n) finish(place, x[i], i);
         }
     } else {
+        if (n > 0) params<DT, V>(a, c, scale, shift);
         join_stats(a, p, stat);
         __syncthreads();
         if (n > 0) {
             constants();
+            const Mx4Place<V> place(a, c);
             const Walk<DT, V> in(a.x, a.x_is, a.x_ps, p, n);
             typename P::type x[2][NV];
             walk<NV>(n, p.rows / p.R, [&](int set, int at) { in.ask(at, x[set]); }, [&](int set, int at, auto some) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
-                    if (i < some) finish(x[set][i], at + i);
+                    if (i < some) finish(place, x[set][i], at + i);
             });
         }
     }

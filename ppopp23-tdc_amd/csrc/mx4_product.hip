@@ -262,25 +262,40 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
 // time, with their codes straight in registers: a block of 32 rows by 64 numbers is one request of 1 KiB.  The waves' sums meet
 // in LDS, in the order of the waves.  XS: x in 4 bits (TDC_MX4), or numbers of that type, which a workgroup makes into 4 bits in LDS
 // by itself: for few rows that costs less than a launch.
-// Eight numbers a thread into codes in LDS: block b of row m at (b M + m) 16, its scale byte behind all codes, words of four steps.
+// `rows` rows of x from row m0 on into codes in LDS, eight numbers a thread, four such runs on their way: block b of row m at
+// (b rows + m) 16, its scale byte behind all codes, words of four steps.
 template <int XS>
-static __device__ __forceinline__ void take_numbers(const ProductArgs &a, unsigned char *codes, unsigned char *scales) {
+static __device__ __forceinline__ void take_numbers(const ProductArgs &a, long long m0, int rows, unsigned char *codes, unsigned char *scales) {
     using P = Pack<XS, 8>;
-    const int M = (int)a.M, octets = a.ksteps * 16;
-    for (int i = threadIdx.x; i < M * octets; i += blockDim.x) {
-        const int m = i / octets, o = i - m * octets, n = (int)min(8ll, a.K - (long long)o * 8);
-        float v[8];
-        if (n == 8) P::up(P::load(a.x, m * a.x_stride + o * 8), v);
-        else {
+    const int octets = a.ksteps * 16;
+    for (int at = threadIdx.x; at < rows * octets; at += 4 * blockDim.x) {
+        typename P::type p[4];
+        int row[4], octet[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j < n ? Num<XS>::up(reinterpret_cast<const typename Num<XS>::type *>(a.x)[m * a.x_stride + o * 8 + j]) : 0.0f;
+        for (int k = 0; k < 4; ++k) {
+            const int i = min(at + k * (int)blockDim.x, rows * octets - 1);      // (a repeated one is not stored)
+            row[k] = i / octets;
+            octet[k] = i - row[k] * octets;
+            const long long from = (m0 + row[k]) * a.x_stride;
+            if (octet[k] * 8 + 8 <= a.K) p[k] = P::load(a.x, from + octet[k] * 8);
+            else {
+                p[k] = typename P::type{};
+#pragma unroll
+                for (int j = 0; j < 7; ++j)
+                    if (octet[k] * 8 + j < a.K) p[k][j] = reinterpret_cast<const typename Num<XS>::type *>(a.x)[from + octet[k] * 8 + j];
+            }
         }
-        float top = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = larger(top, v[j]);
-        const int byte = mx4_scale_byte(quad_larger(top)), b = o >> 2;
-        *reinterpret_cast<unsigned *>(codes + (b * M + m) * 16 + (o & 3) * 4) = mx4_codes(v, mx4_divisor(byte));
-        if ((o & 3) == 0) scales[(b >> 4) * M * 16 + m * 16 + (b & 3) * 4 + (b >> 2 & 3)] = (unsigned char)byte;
+        for (int k = 0; k < 4; ++k) {
+            float v[8], top = 0.0f;
+            P::up(p[k], v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = larger(top, v[j]);
+            const int byte = mx4_scale_byte(quad_larger(top)), b = octet[k] >> 2;
+            if (at + k * (int)blockDim.x >= rows * octets) continue;
+            *reinterpret_cast<unsigned *>(codes + (b * rows + row[k]) * 16 + (octet[k] & 3) * 4) = mx4_codes(v, mx4_divisor(byte));
+            if ((octet[k] & 3) == 0) scales[(b >> 4) * rows * 16 + row[k] * 16 + (b & 3) * 4 + (b >> 2 & 3)] = (unsigned char)byte;
+        }
     }
 }
 
@@ -290,7 +305,7 @@ __global__ void __launch_bounds__(1024) tdc_mx4_product_few_kernel(const Product
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), waves = blockDim.x >> 6, r = lane & 31, q = lane >> 5;
     const long long n0 = (long long)(blockIdx.x / (unsigned)blocks_m) * 32, m0 = (long long)(blockIdx.x % (unsigned)blocks_m) * 32;
     const long long x_blocks = (a.M + 31) >> 5, w_blocks = (a.N + 31) >> 5;
-    const int groups = (a.ksteps + 3) / 4, M = (int)min(a.M, 32ll);
+    const int groups = (a.ksteps + 3) / 4, M = (int)min(a.M - m0, 32ll);      // (rows of this workgroup)
     const long long w_row = min(n0 + r, a.N - 1), x_row = min(m0 + r, a.M - 1);
 
     i4_t w[4][2], x[4][2];
@@ -319,7 +334,7 @@ __global__ void __launch_bounds__(1024) tdc_mx4_product_few_kernel(const Product
         // (the scale bytes past a row's last block)
         for (int i = t; i < M * 16; i += blockDim.x) sx_lds[(groups - 1) * M * 16 + i] = 0;
         __syncthreads();
-        take_numbers<XS>(a, x_lds, sx_lds);
+        take_numbers<XS>(a, m0, M, x_lds, sx_lds);
         __syncthreads();
     }
     f16_t acc;
@@ -348,15 +363,17 @@ __global__ void __launch_bounds__(1024) tdc_mx4_product_few_kernel(const Product
     if constexpr (XS != TDC_MX4) __syncthreads();
     float *const part = reinterpret_cast<float *>(lds);
     using T = typename Num<DT>::type;
+    if (wave < groups) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) part[(wave * 16 + e) * 64 + lane] = acc[e];
+        for (int e = 0; e < 16; ++e) part[(wave * 16 + e) * 64 + lane] = acc[e];
+    }
     __syncthreads();
-    const int rows = (int)min(32ll, a.M - m0);
-    for (int o = t; o < 32 * rows; o += blockDim.x) {
+    const int summed = min(waves, groups);      // (the others had none)
+    for (int o = t; o < 32 * M; o += blockDim.x) {
         const int n = o & 31, m = o >> 5, at = ((n >> 3) * 4 + (n & 3)) * 64 + (n >> 2 & 1) * 32 + m;
         if (n0 + n >= a.N) continue;
         float v = 0.0f;
-        for (int k = 0; k < waves; ++k) v += part[k * 1024 + at];
+        for (int k = 0; k < summed; ++k) v += part[k * 1024 + at];
         if (a.bias) v += param<DT>(a.bias, n0 + n, a.bias_dtype);
         if (a.residual) v += Num<DT>::up(reinterpret_cast<const T *>(a.residual)[(m0 + m) * a.r_stride + n0 + n]);
         v = a.act == TDC_ACT_RELU ? act_of<TDC_ACT_RELU>(v) : a.act == TDC_ACT_SILU ? act_of<TDC_ACT_SILU>(v) : v;
@@ -388,9 +405,10 @@ static int launch_tile(const ProductArgs &a, hipStream_t s) {
 }
 template <int DT, int XS>
 static int launch_few(const ProductArgs &a, hipStream_t s) {
-    // A wave for every 512 numbers of K, four to sixteen of them.
-    const int groups = (a.ksteps + 3) / 4, waves = groups <= 4 ? 4 : groups <= 8 ? 8 : 16;
-    const int x_bytes = XS == TDC_MX4 ? 0 : (int)a.M * (a.ksteps * 64 + groups * 16), lds = std::max(waves * 4096, x_bytes);
+    // A wave for every 512 numbers of K, four to sixteen of them; sixteen also to make many numbers into 4 bits.
+    const int groups = (a.ksteps + 3) / 4, rows = (int)std::min(a.M, 32ll);
+    const int waves = groups > 8 || (XS != TDC_MX4 && rows * a.ksteps > 64) ? 16 : groups > 4 ? 8 : 4;
+    const int x_bytes = XS == TDC_MX4 ? 0 : rows * (a.ksteps * 64 + groups * 16), lds = std::max(std::min(waves, groups) * 4096, x_bytes);
     const unsigned bm = (unsigned)((a.M + 31) / 32), bn = (unsigned)((a.N + 31) / 32);
     tdc_mx4_product_few_kernel<DT, XS><<<bm * bn, waves * 64, lds, s>>>(a, (int)bm);
     return (int)hipGetLastError();
@@ -413,8 +431,12 @@ static int launch_product(const ProductArgs &a, hipStream_t s) {
     return launch_tile<DT, 2, 2>(a, s);
 }
 
-// x as it comes, without a launch of its own: eight rows and 64 Ki numbers at most (34 KiB of LDS), as each workgroup repeats the work.
-bool product_takes_numbers(long long M, long long K) { return M <= 8 && M * mx4_padded(K) <= 65536; }
+// x as it comes, without a launch of its own: 64 Ki numbers a workgroup (34 KiB of LDS), as each repeats the work for its rows; eight
+// rows of any number of weights, more where no compute unit does it twice.
+bool product_takes_numbers(long long M, long long N, long long K) {
+    const long long rows = std::min(M, 32ll), workgroups = ((M + 31) / 32) * ((N + 31) / 32);
+    return rows * mx4_padded(K) <= 65536 && (M <= 8 || workgroups <= 256);
+}
 
 int launch_mx4_product(const ProductArgs &a, int y_dtype, void *stream) {
     const hipStream_t s = (hipStream_t)stream;

@@ -39,9 +39,10 @@ NormPlan norm_plan(const tdc_group_norm_desc &d, bool quantised, bool grad) {
     };
     const bool blocks = quantised && d.C % 32 != 0;
     auto fits = [&](int unit) { return !blocks && unit % Cg == 0 && pixels <= (long long)(most / (unit / n.vec)) * 16; };
-    // Whole cache lines where that leaves a workgroup for every compute unit, half ones else: their neighbours come to the same die.
+    // Whole cache lines where that leaves two workgroups for every compute unit, half ones else: their neighbours come to the same
+    // die.
     n.unit = tile(128);
-    n.whole = fits(n.unit) && batch * ((d.C + n.unit - 1) / n.unit) >= 256;
+    n.whole = fits(n.unit) && batch * ((d.C + n.unit - 1) / n.unit) >= 512;
     if (!n.whole && fits(tile(64))) {
         n.unit = tile(64);
         n.whole = true;
@@ -68,7 +69,7 @@ NormPlan norm_plan(const tdc_group_norm_desc &d, bool quantised, bool grad) {
     n.held = n.vec == widest && (n.chunk_rows + n.threads / vecs - 1) / (n.threads / vecs) <= 4 ? 4 : 16;
     n.slots = n.chunks * n.tiles_per_group;
     const int groups = std::min(n.unit, (n.unit - 1) / Cg + 2);
-    n.lds = grad ? 8 * (n.threads * n.vec + groups) : 12 * n.threads * n.places + 8 * groups;
+    n.lds = grad ? 8 * (n.threads * n.vec + groups) : 12 * n.threads * n.places + 8 * groups + 16 * (n.threads / 64);
     return n;
 }
 size_t stat_bytes(const tdc_group_norm_desc &d, const NormPlan &n) { return sizeof(NormStat) * d.batch * d.groups * n.slots; }
@@ -168,7 +169,7 @@ int linear_check(const tdc_mx4_linear_desc *desc, tdc_mx4_linear_desc &d) {
 }
 size_t linear_codes(const tdc_mx4_linear_desc &d) { return (size_t)mx4_code_bytes(d.M, d.K); }
 size_t linear_ws(const tdc_mx4_linear_desc &d) {
-    return d.x_dtype == TDC_MX4 || product_takes_numbers(d.M, d.K) ? 0 : linear_codes(d) + (size_t)(d.M * mx4_scale_bytes(d.K));
+    return d.x_dtype == TDC_MX4 || product_takes_numbers(d.M, d.N, d.K) ? 0 : linear_codes(d) + (size_t)(d.M * mx4_scale_bytes(d.K));
 }
 
 }  // namespace
@@ -328,7 +329,7 @@ int tdc_mx4_linear(const tdc_mx4_linear_desc *desc, const void *x, const void *x
         if (int st = mx4_check("4-bit product", d.M, d.K, x, x_scales)) return st;
         a.x_codes = (const unsigned char *)x;
         a.x_scales = (const unsigned char *)x_scales;
-    } else if (product_takes_numbers(d.M, d.K)) {
+    } else if (product_takes_numbers(d.M, d.N, d.K)) {
         a.x = x;
         a.x_dtype = d.x_dtype;
         a.x_stride = d.x_stride;

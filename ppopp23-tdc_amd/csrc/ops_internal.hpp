@@ -83,7 +83,7 @@ struct ProductArgs {
     int ksteps;                     // padded K / 128
     int bias_dtype, act;
 };
-bool product_takes_numbers(long long M, long long K);
+bool product_takes_numbers(long long M, long long N, long long K);
 int launch_mx4_product(const ProductArgs &a, int y_dtype, void *stream);
 
 }  // namespace tdc
