@@ -21,41 +21,44 @@ static __device__ __forceinline__ f16_t mfma4(i4_t a, i4_t b, f16_t c, int sa, i
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wa, wb, c, 4, 4, 0, sa, 0, sb);
 }
 
-// Eight neighbouring outputs of a row (those before N): sums with the bias in `v`; residual, activation, store.
-template <int DT, int ACT>
-static __device__ __forceinline__ void finish8(const ProductArgs &a, long long m, long long n, float (&v)[8]) {
+// Eight neighbouring numbers of a row as one request.
+template <int DT>
+struct Eight {
     using T = typename Num<DT>::type;
-    typedef T vec_t __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-    T *const to = reinterpret_cast<T *>(a.y) + m * a.y_stride + n;
-    const int count = (int)min(8ll, a.N - n);
-    if (a.residual) {
-        const T *const add = reinterpret_cast<const T *>(a.residual) + m * a.r_stride + n;
-        vec_t r = {};
-        if (count == 8) r = *reinterpret_cast<const vec_t *>(add);
+    typedef T vec_t __attribute__((ext_vector_type(8)));
+    typedef T mem_t __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
+// The residual of eight neighbouring outputs of a row: zeros where there is none (rows from M on, outputs from N on).
+template <int DT>
+static __device__ __forceinline__ typename Eight<DT>::vec_t residual8(const ProductArgs &a, long long m, long long n) {
+    using T = typename Num<DT>::type;
+    typename Eight<DT>::vec_t r = {};
+    if (a.residual && m < a.M) {
+        const T *const from = reinterpret_cast<const T *>(a.residual) + m * a.r_stride + n;
+        if (n + 8 <= a.N) r = *reinterpret_cast<const typename Eight<DT>::mem_t *>(from);
         else {
 #pragma unroll
             for (int i = 0; i < 7; ++i)
-                if (i < count) r[i] = add[i];
+                if (n + i < a.N) r[i] = from[i];
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += Num<DT>::up(r[i]);
     }
-    vec_t out;
+    return r;
+}
+// Eight neighbouring outputs of a row (those before N): residual on sums with the bias, activation, store.
+template <int DT, int ACT>
+static __device__ __forceinline__ void finish8(const ProductArgs &a, long long m, long long n, const float (&v)[8], typename Eight<DT>::vec_t r) {
+    using T = typename Num<DT>::type;
+    T *const to = reinterpret_cast<T *>(a.y) + m * a.y_stride + n;
+    typename Eight<DT>::vec_t out;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = Num<DT>::down(act_of<ACT>(v[i]));
-    if (count == 8) *reinterpret_cast<vec_t *>(to) = out;
+    for (int i = 0; i < 8; ++i) out[i] = Num<DT>::down(act_of<ACT>(v[i] + Num<DT>::up(r[i])));
+    if (n + 8 <= a.N) *reinterpret_cast<typename Eight<DT>::mem_t *>(to) = out;
     else {
 #pragma unroll
         for (int i = 0; i < 7; ++i)
-            if (i < count) to[i] = out[i];
+            if (n + i < a.N) to[i] = out[i];
     }
 }
-template <int DT>
-static __device__ __forceinline__ void bias8(const ProductArgs &a, long long n, float (&bias)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bias[i] = a.bias && n + i < a.N ? param<DT>(a.bias, n + i, a.bias_dtype) : 0.0f;
-}
-
 // ---- tiles ----
 //
 // A workgroup of four waves owns 64 MB rows of x and 64 NB of w, a wave a quarter of it: MB x NB blocks of 32 x 32.  A step is
@@ -73,11 +76,67 @@ struct Tile {
     static constexpr int M = 64 * MB, N = 64 * NB;
     static constexpr int kBuffer = (M + N) * 64;              // bytes of a step's codes: x, then w
     static constexpr int kScales = (M + N) * 16;              // bytes of four steps' scales
-    static constexpr int kLds = 4 * kBuffer + 2 * kScales;
+    static constexpr int kLds = 4 * kBuffer + 2 * kScales + N * 4;     // (and the bias)
     static constexpr int kX = MB, kChunks = MB + NB;          // requests of a wave and step: of x, in all
     static constexpr int kScaleRequests = (M + N) / 256;      // of a wave and four steps
     static constexpr int kParts = NB / 2;
 };
+
+// Which tile a workgroup has, if any: neighbouring workgroups of a die take tiles of eight rows by as many columns as run at once, which
+// share operands in its L2.
+template <int MB, int NB>
+static __device__ __forceinline__ bool tile_of(int tiles_m, int tiles_n, long long &m0, long long &n0) {
+    const int total = tiles_m * tiles_n, per_die = (total + 7) / 8;
+    const int id = (blockIdx.x & 7) * per_die + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per_die || id >= total) return false;
+    const int group = id / (8 * tiles_n), rest = id - group * 8 * tiles_n, high = min(8, tiles_m - group * 8);
+    m0 = (long long)(group * 8 + rest % high) * Tile<MB, NB>::M;
+    n0 = (long long)(rest / high) * Tile<MB, NB>::N;
+    return true;
+}
+template <int DT>
+static __device__ __forceinline__ float bias_of(const ProductArgs &a, long long n, bool wanted) {
+    return wanted && a.bias && n < a.N ? param<DT>(a.bias, n, a.bias_dtype) : 0.0f;
+}
+
+// A wave's outputs from row m on and from column n on, their bias in LDS.  Of a block a lane has row r of x, and of w 16 u + 8 q ..
+// 16 u + 8 q + 7, u = 0, 1.  The residuals of the next eight columns are on their way while these are finished; the first are
+// handed over.
+template <int DT, int MB, int NB>
+static __device__ __forceinline__ void finish_tile(const ProductArgs &a, const f16_t (&acc)[NB][MB], long long m, long long n, const float *bias,
+                                                   const typename Eight<DT>::vec_t (&first)[MB]) {
+    const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5;
+    auto row = [&](int i) { return m + i * 32 + r; };
+    auto column = [&](int k) { return k / 2 * 32 + k % 2 * 16 + q * 8; };
+    typename Eight<DT>::vec_t res[2][MB];
+    auto finish = [&](auto act) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i) res[0][i] = first[i];
+#pragma unroll
+        for (int k = 0; k < 2 * NB; ++k) {
+            const int c = column(k);
+            if (k + 1 < 2 * NB) {
+#pragma unroll
+                for (int i = 0; i < MB; ++i) res[(k + 1) & 1][i] = residual8<DT>(a, row(i), n + column(k + 1));
+            }
+            if (n + c < a.N) {
+                const float4 lo = *reinterpret_cast<const float4 *>(bias + c), hi = *reinterpret_cast<const float4 *>(bias + c + 4);
+                const float add[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                for (int i = 0; i < MB; ++i) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = acc[k / 2][i][8 * (k % 2) + e] + add[e];
+                    if (row(i) < a.M) finish8<DT, decltype(act)::value>(a, row(i), n + c, v, res[k & 1][i]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);      // (or all residuals are requested first, and spill)
+        }
+    };
+    if (a.act == TDC_ACT_RELU) finish(std::integral_constant<int, TDC_ACT_RELU>{});
+    else if (a.act == TDC_ACT_SILU) finish(std::integral_constant<int, TDC_ACT_SILU>{});
+    else finish(std::integral_constant<int, TDC_ACT_NONE>{});
+}
 
 template <int DT, int MB, int NB>
 __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile_kernel(const ProductArgs a, int tiles_m, int tiles_n) {
@@ -86,12 +145,9 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 31, q = lane >> 5;
     const int wm = wave & 1, wn = wave >> 1;
 
-    // Neighbouring workgroups of a die take tiles of eight rows by as many columns as run at once: they share operands in its L2.
-    const int total = tiles_m * tiles_n, per_die = (total + 7) / 8;
-    const int id = (blockIdx.x & 7) * per_die + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per_die || id >= total) return;
-    const int group = id / (8 * tiles_n), rest = id - group * 8 * tiles_n, high = min(8, tiles_m - group * 8);
-    const long long m0 = (long long)(group * 8 + rest % high) * L::M, n0 = (long long)(rest / high) * L::N;
+    long long m0, n0;
+    if (!tile_of<MB, NB>(tiles_m, tiles_n, m0, n0)) return;
+    const float b = bias_of<DT>(a, n0 + t, t < L::N);
 
     // Requests straight into LDS: 16 bytes a lane, in the order of the lanes, at a wave's own place.
     auto bring = [&](const unsigned char *base, int offset, unsigned char *to) {
@@ -164,11 +220,13 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
 
     // (an odd number of steps is rounded up: the scales past the last are zero, and so is what that step adds)
     const int steps = (a.ksteps + 1) / 2 * 2;
+    float *const bias = reinterpret_cast<float *>(lds_scales + 2 * L::kScales);
     fetch_scales(0);
 #pragma unroll
     for (int s = 0; s < 3; ++s)
 #pragma unroll
         for (int i = 0; i < L::kChunks; ++i) fetch(i, s);
+    if (t < L::N) bias[t] = b;
     meet(Codes{});
     i4_t x[2][MB][2], w[2][2][2];
     int sx[MB][2], sw[NB][2];
@@ -229,31 +287,10 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
     }
     meet(None{});       // (nothing may still be on its way into LDS when the workgroup ends)
 
-    // A lane's outputs of a block: row r of x, and of w 16 u + 8 q .. 16 u + 8 q + 7, u = 0, 1.
-    auto finish = [&](auto act) {
+    typename Eight<DT>::vec_t first[MB];
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const long long n = n0 + wn * 32 * NB + j * 32 + u * 16 + q * 8;
-                if (n >= a.N) continue;
-                float bias[8];
-                bias8<DT>(a, n, bias);
-#pragma unroll
-                for (int i = 0; i < MB; ++i) {
-                    const long long m = m0 + wm * 32 * MB + i * 32 + r;
-                    if (m >= a.M) continue;
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = acc[j][i][8 * u + e] + bias[e];
-                    finish8<DT, decltype(act)::value>(a, m, n, v);
-                    __builtin_amdgcn_sched_barrier(0);      // (or the rows' residuals are all requested first, and spill)
-                }
-            }
-    };
-    if (a.act == TDC_ACT_RELU) finish(std::integral_constant<int, TDC_ACT_RELU>{});
-    else if (a.act == TDC_ACT_SILU) finish(std::integral_constant<int, TDC_ACT_SILU>{});
-    else finish(std::integral_constant<int, TDC_ACT_NONE>{});
+    for (int i = 0; i < MB; ++i) first[i] = residual8<DT>(a, m0 + wm * 32 * MB + i * 32 + r, n0 + wn * 32 * NB + q * 8);
+    finish_tile<DT, MB, NB>(a, acc, m0 + wm * 32 * MB, n0 + wn * 32 * NB, bias + wn * 32 * NB, first);
 }
 
 // ---- few outputs ----
@@ -415,8 +452,8 @@ static int launch_few(const ProductArgs &a, hipStream_t s) {
 }
 
 // Timed in turn over M 16 .. 25088, N 64 .. 8192, K 128 .. 8192 (us):
-//   32 x 32 outputs a workgroup while there are 256 of them, or 512 of long sums: 512 x 512 x 2048 5.5 against 9.7 in tiles of 128,
-//   1024 x 512 x 2048 7.5 against 9.7, but 1024 x 512 x 512 6.7 against 6.6 and 1024 x 1024 x 2048 11.9 against 9.9;
+//   32 x 32 outputs a workgroup while there are 512 of them, or 1024 of short sums: 1024 x 512 x 2048 7.5 against 9.2 in tiles of 128,
+//   1024 x 1024 x 512 5.2 against 6.2, but 1024 x 1024 x 1024 7.6 against 7.3 and 4096 x 512 x 512 8.9 against 6.6;
 //   tiles of 256 for long sums that fill the compute units: 4096 x 8192 x 8192 155 against 171, 25088 x 512 x 8192 65 against 80, but
 //   8192 x 8192 x 2048 122 against 110 (a tile's first loads and its stores run alone) and 1024 x 8192 x 8192 60 against 44.
 template <int DT>
@@ -426,7 +463,7 @@ static int launch_product(const ProductArgs &a, hipStream_t s) {
         return a.x_dtype == TDC_F16 ? launch_few<DT, TDC_F16>(a, s) : launch_few<DT, TDC_BF16>(a, s);
     }
     auto tiles = [&](long long edge) { return ((a.M + edge - 1) / edge) * ((a.N + edge - 1) / edge); };
-    if (tiles(32) <= (a.ksteps >= 8 ? 512 : 256)) return launch_few<DT, TDC_MX4>(a, s);
+    if (tiles(32) <= (a.ksteps <= 4 ? 1024 : 512)) return launch_few<DT, TDC_MX4>(a, s);
     if (a.ksteps >= 32 && tiles(256) >= 192) return launch_tile<DT, 4, 4>(a, s);
     return launch_tile<DT, 2, 2>(a, s);
 }
