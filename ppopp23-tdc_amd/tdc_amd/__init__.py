@@ -4,7 +4,8 @@ from ._lib import (LIB_PATH, ConvDesc, TdcError, Tile, TileInfo, conv_desc, lib,
 
 __all__ = ["LIB_PATH", "ConvDesc", "TdcError", "Tile", "TileInfo", "conv_desc", "lib", "model_enumerate",
            "model_evaluate", "model_select", "set_autotune", "Conv2dPlan", "TKConvOp", "TKConv2dC", "ranks_dict", "partial_tucker2",
-           "group_norm_act", "group_norm_act_mx4", "mx4_quantize", "mx4_linear", "mx4_conv1x1", "Mx4Tensor"]
+           "group_norm_act", "group_norm_act_mx4", "mx4_quantize", "mx4_linear", "mx4_conv1x1", "Mx4Tensor",
+           "GroupNormAct", "TuckerBlockMx4"]
 
 
 def __getattr__(name):
@@ -15,6 +16,8 @@ def __getattr__(name):
         from . import TKConv as module
     elif name in ("group_norm_act", "group_norm_act_mx4", "mx4_quantize", "mx4_linear", "mx4_conv1x1", "Mx4Tensor"):
         from . import channels_last as module
+    elif name in ("GroupNormAct", "TuckerBlockMx4"):
+        from . import mx4_block as module
     else:
         raise AttributeError(name)
     globals()[name] = value = getattr(module, name)

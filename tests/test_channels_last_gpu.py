@@ -458,3 +458,55 @@ def test_offsets_beyond_32_bits():
     wq = tdc_amd.mx4_quantize(torch.eye(32, device="cuda"))
     got = tdc_amd.mx4_linear(flat, wq)
     assert np.array_equal(got.double().cpu().numpy(), ref.mx4(flat.double().cpu().numpy())[2])
+
+
+# ---- together ----
+
+def test_tucker_block_in_4_bits():
+    """The block is its operators one after the other, and near the same block in 32 bits: each of its two products is off by what
+    rounding both operands to 4 bits costs (some 0.1 an operand), which the residual does not share."""
+    torch.manual_seed(3)
+    conv = tdc_amd.TKConv2dC(96, 96, 3, padding=1, hp_dict=tdc_amd.ranks_dict(conv=[40, 32]), name="conv")
+    block = tdc_amd.TuckerBlockMx4(conv, groups=8, rank_groups=5).cuda()
+    with torch.no_grad():
+        block.norm_in.weight.add_(torch.randn(96, device="cuda") * 0.2)
+        block.norm_core.bias.add_(torch.randn(40, device="cuda") * 0.2)
+    x = torch.randn(3, 14, 13, 96, generator=seeded(5)).bfloat16().cuda().permute(0, 3, 1, 2)
+    first0, core0, last0 = (p.detach().clone() for p in (conv.first_kernel, conv.core_kernel, conv.last_kernel))
+    y = block(x)
+    assert y.shape == x.shape and y.dtype == x.dtype and y.is_contiguous(memory_format=torch.channels_last)
+    n, m = block.norm_in, block.norm_core
+    h = tdc_amd.mx4_conv1x1(tdc_amd.group_norm_act_mx4(x, 8, n.weight, n.bias, act="silu"), tdc_amd.mx4_quantize(conv.first_kernel.detach().flatten(1)),
+                            out_dtype=F32)
+    plan = tdc_amd.Conv2dPlan(3, 32, 40, 14, 13, 3, 3, 1, 1).set_weights(conv.core_kernel)
+    h = plan.forward(h.contiguous()).contiguous(memory_format=torch.channels_last)
+    want = tdc_amd.mx4_conv1x1(tdc_amd.group_norm_act_mx4(h, 5, m.weight, m.bias, act="silu"), tdc_amd.mx4_quantize(conv.last_kernel.detach().flatten(1)),
+                               conv.bias.detach(), x, out_dtype=BF16)
+    plan.close()
+    assert torch.equal(y, want) and torch.equal(y, block(x))
+    with torch.no_grad():
+        conv.last_kernel.zero_()
+    assert torch.equal(block(x), (x.float() + conv.bias.view(1, -1, 1, 1)).to(BF16))     # 0 for the product, after the change
+    conv.load_kernels(first0, core0, last0)
+    assert torch.equal(y, block(x))
+    plain = block.plain(x)
+    assert torch.linalg.norm(y.float() - plain) < 0.4 * torch.linalg.norm(plain - x.float())
+    with pytest.raises(ValueError, match="keep its input's size"):
+        tdc_amd.TuckerBlockMx4(tdc_amd.TKConv2dC(8, 8, 3, hp_dict=tdc_amd.ranks_dict(conv=[4, 4]), name="conv"))
+
+
+def test_norm_module_trains():
+    """A few steps of gradient descent through the module: the loss falls as it does in 64 bits on the host, step by step."""
+    g = seeded(9)
+    x, target = torch.randn(4, 24, 6, 6, generator=g), torch.randn(4, 24, 6, 6, generator=g)
+    norm = tdc_amd.GroupNormAct(6, 24, act="silu").cuda()
+    w, b = torch.ones(24, dtype=torch.float64, requires_grad=True), torch.zeros(24, dtype=torch.float64, requires_grad=True)
+    xd = x.cuda().contiguous(memory_format=torch.channels_last)
+    for step in range(5):
+        loss = ((norm(xd) - target.cuda()) ** 2).mean()
+        plain = ((torch.nn.functional.silu(torch.nn.functional.group_norm(x.double(), 6, w, b)) - target.double()) ** 2).mean()
+        assert abs(loss.item() - plain.item()) < 1e-5 * plain.item(), step
+        grads, want = torch.autograd.grad(loss, (norm.weight, norm.bias)), torch.autograd.grad(plain, (w, b))
+        with torch.no_grad():
+            for p, d in ((norm.weight, grads[0]), (norm.bias, grads[1]), (w, want[0]), (b, want[1])):
+                p -= 20 * d
