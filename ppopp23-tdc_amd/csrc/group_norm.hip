@@ -54,8 +54,8 @@ static __device__ __forceinline__ PartSum sum_places(const Part &p, const double
                                                      int run, int at, int step, int lanes) {
     // (a thread row has one pixel more or less: reciprocals of both counts; places by multiplication, exact for so few)
     const int most = rows_of(p, 0), longer = p.rows - (most - 1) * p.R;
-    const float per = 1.0f / mine;
-    const double inv_most = 1.0 / (most * run), inv_less = most > 1 ? 1.0 / ((most - 1) * run) : 0.0;
+    const float per = __builtin_amdgcn_rcpf((float)mine);
+    const double inv_most = inverse(most * run), inv_less = most > 1 ? inverse((most - 1) * run) : 0.0;
     PartSum r{0.0, 0.0f, 0};
     for (int e = at; e < mine * used; e += step) {
         const int row = (int)((e + 0.5f) * per);
@@ -64,7 +64,7 @@ static __device__ __forceinline__ PartSum sum_places(const Part &p, const double
     }
     r.sum = team_sum(r.sum, lanes);
     r.count = team_sum(r.count, lanes);
-    const double mean = r.sum / max(r.count, 1);
+    const double mean = r.sum * inverse(max(r.count, 1));
     for (int e = at; e < mine * used; e += step) {
         const int row = (int)((e + 0.5f) * per), i = row * places + lo + e - row * mine;
         const bool full = row < longer;
@@ -81,22 +81,22 @@ static __device__ __forceinline__ PartSum sum_places(const Part &p, const double
 template <int V, typename Done>
 static __device__ __forceinline__ void join_threads(const NormArgs &a, const Part &p, int n, const double (&s)[V], const float (&q)[V], int run,
                                                     double *sums, float *devs, PartSum *waves, Done done) {
-    const int places = p.vecs * (V / run);      // of a thread row
+    const int places = p.vecs * a.plan.places;      // of a thread row
     if (n > 0) {
-        const int at = p.tr * places + p.tc * (V / run);
+        const int at = p.tr * places + p.tc * a.plan.places;
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (j % run == 0) {
-                sums[at + j / run] = s[j];
-                devs[at + j / run] = q[j];
+            if ((j & (run - 1)) == 0) {
+                sums[at + (j >> a.plan.run_shift)] = s[j];
+                devs[at + (j >> a.plan.run_shift)] = q[j];
             }
     }
     __syncthreads();
     const int used = min(p.R, p.rows), all = a.plan.threads >> 6, wave = threadIdx.x >> 6;
-    auto first = [&](int i) { return (max((p.g0 + i) * a.Cg, p.c0) - p.c0) / run; };
-    auto mine = [&](int i) { return shared_channels(a, p.g0 + i, p.tile) / run; };
+    auto first = [&](int i) { return (max((p.g0 + i) * a.Cg, p.c0) - p.c0) >> a.plan.run_shift; };
+    auto mine = [&](int i) { return shared_channels(a, p.g0 + i, p.tile) >> a.plan.run_shift; };
     if (p.ng < all) {
-        const int share = all / p.ng, i = wave / share, k = wave - i * share;
+        const int share = small_quotient(all, p.ng), i = small_quotient(wave, share), k = wave - i * share;
         if (i < p.ng) {
             const PartSum r = sum_places(p, sums, devs, places, first(i), mine(i), used, run, k * 64 + (threadIdx.x & 63), share * 64, 64);
             if ((threadIdx.x & 63) == 0) waves[wave] = r;
@@ -110,10 +110,10 @@ static __device__ __forceinline__ void join_threads(const NormArgs &a, const Par
                 sum += w[k].sum;
                 count += w[k].count;
             }
-            const double mean = sum / count;
+            const double mean = sum * inverse(count);
             float m2 = 0.0f;
             for (int k = 0; k < share; ++k) {
-                const float d = (float)(w[k].sum / max(w[k].count, 1) - mean);
+                const float d = (float)(w[k].sum * inverse(max(w[k].count, 1)) - mean);
                 m2 += w[k].m2 + w[k].count * d * d;
             }
             done(threadIdx.x, sum, m2);
@@ -147,7 +147,7 @@ static __device__ __forceinline__ void held_sums(int n, typename Pack<DT, V>::ty
     join_run(s, run);
     pack_again(x);
     float mean[V];
-    const double inv = 1.0 / ((double)max(n, 1) * run);
+    const double inv = inverse(max(n, 1) * run);
 #pragma unroll
     for (int j = 0; j < V; ++j) mean[j] = (float)(s[j] * inv);
 #pragma unroll
@@ -176,7 +176,7 @@ static __device__ __forceinline__ void passing_sums(const NormArgs &a, const Par
         q[j] = 0.0f;
     }
     typename P::type x[2][NV];
-    walk<NV>(n, p.rows / p.R, [&](int set, int at) { in.ask(at, x[set]); }, [&](int set, int, auto some) {
+    walk<NV>(n, quotient(p.rows, p.by_R), [&](int set, int at) { in.ask(at, x[set]); }, [&](int set, int, auto some) {
         float four[V];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -191,13 +191,13 @@ static __device__ __forceinline__ void passing_sums(const NormArgs &a, const Par
             }
     });
     double own[V];
-    const double inv = 1.0 / n;
+    const double inv = inverse(n);
 #pragma unroll
     for (int j = 0; j < V; ++j) own[j] = s[j] * inv;
     join_run(s, run);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float d = (float)(own[j] - first[j]), e = (float)(own[j] - s[j] * inv / run);
+        const float d = (float)(own[j] - first[j]), e = (float)(own[j] - s[j] * (inv * (1.0 / V) * a.plan.places));
         q[j] = fmaxf(q[j] - n * d * d, 0.0f) + n * e * e;
     }
     join_run(q, run);
@@ -205,7 +205,7 @@ static __device__ __forceinline__ void passing_sums(const NormArgs &a, const Par
 
 // One group's (mean, rstd); the first workgroup that has it keeps them for the caller.
 static __device__ __forceinline__ float2 finish_stats(const NormArgs &a, const Part &p, int g, double mean, float m2, bool keep) {
-    const float2 st = make_float2((float)mean, 1.0f / sqrtf(m2 / ((float)a.pixels * a.Cg) + a.eps));
+    const float2 st = make_float2((float)mean, 1.0f / sqrtf(m2 * (float)a.per_number + a.eps));
     if (keep) {
         if (a.mean) a.mean[(long long)p.image * a.groups + g] = st.x;
         if (a.rstd) a.rstd[(long long)p.image * a.groups + g] = st.y;
@@ -217,12 +217,12 @@ static __device__ __forceinline__ void join_stats(const NormArgs &a, const Part 
     const Team t = team_of(a.plan.threads, p.ng);
     const NormPlan &n = a.plan;
     for (int i = t.first; i < p.ng; i += t.step) {
-        const int g = p.g0 + i, tile0 = g * a.Cg / n.unit, tiles = ((g + 1) * a.Cg - 1) / n.unit - tile0 + 1;
+        const int g = p.g0 + i, tile0 = tiles_of(a, p, g).x, tiles = tiles_of(a, p, g).y;
         const NormStat *part = a.stat + ((long long)p.image * a.groups + g) * n.slots;
         double sum = 0.0;
         for (int k = 0; k < tiles; ++k)
             for (int c = t.at; c < n.chunks; c += t.lanes) sum += part[c * n.tiles_per_group + k].sum;
-        const double mean = team_sum(sum, t.lanes) / ((double)a.pixels * a.Cg);
+        const double mean = team_sum(sum, t.lanes) * a.per_number;
         float m2 = 0.0f;
         for (int k = 0; k < tiles; ++k) {
             const int channels = shared_channels(a, g, tile0 + k);
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(c
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const Part p = part_of(a, V, blockIdx.x, gridDim.x);
     const int n = rows_of(p, p.tr);
-    const int run = V / a.plan.places, most = a.plan.threads * a.plan.places;
+    const int run = 1 << a.plan.run_shift, most = a.plan.threads * a.plan.places;
     double *const sums = reinterpret_cast<double *>(lds);
     float *const devs = reinterpret_cast<float *>(sums + most);
     PartSum *const waves = reinterpret_cast<PartSum *>(devs + most);
@@ -299,9 +299,11 @@ __global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(c
     const int c = p.c0 + p.tc * V;
     float mean[V], scale[V], shift[V];
     auto constants = [&]() {
+        int g[V];
+        groups_of(a, c, g);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float2 st = stat[(c + j) / a.Cg - p.g0];
+            const float2 st = stat[g[j] - p.g0];
             mean[j] = st.x;
             scale[j] *= st.y;
         }
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(c
         held_sums<DT, V, NV>(n, x, run, s, q);
         if (n > 0) params<DT, V>(a, c, scale, shift);
         join_threads(a, p, n, s, q, run, sums, devs, waves, [&](int i, double sum, float m2) {
-            stat[i] = finish_stats(a, p, p.g0 + i, sum / ((double)a.pixels * a.Cg), m2, true);
+            stat[i] = finish_stats(a, p, p.g0 + i, sum * a.per_number, m2, true);
         });
         __syncthreads();
         if (n > 0) {
@@ -338,12 +340,12 @@ __global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(c
         if (n > 0) {
             constants();
             const Mx4Place<V> place(a, c);
-            const Walk<DT, V> in(a.x, a.x_is, a.x_ps, p, n);
+            const Walk<DT, V> in(a.x, a.x_is, a.x_ps, p, n, true);
             typename P::type x[2][NV];
-            walk<NV>(n, p.rows / p.R, [&](int set, int at) { in.ask(at, x[set]); }, [&](int set, int at, auto some) {
+            walk<NV>(n, quotient(p.rows, p.by_R), [&](int set, int at) { in.ask(at, x[set]); }, [&](int set, int at, auto some) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
-                    if (i < some) finish(place, x[set][i], at + i);
+                    if (i < some) finish(place, x[set][i], n - 1 - at - i);
             });
         }
     }
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(256) tdc_norm_blocks_kernel(const NormArgs a) 
         for (int j = 0; j < 32; ++j) {
             v[j] = 0.0f;
             if (j < n) {
-                const float2 st = stat[(c + j) / a.Cg - p.g0];
+                const float2 st = stat[quotient(c + j, a.plan.by_group) - p.g0];
                 const float gamma = a.gamma ? param<DT>(a.gamma, c + j, a.param_dtype) : 1.0f;
                 const float beta = a.beta ? param<DT>(a.beta, c + j, a.param_dtype) : 0.0f;
                 v[j] = act_of<ACT>(fmaf(Num<DT>::up(in[j]) - st.x, st.y * gamma, beta));

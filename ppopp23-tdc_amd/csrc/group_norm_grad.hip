@@ -71,13 +71,15 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
         hold<DT, V, NV>(a.dy, a.d_is, a.d_ps, p, n, dy[0]);
     }
     float mean[V], rstd[V], gamma[V], beta[V];
+    int g[V];
+    groups_of(a, c, g);
     if (n > 0) {
         params<DT, V>(a, c, gamma, beta);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const long long g = (long long)p.image * a.groups + (c + j) / a.Cg;
-            mean[j] = a.mean[g];
-            rstd[j] = a.rstd[g];
+            const long long at = (long long)p.image * a.groups + g[j];
+            mean[j] = a.mean[at];
+            rstd[j] = a.rstd[at];
         }
     }
     // All pixels of this thread, which has some.
@@ -87,19 +89,20 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
             for (int i = 0; i < NV; ++i)
                 if (i < n) use(0, i, i);
         } else {
-            const Walk<DT, V> in(a.x, a.x_is, a.x_ps, p, n), din(a.dy, a.d_is, a.d_ps, p, n);
-            walk<NV>(n, p.rows / p.R, [&](int set, int at) {
+            constexpr bool back = MODE == kApply;
+            const Walk<DT, V> in(a.x, a.x_is, a.x_ps, p, n, back), din(a.dy, a.d_is, a.d_ps, p, n, back);
+            walk<NV>(n, quotient(p.rows, p.by_R), [&](int set, int at) {
                 in.ask(at, x[set]);
                 din.ask(at, dy[set]);
             }, [&](int set, int at, auto some) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
-                    if (i < some) use(set, i, at + i);
+                    if (i < some) use(set, i, back ? n - 1 - at - i : at + i);
             });
         }
     };
     float2 *const cell = reinterpret_cast<float2 *>(lds), *const stat = cell + (MODE == kApply ? 0 : a.plan.threads * V);
-    const float inv = 1.0f / ((float)a.pixels * a.Cg);
+    const float inv = (float)a.per_number;
     const Team t = team_of(a.plan.threads, p.ng);
     if constexpr (MODE != kApply) {
         if (n > 0) {
@@ -152,7 +155,7 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
     } else {
         const NormPlan &m = a.plan;
         for (int i = t.first; i < p.ng; i += t.step) {
-            const int g = p.g0 + i, tiles = ((g + 1) * a.Cg - 1) / m.unit - g * a.Cg / m.unit + 1;
+            const int g = p.g0 + i, tiles = tiles_of(a, p, g).y;
             const float2 *part = a.part + ((long long)p.image * a.groups + g) * m.slots;
             float s = 0.0f, u = 0.0f;
             for (int k = 0; k < tiles; ++k)
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
     float s1[V], s2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float2 st = stat[(c + j) / a.Cg - p.g0];
+        const float2 st = stat[g[j] - p.g0];
         s1[j] = st.x;
         s2[j] = st.y;
     }

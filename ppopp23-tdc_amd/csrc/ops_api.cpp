@@ -21,6 +21,8 @@ bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (unsigned)(bytes
 
 // `quantised`: tiles end at multiples of 32 channels, the blocks of the result, which is written in one launch only where rows end
 // there too.  `grad`: x and dy are held side by side.
+Divisor divisor(long long by) { return {(unsigned)by, by == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / by)}; }
+
 NormPlan norm_plan(const tdc_group_norm_desc &d, bool quantised, bool grad) {
     NormPlan n{};
     const int Cg = d.C / d.groups, size = dtype_bytes(d.dtype), widest = 16 / size;
@@ -53,21 +55,29 @@ NormPlan norm_plan(const tdc_group_norm_desc &d, bool quantised, bool grad) {
     const long long dealt = n.tiles * batch;
     n.threads = most;
     if (n.whole) {
-        // Few workgroups: many threads with few requests each.  Many: few threads, so that several workgroups share a compute unit.
-        const int held = dealt >= 512 ? 16 : 4;
-        while (n.threads > 64 && n.threads / 2 >= vecs && (long long)(n.threads / 2 / vecs) * held >= pixels) n.threads /= 2;
+        // Few workgroups: many threads with few requests each.  Many: few threads, so that several workgroups share a compute unit,
+        // but two waves for each of its vector units (32 x 14 x 14 x 1024 in 16 bits: 13.5 us, 16.5 with one; 32 x 28 x 28 x 512: 19.2, 20.6
+        // with four, 26.5 with eight).
+        const bool many = dealt >= 512;
+        while (n.threads > 64 && n.threads / 2 >= vecs && (long long)(n.threads / 2 / vecs) * (many ? 16 : 4) >= pixels &&
+               (!many || dealt * n.threads >= 512 * 512)) n.threads /= 2;
         n.chunk_rows = (int)pixels;
     } else {
-        // Workgroups of 256: four to a compute unit, which all kernels have the registers for, as long as each thread has four
-        // pixels to move.
+        // Workgroups of 256: two to a compute unit, as long as each thread has four pixels to move.
         n.threads = std::min(most, 256);
         const int rows = n.threads / vecs;
-        const long long want = std::max(1ll, 1024 / dealt);
+        const long long want = std::max(1ll, 512 / dealt);
         n.chunk_rows = (int)std::min(round_up(pixels, rows), round_up(std::max(4ll * rows, (pixels + want - 1) / want), rows));
     }
     n.chunks = (int)((pixels + n.chunk_rows - 1) / n.chunk_rows);
     n.held = n.vec == widest && (n.chunk_rows + n.threads / vecs - 1) / (n.threads / vecs) <= 4 ? 4 : 16;
     n.slots = n.chunks * n.tiles_per_group;
+    n.run_shift = __builtin_ctz(n.vec / n.places);
+    n.by_tiles = divisor(n.tiles);
+    n.by_chunks = divisor(n.chunks);
+    n.by_group = divisor(Cg);
+    n.by_rows[0] = divisor(n.threads / vecs);
+    n.by_rows[1] = divisor(n.threads / ((d.C - (n.tiles - 1) * n.unit) / n.vec));
     const int groups = std::min(n.unit, (n.unit - 1) / Cg + 2);
     n.lds = grad ? 8 * (n.threads * n.vec + groups) : 12 * n.threads * n.places + 8 * groups + 16 * (n.threads / 64);
     return n;
@@ -220,6 +230,7 @@ int tdc_group_norm_forward(const tdc_group_norm_desc *desc, const void *x, const
     a.rstd = rstd;
     a.stat = (NormStat *)ws;
     a.plan = plan;
+    a.per_number = 1.0 / ((double)std::max<long long>(d.pixels, 1) * (d.C / d.groups));
     return launched("group norm", launch_norm_forward(a, d.dtype, stream));
 }
 TDC_ENTRY_END
@@ -238,6 +249,7 @@ int tdc_group_norm_forward_mx4(const tdc_group_norm_desc *desc, const void *x, c
     a.scales = (unsigned char *)scales;
     a.stat = (NormStat *)ws;
     a.plan = plan;
+    a.per_number = 1.0 / ((double)std::max<long long>(d.pixels, 1) * (d.C / d.groups));
     return launched("group norm", launch_norm_forward(a, d.dtype, stream));
 }
 TDC_ENTRY_END
@@ -271,6 +283,7 @@ int tdc_group_norm_backward(const tdc_group_norm_desc *desc, const void *x, cons
     a.dgamma = dgamma;
     a.dbeta = dbeta;
     a.plan = plan;
+    a.per_number = 1.0 / ((double)std::max<long long>(d.pixels, 1) * (d.C / d.groups));
     a.part = (float2 *)ws;
     a.chan = (float *)((char *)ws + part_bytes(d, a.plan));
     return launched("group norm", launch_norm_backward(a, d.dtype, stream));

@@ -24,6 +24,12 @@ __host__ __device__ inline long long mx4_block_at(long long rows, long long row,
 // Scale bytes of a row.
 inline long long mx4_scale_bytes(long long K) { return round_up(K, 512) / 32; }
 
+// A divisor known before the launch, for quotients of unsigned numbers without a division (of which the compiler makes 25
+// instructions): mul = floor(2^32 / by) gives the quotient or one less.
+struct Divisor {
+    unsigned by, mul;
+};
+
 // How a norm's work is dealt out.  A workgroup of `threads` owns `unit` channels (unit / vec vectors, a thread each) of `chunk_rows`
 // pixels of one image, at most `held` pixels a thread, which it keeps in registers.  Where one workgroup holds all pixels
 // (chunks = 1) a norm is one launch; else `slots` partial results per image and group meet in a second one.
@@ -40,6 +46,9 @@ struct NormPlan {
     int places;         // sums a thread keeps apart: its vector may span groups
     int lds;            // bytes
     bool whole;         // one workgroup has all pixels and channels of its groups
+    int run_shift;      // log2 of the channels of a vector that share a place
+    Divisor by_tiles, by_chunks, by_group;
+    Divisor by_rows[2]; // the pixels that its threads move at a time: a workgroup of `unit` channels, the last one across the channels
 };
 
 // Partial statistics of one group: the sum, and the squared deviations from its mean.
@@ -61,6 +70,7 @@ struct NormArgs {
     long long rows;                 // batch * pixels
     int batch, pixels, C, groups, Cg, act, param_dtype;
     float eps;
+    double per_number;              // 1 / (pixels * Cg)
     NormPlan plan;
 };
 
