@@ -99,38 +99,46 @@ static __device__ __forceinline__ float bias_of(const ProductArgs &a, long long 
     return wanted && a.bias && n < a.N ? param<DT>(a.bias, n, a.bias_dtype) : 0.0f;
 }
 
-// A wave's outputs from row m on and from column n on, their bias in LDS.  Of a block a lane has row r of x, and of w 16 u + 8 q ..
-// 16 u + 8 q + 7, u = 0, 1.  The residuals of the next eight columns are on their way while these are finished; the first are
-// handed over.
+// A wave's outputs from row m on and from column n on; `bias` is that of its columns, `stage` its own 4 KiB NB of LDS.  Of a block a lane
+// has row r of x, and of w 16 u + 8 q .. 16 u + 8 q + 7, u = 0, 1: 32 rows at a time go through LDS (16 bytes are moved by the row, so
+// that neither side meets a bank twice), from where a lane takes eight outputs of a row and its neighbours those beside them: residuals
+// and outputs are whole cache lines.  The residuals of the next 32 rows are on their way while these are finished.
 template <int DT, int MB, int NB>
 static __device__ __forceinline__ void finish_tile(const ProductArgs &a, const f16_t (&acc)[NB][MB], long long m, long long n, const float *bias,
-                                                   const typename Eight<DT>::vec_t (&first)[MB]) {
-    const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5;
-    auto row = [&](int i) { return m + i * 32 + r; };
-    auto column = [&](int k) { return k / 2 * 32 + k % 2 * 16 + q * 8; };
-    typename Eight<DT>::vec_t res[2][MB];
+                                                   unsigned char *stage) {
+    constexpr int kAcross = NB * 4, kDown = 64 / kAcross, kTurns = 32 / kDown;     // lanes of a row, rows at a time
+    const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5, down = lane / kAcross, c = lane % kAcross * 8;
+    auto place = [&](int row, int chunk) { return reinterpret_cast<float4 *>(stage + row * NB * 128 + (chunk ^ (row & 15)) * 16); };
+    const float4 lo = *reinterpret_cast<const float4 *>(bias + c), hi = *reinterpret_cast<const float4 *>(bias + c + 4);
+    const float add[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     auto finish = [&](auto act) {
+        typename Eight<DT>::vec_t res[2][kTurns];
+        auto ask = [&](int i) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) res[0][i] = first[i];
+            for (int s = 0; s < kTurns; ++s) res[i & 1][s] = residual8<DT>(a, m + i * 32 + s * kDown + down, n + c);
+        };
+        ask(0);
 #pragma unroll
-        for (int k = 0; k < 2 * NB; ++k) {
-            const int c = column(k);
-            if (k + 1 < 2 * NB) {
+        for (int i = 0; i < MB; ++i) {
 #pragma unroll
-                for (int i = 0; i < MB; ++i) res[(k + 1) & 1][i] = residual8<DT>(a, row(i), n + column(k + 1));
-            }
-            if (n + c < a.N) {
-                const float4 lo = *reinterpret_cast<const float4 *>(bias + c), hi = *reinterpret_cast<const float4 *>(bias + c + 4);
-                const float add[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            for (int k = 0; k < 2 * NB; ++k)
 #pragma unroll
-                for (int i = 0; i < MB; ++i) {
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = acc[k / 2][i][8 * (k % 2) + e] + add[e];
-                    if (row(i) < a.M) finish8<DT, decltype(act)::value>(a, row(i), n + c, v, res[k & 1][i]);
+                for (int h = 0; h < 2; ++h) {
+                    const int e = 8 * (k % 2) + 4 * h;
+                    const f16_t &v = acc[k / 2][i];
+                    *place(r, k * 4 + q * 2 + h) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                 }
+            if (i + 1 < MB) ask(i + 1);
+            asm volatile("" ::: "memory");      // (a wave's own LDS operations come in order)
+#pragma unroll
+            for (int s = 0; s < kTurns; ++s) {
+                const int row = s * kDown + down;
+                const float4 u = *place(row, c / 4), w = *place(row, c / 4 + 1);
+                const float v[8] = {u.x + add[0], u.y + add[1], u.z + add[2], u.w + add[3], w.x + add[4], w.y + add[5], w.z + add[6], w.w + add[7]};
+                if (m + i * 32 + row < a.M && n + c < a.N) finish8<DT, decltype(act)::value>(a, m + i * 32 + row, n + c, v, res[i & 1][s]);
             }
-            __builtin_amdgcn_sched_barrier(0);      // (or all residuals are requested first, and spill)
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     if (a.act == TDC_ACT_RELU) finish(std::integral_constant<int, TDC_ACT_RELU>{});
@@ -287,10 +295,7 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
     }
     meet(None{});       // (nothing may still be on its way into LDS when the workgroup ends)
 
-    typename Eight<DT>::vec_t first[MB];
-#pragma unroll
-    for (int i = 0; i < MB; ++i) first[i] = residual8<DT>(a, m0 + wm * 32 * MB + i * 32 + r, n0 + wn * 32 * NB + q * 8);
-    finish_tile<DT, MB, NB>(a, acc, m0 + wm * 32 * MB, n0 + wn * 32 * NB, bias + wn * 32 * NB, first);
+    finish_tile<DT, MB, NB>(a, acc, m0 + wm * 32 * MB, n0 + wn * 32 * NB, bias + wn * 32 * NB, lds + wave * NB * 4096);
 }
 
 // ---- few outputs ----
