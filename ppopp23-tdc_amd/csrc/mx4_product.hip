@@ -80,6 +80,9 @@ struct Tile {
     static constexpr int kX = MB, kChunks = MB + NB;          // requests of a wave and step: of x, in all
     static constexpr int kScaleRequests = (M + N) / 256;      // of a wave and four steps
     static constexpr int kParts = NB / 2;
+    // Where all steps are in LDS at once: as many buffers, and what the outputs pass through.
+    static constexpr __host__ __device__ int short_buffers(int steps) { return steps > 2 ? steps : 2; }
+    static constexpr __host__ __device__ int short_lds(int steps) { return short_buffers(steps) * kBuffer + kScales + N * 4; }
 };
 
 // Which tile a workgroup has, if any: neighbouring workgroups of a die take tiles of eight rows by as many columns as run at once, which
@@ -93,6 +96,33 @@ static __device__ __forceinline__ bool tile_of(int tiles_m, int tiles_n, long lo
     m0 = (long long)(group * 8 + rest % high) * Tile<MB, NB>::M;
     n0 = (long long)(rest / high) * Tile<MB, NB>::N;
     return true;
+}
+// A request straight into LDS: 16 bytes a lane, from `at` + `offset` on, in the order of the lanes.
+static __device__ __forceinline__ void bring(const unsigned char *base, int at, int offset, unsigned char *to) {
+    const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(base), 0, 0x7fffffff, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)to, 16, at, offset, 0, 0);
+}
+// Codes of a step for a tile: request i of a wave is half a block of 32 rows, of x for i below kX, of w from there on.  (Blocks past the
+// last repeat it: their products go nowhere.)
+template <int MB, int NB>
+static __device__ __forceinline__ const unsigned char *codes_of(const ProductArgs &a, int i, long long step, long long m0, long long n0) {
+    const bool of_x = i < Tile<MB, NB>::kX;
+    return (of_x ? a.x_codes : a.w_codes) + (step * (((of_x ? a.M : a.N) + 31) >> 5) + ((of_x ? m0 : n0) >> 5)) * 2048;
+}
+template <int MB, int NB>
+static __device__ __forceinline__ int chunk_of(const ProductArgs &a, int i, int wave, long long m0, long long n0) {
+    using L = Tile<MB, NB>;
+    const int c = (i < L::kX ? i : i - L::kX) * 4 + wave;
+    return (int)min((long long)(c / 2), (i < L::kX ? ((a.M + 31) >> 5) - (m0 >> 5) : ((a.N + 31) >> 5) - (n0 >> 5)) - 1) * 2048 + c % 2 * 1024;
+}
+// Waits until all but the wave's newest `left` requests have come and its LDS operations are done, then for the other waves.  (A fence in
+// place of the waits would wait for every request.)
+template <int left>
+static __device__ __forceinline__ void meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((left & 15) | (left >> 4) << 14 | 7 << 4);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 template <int DT>
 static __device__ __forceinline__ float bias_of(const ProductArgs &a, long long n, bool wanted) {
@@ -157,23 +187,12 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
     if (!tile_of<MB, NB>(tiles_m, tiles_n, m0, n0)) return;
     const float b = bias_of<DT>(a, n0 + t, t < L::N);
 
-    // Requests straight into LDS: 16 bytes a lane, in the order of the lanes, at a wave's own place.
-    auto bring = [&](const unsigned char *base, int offset, unsigned char *to) {
-        const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(base), 0, 0x7fffffff, 0x00020000);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)to, 16, lane * 16, offset, 0, 0);
-    };
-    // Codes: request i of a wave is half a block of 32 rows.  (Blocks past the last repeat it: their products go nowhere.)
-    const long long x_blocks = (a.M + 31) >> 5, w_blocks = (a.N + 31) >> 5;
+    // Codes: request i of a wave.
     int from[L::kChunks];
 #pragma unroll
-    for (int i = 0; i < L::kChunks; ++i) {
-        const int c = (i < L::kX ? i : i - L::kX) * 4 + wave;
-        from[i] = (int)min((long long)(c / 2), (i < L::kX ? x_blocks - (m0 >> 5) : w_blocks - (n0 >> 5)) - 1) * 2048 + c % 2 * 1024;
-    }
+    for (int i = 0; i < L::kChunks; ++i) from[i] = chunk_of<MB, NB>(a, i, wave, m0, n0);
     auto fetch = [&](int i, int step) {
-        const long long k = min(step, a.ksteps - 1);
-        const unsigned char *const base = i < L::kX ? a.x_codes + (k * x_blocks + (m0 >> 5)) * 2048 : a.w_codes + (k * w_blocks + (n0 >> 5)) * 2048;
-        bring(base, from[i], lds + (step & 3) * L::kBuffer + (i * 4 + wave) * 1024);
+        bring(codes_of<MB, NB>(a, i, min(step, a.ksteps - 1), m0, n0), lane * 16, from[i], lds + (step & 3) * L::kBuffer + (i * 4 + wave) * 1024);
     };
     // Scales of four steps: rows of x, then of w, a row a thread.
     const int groups = (a.ksteps + 3) / 4, last_m = (int)min((long long)L::M, a.M - m0) - 1, last_n = (int)min((long long)L::N, a.N - n0) - 1;
@@ -186,8 +205,7 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
             const bool of_x = i * 256 + wave * 64 < L::M;
             const unsigned char *const base = of_x ? a.x_scales + (at * a.M + m0) * 16 : a.w_scales + (at * a.N + n0) * 16;
             const int row = i * 256 + t, in = of_x ? min(row, last_m) : min(row - L::M, last_n);
-            const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(base), 0, 0x7fffffff, 0x00020000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)(to + i * 4096), 16, in * 16, 0, 0, 0);
+            bring(base, in * 16, 0, to + i * 4096);
         }
     };
 
@@ -206,18 +224,6 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
             for (int j = 0; j < NB; ++j) sw[j][h] = *reinterpret_cast<const int *>(at + (L::M + w_row + j * 32) * 16 + h * 8);
         }
     };
-    // Waits until all but the wave's newest `left` requests have come and its LDS reads are done, then for the other waves.  (A fence
-    // in place of the waits would wait for every request.)
-    auto meet = [&](auto left) {
-        constexpr int n = decltype(left)::value;
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 7 << 4);
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
-    using None = std::integral_constant<int, 0>;
-    using Codes = std::integral_constant<int, L::kChunks>;
-
     f16_t acc[NB][MB];
 #pragma unroll
     for (int j = 0; j < NB; ++j)
@@ -235,7 +241,7 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
 #pragma unroll
         for (int i = 0; i < L::kChunks; ++i) fetch(i, s);
     if (t < L::N) bias[t] = b;
-    meet(Codes{});
+    meet<L::kChunks>();
     i4_t x[2][MB][2], w[2][2][2];
     int sx[MB][2], sw[NB][2];
 #pragma unroll
@@ -279,7 +285,7 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
 #pragma unroll
             for (int j = 0; j < NB; ++j) sw[j][h] = (int)((unsigned)sw[j][h] >> 8);
         }
-        meet(Codes{});      // (the codes of the step after the next have to be there: all requests but this step's)
+        meet<L::kChunks>();      // (the codes of the step after the next have to be there: all requests but this step's)
     };
     // (no branch stands between a step's requests and its matrix instructions, or the compiler moves these behind the barrier; the
     // last three steps bring codes that no one needs)
@@ -293,9 +299,71 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
         }
         read_scales(g + 1, sx, sw);
     }
-    meet(None{});       // (nothing may still be on its way into LDS when the workgroup ends)
+    meet<0>();       // (nothing may still be on its way into LDS when the workgroup ends)
 
     finish_tile<DT, MB, NB>(a, acc, m0 + wm * 32 * MB, n0 + wn * 32 * NB, bias + wn * 32 * NB, lds + wave * NB * 4096);
+}
+
+// ---- short sums ----
+//
+// Bound by the outputs' bytes, and by the way there.  Tiles of 128 x 128 as above, but all codes of up to 512 numbers of a row are in
+// LDS at once, asked for together and waited for once; up to 256 numbers leave room for three workgroups on a compute unit, of which
+// one can store while others load.  (Making x into 4 bits here as well, once for every tile across, took longer than a launch of its
+// own that leaves codes: 25088 x 128 x 512 18.5 us against 17.6, 4096 x 512 x 4096 41 against 22.)
+template <int DT>
+__global__ void __launch_bounds__(256, (DT == TDC_F32 ? 2 : 3)) tdc_mx4_product_short_kernel(const ProductArgs a, int tiles_m, int tiles_n) {
+    using L = Tile<2, 2>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 31, q = lane >> 5;
+    const int wm = wave & 1, wn = wave >> 1;
+    long long m0, n0;
+    if (!tile_of<2, 2>(tiles_m, tiles_n, m0, n0)) return;
+    const float b = bias_of<DT>(a, n0 + t, t < L::N);
+    unsigned char *const lds_scales = lds + L::short_buffers(a.ksteps) * L::kBuffer;
+    float *const bias = reinterpret_cast<float *>(lds_scales + L::kScales);
+#pragma unroll
+    for (int i = 0; i < L::kChunks; ++i) {
+        const int from = chunk_of<2, 2>(a, i, wave, m0, n0);
+        for (int step = 0; step < a.ksteps; ++step)
+            bring(codes_of<2, 2>(a, i, step, m0, n0), lane * 16, from, lds + step * L::kBuffer + (i * 4 + wave) * 1024);
+    }
+    // Scales: rows of x, then of w, a row a thread.
+    if (wave < 2) bring(a.x_scales + m0 * 16, (int)min((long long)t, a.M - m0 - 1) * 16, 0, lds_scales + wave * 1024);
+    else bring(a.w_scales + n0 * 16, (int)min((long long)t - L::M, a.N - n0 - 1) * 16, 0, lds_scales + wave * 1024);
+    if (t < L::N) bias[t] = b;
+    meet<0>();
+    // Row r of a block; its places q and 2 + q for the two halves of a step.
+    const int w_in = weight_row(r), x_at = wm * 4096 + q * 512 + r * 16, w_at = L::M * 64 + wn * 4096 + q * 512 + w_in * 16;
+    int sx[2][2], sw[2][2];
+    f16_t acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            sx[i][h] = *reinterpret_cast<const int *>(lds_scales + (wm * 64 + i * 32 + r) * 16 + q * 4 + h * 8);
+            sw[i][h] = *reinterpret_cast<const int *>(lds_scales + (L::M + wn * 64 + i * 32 + w_in) * 16 + q * 4 + h * 8);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][h][e] = 0.0f;
+        }
+    for (int step = 0; step < a.ksteps; ++step) {
+        const unsigned char *const at = lds + step * L::kBuffer;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            i4_t x[2], w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                x[i] = *reinterpret_cast<const i4_t *>(at + x_at + i * 2048 + h * 1024);
+                w[i] = *reinterpret_cast<const i4_t *>(at + w_at + i * 2048 + h * 1024);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    acc[j][i] = mfma4(w[j], x[i], acc[j][i], (int)((unsigned)sw[j][h] >> 8 * step), (int)((unsigned)sx[i][h] >> 8 * step));
+        }
+    }
+    meet<0>();
+    finish_tile<DT, 2, 2>(a, acc, m0 + wm * 64, n0 + wn * 64, bias + wn * 64, lds + wave * 8192);
 }
 
 // ---- few outputs ----
@@ -316,7 +384,7 @@ static __device__ __forceinline__ void take_numbers(const ProductArgs &a, long l
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int i = min(at + k * (int)blockDim.x, rows * octets - 1);      // (a repeated one is not stored)
-            row[k] = i / octets;
+            row[k] = small_quotient(i, octets);
             octet[k] = i - row[k] * octets;
             const long long from = (m0 + row[k]) * a.x_stride;
             if (octet[k] * 8 + 8 <= a.K) p[k] = P::load(a.x, from + octet[k] * 8);
@@ -445,6 +513,17 @@ static int launch_tile(const ProductArgs &a, hipStream_t s) {
     fn<<<grid, 256, L::kLds, s>>>(a, tm, tn);
     return (int)hipGetLastError();
 }
+template <int DT>
+static int launch_short(const ProductArgs &a, hipStream_t s) {
+    using L = Tile<2, 2>;
+    static unsigned long long done = 0;
+    auto *const fn = &tdc_mx4_product_short_kernel<DT>;
+    if (int e = allow_lds((const void *)fn, L::short_lds(4), done)) return e;
+    const int tm = (int)((a.M + L::M - 1) / L::M), tn = (int)((a.N + L::N - 1) / L::N);
+    const unsigned grid = (unsigned)(((long long)tm * tn + 7) / 8 * 8);
+    fn<<<grid, 256, L::short_lds(a.ksteps), s>>>(a, tm, tn);
+    return (int)hipGetLastError();
+}
 template <int DT, int XS>
 static int launch_few(const ProductArgs &a, hipStream_t s) {
     // A wave for every 512 numbers of K, four to sixteen of them; sixteen also to make many numbers into 4 bits.
@@ -456,11 +535,13 @@ static int launch_few(const ProductArgs &a, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
-// Timed in turn over M 16 .. 25088, N 64 .. 8192, K 128 .. 8192 (us):
-//   32 x 32 outputs a workgroup while there are 512 of them, or 1024 of short sums: 1024 x 512 x 2048 7.5 against 9.2 in tiles of 128,
-//   1024 x 1024 x 512 5.2 against 6.2, but 1024 x 1024 x 1024 7.6 against 7.3 and 4096 x 512 x 512 8.9 against 6.6;
-//   tiles of 256 for long sums that fill the compute units: 4096 x 8192 x 8192 155 against 171, 25088 x 512 x 8192 65 against 80, but
-//   8192 x 8192 x 2048 122 against 110 (a tile's first loads and its stores run alone) and 1024 x 8192 x 8192 60 against 44.
+// Timed in turn over M 16 .. 100352, N 64 .. 8192, K 64 .. 8192 (us, M x N x K):
+//   32 x 32 outputs a workgroup while there are 512 of them, or 1024 of short sums: 1024 x 512 x 2048 7.5 against 9.6 in tiles of 128,
+//   1024 x 1024 x 512 5.3 against 6.6, but 1024 x 1024 x 1024 7.6 against 7.6 and 2048 x 1024 x 512 9.0 against 6.9;
+//   all steps at once up to 512 numbers: 25088 x 512 x 128 12.6 against 15.0 step by step, 100352 x 256 x 64 17.9 against 24.0, 4096 x 4096
+//   x 512 16.9 against 17.6 (more than 512 would leave a compute unit one workgroup);
+//   tiles of 256 for long sums that fill the compute units: 4096 x 8192 x 8192 164 against 184, 25088 x 512 x 8192 69 against 78, but
+//   8192 x 8192 x 2048 114 against 112 (a tile's first loads and its stores run alone) and 1024 x 8192 x 8192 64 against 45.
 template <int DT>
 static int launch_product(const ProductArgs &a, hipStream_t s) {
     if (a.x) {
@@ -469,6 +550,7 @@ static int launch_product(const ProductArgs &a, hipStream_t s) {
     }
     auto tiles = [&](long long edge) { return ((a.M + edge - 1) / edge) * ((a.N + edge - 1) / edge); };
     if (tiles(32) <= (a.ksteps <= 4 ? 1024 : 512)) return launch_few<DT, TDC_MX4>(a, s);
+    if (a.ksteps <= 4) return launch_short<DT>(a, s);
     if (a.ksteps >= 32 && tiles(256) >= 192) return launch_tile<DT, 4, 4>(a, s);
     return launch_tile<DT, 2, 2>(a, s);
 }

@@ -6,12 +6,11 @@
 
 namespace tdc {
 
-// Quotients: of numbers below 2^32, and of two below 2^20 (an approximate reciprocal is near enough for those).
+// The quotient of a number below 2^32.
 static __device__ __forceinline__ unsigned quotient(unsigned n, const Divisor &d) {
     const unsigned q = __umulhi(n, d.mul);
     return q + (n - q * d.by >= d.by);
 }
-static __device__ __forceinline__ int small_quotient(int n, int d) { return (int)((n + 0.5f) * __builtin_amdgcn_rcpf((float)d)); }
 // 1 / n to the last bits of a double: two steps of Newton's method from 23 bits.
 static __device__ __forceinline__ double inverse(int n) {
     double r = __builtin_amdgcn_rcpf((float)n);

@@ -128,4 +128,7 @@ __device__ __forceinline__ float quad_larger(float top) {
     return larger(top, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, top), 0x4E, 0xf, 0xf, true)));
 }
 
+// The quotient of two numbers below 2^20: an approximate reciprocal is near enough for those.
+static __device__ __forceinline__ int small_quotient(int n, int d) { return (int)((n + 0.5f) * __builtin_amdgcn_rcpf((float)d)); }
+
 }  // namespace tdc

@@ -323,6 +323,21 @@ def test_product_of_whole_numbers_is_exact():
         assert torch.equal(y.cpu().double(), x.double() @ w.double().t())
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M,N,K", [(4400, 4500, 4200), (6200, 12400, 4096)])
+def test_product_of_more_tiles_than_compute_units_is_exact(dtype, M, N, K):
+    """Workgroups that take one tile after the other, the last ones not all of them: sums of quarters, exact in fp32 in any order."""
+    g = torch.Generator(device="cuda").manual_seed(23)
+    values = torch.tensor([0.0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.5, -1, -1.5, -2, -3, -4, -6], device="cuda")
+    x, w = (values[torch.randint(0, 15, (n, K), generator=g, device="cuda")] for n in (M, N))
+    x[:, ::32] = 6.0
+    w[:, ::32] = 6.0
+    bias, residual = (torch.randint(-9, 10, n, generator=g, device="cuda").float() for n in ((N,), (M, N)))
+    want = torch.relu(x @ w.t() / 64 + bias + residual).to(dtype)
+    y = tdc_amd.mx4_linear(x / 64, tdc_amd.mx4_quantize(w), bias, residual.to(dtype), act="relu", out_dtype=dtype)
+    assert torch.equal(y, want)
+
+
 def test_product_strides_axes_and_specials():
     base = numbers(6, 6, 9, 200).cuda()
     x = base[:, :, 20:170]
