@@ -130,15 +130,15 @@ static __device__ __forceinline__ float bias_of(const ProductArgs &a, long long 
 }
 
 // A wave's outputs from row m on and from column n on; `bias` is that of its columns, `stage` its own 4 KiB NB of LDS.  Of a block a lane
-// has row r of x, and of w 16 u + 8 q .. 16 u + 8 q + 7, u = 0, 1: 32 rows at a time go through LDS (16 bytes are moved by the row, so
-// that neither side meets a bank twice), from where a lane takes eight outputs of a row and its neighbours those beside them: residuals
+// has row r of x, and of w 16 u + 8 q .. 16 u + 8 q + 7, u = 0, 1: 32 rows at a time go through LDS (the first halves of a row's eights before
+// the second ones, 16 bytes moved by the row, so that neither side meets a bank twice), from where a lane takes eight outputs of a row and its neighbours those beside them: residuals
 // and outputs are whole cache lines.  The residuals of the next 32 rows are on their way while these are finished.
 template <int DT, int MB, int NB>
 static __device__ __forceinline__ void finish_tile(const ProductArgs &a, const f16_t (&acc)[NB][MB], long long m, long long n, const float *bias,
                                                    unsigned char *stage) {
     constexpr int kAcross = NB * 4, kDown = 64 / kAcross, kTurns = 32 / kDown;     // lanes of a row, rows at a time
     const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5, down = lane / kAcross, c = lane % kAcross * 8;
-    auto place = [&](int row, int chunk) { return reinterpret_cast<float4 *>(stage + row * NB * 128 + (chunk ^ (row & 15)) * 16); };
+    auto place = [&](int row, int eight, int half) { return reinterpret_cast<float4 *>(stage + row * NB * 128 + (half * kAcross + eight ^ (row & 15)) * 16); };
     const float4 lo = *reinterpret_cast<const float4 *>(bias + c), hi = *reinterpret_cast<const float4 *>(bias + c + 4);
     const float add[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     auto finish = [&](auto act) {
@@ -156,14 +156,14 @@ static __device__ __forceinline__ void finish_tile(const ProductArgs &a, const f
                 for (int h = 0; h < 2; ++h) {
                     const int e = 8 * (k % 2) + 4 * h;
                     const f16_t &v = acc[k / 2][i];
-                    *place(r, k * 4 + q * 2 + h) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    *place(r, k * 2 + q, h) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                 }
             if (i + 1 < MB) ask(i + 1);
             asm volatile("" ::: "memory");      // (a wave's own LDS operations come in order)
 #pragma unroll
             for (int s = 0; s < kTurns; ++s) {
                 const int row = s * kDown + down;
-                const float4 u = *place(row, c / 4), w = *place(row, c / 4 + 1);
+                const float4 u = *place(row, c / 8, 0), w = *place(row, c / 8, 1);
                 const float v[8] = {u.x + add[0], u.y + add[1], u.z + add[2], u.w + add[3], w.x + add[4], w.y + add[5], w.z + add[6], w.w + add[7]};
                 if (m + i * 32 + row < a.M && n + c < a.N) finish8<DT, decltype(act)::value>(a, m + i * 32 + row, n + c, v, res[i & 1][s]);
             }
