@@ -9,6 +9,11 @@
 // kept per channel: weighted by gamma and added over a group they are the two group means, and added over workgroups the
 // parameters' gradients (by the first workgroups of the second launch, or in a launch of their own).  No atomics, the
 // same order on every run.
+//
+// Sums over a thread's pixels are short chains in fp32, joined in trees: dz and dz xh have no common offset to lose.
+//
+// Measured: 32 x 112 x 112 x 128 in 16 bits, silu: 40 us for the sums (5.1 TB/s) and 55 for dx (5.6), the vector unit busy for 60 to 70 % beside
+// the memory.  3 x 13 x 17 x 114, one launch and that of the parameters: 7.7 and 2.7 us, in a backward pass of which the host has some 50.
 #include "norm_device.hpp"
 
 namespace tdc {

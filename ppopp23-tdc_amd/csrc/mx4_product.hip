@@ -68,6 +68,11 @@ static __device__ __forceinline__ void finish8(const ProductArgs &a, long long m
 // that one wave to a SIMD keeps the matrix unit fed across its one barrier a step.  LDS holds the codes as they lie in
 // memory: a block's read is 1 KiB in a row, which meets no bank twice.
 //
+// Measured, tiles of 256, 8192 x 8192 x 8192 in random codes: 316 us, 3.5 PFLOP/s; 237 on zeros, 4.7, so that a quarter of it is the clock that
+// the power leaves.  Without the outputs 294 and 202, without new codes besides 233 and 181 (registers only: 172 and 124).  The same
+// workgroups going from tile to tile, the next one's codes on their way while this one's outputs leave, took as long: the work saved is
+// waiting, which needs no power.
+//
 // The row of w that is row r of a block: bits 2 and 3 change places, which makes a lane's outputs 8 i .. 8 i + 7 neighbours.
 static __device__ __forceinline__ int weight_row(int r) { return (r & 19) | (r & 4) << 1 | (r & 8) >> 1; }
 
@@ -309,7 +314,10 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
 // Bound by the outputs' bytes, and by the way there.  Tiles of 128 x 128 as above, but all codes of up to 512 numbers of a row are in
 // LDS at once, asked for together and waited for once; up to 256 numbers leave room for three workgroups on a compute unit, of which
 // one can store while others load.  (Making x into 4 bits here as well, once for every tile across, took longer than a launch of its
-// own that leaves codes: 25088 x 128 x 512 18.5 us against 17.6, 4096 x 512 x 4096 41 against 22.)
+// own that leaves codes: 25088 rows of 128 by 512 18.5 us against 17.6, 4096 of 512 by 4096 41 against 22.)
+//
+// Measured: 25088 rows of 128 by 512, outputs in bf16: 12.6 us, 16.4 with a residual (51 MB and 3.2 TB/s of it, two and a half us the launch);
+// 5.2 of the 12.6 are the stores, 3 the way of the sums through LDS.
 template <int DT>
 __global__ void __launch_bounds__(256, (DT == TDC_F32 ? 2 : 3)) tdc_mx4_product_short_kernel(const ProductArgs a, int tiles_m, int tiles_n) {
     using L = Tile<2, 2>;
@@ -372,6 +380,9 @@ __global__ void __launch_bounds__(256, (DT == TDC_F32 ? 2 : 3)) tdc_mx4_product_
 // time, with their codes straight in registers: a block of 32 rows by 64 numbers is one request of 1 KiB.  The waves' sums meet
 // in LDS, in the order of the waves.  XS: x in 4 bits (TDC_MX4), or numbers of that type, which a workgroup makes into 4 bits in LDS
 // by itself: for few rows that costs less than a launch.
+//
+// Measured: one row of 4096 by 16384 weights, x in bf16: 8.0 to 9.6 us (36 MB, 3.7 to 4.5 TB/s); 33 rows of 2000 by 1001, x in fp32: 11.4, a chain
+// of latencies (x, its codes, weights, the waves' sums); 196 rows of 1024 by 256 in 4 bits: 5.6.
 // `rows` rows of x from row m0 on into codes in LDS, eight numbers a thread, four such runs on their way: block b of row m at
 // (b rows + m) 16, its scale byte behind all codes, words of four steps.
 template <int XS>
