@@ -4,8 +4,8 @@
 //
 // Memory traffic.  A workgroup owns `unit` neighbouring channels (whole groups, unless one group is wider than that) of a run of
 // pixels, and holds them in registers: a thread asks for `vec` channels of every R-th pixel, all requests at once.  Where the
-// pixels of an image fit (up to 256 KiB a workgroup) that is all: x is read once, the statistics meet in LDS, y is written.
-// Else one launch leaves partial statistics, and a second reads x again and joins, while it comes, the partial results of its own
+// pixels of an image fit (up to 256 KiB a workgroup), and that does not leave most of the chip idle, that is all: x is read once, the
+// statistics meet in LDS, y is written.  Else one launch leaves partial statistics, and a second reads x again and joins, while it comes, the partial results of its own
 // groups: no atomics, no third launch, the same order on every run.  These two are made of many small workgroups whose threads have
 // four requests on their way while they work on four.
 //
@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(c
     using P = Pack<DT, V>;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const Part p = part_of(a, V, blockIdx.x, gridDim.x);
-    const int n = rows_of(p, p.tr);
+    // (a vector past the last channel has no numbers; in 4 bits it fills a block up with zeros)
+    const int c = p.c0 + p.tc * V, all = rows_of(p, p.tr), n = c < a.C ? all : 0;
     const int run = 1 << a.plan.run_shift, most = a.plan.threads * a.plan.places;
     double *const sums = reinterpret_cast<double *>(lds);
     float *const devs = reinterpret_cast<float *>(sums + most);
@@ -302,8 +303,9 @@ __global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(c
         join_threads(a, p, n, s, q, run, sums, devs, waves, [&](int i, double sum, float m2) { a.stat[slot_of(a, p, p.g0 + i)] = NormStat{sum, m2}; });
         return;
     }
-    const int c = p.c0 + p.tc * V;
     float mean[V], scale[V], shift[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) mean[j] = scale[j] = shift[j] = 0.0f;
     auto constants = [&]() {
         int g[V];
         groups_of(a, c, g);
@@ -332,33 +334,40 @@ __global__ void __launch_bounds__(MODE == kWhole ? 1024 : 256) tdc_norm_kernel(c
             stat[i] = finish_stats(a, p, p.g0 + i, sum * a.per_number, m2, true);
         });
         __syncthreads();
-        if (n > 0) {
-            constants();
+        if (all > 0) {
+            if (n > 0) constants();
             const Mx4Place<V> place(a, c);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (i < n) finish(place, x[i], i);
+                if (i < all) finish(place, x[i], i);
         }
     } else {
         if (n > 0) params<DT, V>(a, c, scale, shift);
         join_stats(a, p, stat);
         __syncthreads();
-        if (n > 0) {
-            constants();
+        if (all > 0) {
+            if (n > 0) constants();
             const Mx4Place<V> place(a, c);
-            const Walk<DT, V> in(a.x, a.x_is, a.x_ps, p, n, true);
+            Part there = p;
+            if (n == 0) there.tc = 0;
+            const Walk<DT, V> in(a.x, a.x_is, a.x_ps, there, all, true);
             typename P::type x[2][NV];
-            walk<NV>(n, quotient(p.rows, p.by_R), [&](int set, int at) { in.ask(at, x[set]); }, [&](int set, int at, auto some) {
+            walk<NV>(all, quotient(p.rows, p.by_R), [&](int set, int at) { in.ask(at, x[set]); }, [&](int set, int at, auto some) {
+                if (MX4 && a.plan.round) {
+#pragma unroll
+                    for (int i = 0; i < NV; ++i)
+                        if (n == 0) x[set][i] = typename P::type{};
+                }
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
-                    if (i < some) finish(place, x[set][i], n - 1 - at - i);
+                    if (i < some) finish(place, x[set][i], all - 1 - at - i);
             });
         }
     }
     if (MX4 && p.c0 + p.width == a.C) store_mx4_padding(a, p);
 }
 
-// The second half into 4 bits where a row's blocks and vectors do not fit together: a thread takes a block of 32 channels of a pixel.
+// The second half into 4 bits where the channels are no whole number of vectors: a thread takes a block of 32 channels of a pixel.
 template <int DT, int ACT>
 __global__ void __launch_bounds__(256) tdc_norm_blocks_kernel(const NormArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
@@ -414,8 +423,7 @@ template <int DT, int ACT>
 static int by_shape(const NormArgs &a, hipStream_t s) {
     constexpr int VM = DT == TDC_F32 ? 4 : 8;
     const NormPlan &n = a.plan;
-    if (a.codes && (a.C % 32 || n.vec != VM)) {
-        if (n.vec == VM) return run_blocks<DT, VM, ACT>(a, s);
+    if (a.codes && n.vec != VM) {
         return n.vec == 2 ? run_blocks<DT, 2, ACT>(a, s) : run_blocks<DT, 1, ACT>(a, s);
     }
     if (a.codes) return n.held == 4 ? run<DT, VM, 4, ACT, true>(a, s) : run<DT, VM, 16, ACT, true>(a, s);

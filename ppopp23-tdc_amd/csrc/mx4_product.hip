@@ -135,15 +135,18 @@ static __device__ __forceinline__ float bias_of(const ProductArgs &a, long long 
 }
 
 // A wave's outputs from row m on and from column n on; `bias` is that of its columns, `stage` its own 4 KiB NB of LDS.  Of a block a lane
-// has row r of x, and of w 16 u + 8 q .. 16 u + 8 q + 7, u = 0, 1: 32 rows at a time go through LDS (the first halves of a row's eights before
-// the second ones, 16 bytes moved by the row, so that neither side meets a bank twice), from where a lane takes eight outputs of a row and its neighbours those beside them: residuals
-// and outputs are whole cache lines.  The residuals of the next 32 rows are on their way while these are finished.
+// has row r of x, and of w 16 u + 8 q .. 16 u + 8 q + 7, u = 0, 1.  32 rows at a time go through LDS, where a lane takes eight outputs of a
+// row and its neighbours those beside them: residuals and outputs are whole cache lines.  (The first halves of a row's eights lie
+// before the second ones, 16 bytes moved by the row, so that neither side meets a bank twice.)  The residuals of the next 32 rows are on
+// their way while these are finished.
 template <int DT, int MB, int NB>
 static __device__ __forceinline__ void finish_tile(const ProductArgs &a, const f16_t (&acc)[NB][MB], long long m, long long n, const float *bias,
                                                    unsigned char *stage) {
     constexpr int kAcross = NB * 4, kDown = 64 / kAcross, kTurns = 32 / kDown;     // lanes of a row, rows at a time
     const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5, down = lane / kAcross, c = lane % kAcross * 8;
-    auto place = [&](int row, int eight, int half) { return reinterpret_cast<float4 *>(stage + row * NB * 128 + (half * kAcross + eight ^ (row & 15)) * 16); };
+    auto place = [&](int row, int eight, int half) {
+        return reinterpret_cast<float4 *>(stage + row * NB * 128 + ((half * kAcross + eight) ^ (row & 15)) * 16);
+    };
     const float4 lo = *reinterpret_cast<const float4 *>(bias + c), hi = *reinterpret_cast<const float4 *>(bias + c + 4);
     const float add[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     auto finish = [&](auto act) {

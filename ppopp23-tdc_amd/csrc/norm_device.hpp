@@ -40,7 +40,7 @@ static __device__ __forceinline__ Part part_of(const NormArgs &a, int vec, unsig
     p.chunk = across - p.image * n.chunks;
     p.c0 = p.tile * n.unit;
     p.width = min(n.unit, a.C - p.c0);
-    p.vecs = p.width >> __builtin_ctz(vec);
+    p.vecs = ((p.width + n.round) & ~n.round) >> __builtin_ctz(vec);
     p.by_R = n.by_rows[p.width < n.unit];
     p.R = p.by_R.by;
     p.tr = small_quotient(threadIdx.x, p.vecs);

@@ -39,19 +39,30 @@ NormPlan norm_plan(const tdc_group_norm_desc &d, bool quantised, bool grad) {
         const int unit = std::max(1, (bytes / size + whole - 1) / whole) * whole;
         return std::min(std::min(unit, across * n.vec / whole * whole), d.C);
     };
-    const bool blocks = quantised && d.C % 32 != 0;
-    auto fits = [&](int unit) { return !blocks && unit % Cg == 0 && pixels <= (long long)(most / (unit / n.vec)) * 16; };
+    const bool blocks = quantised && n.vec != widest;
+    n.round = quantised && !blocks && d.C % 32 ? 31 : 0;
+    auto vectors = [&](int width) { return ((width + n.round) & ~n.round) / n.vec; };
+    auto fits = [&](int unit) { return !blocks && unit % Cg == 0 && pixels <= (long long)(most / vectors(unit)) * 16; };
+    // One launch pays where a workgroup has little to do, or every compute unit something (bf16, silu, us, one launch against two):
+    // forward, 25 Ki numbers a workgroup 9.4 against 10.7; 51 Ki, 8 workgroups 12.5 against 11.0, 256 18.5 against 22.6; 100 Ki, 16 workgroups
+    // 17.8 against 11.3 (28 against 12.5 into 4 bits), 128 23.1 against 22.7, 256 34.2 against 36.5.  Gradient, where the parameters need
+    // a second launch in either case: 6 Ki 10.4 against 11.9; 25 Ki, 8 workgroups 16.3 against 12.0, 256 21.8 against 23.1; 51 Ki, 256 36
+    // against 32.
+    auto pays = [&](int unit) {
+        const long long numbers = unit * pixels, workgroups = batch * ((d.C + unit - 1) / unit);
+        return numbers <= (grad ? 8192 : 32768) || (workgroups >= 256 && (!grad || numbers <= 32768));
+    };
     // Whole cache lines where that leaves two workgroups for every compute unit, half ones else: their neighbours come to the same
     // die.
     n.unit = tile(128);
-    n.whole = fits(n.unit) && batch * ((d.C + n.unit - 1) / n.unit) >= 512;
-    if (!n.whole && fits(tile(64))) {
+    n.whole = fits(n.unit) && batch * ((d.C + n.unit - 1) / n.unit) >= 512 && pays(n.unit);
+    if (!n.whole && fits(tile(64)) && pays(tile(64))) {
         n.unit = tile(64);
         n.whole = true;
     }
     n.tiles = (d.C + n.unit - 1) / n.unit;
     n.tiles_per_group = n.unit % Cg == 0 ? 1 : std::min(n.tiles, (Cg + n.unit - 2) / n.unit + 1);
-    const int vecs = n.unit / n.vec;
+    const int vecs = vectors(n.unit);
     const long long dealt = n.tiles * batch;
     n.threads = most;
     if (n.whole) {
@@ -77,7 +88,7 @@ NormPlan norm_plan(const tdc_group_norm_desc &d, bool quantised, bool grad) {
     n.by_chunks = divisor(n.chunks);
     n.by_group = divisor(Cg);
     n.by_rows[0] = divisor(n.threads / vecs);
-    n.by_rows[1] = divisor(n.threads / ((d.C - (n.tiles - 1) * n.unit) / n.vec));
+    n.by_rows[1] = divisor(n.threads / vectors(d.C - (n.tiles - 1) * n.unit));
     const int groups = std::min(n.unit, (n.unit - 1) / Cg + 2);
     n.lds = grad ? 8 * (n.threads * n.vec + groups) : 12 * n.threads * n.places + 8 * groups + 16 * (n.threads / 64);
     return n;

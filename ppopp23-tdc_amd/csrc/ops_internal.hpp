@@ -46,6 +46,7 @@ struct NormPlan {
     int places;         // sums a thread keeps apart: its vector may span groups
     int lds;            // bytes
     bool whole;         // one workgroup has all pixels and channels of its groups
+    int round;          // 31 where a row's last block of 32 is not full: its vectors are counted as if it were, else 0
     int run_shift;      // log2 of the channels of a vector that share a place
     Divisor by_tiles, by_chunks, by_group;
     Divisor by_rows[2]; // the pixels that its threads move at a time: a workgroup of `unit` channels, the last one across the channels

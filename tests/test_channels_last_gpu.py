@@ -475,6 +475,24 @@ def test_offsets_beyond_32_bits():
     assert np.array_equal(got.double().cpu().numpy(), ref.mx4(flat.double().cpu().numpy())[2])
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape,groups", [((2, 264, 50, 14), 8), ((1, 944, 22, 17), 16), ((3, 40, 70, 31), 5), ((5, 36, 9, 9), 3), ((70, 72, 6, 6), 9),
+                                          ((1, 2056, 40, 3), 8), ((2, 24, 1, 1), 1), ((9, 296, 61, 61), 37)])
+def test_norm_into_4_bits_where_the_last_block_is_not_full(shape, groups, dtype):
+    test_norm_into_4_bits(shape, groups, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_norm_into_4_bits_takes_nothing_from_beside_its_channels(dtype):
+    for B, C, S, groups in ((2, 40, 9, 5), (1, 72, 3000, 9), (1, 72, 800, 9)):
+        x = numbers(61, B, S, C).to(dtype).cuda()
+        wide = torch.full((B, S, C + 56), float("nan"), dtype=dtype, device="cuda")
+        wide[..., 24:24 + C] = x
+        want, got = (tdc_amd.group_norm_act_mx4(t.permute(0, 2, 1), groups, act="silu") for t in (x, wide[..., 24:24 + C]))
+        assert torch.equal(want.dequantize(), got.dequantize()) and torch.equal(want.scales, got.scales)     # (codes past the last row are anything)
+        assert got.dequantize().isfinite().all()
+
+
 # ---- together ----
 
 def test_tucker_block_in_4_bits():
