@@ -74,11 +74,12 @@ NormPlan norm_plan(const tdc_group_norm_desc &d, bool quantised, bool grad) {
                (!many || dealt * n.threads >= 512 * 512)) n.threads /= 2;
         n.chunk_rows = (int)pixels;
     } else {
-        // Workgroups of 256: two to a compute unit, as long as each thread has four pixels to move.
+        // Workgroups of 256: two to a compute unit, as long as each thread has four pixels to move, and at most 256 (a sum in fp32 is no
+        // longer than that before it meets others).
         n.threads = std::min(most, 256);
         const int rows = n.threads / vecs;
         const long long want = std::max(1ll, 512 / dealt);
-        n.chunk_rows = (int)std::min(round_up(pixels, rows), round_up(std::max(4ll * rows, (pixels + want - 1) / want), rows));
+        n.chunk_rows = (int)std::min(round_up(pixels, rows), round_up(std::clamp((pixels + want - 1) / want, 4ll * rows, 256ll * rows), rows));
     }
     n.chunks = (int)((pixels + n.chunk_rows - 1) / n.chunk_rows);
     n.held = n.vec == widest && (n.chunk_rows + n.threads / vecs - 1) / (n.threads / vecs) <= 4 ? 4 : 16;

@@ -493,6 +493,12 @@ def test_norm_into_4_bits_takes_nothing_from_beside_its_channels(dtype):
         assert got.dequantize().isfinite().all()
 
 
+@pytest.mark.parametrize("shape,groups,dtype", [((1, 4, 1100, 1000), 2, F32), ((1, 24, 700, 500), 3, BF16)])
+def test_norm_of_one_image_of_many_pixels(shape, groups, dtype):
+    test_norm_forward(shape, groups, dtype)
+    test_norm_gradients(shape, groups, dtype)
+
+
 # ---- together ----
 
 def test_tucker_block_in_4_bits():
