@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(256, (DT == TDC_F32 ? 2 : 3)) tdc_mx4_product_
 // in LDS, in the order of the waves.  XS: x in 4 bits (TDC_MX4), or numbers of that type, which a workgroup makes into 4 bits in LDS
 // by itself: for few rows that costs less than a launch.
 //
-// Measured: one row of 4096 by 16384 weights, x in bf16: 8.0 to 9.6 us (36 MB, 3.7 to 4.5 TB/s); 33 rows of 2000 by 1001, x in fp32: 11.4, a chain
+// Measured: one row of 4096 by 16384 weights, x in bf16: 8.0 to 9.8 us (36 MB, 3.7 to 4.5 TB/s); 33 rows of 2000 by 1001, x in fp32: 11.4, a chain
 // of latencies (x, its codes, weights, the waves' sums); 196 rows of 1024 by 256 in 4 bits: 5.6.
 // `rows` rows of x from row m0 on into codes in LDS, eight numbers a thread, four such runs on their way: block b of row m at
 // (b rows + m) 16, its scale byte behind all codes, words of four steps.
