@@ -10,9 +10,10 @@
 // four requests on their way while they work on four.
 //
 // Mean: summed in 64 bits (an add of which costs the vector unit what one in 32 does), so that it is off by the rounding of its
-// last conversion alone, however the numbers cancel.  Variance: a thread sums the squared deviations from its own mean (or its first
-// number), and those of threads and workgroups are joined by M2 = sum M2_i + n_i (mean_i - mean)^2: an offset common to a group
-// cancels before it is squared.  Everything else between load and store is fp32.
+// last conversion alone, however the numbers cancel.  Variance: a thread sums the squared deviations of the numbers it holds from their own
+// mean, of numbers that pass from the first of them in 64 bits, and those of threads and workgroups are joined by
+// M2 = sum M2_i + n_i (mean_i - mean)^2: an offset common to a group cancels before it is squared, and a number far out is no reference that
+// costs the others theirs.  Everything else between load and store is fp32.
 //
 // Measured (16 bits): 32 x 56 x 56 x 256, relu, one launch: 21.7 us, 4.7 TB/s where a copy of that size reaches 5.1.  32 x 112 x 112 x 128,
 // silu, two launches: 31 us of statistics behind another kernel's write-back (25 by themselves, 4.1 TB/s) and 34.5 for the rest, 6.0 TB/s as
@@ -167,8 +168,9 @@ static __device__ __forceinline__ void held_sums(int n, typename Pack<DT, V>::ty
     join_run(q, run);
 }
 
-// Of any number of pixels: the deviations from a channel's first number, an error of which is one part in n of the deviations that this
-// number itself has, then moved to the mean of the place.
+// Of any number of pixels: the deviations from a channel's first number, then moved to the mean of the place.  Where that first number lies far
+// out the sum of squares is up to n times what remains, so it is one of doubles (which add and multiply at the rate of floats): in fp32 an
+// image with one number in its corner had a variance up to 1e-3 off at 256 pixels a thread.
 template <int DT, int V, int NV>
 static __device__ __forceinline__ void passing_sums(const NormArgs &a, const Part &p, int n, int run, double (&s)[V], float (&q)[V]) {
     using P = Pack<DT, V>;
@@ -176,14 +178,11 @@ static __device__ __forceinline__ void passing_sums(const NormArgs &a, const Par
     const Walk<DT, V> in(a.x, a.x_is, a.x_ps, p, n);
     float first[V];
     P::up(P::load(in.base, in.at), first);
+    double dev[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        s[j] = 0.0;
-        q[j] = 0.0f;
-    }
+    for (int j = 0; j < V; ++j) s[j] = dev[j] = 0.0;
     typename P::type x[2][NV];
     walk<NV>(n, quotient(p.rows, p.by_R), [&](int set, int at) { in.ask(at, x[set]); }, [&](int set, int, auto some) {
-        float four[V];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             if (i < some) {
@@ -191,20 +190,26 @@ static __device__ __forceinline__ void passing_sums(const NormArgs &a, const Par
                 P::up(x[set][i], v);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    add_up<DT>(i, i == some - 1, v[j], four[j], s[j]);
-                    q[j] = fmaf(v[j] - first[j], v[j] - first[j], q[j]);
+                    const double d = (double)v[j] - (double)first[j];
+                    s[j] += d;
+                    dev[j] = fma(d, d, dev[j]);
                 }
             }
     });
     double own[V];
     const double inv = inverse(n);
 #pragma unroll
-    for (int j = 0; j < V; ++j) own[j] = s[j] * inv;
+    for (int j = 0; j < V; ++j) {
+        own[j] = s[j] * inv;      // (about the first number)
+        dev[j] = fmax(dev[j] - s[j] * own[j], 0.0);
+        own[j] += first[j];
+        s[j] = fma(n, (double)first[j], s[j]);
+    }
     join_run(s, run);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float d = (float)(own[j] - first[j]), e = (float)(own[j] - s[j] * (inv * (1.0 / V) * a.plan.places));
-        q[j] = fmaxf(q[j] - n * d * d, 0.0f) + n * e * e;
+        const double e = own[j] - s[j] * (inv * (1.0 / V) * a.plan.places);
+        q[j] = (float)fma(n * e, e, dev[j]);
     }
     join_run(q, run);
 }

@@ -549,3 +549,57 @@ def test_norm_module_trains():
         with torch.no_grad():
             for p, d in ((norm.weight, grads[0]), (norm.bias, grads[1]), (w, want[0]), (b, want[1])):
                 p -= 20 * d
+
+
+# ---- sums that meet large and small numbers ----
+
+def check_forward_on_device(y, x, groups, what):
+    """check_forward without parameters, for tensors that are long work for the host: in 64 bits by torch."""
+    v = x.double().permute(0, 2, 3, 1).reshape(x.shape[0], -1, groups, x.shape[1] // groups)
+    mean = v.mean((1, 3), keepdim=True)
+    v = v - mean
+    rstd = 1 / torch.sqrt((v * v).mean((1, 3), keepdim=True) + 1e-5)
+    want = v * rstd
+    bound = E * want.abs() + 16 * E * (want.abs() + mean.abs() * rstd)
+    off = (y.double().permute(0, 2, 3, 1).reshape(v.shape) - want).abs()
+    assert bool((off <= bound).all()), (what, float((off / bound.clamp(min=1e-300)).max()))
+
+
+@pytest.mark.parametrize("shape,groups", [((1, 128, 112, 112), 32), ((1, 3, 1460, 1460), 1), ((1, 4, 2535, 2535), 2), ((1, 1, 5800, 5800), 1),
+                                          ((8, 16, 1024, 1024), 4)])
+def test_norm_of_images_that_begin_with_outliers(shape, groups):
+    """The first number of a thread holds nearly all of its variance: fp32, two launches, 4 (the first shape) to 256 pixels a thread."""
+    B, C, H, W = shape
+    g = torch.Generator(device="cuda").manual_seed(71)
+    for what in ("impulse", "a few among small ones", "another first row"):
+        x = torch.zeros(B, H, W, C, device="cuda")
+        if what == "impulse":
+            x[:, 0, 0] = 1 + 3 * torch.rand(B, C, generator=g, device="cuda")
+        elif what == "another first row":
+            x += 0.3
+            x[:, 0] = 40.0
+        else:
+            x.normal_(generator=g).mul_(0.05)
+            x.view(B, -1, C)[:, :300] += 1 + 3 * torch.rand(B, 300, C, generator=g, device="cuda")
+        x = x.permute(0, 3, 1, 2)
+        check_forward_on_device(tdc_amd.group_norm_act(x, groups), x, groups, what)
+
+
+@pytest.mark.parametrize("S", [896 * 896, 2048 * 2048])
+def test_norm_into_4_bits_of_an_image_that_begins_with_an_outlier(S):
+    """Numbers that lie 1e-5 of themselves from halfway between two codes, ten times their fp32 error, take the code of their side."""
+    C, big = 32, float(np.float32(2.7))      # (its square is not exact in fp32)
+    x = torch.zeros(1, S, C, device="cuda")
+    x[:, 0] = big
+    mean = big / S
+    rstd = 1 / math.sqrt(big * mean - mean * mean + 1e-5)
+    first = (big - mean) * rstd
+    gamma = np.full(C, 2.5 / first)
+    beta = np.where(np.arange(C) % 2 == 0, -2.5e-5, 2.5e-5)
+    gamma[0], beta[0] = 6.0 / first, 0.0      # (the block's scale is 1)
+    gamma, beta = torch.from_numpy(gamma).float(), torch.from_numpy(beta).float()
+    z = first * gamma.double().numpy() + beta.double().numpy()
+    assert np.abs(z[1:] - 2.5).min() > 2e-5
+    q = tdc_amd.group_norm_act_mx4(x.permute(0, 2, 1), 1, gamma.cuda(), beta.cuda())
+    got = q.dequantize()[0, 0].double().cpu().numpy()
+    assert np.array_equal(got, ref.mx4(z[None])[2][0])
