@@ -10,7 +10,9 @@
 // parameters' gradients (by the first workgroups of the second launch, or in a launch of their own).  No atomics, the
 // same order on every run.
 //
-// Sums over a thread's pixels are chains of at most 256 in fp32, joined by others': dz and dz xh have no common offset to lose.
+// Sums over a thread's pixels are chains of at most 256 in fp32: dz and dz xh have no common offset to lose.  Where they meet others' they are
+// added in 64 bits, for there is no limit to how many of them there are: 3e5 images of two pixels with one dy everywhere, whose additions
+// are all rounded the same way, had dbeta 2e-5 off.
 //
 // Measured: 32 x 112 x 112 x 128 in 16 bits, silu: 40 us for the sums (5.1 TB/s) and 55 for dx (5.6), the vector unit busy for 60 to 70 % beside
 // the memory.  28 x 28 x 256: 12 us, latencies of two launches; 14 x 14 x 1024: 10.4, one launch and that of the parameters.
@@ -35,9 +37,9 @@ static __device__ __forceinline__ void slopes(const typename Pack<DT, V>::type &
 }
 
 // The parameters' gradients: a workgroup of 256 adds up 4 of the 2 C columns of the per-channel sums.
-static __device__ __forceinline__ void add_params(const NormArgs &a, unsigned block, float *sum) {
+static __device__ __forceinline__ void add_params(const NormArgs &a, unsigned block, double *sum) {
     const int col = block * 4 + (threadIdx.x & 3), lane = threadIdx.x >> 2, rows = a.batch * a.plan.chunks;
-    float s = 0.0f;
+    double s = 0.0;
     if (col < 2 * a.C) {
 #pragma unroll 8
         for (int r = lane; r < rows; r += 64) s += a.chan[(long long)r * 2 * a.C + col];
@@ -50,11 +52,11 @@ static __device__ __forceinline__ void add_params(const NormArgs &a, unsigned bl
     }
     if (lane == 0 && col < 2 * a.C) {
         float *const to = col < a.C ? a.dbeta : a.dgamma;
-        if (to) to[col < a.C ? col : col - a.C] = sum[threadIdx.x];
+        if (to) to[col < a.C ? col : col - a.C] = (float)sum[threadIdx.x];
     }
 }
 static __global__ void __launch_bounds__(256) tdc_norm_param_grad_kernel(const NormArgs a) {
-    __shared__ float sum[256];
+    __shared__ double sum[256];
     add_params(a, blockIdx.x, sum);
 }
 
@@ -64,7 +66,7 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
     using P = Pack<DT, V>;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     if (MODE == kApply && blockIdx.x < param_blocks) {
-        add_params(a, blockIdx.x, reinterpret_cast<float *>(lds));
+        add_params(a, blockIdx.x, reinterpret_cast<double *>(lds));
         return;
     }
     const Part p = part_of(a, V, blockIdx.x - param_blocks, gridDim.x - param_blocks);
@@ -107,7 +109,7 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
         }
     };
     float2 *const cell = reinterpret_cast<float2 *>(lds), *const stat = cell + (MODE == kApply ? 0 : a.plan.threads * V);
-    const float inv = (float)a.per_number;
+    const double inv = a.per_number;
     const Team t = team_of(a.plan.threads, p.ng);
     if constexpr (MODE != kApply) {
         if (n > 0) {
@@ -130,12 +132,13 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
         float *const chan = a.chan + ((long long)p.image * a.plan.chunks + p.chunk) * 2 * a.C + p.c0;
         const int used = min(p.R, p.rows);
         for (int ch = threadIdx.x; ch < p.width; ch += a.plan.threads) {
-            float2 s = cell[ch];
-            for (int r = 1; r < used; ++r) {
+            double z = 0.0, u = 0.0;
+            for (int r = 0; r < used; ++r) {
                 const float2 e = cell[r * p.width + ch];
-                s.x += e.x;
-                s.y += e.y;
+                z += e.x;
+                u += e.y;
             }
+            const float2 s = make_float2((float)z, (float)u);
             chan[ch] = s.x;
             chan[a.C + ch] = s.y;
             const float w = a.gamma ? param<DT>(a.gamma, p.c0 + ch, a.param_dtype) : 1.0f;
@@ -144,7 +147,7 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
         __syncthreads();
         for (int i = t.first; i < p.ng; i += t.step) {
             const int g = p.g0 + i, lo = max(g * a.Cg, p.c0) - p.c0, channels = shared_channels(a, g, p.tile);
-            float s = 0.0f, u = 0.0f;
+            double s = 0.0, u = 0.0;
             for (int e = t.at; e < channels; e += t.lanes) {
                 s += cell[lo + e].x;
                 u += cell[lo + e].y;
@@ -152,8 +155,8 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
             s = team_sum(s, t.lanes);
             u = team_sum(u, t.lanes);
             if (t.at == 0) {
-                if (MODE == kSums) a.part[slot_of(a, p, g)] = make_float2(s, u);
-                else stat[i] = make_float2(s * inv, u * inv);
+                if (MODE == kSums) a.part[slot_of(a, p, g)] = make_float2((float)s, (float)u);
+                else stat[i] = make_float2((float)(s * inv), (float)(u * inv));
             }
         }
         if (MODE == kSums) return;
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
         for (int i = t.first; i < p.ng; i += t.step) {
             const int g = p.g0 + i, tiles = tiles_of(a, p, g).y;
             const float2 *part = a.part + ((long long)p.image * a.groups + g) * m.slots;
-            float s = 0.0f, u = 0.0f;
+            double s = 0.0, u = 0.0;
             for (int k = 0; k < tiles; ++k)
                 for (int e = t.at; e < m.chunks; e += t.lanes) {
                     const float2 v = part[e * m.tiles_per_group + k];
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(MODE == kWhole ? 512 : 256) tdc_norm_grad_kern
                 }
             s = team_sum(s, t.lanes) * inv;
             u = team_sum(u, t.lanes) * inv;
-            if (t.at == 0) stat[i] = make_float2(s, u);
+            if (t.at == 0) stat[i] = make_float2((float)s, (float)u);
         }
     }
     __syncthreads();

@@ -603,3 +603,17 @@ def test_norm_into_4_bits_of_an_image_that_begins_with_an_outlier(S):
     q = tdc_amd.group_norm_act_mx4(x.permute(0, 2, 1), 1, gamma.cuda(), beta.cuda())
     got = q.dequantize()[0, 0].double().cpu().numpy()
     assert np.array_equal(got, ref.mx4(z[None])[2][0])
+
+
+@pytest.mark.parametrize("shape,groups", [((1 << 20, 16), 2), ((300001, 3, 2, 1), 1), ((1, 1, 1500, 1500), 1)])
+def test_norm_gradients_of_many_rows_with_one_slope(shape, groups):
+    """dy as a mean's backward gives it, the same everywhere: every step of a long fp32 sum of it is rounded the same way."""
+    g = torch.Generator(device="cuda").manual_seed(73)
+    B, C, *space = shape
+    x = torch.randn(B, *space, C, generator=g, device="cuda").movedim(-1, 1)
+    gamma, beta = torch.rand(C, generator=g, device="cuda") + 0.5, torch.randn(C, generator=g, device="cuda")
+    for act in ("none", "silu"):
+        leaves = [t.detach().requires_grad_() for t in (x, gamma, beta)]
+        dy = torch.full((), 0.3, device="cuda").expand(shape)
+        grads = torch.autograd.grad(tdc_amd.group_norm_act(leaves[0], groups, leaves[1], leaves[2], act=act), leaves, dy)
+        check_grads(x, gamma.double().cpu().numpy(), beta.double().cpu().numpy(), dy, grads, groups, act, f"{shape} {act}")
