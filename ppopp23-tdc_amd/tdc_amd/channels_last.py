@@ -11,6 +11,7 @@ tensors' device; scratch comes from torch's allocator, call by call.
 from __future__ import annotations
 
 import ctypes
+import warnings
 from ctypes import byref
 
 import torch
@@ -63,6 +64,15 @@ def _vector(t, n, dtype, device, what):
         raise TypeError(f"{what} has to be float32 or {dtype}: got {t.dtype}")
     if n > 1 and t.stride(0) != 1:
         raise ValueError(f"{what} must be contiguous")
+
+
+def _wants(t):
+    """Whether a gradient would have to reach t."""
+    return t is not None and getattr(t, "requires_grad", False) and torch.is_grad_enabled()
+
+
+def _no_gradient(what, name):
+    raise RuntimeError(f"{what} has no gradient, and {name} requires one: call it under torch.no_grad(), or on {name}.detach()")
 
 
 def _ptr(t):
@@ -339,8 +349,10 @@ def _quantize(x):
 def mx4_quantize(x):
     """``x`` [..., K] in microscaled 4-bit floating point: each block of 32 along the last axis is scaled by the power of two that
     takes its largest magnitude into [4, 8) and rounded to nearest (halfway to the even code, saturating at 6).  A block with
-    an infinity or a NaN stands for NaNs."""
+    an infinity or a NaN stands for NaNs.  Has no gradient: weights that train are put into 4 bits under ``torch.no_grad()``."""
     _number_tensor(x, "x")
+    if _wants(x):
+        _no_gradient("mx4_quantize", "x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"expected x [..., K] with K at least 1, got {tuple(x.shape)}")
     return _on(x, _quantize, x)
@@ -348,9 +360,12 @@ def mx4_quantize(x):
 
 def group_norm_act_mx4(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
     """``group_norm_act`` with its result in 4 bits, quantised from the 32-bit values: an ``Mx4Tensor`` of shape
-    [batch, ..., channels] for ``mx4_conv1x1``.  Has no gradient."""
-    if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
+    [batch, ..., channels] for ``mx4_conv1x1``.  Has no gradient: an ``x`` that requires one is refused, ``weight`` and ``bias`` that
+    do are taken as they are, with a warning."""
+    if _wants(x):
         raise RuntimeError("group_norm_act_mx4 has no gradient: call it under torch.no_grad(), or use group_norm_act")
+    if _wants(weight) or _wants(bias):
+        warnings.warn("group_norm_act_mx4 has no gradient: weight and bias get none from it (torch.no_grad() says that this is meant)", stacklevel=2)
     return _on(x, _norm_mx4, x, groups, weight, bias, eps, act)
 
 
@@ -379,10 +394,14 @@ def _linear(x, weight, bias, residual, act, out_dtype, pixels):
     quantised = type(x) is Mx4Tensor
     if not quantised:
         _number_tensor(x, "x")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("the 4-bit product has no gradient: call it under torch.no_grad()")
+        if _wants(x):
+            _no_gradient("the 4-bit product", "x")
         if x.dim() < 1:
             raise ValueError("expected x [..., K]")
+    if _wants(bias):
+        _no_gradient("the 4-bit product", "bias")
+    if _wants(residual):
+        _no_gradient("the 4-bit product", "residual")
     shape = x.shape
     if shape[-1] != weight.K:
         raise ValueError(f"x has {shape[-1]} numbers a row, weight {weight.K}")
@@ -436,7 +455,7 @@ def mx4_linear(x, weight, bias=None, residual=None, act="none", out_dtype=None):
 
     ``weight`` is an ``Mx4Tensor`` [N, K]; ``x`` [..., K] is numbers (float32, float16, bfloat16), quantised on the way, or an
     ``Mx4Tensor``.  ``out_dtype`` is x's type unless given (bfloat16 for an Mx4Tensor); ``residual`` [..., N] is of that type,
-    ``bias`` [N] of it or float32.  Has no gradient."""
+    ``bias`` [N] of it or float32.  Has no gradient: an ``x``, ``bias`` or ``residual`` that requires one is refused."""
     return _linear(x, weight, bias, residual, act, out_dtype, False)
 
 

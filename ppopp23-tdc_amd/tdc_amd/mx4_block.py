@@ -34,7 +34,9 @@ class GroupNormAct(nn.Module):
         return group_norm_act(x, self.groups, self.weight, self.bias, self.eps, self.act)
 
     def mx4(self, x):
-        """The result in 4 bits, for ``mx4_conv1x1``."""
+        """The result in 4 bits, for ``mx4_conv1x1``; without a gradient, so that parameters that train need ``torch.no_grad()``."""
+        if torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters()):
+            raise RuntimeError("the norm into 4 bits has no gradient, and its parameters require one: call it under torch.no_grad()")
         return group_norm_act_mx4(x, self.groups, self.weight, self.bias, self.eps, self.act)
 
     def extra_repr(self):

@@ -617,3 +617,38 @@ def test_norm_gradients_of_many_rows_with_one_slope(shape, groups):
         dy = torch.full((), 0.3, device="cuda").expand(shape)
         grads = torch.autograd.grad(tdc_amd.group_norm_act(leaves[0], groups, leaves[1], leaves[2], act=act), leaves, dy)
         check_grads(x, gamma.double().cpu().numpy(), beta.double().cpu().numpy(), dy, grads, groups, act, f"{shape} {act}")
+
+
+# ---- derivatives that the operators do not have ----
+
+def test_4_bit_operators_refuse_what_wants_a_gradient():
+    """None of them drops a gradient without a word: whatever would have to get one is refused, and taken under no_grad."""
+    x = torch.randn(2, 64, 3, 4, device="cuda").contiguous(memory_format=torch.channels_last)
+    wq = tdc_amd.mx4_quantize(torch.randn(64, 64, device="cuda"))
+    bias, xq = torch.randn(64, device="cuda"), tdc_amd.group_norm_act_mx4(x, 4)
+    norm = tdc_amd.GroupNormAct(4, 64).cuda()
+
+    def wanting(t):
+        return t.detach().clone(memory_format=torch.preserve_format).requires_grad_()
+
+    calls = {
+        "x": lambda: tdc_amd.mx4_conv1x1(wanting(x), wq),
+        "bias": lambda: tdc_amd.mx4_conv1x1(x, wq, wanting(bias)),
+        "residual": lambda: tdc_amd.mx4_conv1x1(xq, wq, bias, wanting(x), out_dtype=F32),
+        "residual with a history": lambda: tdc_amd.mx4_conv1x1(xq, wq, None, wanting(x) * 2, out_dtype=F32),
+        "residual of rows": lambda: tdc_amd.mx4_linear(torch.randn(3, 64, device="cuda"), wq, residual=wanting(torch.randn(3, 64, device="cuda"))),
+        "quantised": lambda: tdc_amd.mx4_quantize(wanting(x)),
+        "norm into 4 bits": lambda: tdc_amd.group_norm_act_mx4(wanting(x), 4),
+        "the module's parameters": lambda: norm.mx4(x),
+    }
+    for what, call in calls.items():
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+            pytest.fail(what)
+        with torch.no_grad():
+            call()
+    # as an argument of the function they are taken as numbers, with a warning
+    with pytest.warns(UserWarning, match="no gradient"):
+        q = tdc_amd.group_norm_act_mx4(x, 4, norm.weight, norm.bias)
+    with torch.no_grad():
+        assert torch.equal(q.dequantize(), norm.mx4(x).dequantize())
