@@ -15,6 +15,7 @@ import warnings
 from ctypes import byref
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -69,6 +70,14 @@ def _vector(t, n, dtype, device, what):
 def _wants(t):
     """Whether a gradient would have to reach t."""
     return t is not None and getattr(t, "requires_grad", False) and torch.is_grad_enabled()
+
+
+def _no_tangent(what, *tensors):
+    """Refuses dual tensors of forward mode: they need not require a gradient, and their tangents would be lost."""
+    if getattr(forward_ad, "_current_level", 0) < 0:      # (no level is open: the usual call)
+        return
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no derivative in forward mode")
 
 
 def _no_gradient(what, name):
@@ -205,6 +214,7 @@ class _GroupNormAct(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
+        _no_tangent("the gradient of group_norm_act", dy)
         groups, eps, act = ctx.how
         plan = _norm_for(x, groups, weight, bias, eps, act, dy.stride())
         dev, C = x.device, x.shape[1]
@@ -241,7 +251,8 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
 
     Mean and variance are those of one image and group of channels, in 32 bits; ``act`` is "none", "relu" or "silu".  ``x``
     may be float32, float16 or bfloat16 and a channel slice of a wider tensor; ``weight`` and ``bias`` [channels] float32 or
-    of x's type.  The result is dense channels last, of x's type.  Differentiable once, in x, weight and bias."""
+    of x's type.  The result is dense channels last, of x's type.  Differentiable once, backwards, in x, weight and bias."""
+    _no_tangent("group_norm_act", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         return _on(x, _GroupNormAct.apply, x, weight, bias, groups, eps, act)
@@ -351,6 +362,7 @@ def mx4_quantize(x):
     takes its largest magnitude into [4, 8) and rounded to nearest (halfway to the even code, saturating at 6).  A block with
     an infinity or a NaN stands for NaNs.  Has no gradient: weights that train are put into 4 bits under ``torch.no_grad()``."""
     _number_tensor(x, "x")
+    _no_tangent("mx4_quantize", x)
     if _wants(x):
         _no_gradient("mx4_quantize", "x")
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -362,6 +374,7 @@ def group_norm_act_mx4(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
     """``group_norm_act`` with its result in 4 bits, quantised from the 32-bit values: an ``Mx4Tensor`` of shape
     [batch, ..., channels] for ``mx4_conv1x1``.  Has no gradient: an ``x`` that requires one is refused, ``weight`` and ``bias`` that
     do are taken as they are, with a warning."""
+    _no_tangent("group_norm_act_mx4", x, weight, bias)
     if _wants(x):
         raise RuntimeError("group_norm_act_mx4 has no gradient: call it under torch.no_grad(), or use group_norm_act")
     if _wants(weight) or _wants(bias):
@@ -398,6 +411,7 @@ def _linear(x, weight, bias, residual, act, out_dtype, pixels):
             _no_gradient("the 4-bit product", "x")
         if x.dim() < 1:
             raise ValueError("expected x [..., K]")
+    _no_tangent("the 4-bit product", x, bias, residual)
     if _wants(bias):
         _no_gradient("the 4-bit product", "bias")
     if _wants(residual):

@@ -652,3 +652,27 @@ def test_4_bit_operators_refuse_what_wants_a_gradient():
         q = tdc_amd.group_norm_act_mx4(x, 4, norm.weight, norm.bias)
     with torch.no_grad():
         assert torch.equal(q.dequantize(), norm.mx4(x).dequantize())
+
+
+def test_tangents_are_refused():
+    """Forward mode: a dual tensor need not require a gradient, and its tangent would be lost."""
+    from torch.autograd import forward_ad
+    x = torch.randn(2, 64, 3, 4, device="cuda").contiguous(memory_format=torch.channels_last)
+    w = torch.ones(64, device="cuda")
+    wq = tdc_amd.mx4_quantize(torch.randn(64, 64, device="cuda"))
+    residual = torch.randn(2, 64, 3, 4, device="cuda")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: tdc_amd.group_norm_act(dual, 4), lambda: tdc_amd.group_norm_act(x, 4, forward_ad.make_dual(w, w)),
+                     lambda: tdc_amd.group_norm_act(x, 4, None, forward_ad.make_dual(w, w)), lambda: tdc_amd.group_norm_act_mx4(dual, 4),
+                     lambda: tdc_amd.mx4_quantize(dual), lambda: tdc_amd.mx4_conv1x1(dual, wq),
+                     lambda: tdc_amd.mx4_conv1x1(x, wq, None, forward_ad.make_dual(residual, residual))):
+            with pytest.raises(RuntimeError, match="forward mode"):
+                call()
+        want = tdc_amd.group_norm_act(x, 4, w)
+    assert torch.equal(want, tdc_amd.group_norm_act(x, 4, w))
+    leaf = x.detach().requires_grad_()
+    y = tdc_amd.group_norm_act(leaf, 4)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward mode"):
+            torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
