@@ -291,6 +291,10 @@ class Mx4Tensor:
         t.shape, t.rows, t.K, t.device, t.index = shape, rows, K, device, index
         return t
 
+    def __reduce__(self):
+        # (a copy, also one from a file, finds its addresses anew)
+        return _mx4_again, (self.codes, self.scales, self.shape)
+
     def _byte_shapes(self):
         return ((self.K + 127) // 128, (self.rows + 31) // 32, 4, 32, 16), ((self.K + 511) // 512, self.rows, 16)
 
@@ -326,6 +330,14 @@ class Mx4Tensor:
 
     def __repr__(self):
         return f"Mx4Tensor(shape={self.shape}, device={self.device})"
+
+
+def _mx4_again(codes, scales, shape):
+    t = Mx4Tensor.__new__(Mx4Tensor)
+    t.shape, t.K, t.rows = shape, shape[-1], _product(shape[:-1])
+    t.device, t.index, t._held = codes.device, codes.get_device(), (codes, scales)
+    t._codes_at, t._scales_at = codes.data_ptr(), scales.data_ptr()
+    return t
 
 
 def _product(shape):

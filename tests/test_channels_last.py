@@ -1,5 +1,7 @@
 """What the channels-last operators refuse (no GPU needed), and their 64-bit oracle against hand-worked numbers."""
+import copy
 import ctypes
+import pickle
 
 import numpy as np
 import pytest
@@ -145,3 +147,14 @@ def test_oracle_of_4_bit_numbers():
     assert values[0, :10].tolist() == [6, 4, 4, 2, 2, 1, 0, 0, -6, 6]
     assert codes[0, :10].tolist() == [7, 6, 6, 4, 4, 2, 0, 8, 15, 7]
     assert values[0, 32:35].tolist() == [6 / 64, -3 / 64, 0]      # 0.1 * 64 = 6.4, 0.05 * 64 = 3.2
+
+
+def test_copies_of_a_4_bit_tensor_have_their_own_addresses():
+    """What kernels are handed is where a copy's own bytes lie, not where the original's lay."""
+    q = tdc_amd.Mx4Tensor._new(6, 200, (2, 3, 200), torch.device("cpu"), -1)
+    q._held.random_(0, 255, generator=torch.Generator().manual_seed(1))
+    for other in (copy.copy(q), copy.deepcopy(q), pickle.loads(pickle.dumps(q)), copy.deepcopy(pickle.loads(pickle.dumps(q)))):
+        assert (other.shape, other.rows, other.K, other.device) == (q.shape, 6, 200, q.device)
+        assert torch.equal(other.codes, q.codes) and torch.equal(other.scales, q.scales)
+        assert other._codes_at == other.codes.data_ptr() and other._scales_at == other.scales.data_ptr()
+    assert copy.deepcopy(q)._codes_at != q._codes_at

@@ -676,3 +676,25 @@ def test_tangents_are_refused():
     with forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="forward mode"):
             torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+def test_copies_of_a_4_bit_tensor():
+    import copy
+    import io
+    x = numbers(91, 5, 70, 300).cuda()
+    q = tdc_amd.mx4_quantize(x)
+    file = io.BytesIO()
+    torch.save(q, file)
+    file.seek(0)
+    copies = [copy.deepcopy(q), torch.load(file, weights_only=False), copy.copy(q)]
+    want = q.dequantize()
+    del q
+    torch.full((1 << 20,), 7.0, device="cuda")      # (what the original held may be another's by now)
+    for other in copies:
+        assert torch.equal(other.dequantize(), want)
+    file.seek(0)
+    away = torch.load(file, map_location="cpu", weights_only=False)
+    with pytest.raises(ValueError):
+        away.dequantize()
+    with pytest.raises(ValueError):
+        tdc_amd.mx4_linear(away, tdc_amd.mx4_quantize(torch.ones(4, 300, device="cuda")))
