@@ -11,6 +11,8 @@ far apart they are:
 """
 from __future__ import annotations
 
+import threading
+
 import torch
 from torch import nn
 from torch.nn import functional as F
@@ -48,7 +50,8 @@ class TuckerBlockMx4(nn.Module):
 
     ``forward`` takes and returns channels-last tensors [batch, channels, height, width]; ``x`` is added to the result where
     the channels agree.  The factors are put into 4 bits, and the core packed, when first used and again when the parameters'
-    version counters have moved; writes those do not see (``.data``) need ``invalidate()``."""
+    version counters have moved; writes those do not see (``.data``) need ``invalidate()``.  Threads may share a block: their
+    calls queue their work one at a time."""
 
     MAX_CACHED_SHAPES = 8   # plans of the core kept, least recently used first out
 
@@ -60,12 +63,24 @@ class TuckerBlockMx4(nn.Module):
         self.conv = conv
         self.norm_in = GroupNormAct(groups, conv.in_channels, act=act)
         self.norm_core = GroupNormAct(rank_groups, conv.out_rank, act=act)
-        self.invalidate()
+        self._forget()
+
+    def _forget(self):
+        self._turn = threading.RLock()      # of the thread whose call compares, packs, queues or closes
+        self._factors, self._plans, self._stamp = None, {}, None
+
+    def __getstate__(self):      # (a copy packs its own)
+        return {k: v for k, v in self.__dict__.items() if k not in ("_turn", "_factors", "_plans", "_stamp")}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._forget()
 
     def invalidate(self):
-        for plan in getattr(self, "_plans", {}).values():
-            plan.close()
-        self._factors, self._plans, self._stamp = None, {}, None
+        with self._turn:
+            for plan in self._plans.values():
+                plan.close()
+            self._factors, self._plans, self._stamp = None, {}, None
 
     def _apply(self, fn, *args, **kwargs):
         out = super()._apply(fn, *args, **kwargs)
@@ -85,12 +100,16 @@ class TuckerBlockMx4(nn.Module):
 
     @torch.no_grad()
     def forward(self, x):
+        with self._turn:
+            return self._queue(x)
+
+    def _queue(self, x):
         c = self.conv
         stamp = tuple((p.data_ptr(), p._version) for p in (c.first_kernel, c.core_kernel, c.last_kernel))
         if stamp != self._stamp:
             self.invalidate()
-            self._stamp = stamp
             self._factors = mx4_quantize(c.first_kernel.flatten(1)), mx4_quantize(c.last_kernel.flatten(1))
+            self._stamp = stamp
         first, last = self._factors
         h = mx4_conv1x1(self.norm_in.mx4(x), first, out_dtype=torch.float32)
         h = self._core(tuple(h.shape)).forward(h.contiguous())

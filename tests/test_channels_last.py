@@ -2,6 +2,7 @@
 import copy
 import ctypes
 import pickle
+import threading
 
 import numpy as np
 import pytest
@@ -158,3 +159,131 @@ def test_copies_of_a_4_bit_tensor_have_their_own_addresses():
         assert torch.equal(other.codes, q.codes) and torch.equal(other.scales, q.scales)
         assert other._codes_at == other.codes.data_ptr() and other._scales_at == other.scales.data_ptr()
     assert copy.deepcopy(q)._codes_at != q._codes_at
+
+
+# ---- the block's host side, with stand-ins for everything that needs a device ----
+
+class StandIn:
+    """The block's operators and plans on the host; `calls` names them in order, `at[name]` runs inside the call of that name."""
+
+    def __init__(self, monkeypatch):
+        from tdc_amd import mx4_block
+        self.calls, self.at, self.plans = [], {}, []
+        outer = self
+
+        def said(name):
+            outer.calls.append(name)
+            outer.at.get(name, lambda: None)()
+
+        class Plan:
+            def __init__(self, B, C, N, H, W, *rest):
+                self.open, self.shape, self._h = True, (B, N, H, W), ctypes.c_void_p(1)
+                outer.plans.append(self)
+
+            def set_weights(self, w):
+                said("set_weights")
+                return self
+
+            def forward(self, x):
+                said("core")
+                assert self.open, "the plan was closed while it was in use"
+                return torch.zeros(self.shape)
+
+            def close(self):
+                said("close")
+                self.open = False
+
+        def product(x, w, bias=None, residual=None, out_dtype=None):
+            said("product")
+            return torch.zeros(x.shape[0], w.shape[0], *x.shape[2:])
+
+        def quantize(w):
+            said("quantize")
+            return w.clone()
+
+        for name, value in (("Conv2dPlan", Plan), ("mx4_conv1x1", product), ("mx4_quantize", quantize)):
+            monkeypatch.setattr(mx4_block, name, value)
+        monkeypatch.setattr(mx4_block.GroupNormAct, "mx4", lambda norm, x: x)
+        conv = tdc_amd.TKConv2dC(8, 8, 3, padding=1, hp_dict=tdc_amd.ranks_dict(conv=[4, 4]), name="conv")
+        self.block = tdc_amd.TuckerBlockMx4(conv, groups=2, rank_groups=2)
+        self.x = torch.zeros(2, 8, 5, 5).contiguous(memory_format=torch.channels_last)
+
+
+def in_threads(*bodies):
+    """Runs them, each in a thread; their errors."""
+    errors = []
+
+    def guarded(body):
+        try:
+            body()
+        except BaseException as e:  # noqa: B036
+            errors.append(e)
+
+    threads = [threading.Thread(target=guarded, args=(b,)) for b in bodies]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(20)
+        assert not t.is_alive()
+    return errors
+
+
+def test_block_is_built_once_for_two_threads(monkeypatch):
+    s, inside, second = StandIn(monkeypatch), threading.Event(), threading.Event()
+
+    def first_factor():
+        inside.set()
+        second.wait(0.5)      # (the other thread comes meanwhile, and is held or goes wrong)
+
+    s.at["quantize"] = first_factor
+
+    def other():
+        assert inside.wait(10)
+        s.block(s.x)
+        second.set()
+
+    assert in_threads(lambda: s.block(s.x), other) == []
+    assert s.calls.count("quantize") == 2 and s.calls.count("core") == 2 and len(s.plans) == 1
+
+
+def test_block_is_not_invalidated_under_a_call(monkeypatch):
+    s, inside, done = StandIn(monkeypatch), threading.Event(), threading.Event()
+    s.block(s.x)
+
+    def core():
+        inside.set()
+        done.wait(0.5)
+
+    s.at["core"] = core
+
+    def other():
+        assert inside.wait(10)
+        s.block.invalidate()
+        done.set()
+
+    assert in_threads(lambda: s.block(s.x), other) == []
+    assert not s.plans[0].open
+    s.block(s.x)
+    assert len(s.plans) == 2 and s.plans[1].open
+
+
+def test_block_that_could_not_be_built_is_built_by_the_next_call(monkeypatch):
+    s = StandIn(monkeypatch)
+
+    def fails():
+        del s.at["quantize"]
+        raise MemoryError
+
+    s.at["quantize"] = fails
+    with pytest.raises(MemoryError):
+        s.block(s.x)
+    assert s.block(s.x).shape == (2, 8, 5, 5)
+
+
+def test_block_is_copied_without_what_it_keeps(monkeypatch):
+    s = StandIn(monkeypatch)
+    s.block(s.x)
+    other = copy.deepcopy(s.block)
+    assert other(s.x).shape == (2, 8, 5, 5) and len(s.plans) == 2 and s.plans[0].open
+    s.block(s.x)
+    assert len(s.plans) == 2
