@@ -67,10 +67,10 @@ class TuckerBlockMx4(nn.Module):
 
     def _forget(self):
         self._turn = threading.RLock()      # of the thread whose call compares, packs, queues or closes
-        self._factors, self._plans, self._stamp = None, {}, None
+        self._factors, self._plans, self._packed, self._stamp = None, {}, None, None
 
     def __getstate__(self):      # (a copy packs its own)
-        return {k: v for k, v in self.__dict__.items() if k not in ("_turn", "_factors", "_plans", "_stamp")}
+        return {k: v for k, v in self.__dict__.items() if k not in ("_turn", "_factors", "_plans", "_packed", "_stamp")}
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -80,7 +80,7 @@ class TuckerBlockMx4(nn.Module):
         with self._turn:
             for plan in self._plans.values():
                 plan.close()
-            self._factors, self._plans, self._stamp = None, {}, None
+            self._factors, self._plans, self._packed, self._stamp = None, {}, None, None
 
     def _apply(self, fn, *args, **kwargs):
         out = super()._apply(fn, *args, **kwargs)
@@ -105,11 +105,12 @@ class TuckerBlockMx4(nn.Module):
 
     def _queue(self, x):
         c = self.conv
-        stamp = tuple((p.data_ptr(), p._version) for p in (c.first_kernel, c.core_kernel, c.last_kernel))
+        packed = c.first_kernel, c.core_kernel, c.last_kernel
+        stamp = tuple((id(p), p.data_ptr(), p._version) for p in packed)
         if stamp != self._stamp:
             self.invalidate()
             self._factors = mx4_quantize(c.first_kernel.flatten(1)), mx4_quantize(c.last_kernel.flatten(1))
-            self._stamp = stamp
+            self._packed, self._stamp = packed, stamp      # (parameters that are held keep their ids to themselves)
         first, last = self._factors
         h = mx4_conv1x1(self.norm_in.mx4(x), first, out_dtype=torch.float32)
         h = self._core(tuple(h.shape)).forward(h.contiguous())

@@ -287,3 +287,16 @@ def test_block_is_copied_without_what_it_keeps(monkeypatch):
     assert other(s.x).shape == (2, 8, 5, 5) and len(s.plans) == 2 and s.plans[0].open
     s.block(s.x)
     assert len(s.plans) == 2
+
+
+def test_block_sees_another_parameter_in_the_same_place(monkeypatch):
+    """A new parameter may lie where the old one lay, with the same version."""
+    s, held = StandIn(monkeypatch), np.zeros((4, 8, 1, 1), np.float32)
+    s.block.conv.first_kernel = torch.nn.Parameter(torch.from_numpy(held))
+    s.block(s.x)
+    held += 1
+    s.block.conv.first_kernel = torch.nn.Parameter(torch.from_numpy(held))
+    s.block(s.x)
+    assert s.calls.count("quantize") == 4
+    s.block(s.x)
+    assert s.calls.count("quantize") == 4
