@@ -17,7 +17,7 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
-from .channels_last import group_norm_act, group_norm_act_mx4, mx4_conv1x1, mx4_quantize
+from .channels_last import _on, group_norm_act, group_norm_act_mx4, mx4_conv1x1, mx4_quantize
 from .conv import Conv2dPlan
 
 
@@ -101,7 +101,7 @@ class TuckerBlockMx4(nn.Module):
     @torch.no_grad()
     def forward(self, x):
         with self._turn:
-            return self._queue(x)
+            return _on(x, self._queue, x)      # (the core works on the current device)
 
     def _queue(self, x):
         c = self.conv

@@ -300,3 +300,35 @@ def test_block_sees_another_parameter_in_the_same_place(monkeypatch):
     assert s.calls.count("quantize") == 4
     s.block(s.x)
     assert s.calls.count("quantize") == 4
+
+
+class OnDevice(torch.Tensor):
+    """A host tensor that says it lies on the second device."""
+    is_cuda = property(lambda self: True)
+    device = property(lambda self: torch.device("cuda", 1))
+
+    def get_device(self):
+        return 1
+
+
+def test_block_works_on_the_device_of_its_input(monkeypatch):
+    from tdc_amd import channels_last
+    s, current = StandIn(monkeypatch), [0]
+
+    class Device:
+        def __init__(self, device):
+            self.index = torch.device(device).index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *error):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(channels_last, "_device", lambda: current[0])
+    seen = []
+    for name in ("set_weights", "core"):
+        s.at[name] = lambda: seen.append(current[0])
+    s.block(s.x.as_subclass(OnDevice))
+    assert seen == [1, 1] and current == [0]
