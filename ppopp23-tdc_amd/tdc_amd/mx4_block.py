@@ -18,7 +18,7 @@ from torch import nn
 from torch.nn import functional as F
 
 from .channels_last import _on, group_norm_act, group_norm_act_mx4, mx4_conv1x1, mx4_quantize
-from .conv import Conv2dPlan
+from .conv import Conv2dPlan, _raw_stream
 
 
 class GroupNormAct(nn.Module):
@@ -51,7 +51,9 @@ class TuckerBlockMx4(nn.Module):
     ``forward`` takes and returns channels-last tensors [batch, channels, height, width]; ``x`` is added to the result where
     the channels agree.  The factors are put into 4 bits, and the core packed, when first used and again when the parameters'
     version counters have moved; writes those do not see (``.data``) need ``invalidate()``.  Threads may share a block: their
-    calls queue their work one at a time."""
+    calls queue their work one at a time, and a call on another stream than the last one's waits for that stream on the device (the
+    core's scratch belongs to the block).  A captured call waits for nothing outside its graph: its replays must not overlap other
+    calls, and neither packing nor ``invalidate()`` may happen in a capture."""
 
     MAX_CACHED_SHAPES = 8   # plans of the core kept, least recently used first out
 
@@ -68,9 +70,10 @@ class TuckerBlockMx4(nn.Module):
     def _forget(self):
         self._turn = threading.RLock()      # of the thread whose call compares, packs, queues or closes
         self._factors, self._plans, self._packed, self._stamp = None, {}, None, None
+        self._last = None, None      # the last call's stream, as its handle and itself
 
     def __getstate__(self):      # (a copy packs its own)
-        return {k: v for k, v in self.__dict__.items() if k not in ("_turn", "_factors", "_plans", "_packed", "_stamp")}
+        return {k: v for k, v in self.__dict__.items() if k not in ("_turn", "_factors", "_plans", "_packed", "_stamp", "_last")}
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -78,6 +81,8 @@ class TuckerBlockMx4(nn.Module):
 
     def invalidate(self):
         with self._turn:
+            if self._factors is not None and self._factors[0].device.type == "cuda":
+                torch.cuda.synchronize(self._factors[0].device)      # (streams other than the one they were made on may be reading)
             for plan in self._plans.values():
                 plan.close()
             self._factors, self._plans, self._packed, self._stamp = None, {}, None, None
@@ -105,11 +110,20 @@ class TuckerBlockMx4(nn.Module):
 
     def _queue(self, x):
         c = self.conv
+        if x.is_cuda:
+            stream = _raw_stream(x.get_device())
+            if stream != self._last[0] and not torch.cuda.is_current_stream_capturing():
+                now = torch.cuda.current_stream()
+                if self._last[1] is not None:
+                    now.wait_stream(self._last[1])
+                self._last = stream, now
         packed = c.first_kernel, c.core_kernel, c.last_kernel
         stamp = tuple((id(p), p.data_ptr(), p._version) for p in packed)
         if stamp != self._stamp:
             self.invalidate()
             self._factors = mx4_quantize(c.first_kernel.flatten(1)), mx4_quantize(c.last_kernel.flatten(1))
+            if x.is_cuda:
+                torch.cuda.current_stream().synchronize()      # (whatever stream uses them next)
             self._packed, self._stamp = packed, stamp      # (parameters that are held keep their ids to themselves)
         first, last = self._factors
         h = mx4_conv1x1(self.norm_in.mx4(x), first, out_dtype=torch.float32)

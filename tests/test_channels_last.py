@@ -311,9 +311,37 @@ class OnDevice(torch.Tensor):
         return 1
 
 
+class Streams:
+    """Streams of a device by their numbers: what waits for what is noted among the stand-in's calls."""
+
+    def __init__(self, monkeypatch, s):
+        from tdc_amd import mx4_block
+        self.now, self.capturing = 1, False
+        outer = self
+
+        class Stream:
+            def __init__(self, number):
+                self.number = number
+
+            def synchronize(self):
+                s.calls.append(f"host waits for {self.number}")
+
+            def wait_stream(self, other):
+                s.calls.append(f"{self.number} waits for {other.number}")
+
+        monkeypatch.setattr(mx4_block, "_raw_stream", lambda device: outer.now, raising=False)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream(outer.now))
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: outer.capturing)
+        monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: s.calls.append("host waits for all"))
+        product, quantize = mx4_block.mx4_conv1x1, mx4_block.mx4_quantize
+        monkeypatch.setattr(mx4_block, "mx4_quantize", lambda w: quantize(w).detach().as_subclass(OnDevice))
+        monkeypatch.setattr(mx4_block, "mx4_conv1x1", lambda *a, **k: product(*a, **k).as_subclass(OnDevice))
+
+
 def test_block_works_on_the_device_of_its_input(monkeypatch):
     from tdc_amd import channels_last
     s, current = StandIn(monkeypatch), [0]
+    Streams(monkeypatch, s)
 
     class Device:
         def __init__(self, device):
@@ -332,3 +360,30 @@ def test_block_works_on_the_device_of_its_input(monkeypatch):
         s.at[name] = lambda: seen.append(current[0])
     s.block(s.x.as_subclass(OnDevice))
     assert seen == [1, 1] and current == [0]
+
+
+def test_block_is_ordered_across_streams(monkeypatch):
+    """Factors are there for every stream before the first one uses them; a call on another stream than the last one's waits for it, for
+    the core's scratch is theirs in turn; nothing is freed that a stream may still read.  A capture cannot wait for what lies outside."""
+    from tdc_amd import mx4_block
+    s = StandIn(monkeypatch)
+    streams = Streams(monkeypatch, s)
+    monkeypatch.setattr(mx4_block, "_on", lambda t, call, *args: call(*args))
+    x = s.x.as_subclass(OnDevice)
+
+    def calls(now, capturing=False):
+        s.calls.clear()
+        streams.now, streams.capturing = now, capturing
+        s.block(x)
+        return s.calls
+
+    c = calls(1)
+    assert max(i for i, n in enumerate(c) if n == "quantize") < c.index("host waits for 1") < c.index("product")
+    assert calls(1) == ["product", "core", "product"]
+    assert calls(2) == ["2 waits for 1", "product", "core", "product"]
+    assert calls(2) == ["product", "core", "product"]
+    assert calls(7, capturing=True) == ["product", "core", "product"]
+    assert calls(1) == ["1 waits for 2", "product", "core", "product"]
+    s.calls.clear()
+    s.block.invalidate()
+    assert s.calls[0] == "host waits for all" and "close" in s.calls

@@ -698,3 +698,33 @@ def test_copies_of_a_4_bit_tensor():
         away.dequantize()
     with pytest.raises(ValueError):
         tdc_amd.mx4_linear(away, tdc_amd.mx4_quantize(torch.ones(4, 300, device="cuda")))
+
+
+def test_tucker_block_on_streams_and_in_a_graph():
+    """Same results on two streams in turn, nothing between, after the weights have changed, and from a graph captured on a stream that the block has not seen."""
+    torch.manual_seed(4)
+    conv = tdc_amd.TKConv2dC(96, 96, 3, padding=1, hp_dict=tdc_amd.ranks_dict(conv=[40, 32]), name="conv")
+    block = tdc_amd.TuckerBlockMx4(conv, groups=8, rank_groups=5).cuda()
+    xs = [torch.randn(4, 28, 28, 96, device="cuda").bfloat16().permute(0, 3, 1, 2) for _ in range(6)]
+    sides = torch.cuda.Stream(), torch.cuda.Stream()
+    for change in range(2):
+        with torch.no_grad():
+            conv.first_kernel.mul_(1.5)
+        torch.cuda.synchronize()
+        got = []
+        for i, x in enumerate(xs):
+            with torch.cuda.stream(sides[i % 2]):
+                got.append(block(x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, block(x)) for x, y in zip(xs, got)), change
+    graph, x = torch.cuda.CUDAGraph(), xs[0].clone(memory_format=torch.channels_last)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        held = block(x)
+    for rep in range(4):
+        x.copy_(xs[rep + 1])
+        want = block(x)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want), rep
