@@ -97,9 +97,13 @@ __global__ void __launch_bounds__(256) tdc_mx4_dequantize_kernel(const unsigned 
     }
 }
 
+static long long workgroups(long long rows, int runs) { return (rows + kRows - 1) / kRows * runs; }
+static int runs_of(long long K) { return (int)((mx4_padded(K) / 128 + kSteps - 1) / kSteps); }
+long long mx4_work_items(long long rows, long long K) { return workgroups(rows, runs_of(K)) * 256; }
+
 int launch_mx4_quantize(const void *x, int dtype, long long rows, long long K, long long stride, void *codes, void *scales, void *stream) {
-    const int groups = (int)(mx4_padded(K) / 128), runs = (groups + kSteps - 1) / kSteps;
-    const unsigned grid = (unsigned)((rows + kRows - 1) / kRows * runs);
+    const int groups = (int)(mx4_padded(K) / 128), runs = runs_of(K);
+    const unsigned grid = (unsigned)workgroups(rows, runs);
     const hipStream_t s = (hipStream_t)stream;
     auto *c = (unsigned *)codes, *e = (unsigned *)scales;
     if (dtype == TDC_F32) tdc_mx4_quantize_kernel<TDC_F32><<<grid, 256, 0, s>>>(x, rows, K, stride, groups, runs, c, e);
@@ -110,8 +114,8 @@ int launch_mx4_quantize(const void *x, int dtype, long long rows, long long K, l
 
 int launch_mx4_dequantize(const void *codes, const void *scales, long long rows, long long K, void *y, int dtype, long long stride,
                           void *stream) {
-    const int groups = (int)(mx4_padded(K) / 128), runs = (groups + kSteps - 1) / kSteps;
-    const unsigned grid = (unsigned)((rows + kRows - 1) / kRows * runs);
+    const int groups = (int)(mx4_padded(K) / 128), runs = runs_of(K);
+    const unsigned grid = (unsigned)workgroups(rows, runs);
     const hipStream_t s = (hipStream_t)stream;
     auto *c = (const unsigned *)codes, *e = (const unsigned *)scales;
     if (dtype == TDC_F32) tdc_mx4_dequantize_kernel<TDC_F32><<<grid, 256, 0, s>>>(c, e, rows, K, groups, runs, y, stride);

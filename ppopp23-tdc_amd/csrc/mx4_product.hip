@@ -538,11 +538,14 @@ static int launch_short(const ProductArgs &a, hipStream_t s) {
     fn<<<grid, 256, L::short_lds(a.ksteps), s>>>(a, tm, tn);
     return (int)hipGetLastError();
 }
+// A wave for every 512 numbers of K, four to sixteen of them; sixteen also to make many numbers into 4 bits.
+static int few_waves(long long M, int ksteps, bool numbers) {
+    const int groups = (ksteps + 3) / 4;
+    return groups > 8 || (numbers && std::min(M, 32ll) * ksteps > 64) ? 16 : groups > 4 ? 8 : 4;
+}
 template <int DT, int XS>
 static int launch_few(const ProductArgs &a, hipStream_t s) {
-    // A wave for every 512 numbers of K, four to sixteen of them; sixteen also to make many numbers into 4 bits.
-    const int groups = (a.ksteps + 3) / 4, rows = (int)std::min(a.M, 32ll);
-    const int waves = groups > 8 || (XS != TDC_MX4 && rows * a.ksteps > 64) ? 16 : groups > 4 ? 8 : 4;
+    const int groups = (a.ksteps + 3) / 4, rows = (int)std::min(a.M, 32ll), waves = few_waves(a.M, a.ksteps, XS != TDC_MX4);
     const int x_bytes = XS == TDC_MX4 ? 0 : rows * (a.ksteps * 64 + groups * 16), lds = std::max(std::min(waves, groups) * 4096, x_bytes);
     const unsigned bm = (unsigned)((a.M + 31) / 32), bn = (unsigned)((a.N + 31) / 32);
     tdc_mx4_product_few_kernel<DT, XS><<<bm * bn, waves * 64, lds, s>>>(a, (int)bm);
@@ -556,17 +559,25 @@ static int launch_few(const ProductArgs &a, hipStream_t s) {
 //   x 512 16.9 against 17.6 (more than 512 would leave a compute unit one workgroup);
 //   tiles of 256 for long sums that fill the compute units: 4096 x 8192 x 8192 164 against 184, 25088 x 512 x 8192 69 against 78, but
 //   8192 x 8192 x 2048 114 against 112 (a tile's first loads and its stores run alone) and 1024 x 8192 x 8192 64 against 45.
+static long long tiles(long long M, long long N, long long edge) { return ((M + edge - 1) / edge) * ((N + edge - 1) / edge); }
+enum { kFew, kShort, kTiles128, kTiles256 };
+static int pick(long long M, long long N, int ksteps) {
+    if (tiles(M, N, 32) <= (ksteps <= 4 ? 1024 : 512)) return kFew;
+    if (ksteps <= 4) return kShort;
+    return ksteps >= 32 && tiles(M, N, 256) >= 192 ? kTiles256 : kTiles128;
+}
 template <int DT>
 static int launch_product(const ProductArgs &a, hipStream_t s) {
     if (a.x) {
         if (a.x_dtype == TDC_F32) return launch_few<DT, TDC_F32>(a, s);
         return a.x_dtype == TDC_F16 ? launch_few<DT, TDC_F16>(a, s) : launch_few<DT, TDC_BF16>(a, s);
     }
-    auto tiles = [&](long long edge) { return ((a.M + edge - 1) / edge) * ((a.N + edge - 1) / edge); };
-    if (tiles(32) <= (a.ksteps <= 4 ? 1024 : 512)) return launch_few<DT, TDC_MX4>(a, s);
-    if (a.ksteps <= 4) return launch_short<DT>(a, s);
-    if (a.ksteps >= 32 && tiles(256) >= 192) return launch_tile<DT, 4, 4>(a, s);
-    return launch_tile<DT, 2, 2>(a, s);
+    switch (pick(a.M, a.N, a.ksteps)) {
+        case kFew: return launch_few<DT, TDC_MX4>(a, s);
+        case kShort: return launch_short<DT>(a, s);
+        case kTiles256: return launch_tile<DT, 4, 4>(a, s);
+        default: return launch_tile<DT, 2, 2>(a, s);
+    }
 }
 
 // x as it comes, without a launch of its own: 64 Ki numbers a workgroup (34 KiB of LDS), as each repeats the work for its rows; eight
@@ -574,6 +585,14 @@ static int launch_product(const ProductArgs &a, hipStream_t s) {
 bool product_takes_numbers(long long M, long long N, long long K) {
     const long long rows = std::min(M, 32ll), workgroups = ((M + 31) / 32) * ((N + 31) / 32);
     return rows * mx4_padded(K) <= 65536 && (M <= 8 || workgroups <= 256);
+}
+
+long long product_work_items(long long M, long long N, long long K, bool numbers) {
+    const int ksteps = (int)(mx4_padded(K) / 128);
+    const bool taken = numbers && product_takes_numbers(M, N, K);
+    const int kernel = taken ? kFew : pick(M, N, ksteps);
+    if (kernel == kFew) return tiles(M, N, 32) * few_waves(M, ksteps, taken) * 64;
+    return (tiles(M, N, kernel == kTiles256 ? 256 : 128) + 7) / 8 * 8 * 256;
 }
 
 int launch_mx4_product(const ProductArgs &a, int y_dtype, void *stream) {

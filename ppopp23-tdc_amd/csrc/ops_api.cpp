@@ -15,6 +15,7 @@ int launched(const char *what, int err) {
     return err ? api_fail(TDC_ERR_HIP, std::string(what) + ": " + hipGetErrorString((hipError_t)err)) : (int)TDC_OK;
 }
 bool number(int dtype) { return dtype == TDC_F32 || dtype == TDC_F16 || dtype == TDC_BF16; }
+constexpr long long kMostItems = (1ll << 32) - 1;      // of a launch
 bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (unsigned)(bytes - 1)) == 0; }
 
 // ---- group norm ----
@@ -120,10 +121,13 @@ int norm_check(const tdc_group_norm_desc *desc, tdc_group_norm_desc &d) {
         if (*pair.second == 0) *pair.second = d.pixels * *pair.first;
         if (d.batch > 1 && *pair.second < image) return invalid("group norm: an image stride below one image");
     }
-    for (bool grad : {false, true}) {
-        const NormPlan n = norm_plan(d, false, grad);
-        if ((long long)d.batch * n.tiles * n.chunks > (1ll << 30) || n.slots > (1 << 24)) return invalid("group norm: too large");
-    }
+    return TDC_OK;
+}
+// Whether the plan's launches can be made (the gradient's second one has workgroups for the parameters as well).
+int plan_check(const tdc_group_norm_desc &d, const NormPlan &n, bool grad) {
+    const long long workgroups = (long long)d.batch * n.tiles * n.chunks + (grad ? (2ll * d.C + 3) / 4 : 0);
+    if (workgroups > kMostItems / std::max(n.threads, grad ? 256 : 0) || n.slots > (1 << 24))
+        return invalid("group norm: too large, a launch has fewer than 2^32 work items");
     return TDC_OK;
 }
 
@@ -160,6 +164,7 @@ int ws_check(const char *what, const void *ws, size_t have, size_t need) {
 int mx4_range(const char *what, long long rows, long long K) {
     if (rows < 0 || K < 1) return invalid(std::string(what) + ": rows has to be 0 and K 1 at least");
     if (K > (1ll << 30) || rows > (1ll << 35) / mx4_padded(K) * 32) return invalid(std::string(what) + ": more numbers than 2^40");
+    if (mx4_work_items(rows, K) > kMostItems) return invalid(std::string(what) + ": too many rows, a launch has fewer than 2^32 work items");
     return TDC_OK;
 }
 int mx4_check(const char *what, long long rows, long long K, const void *codes, const void *scales) {
@@ -176,7 +181,7 @@ int linear_check(const tdc_mx4_linear_desc *desc, tdc_mx4_linear_desc &d) {
     if (!desc) return invalid("4-bit product: null descriptor");
     d = *desc;
     if (d.M < 0 || d.N < 0 || d.K < 1) return invalid("4-bit product: M, N and K have to be 0, 0 and 1 at least");
-    if (d.K > (1ll << 24) || d.M > (1ll << 34) || d.N > (1ll << 34) || d.M * d.N > (1ll << 40))
+    if (d.K > (1ll << 24) || d.M > (1ll << 34) || d.N > (1ll << 34) || d.M > (1ll << 40) / std::max<long long>(d.N, 1))
         return invalid("4-bit product: K above 2^24 or M * N above 2^40");
     if (d.x_dtype != TDC_MX4 && !number(d.x_dtype)) return invalid("4-bit product: unknown x_dtype");
     if (!number(d.y_dtype)) return invalid("4-bit product: y_dtype has to be TDC_F32, TDC_F16 or TDC_BF16");
@@ -187,6 +192,10 @@ int linear_check(const tdc_mx4_linear_desc *desc, tdc_mx4_linear_desc &d) {
     if (!d.residual_stride) d.residual_stride = d.N;
     if (d.x_dtype != TDC_MX4 && d.M > 1 && d.x_stride < d.K) return invalid("4-bit product: a row stride of x below K");
     if (d.M > 1 && (d.y_stride < d.N || d.residual_stride < d.N)) return invalid("4-bit product: a row stride below N");
+    const bool numbers = d.x_dtype != TDC_MX4;
+    if (product_work_items(d.M, d.N, d.K, numbers) > kMostItems ||
+        (numbers && !product_takes_numbers(d.M, d.N, d.K) && mx4_work_items(d.M, d.K) > kMostItems))
+        return invalid("4-bit product: too large, a launch has fewer than 2^32 work items");
     return TDC_OK;
 }
 size_t linear_codes(const tdc_mx4_linear_desc &d) { return (size_t)mx4_code_bytes(d.M, d.K); }
@@ -211,8 +220,11 @@ extern "C" {
 int tdc_group_norm_workspace(const tdc_group_norm_desc *desc, size_t *forward_bytes, size_t *backward_bytes) TDC_ENTRY {
     tdc_group_norm_desc d;
     if (int st = norm_check(desc, d)) return st;
-    if (forward_bytes) *forward_bytes = forward_ws(d, norm_plan(d, false, false));
-    if (backward_bytes) *backward_bytes = backward_ws(d, norm_plan(d, false, true));
+    const NormPlan forward = norm_plan(d, false, false), backward = norm_plan(d, false, true);
+    if (int st = plan_check(d, forward, false)) return st;
+    if (int st = plan_check(d, backward, true)) return st;
+    if (forward_bytes) *forward_bytes = forward_ws(d, forward);
+    if (backward_bytes) *backward_bytes = backward_ws(d, backward);
     return TDC_OK;
 }
 TDC_ENTRY_END
@@ -221,7 +233,9 @@ int tdc_group_norm_mx4_workspace(const tdc_group_norm_desc *desc, size_t *bytes)
     tdc_group_norm_desc d;
     if (int st = norm_check(desc, d)) return st;
     if (!bytes) return invalid("group norm: null argument");
-    *bytes = forward_ws(d, norm_plan(d, true, false));
+    const NormPlan plan = norm_plan(d, true, false);
+    if (int st = plan_check(d, plan, false)) return st;
+    *bytes = forward_ws(d, plan);
     return TDC_OK;
 }
 TDC_ENTRY_END
@@ -233,6 +247,7 @@ int tdc_group_norm_forward(const tdc_group_norm_desc *desc, const void *x, const
     if (!d.batch || !d.pixels) return TDC_OK;
     if (!x || !y) return invalid("group norm: null x or y");
     const NormPlan plan = norm_plan(d, false, false);
+    if (int st = plan_check(d, plan, false)) return st;
     if (int st = ws_check("group norm", ws, ws_bytes, forward_ws(d, plan))) return st;
     NormArgs a = norm_args(d, x, gamma, beta);
     a.out = y;
@@ -253,8 +268,9 @@ int tdc_group_norm_forward_mx4(const tdc_group_norm_desc *desc, const void *x, c
     if (int st = norm_check(desc, d)) return st;
     if (!d.batch || !d.pixels) return TDC_OK;
     if (!x) return invalid("group norm: null x");
-    if (int st = mx4_check("group norm", d.batch * d.pixels, d.C, codes, scales)) return st;
     const NormPlan plan = norm_plan(d, true, false);
+    if (int st = plan_check(d, plan, false)) return st;
+    if (int st = mx4_check("group norm", d.batch * d.pixels, d.C, codes, scales)) return st;
     if (int st = ws_check("group norm", ws, ws_bytes, forward_ws(d, plan))) return st;
     NormArgs a = norm_args(d, x, gamma, beta);
     a.codes = (unsigned char *)codes;
@@ -282,6 +298,7 @@ int tdc_group_norm_backward(const tdc_group_norm_desc *desc, const void *x, cons
     }
     if (!x || !dy || !mean || !rstd) return invalid("group norm: null x, dy, mean or rstd");
     const NormPlan plan = norm_plan(d, false, true);
+    if (int st = plan_check(d, plan, true)) return st;
     if (int st = ws_check("group norm", ws, ws_bytes, backward_ws(d, plan))) return st;
     NormArgs a = norm_args(d, x, gamma, beta);
     a.dy = dy;

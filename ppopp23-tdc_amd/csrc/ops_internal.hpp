@@ -79,6 +79,7 @@ struct NormArgs {
 int launch_norm_forward(const NormArgs &a, int dtype, void *stream);
 int launch_norm_backward(const NormArgs &a, int dtype, void *stream);
 
+long long mx4_work_items(long long rows, long long K);      // of either launch
 int launch_mx4_quantize(const void *x, int dtype, long long rows, long long K, long long stride, void *codes, void *scales, void *stream);
 int launch_mx4_dequantize(const void *codes, const void *scales, long long rows, long long K, void *y, int dtype, long long stride,
                           void *stream);
@@ -95,6 +96,7 @@ struct ProductArgs {
     int bias_dtype, act;
 };
 bool product_takes_numbers(long long M, long long N, long long K);
+long long product_work_items(long long M, long long N, long long K, bool numbers);
 int launch_mx4_product(const ProductArgs &a, int y_dtype, void *stream);
 
 }  // namespace tdc

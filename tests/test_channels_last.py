@@ -387,3 +387,43 @@ def test_block_is_ordered_across_streams(monkeypatch):
     s.calls.clear()
     s.block.invalidate()
     assert s.calls[0] == "host waits for all" and "close" in s.calls
+
+
+# ---- sizes that no launch can have ----
+
+def test_4_bit_numbers_of_more_rows_than_a_launch_has():
+    """A launch has fewer than 2^32 work items: 16 rows (and 512 numbers of each) take 256."""
+    L, c, s = tdc_amd.lib(), ctypes.c_size_t(), ctypes.c_size_t()
+    for rows, K in (((1 << 28) - 15, 32), ((1 << 27) - 15, 513), (1 << 28, 512), (1 << 33, 128), ((1 << 26) - 15, 2000)):
+        for call in (lambda: L.tdc_mx4_sizes(rows, K, ctypes.byref(c), ctypes.byref(s)), lambda: L.tdc_mx4_quantize(16, 1, rows, K, 0, 16, 16, None),
+                     lambda: L.tdc_mx4_dequantize(16, 16, rows, K, 16, 1, 0, None)):
+            assert call() == INVALID and "2^32" in error(), (rows, K)
+    for rows, K in (((1 << 28) - 16, 512), ((1 << 27) - 16, 513), ((1 << 26) - 16, 2000)):
+        assert L.tdc_mx4_sizes(rows, K, ctypes.byref(c), ctypes.byref(s)) == 0
+        assert c.value >= rows * K // 2
+
+
+@pytest.mark.parametrize("desc", [dict(batch=1 << 26, C=2048, groups=32, dtype=2, pixels=1), dict(batch=1 << 24, C=16, groups=2, pixels=1 << 16),
+                                  dict(batch=(1 << 31) - 1, C=8, groups=1, pixels=1)])
+def test_norms_of_more_workgroups_than_a_launch_has(desc):
+    L, d, a, b = tdc_amd.lib(), norm(**desc), ctypes.c_size_t(), ctypes.c_size_t()
+    assert L.tdc_group_norm_workspace(ctypes.byref(d), ctypes.byref(a), ctypes.byref(b)) == INVALID and "too large" in error()
+    assert L.tdc_group_norm_mx4_workspace(ctypes.byref(d), ctypes.byref(a)) == INVALID and "too large" in error()
+    assert L.tdc_group_norm_forward(ctypes.byref(d), 16, None, None, 16, None, None, 16, 1 << 60, None) == INVALID
+    assert L.tdc_group_norm_forward_mx4(ctypes.byref(d), 16, None, None, 16, 16, 16, 1 << 60, None) == INVALID
+    assert L.tdc_group_norm_backward(ctypes.byref(d), 16, 16, None, None, 16, 16, 16, None, None, 16, 1 << 60, None) == INVALID
+
+
+@pytest.mark.parametrize("desc", [dict(M=8, N=1 << 31, K=32, x_dtype=1), dict(M=1 << 31, N=64, K=512, x_dtype=3),
+                                  dict(M=1 << 29, N=64, K=64, x_dtype=2), dict(M=1 << 33, N=64, K=8192, x_dtype=3)])
+def test_products_of_more_tiles_than_a_launch_has(desc):
+    L, n, d = tdc_amd.lib(), ctypes.c_size_t(), linear(**desc)
+    assert L.tdc_mx4_linear_workspace(ctypes.byref(d), ctypes.byref(n)) == INVALID and "2^32" in error()
+    assert L.tdc_mx4_linear(ctypes.byref(d), 16, 16, 16, 16, None, None, 16, 16, 1 << 60, None) == INVALID
+
+
+def test_products_of_more_outputs_than_64_bits_count():
+    L, n = tdc_amd.lib(), ctypes.c_size_t()
+    for size in (1 << 32, 1 << 34):
+        d = linear(M=size, N=size)
+        assert L.tdc_mx4_linear_workspace(ctypes.byref(d), ctypes.byref(n)) == INVALID and "2^40" in error()
