@@ -554,15 +554,19 @@ def test_norm_module_trains():
 # ---- sums that meet large and small numbers ----
 
 def check_forward_on_device(y, x, groups, what):
-    """check_forward without parameters, for tensors that are long work for the host: in 64 bits by torch."""
-    v = x.double().permute(0, 2, 3, 1).reshape(x.shape[0], -1, groups, x.shape[1] // groups)
-    mean = v.mean((1, 3), keepdim=True)
-    v = v - mean
-    rstd = 1 / torch.sqrt((v * v).mean((1, 3), keepdim=True) + 1e-5)
-    want = v * rstd
-    bound = E * want.abs() + 16 * E * (want.abs() + mean.abs() * rstd)
-    off = (y.double().permute(0, 2, 3, 1).reshape(v.shape) - want).abs()
-    assert bool((off <= bound).all()), (what, float((off / bound.clamp(min=1e-300)).max()))
+    """check_forward without parameters, for tensors that are long work for the host, which only adds up the statistics (torch's
+    reductions of many numbers to few, on the device, are not always right)."""
+    B, C = x.shape[:2]
+    for b in range(B):
+        v, got = (t[b].permute(1, 2, 0).reshape(-1, groups, C // groups).double() for t in (x, y))
+        host = v.cpu().numpy()
+        mean = host.mean(axis=(0, 2), keepdims=True)
+        rstd = 1 / np.sqrt(((host - mean) ** 2).mean(axis=(0, 2), keepdims=True) + 1e-5)
+        mean, rstd = torch.from_numpy(mean).cuda(), torch.from_numpy(rstd).cuda()
+        want = (v - mean) * rstd
+        bound = E * want.abs() + 16 * E * (want.abs() + mean.abs() * rstd)
+        far = ((got - want).abs() / bound.clamp(min=1e-300)).amax(dim=2).cpu().numpy().max()
+        assert far <= 1, (what, b, far)
 
 
 @pytest.mark.parametrize("shape,groups", [((1, 128, 112, 112), 32), ((1, 3, 1460, 1460), 1), ((1, 4, 2535, 2535), 2), ((1, 1, 5800, 5800), 1),
