@@ -163,7 +163,8 @@ _norms = _Cache()
 
 
 def _norm_for(x, groups, weight, bias, eps, act, y_stride=None):
-    wd = weight.dtype if weight is not None else bias.dtype if bias is not None else None
+    given = weight if weight is not None else bias
+    wd = getattr(given, "dtype", None)
     key = (x.shape, x.stride(), y_stride, x.dtype, x.device, wd, weight is None, bias is None, groups, eps, act)
     plan = _norms.get(key)
     if plan is None:
@@ -173,10 +174,12 @@ def _norm_for(x, groups, weight, bias, eps, act, y_stride=None):
         C = x.shape[1]
         if isinstance(groups, bool) or not isinstance(groups, int) or groups < 1 or C % groups:
             raise ValueError(f"groups has to be a whole number that divides the {C} channels: got {groups!r}")
+        _vector(weight, C, x.dtype, x.device, "weight")
+        _vector(bias, C, x.dtype, x.device, "bias")
         plan = _norms.keep(key, _Norm(tuple(x.shape), x.stride(), y_stride, x.dtype, wd or torch.float32, groups, float(eps), _act(act)))
     if weight is not None or bias is not None:
         for t, what in ((weight, "weight"), (bias, "bias")):
-            if t is not None and (t.dtype != wd or t.dim() != 1 or t.shape[0] != x.shape[1] or t.device != x.device or not t.is_contiguous()):
+            if t is not None and (getattr(t, "dtype", None) != wd or wd is None or t.dim() != 1 or t.shape[0] != x.shape[1] or t.device != x.device or not t.is_contiguous()):
                 _vector(t, x.shape[1], x.dtype, x.device, what)
                 raise TypeError("weight and bias have to be of one type")
         if wd != torch.float32 and wd != x.dtype:
@@ -253,8 +256,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none"):
     may be float32, float16 or bfloat16 and a channel slice of a wider tensor; ``weight`` and ``bias`` [channels] float32 or
     of x's type.  The result is dense channels last, of x's type.  Differentiable once, backwards, in x, weight and bias."""
     _no_tangent("group_norm_act", x, weight, bias)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
+    if torch.is_grad_enabled() and (x.requires_grad or getattr(weight, "requires_grad", False) or getattr(bias, "requires_grad", False)):
         return _on(x, _GroupNormAct.apply, x, weight, bias, groups, eps, act)
     return _on(x, _norm_forward, x, groups, weight, bias, eps, act, False)[0]
 

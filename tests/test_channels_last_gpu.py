@@ -732,3 +732,22 @@ def test_tucker_block_on_streams_and_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(held, want), rep
+
+
+# ---- arguments ----
+
+def test_norm_parameters_of_other_types_are_refused_by_name():
+    x = torch.randn(2, 8, 3, 3, device="cuda").contiguous(memory_format=torch.channels_last)
+    w = torch.ones(8, device="cuda")
+    for call in (tdc_amd.group_norm_act, tdc_amd.group_norm_act_mx4):
+        for bad in (w.double(), w.int()):
+            with pytest.raises(TypeError, match="weight has to be float32"):
+                call(x, 2, bad)
+            with pytest.raises(TypeError, match="bias has to be float32"):
+                call(x, 2, None, bad)
+        with pytest.raises(ValueError, match="weight must be a tensor"):
+            call(x, 2, [1.0] * 8)
+        with pytest.raises(ValueError, match="bias must be a tensor"):
+            call(x, 2, w, 1.0)
+        with pytest.raises(ValueError, match="weight must be a tensor"):
+            call(x, 2, w.cpu())
