@@ -353,7 +353,7 @@ def _rows(t):
     """t as evenly spaced rows of neighbouring numbers (copied if it is not), and the distance between rows."""
     K = t.shape[-1]
     if t.dim() != 2:
-        t = t.reshape(-1, K)
+        t = t.reshape(_product(t.shape[:-1]), K)
     step = t.stride(0) if t.shape[0] > 1 else K
     if (K > 1 and t.stride(1) != 1) or step < K:
         t = t.contiguous()

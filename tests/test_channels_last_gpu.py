@@ -751,3 +751,16 @@ def test_norm_parameters_of_other_types_are_refused_by_name():
             call(x, 2, w, 1.0)
         with pytest.raises(ValueError, match="weight must be a tensor"):
             call(x, 2, w.cpu())
+
+
+def test_product_with_no_outputs_or_no_rows():
+    none, some = tdc_amd.mx4_quantize(torch.empty(0, 64, device="cuda")), tdc_amd.mx4_quantize(torch.ones(5, 64, device="cuda"))
+    for lead in ((2, 3), (0, 3), (4,), ()):
+        x = torch.ones(*lead, 64, device="cuda")
+        for w, N in ((none, 0), (some, 5)):
+            for residual in (None, torch.ones(*lead, N, device="cuda")):
+                y = tdc_amd.mx4_linear(x, w, torch.ones(N, device="cuda"), residual)
+                assert y.shape == (*lead, N)
+                assert bool((y == 65 + (residual is not None)).all())
+    x = torch.ones(2, 64, 3, 3, device="cuda").contiguous(memory_format=torch.channels_last)
+    assert tdc_amd.mx4_conv1x1(x, none, residual=torch.ones(2, 0, 3, 3, device="cuda")).shape == (2, 0, 3, 3)
