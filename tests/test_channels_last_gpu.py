@@ -764,3 +764,36 @@ def test_product_with_no_outputs_or_no_rows():
                 assert bool((y == 65 + (residual is not None)).all())
     x = torch.ones(2, 64, 3, 3, device="cuda").contiguous(memory_format=torch.channels_last)
     assert tdc_amd.mx4_conv1x1(x, none, residual=torch.ones(2, 0, 3, 3, device="cuda")).shape == (2, 0, 3, 3)
+
+
+# ---- what only the C entries have ----
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape,groups", [((2, 64, 9, 9), 8), ((3, 48, 70, 90), 4), ((2, 33, 5, 9), 1), ((1, 4104, 40, 5), 1), ((1, 2600, 1, 9), 1300)])
+def test_norm_into_a_slice_and_its_statistics(shape, groups, dtype):
+    """y with strides of its own (nothing beside it is touched), mean and rstd as the entry returns them: off by some ten roundings of what
+    they come from."""
+    from tdc_amd import _lib
+    x, gamma, beta = norm_case(93, shape, dtype)
+    B, C, pixels = shape[0], shape[1], math.prod(shape[2:])
+    wide = torch.full((B, pixels + 2, C + 5), -7.0, dtype=dtype, device="cuda")
+    y = wide[:, 1:1 + pixels, 3:3 + C]
+    kind = {F32: 0, F16: 1, BF16: 2}[dtype]
+    desc = _lib.GroupNormDesc(B, C, groups, 2, kind, 0, 1e-5, 0, pixels, 0, 0, y.stride(1), y.stride(0))
+    need = ctypes.c_size_t()
+    assert tdc_amd.lib().tdc_group_norm_workspace(ctypes.byref(desc), ctypes.byref(need), None) == 0
+    ws = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda")
+    stats = torch.full((2, B, groups), float("nan"), device="cuda")
+    gd, bd = gamma.cuda(), beta.cuda()
+    assert tdc_amd.lib().tdc_group_norm_forward(ctypes.byref(desc), x.data_ptr(), gd.data_ptr(), bd.data_ptr(), y.data_ptr(), stats[0].data_ptr(),
+                                                stats[1].data_ptr(), ws.data_ptr(), need.value, torch.cuda.current_stream().cuda_stream) == 0
+    check_forward(y.permute(0, 2, 1), x.reshape(B, C, pixels), groups, gamma.double().numpy(), beta.double().numpy(), "silu")
+    beside = torch.ones_like(wide, dtype=torch.bool)
+    beside[:, 1:1 + pixels, 3:3 + C] = False
+    assert bool((wide[beside] == -7.0).all())
+    v = rows(x).reshape(B, pixels, groups, C // groups)
+    mean, var = v.mean(axis=(1, 3)), v.var(axis=(1, 3))
+    got = stats.double().cpu().numpy()
+    rstd = 1 / np.sqrt(var + 1e-5)
+    assert (np.abs(got[0] - mean) <= E * np.abs(mean) + 1e-12 * np.abs(v).max()).all()
+    assert (np.abs(got[1] / rstd - 1) <= 10 * E).all()
