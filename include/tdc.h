@@ -411,7 +411,8 @@ int tdc_get_autotune(void);
  * between calls: a call's scratch is the `ws` it is handed (at least the bytes the *_workspace function names for the
  * same descriptor, 16-byte aligned, not shared by calls that can overlap on the device).  Nothing is allocated, nothing is
  * waited for, results are the same on every run, and calls may be captured into a HIP graph.  Outputs must not overlap
- * inputs.  Sizes of zero are legal and launch nothing. */
+ * inputs.  Sizes of zero are legal and launch nothing; sizes for which a launch would need 2^32 work items (some 2^24
+ * workgroups, as of 2^28 rows of up to 512 numbers into 4 bits) are refused. */
 typedef enum tdc_dtype { TDC_F32 = 0, TDC_F16 = 1, TDC_BF16 = 2, TDC_MX4 = 3 } tdc_dtype;
 typedef enum tdc_act { TDC_ACT_NONE = 0, TDC_ACT_RELU = 1, TDC_ACT_SILU = 2 } tdc_act;
 

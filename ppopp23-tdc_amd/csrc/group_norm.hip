@@ -16,7 +16,7 @@
 // costs the others theirs.  Everything else between load and store is fp32.
 //
 // Measured (16 bits): 32 x 56 x 56 x 256, relu, one launch: 21.7 us, 4.7 TB/s where a copy of that size reaches 5.1.  32 x 112 x 112 x 128,
-// silu, two launches: 31 us of statistics behind another kernel's write-back (25 by themselves, 4.1 TB/s) and 34.5 for the rest, 6.0 TB/s as
+// silu, two launches: 31.5 us of statistics behind another kernel's write-back (3.3 TB/s) and 35 for the rest, 5.9 TB/s as
 // part of x comes from the caches.  32 x 28 x 28 x 512, silu, into 4 bits: 17.2 us, of which the vector unit is busy for 62 % (25
 // instructions a number: two passes over the statistics, exp2 and a reciprocal, scale and codes) in turn with the loads.  One image of
 // 7 x 7 x 512: 5.0 us, of which an empty launch is 2.5.

@@ -14,7 +14,7 @@
 // added in 64 bits, for there is no limit to how many of them there are: 3e5 images of two pixels with one dy everywhere, whose additions
 // are all rounded the same way, had dbeta 2e-5 off.
 //
-// Measured: 32 x 112 x 112 x 128 in 16 bits, silu: 40 us for the sums (5.1 TB/s) and 55 for dx (5.6), the vector unit busy for 60 to 70 % beside
+// Measured: 32 x 112 x 112 x 128 in 16 bits, silu: 40.5 us for the sums (5.1 TB/s) and 55.5 for dx (5.5), the vector unit busy for 60 to 70 % beside
 // the memory.  28 x 28 x 256: 12 us, latencies of two launches; 14 x 14 x 1024: 10.4, one launch and that of the parameters.
 #include "norm_device.hpp"
 

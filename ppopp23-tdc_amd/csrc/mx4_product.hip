@@ -69,9 +69,10 @@ static __device__ __forceinline__ void finish8(const ProductArgs &a, long long m
 // memory: a block's read is 1 KiB in a row, which meets no bank twice.
 //
 // Measured, tiles of 256, 8192 x 8192 x 8192 in random codes: 316 us, 3.5 PFLOP/s; 237 on zeros, 4.7, so that a quarter of it is the clock that
-// the power leaves.  Without the outputs 294 and 202, without new codes besides 233 and 181 (registers only: 172 and 124).  The same
-// workgroups going from tile to tile, the next one's codes on their way while this one's outputs leave, took as long: the work saved is
-// waiting, which needs no power.
+// the power leaves.  Without the outputs 294 and 202, without new codes besides 233 and 181 (registers only: 172 and 124).  On zeros, where
+// power does not bind, half of the matrix unit's time is idle all the same; on random codes matrix instructions take half of the busy
+// cycles and LDS 28 %: one wave a SIMD with a barrier every step keeps neither full.  The same workgroups going from tile to tile, the next one's codes on their way while this one's outputs
+// leave, took as long.
 //
 // The row of w that is row r of a block: bits 2 and 3 change places, which makes a lane's outputs 8 i .. 8 i + 7 neighbours.
 static __device__ __forceinline__ int weight_row(int r) { return (r & 19) | (r & 4) << 1 | (r & 8) >> 1; }
@@ -384,8 +385,8 @@ __global__ void __launch_bounds__(256, (DT == TDC_F32 ? 2 : 3)) tdc_mx4_product_
 // in LDS, in the order of the waves.  XS: x in 4 bits (TDC_MX4), or numbers of that type, which a workgroup makes into 4 bits in LDS
 // by itself: for few rows that costs less than a launch.
 //
-// Measured: one row of 4096 by 16384 weights, x in bf16: 8.0 to 9.8 us (36 MB, 3.7 to 4.5 TB/s); 33 rows of 2000 by 1001, x in fp32: 11.4, a chain
-// of latencies (x, its codes, weights, the waves' sums); 196 rows of 1024 by 256 in 4 bits: 5.6.
+// Measured: one row of 4096 by 16384 weights, x in bf16: 8.0 to 9.8 us (36 MB, 3.7 to 4.5 TB/s); 33 rows of 2000 by 1001, x in fp32: 11.4, 64
+// workgroups of which every one across makes the same 32 rows into 4 bits, one after the other with weights and sums; 196 rows of 1024 by 256 in 4 bits: 5.6.
 // `rows` rows of x from row m0 on into codes in LDS, eight numbers a thread, four such runs on their way: block b of row m at
 // (b rows + m) 16, its scale byte behind all codes, words of four steps.
 template <int XS>
@@ -552,7 +553,8 @@ static int launch_few(const ProductArgs &a, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
-// Timed in turn over M 16 .. 100352, N 64 .. 8192, K 64 .. 8192 (us, M x N x K):
+// Timed in turn over M 16 .. 100352, N 64 .. 8192, K 64 .. 8192 (us, M x N x K), and carried on beyond: few rows of x by very many weights
+// (N from 49152 on with K from 4096) run tiles whose rows are mostly empty, untimed:
 //   32 x 32 outputs a workgroup while there are 512 of them, or 1024 of short sums: 1024 x 512 x 2048 7.5 against 9.6 in tiles of 128,
 //   1024 x 1024 x 512 5.3 against 6.6, but 1024 x 1024 x 1024 7.6 against 7.6 and 2048 x 1024 x 512 9.0 against 6.9;
 //   all steps at once up to 512 numbers: 25088 x 512 x 128 12.6 against 15.0 step by step, 100352 x 256 x 64 17.9 against 24.0, 4096 x 4096

@@ -46,7 +46,8 @@ NormPlan norm_plan(const tdc_group_norm_desc &d, bool quantised, bool grad) {
     auto fits = [&](int unit) { return !blocks && unit % Cg == 0 && pixels <= (long long)(most / vectors(unit)) * 16; };
     // One launch pays where a workgroup has little to do, or every compute unit something (bf16, silu, us, one launch against two):
     // forward, 25 Ki numbers a workgroup 9.4 against 10.7; 51 Ki, 8 workgroups 12.5 against 11.0, 256 18.5 against 22.6; 100 Ki, 16 workgroups
-    // 17.8 against 11.3 (28 against 12.5 into 4 bits), 128 23.1 against 22.7, 256 34.2 against 36.5.  Gradient, where the parameters need
+    // 17.8 against 11.3 (28 against 12.5 into 4 bits), 128 23.1 against 22.7, 256 34.2 against 36.5 (fp32, with twice the bytes, goes by the
+    // same counts, untimed).  Gradient, where the parameters need
     // a second launch in either case: 6 Ki 10.4 against 11.9; 25 Ki, 8 workgroups 16.3 against 12.0, 256 21.8 against 23.1; 51 Ki, 256 36
     // against 32.
     auto pays = [&](int unit) {

@@ -69,7 +69,9 @@ __device__ __forceinline__ float param(const void *p, long long i, int param_dty
     return reinterpret_cast<const float *>(p)[i];
 }
 
-// 1 / (1 + e^-z), by the exponential to base two and the reciprocal of the hardware (1 ulp each).
+// 1 / (1 + e^-z), by the exponential to base two and the reciprocal of the hardware (1 ulp each).  Its argument z log2 e is rounded once
+// to fp32, which makes e^-z |z| 2^-24 of itself less exact (1e-6 at z = -20): where |z| is large the activation is small against the
+// norm's own error of z, by which its results are judged.
 __device__ __forceinline__ float sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
 }
