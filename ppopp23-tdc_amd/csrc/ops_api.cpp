@@ -124,10 +124,10 @@ int norm_check(const tdc_group_norm_desc *desc, tdc_group_norm_desc &d) {
     }
     return TDC_OK;
 }
-// Whether the plan's launches can be made (the gradient's second one has workgroups for the parameters as well).
+// Whether the plan's launches can be made.  (The gradient has workgroups of 256 for the parameters: in its second launch, or by themselves.)
 int plan_check(const tdc_group_norm_desc &d, const NormPlan &n, bool grad) {
-    const long long workgroups = (long long)d.batch * n.tiles * n.chunks + (grad ? (2ll * d.C + 3) / 4 : 0);
-    if (workgroups > kMostItems / std::max(n.threads, grad ? 256 : 0) || n.slots > (1 << 24))
+    const double items = (double)d.batch * n.tiles * n.chunks * n.threads, params = grad ? (2.0 * d.C + 3) / 4 * 256 : 0.0;
+    if ((n.whole ? std::max(items, params) : items + params) > kMostItems || (double)n.chunks * n.tiles_per_group > (1 << 24))
         return invalid("group norm: too large, a launch has fewer than 2^32 work items");
     return TDC_OK;
 }

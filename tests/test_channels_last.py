@@ -404,7 +404,9 @@ def test_4_bit_numbers_of_more_rows_than_a_launch_has():
 
 
 @pytest.mark.parametrize("desc", [dict(batch=1 << 26, C=2048, groups=32, dtype=2, pixels=1), dict(batch=1 << 24, C=16, groups=2, pixels=1 << 16),
-                                  dict(batch=(1 << 31) - 1, C=8, groups=1, pixels=1)])
+                                  dict(batch=(1 << 31) - 1, C=8, groups=1, pixels=1),
+                                  dict(batch=(1 << 31) - 1, C=1 << 23, groups=1, pixels=(1 << 31) - 1),
+                                  dict(batch=1 << 16, C=1 << 23, groups=1 << 23, pixels=(1 << 31) - 1)])
 def test_norms_of_more_workgroups_than_a_launch_has(desc):
     L, d, a, b = tdc_amd.lib(), norm(**desc), ctypes.c_size_t(), ctypes.c_size_t()
     assert L.tdc_group_norm_workspace(ctypes.byref(d), ctypes.byref(a), ctypes.byref(b)) == INVALID and "too large" in error()
@@ -427,3 +429,11 @@ def test_products_of_more_outputs_than_64_bits_count():
     for size in (1 << 32, 1 << 34):
         d = linear(M=size, N=size)
         assert L.tdc_mx4_linear_workspace(ctypes.byref(d), ctypes.byref(n)) == INVALID and "2^40" in error()
+
+
+@pytest.mark.parametrize("desc", [dict(batch=1 << 25, C=64, groups=8, dtype=2, pixels=1), dict(batch=(1 << 26) - 1, C=16, groups=2, pixels=1),
+                                  dict(batch=1, C=(1 << 24) - 1, groups=1, pixels=1)])
+def test_norms_of_nearly_as_many_work_items_as_a_launch_has(desc):
+    L, d, a, b = tdc_amd.lib(), norm(**desc), ctypes.c_size_t(), ctypes.c_size_t()
+    assert L.tdc_group_norm_workspace(ctypes.byref(d), ctypes.byref(a), ctypes.byref(b)) == 0
+    assert L.tdc_group_norm_mx4_workspace(ctypes.byref(d), ctypes.byref(a)) == 0
