@@ -65,7 +65,7 @@ def listed():
         # A training step over a large feature map that keeps the sum in 8 bits for the backward pass.
         _norm("rms_train", "rms_train_100352x512_bf16_mx8", 32 * 56 * 56, 512, True, "bf16", "mx8"),
         # A ragged batch through a classifier in 8 bits, with a K that ends inside a block.
-        _product("mx8_linear", "mx8_linear_33x2000x1001_f32", 33, 2000, 1001, "relu", True, False, "f32"),
+        _product("mx8_linear", "mx8_linear_33x2000x1001_f16", 33, 2000, 1001, "relu", True, False, "f16"),
         # A large product in 8 bits, its input quantised on the way.
         _product("mx8_linear", "mx8_linear_8192x8192x8192_bf16", 8192, 8192, 8192, "none", False, False, "bf16"),
         # residual -> norm -> product in 8 bits, for a serving batch of the second stage.
@@ -91,8 +91,7 @@ def draw(rng):
         if train and N < 64:
             act = "silu"        # (few outputs: one whose sign rounding decides would show in dx)
         return _product(kind, None, M, K, N, act, rng.random() < 0.5, rng.random() < 0.3,
-                        "f32" if kind == "mx8_linear" and rng.random() < 0.25 else dtype,
-                        "mx8" if train and rng.random() < 0.4 else "none")
+                        dtype, "mx8" if train and rng.random() < 0.4 else "none")
     if kind in ("rms", "rms_train"):
         dtype = rng.choice((dtype, dtype, "f32"))
         while True:
