@@ -5,15 +5,10 @@
 // neighbouring outputs of one row.  (16x16x128 does as much per instruction but takes the matrix unit 35 cycles where 32x32x64, with
 // twice the work, takes 36: registers only, one wave a SIMD, 4.6 against 8.9 PFLOP/s, 6.4 on random numbers for their power.)
 #include <algorithm>
-#include <type_traits>
 
-#include "ops_device.hpp"
+#include "product_device.hpp"
 
 namespace tdc {
-
-typedef int i4_t __attribute__((ext_vector_type(4)));
-typedef int i8_t __attribute__((ext_vector_type(8)));
-typedef float f16_t __attribute__((ext_vector_type(16)));
 
 // One matrix instruction; the low bytes of the scale words are this step's.
 static __device__ __forceinline__ f16_t mfma4(i4_t a, i4_t b, f16_t c, int sa, int sb) {
@@ -21,44 +16,6 @@ static __device__ __forceinline__ f16_t mfma4(i4_t a, i4_t b, f16_t c, int sa, i
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wa, wb, c, 4, 4, 0, sa, 0, sb);
 }
 
-// Eight neighbouring numbers of a row as one request.
-template <int DT>
-struct Eight {
-    using T = typename Num<DT>::type;
-    typedef T vec_t __attribute__((ext_vector_type(8)));
-    typedef T mem_t __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-};
-// The residual of eight neighbouring outputs of a row: zeros where there is none (rows from M on, outputs from N on).
-template <int DT>
-static __device__ __forceinline__ typename Eight<DT>::vec_t residual8(const ProductArgs &a, long long m, long long n) {
-    using T = typename Num<DT>::type;
-    typename Eight<DT>::vec_t r = {};
-    if (a.residual && m < a.M) {
-        const T *const from = reinterpret_cast<const T *>(a.residual) + m * a.r_stride + n;
-        if (n + 8 <= a.N) r = *reinterpret_cast<const typename Eight<DT>::mem_t *>(from);
-        else {
-#pragma unroll
-            for (int i = 0; i < 7; ++i)
-                if (n + i < a.N) r[i] = from[i];
-        }
-    }
-    return r;
-}
-// Eight neighbouring outputs of a row (those before N): residual on sums with the bias, activation, store.
-template <int DT, int ACT>
-static __device__ __forceinline__ void finish8(const ProductArgs &a, long long m, long long n, const float (&v)[8], typename Eight<DT>::vec_t r) {
-    using T = typename Num<DT>::type;
-    T *const to = reinterpret_cast<T *>(a.y) + m * a.y_stride + n;
-    typename Eight<DT>::vec_t out;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = Num<DT>::down(act_of<ACT>(v[i] + Num<DT>::up(r[i])));
-    if (n + 8 <= a.N) *reinterpret_cast<typename Eight<DT>::mem_t *>(to) = out;
-    else {
-#pragma unroll
-        for (int i = 0; i < 7; ++i)
-            if (n + i < a.N) to[i] = out[i];
-    }
-}
 // ---- tiles ----
 //
 // A workgroup of four waves owns 64 MB rows of x and 64 NB of w, a wave a quarter of it: MB x NB blocks of 32 x 32.  A step is
@@ -74,9 +31,6 @@ static __device__ __forceinline__ void finish8(const ProductArgs &a, long long m
 // cycles and LDS 28 %: one wave a SIMD with a barrier every step keeps neither full.  The same workgroups going from tile to tile, the next one's codes on their way while this one's outputs
 // leave, took as long.
 //
-// The row of w that is row r of a block: bits 2 and 3 change places, which makes a lane's outputs 8 i .. 8 i + 7 neighbours.
-static __device__ __forceinline__ int weight_row(int r) { return (r & 19) | (r & 4) << 1 | (r & 8) >> 1; }
-
 template <int MB, int NB>
 struct Tile {
     static constexpr int M = 64 * MB, N = 64 * NB;
@@ -103,11 +57,6 @@ static __device__ __forceinline__ bool tile_of(int tiles_m, int tiles_n, long lo
     n0 = (long long)(rest / high) * Tile<MB, NB>::N;
     return true;
 }
-// A request straight into LDS: 16 bytes a lane, from `at` + `offset` on, in the order of the lanes.
-static __device__ __forceinline__ void bring(const unsigned char *base, int at, int offset, unsigned char *to) {
-    const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(base), 0, 0x7fffffff, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)to, 16, at, offset, 0, 0);
-}
 // Codes of a step for a tile: request i of a wave is half a block of 32 rows, of x for i below kX, of w from there on.  (Blocks past the
 // last repeat it: their products go nowhere.)
 template <int MB, int NB>
@@ -121,70 +70,6 @@ static __device__ __forceinline__ int chunk_of(const ProductArgs &a, int i, int 
     const int c = (i < L::kX ? i : i - L::kX) * 4 + wave;
     return (int)min((long long)(c / 2), (i < L::kX ? ((a.M + 31) >> 5) - (m0 >> 5) : ((a.N + 31) >> 5) - (n0 >> 5)) - 1) * 2048 + c % 2 * 1024;
 }
-// Waits until all but the wave's newest `left` requests have come and its LDS operations are done, then for the other waves.  (A fence in
-// place of the waits would wait for every request.)
-template <int left>
-static __device__ __forceinline__ void meet() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt((left & 15) | (left >> 4) << 14 | 7 << 4);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-template <int DT>
-static __device__ __forceinline__ float bias_of(const ProductArgs &a, long long n, bool wanted) {
-    return wanted && a.bias && n < a.N ? param<DT>(a.bias, n, a.bias_dtype) : 0.0f;
-}
-
-// A wave's outputs from row m on and from column n on; `bias` is that of its columns, `stage` its own 4 KiB NB of LDS.  Of a block a lane
-// has row r of x, and of w 16 u + 8 q .. 16 u + 8 q + 7, u = 0, 1.  32 rows at a time go through LDS, where a lane takes eight outputs of a
-// row and its neighbours those beside them: residuals and outputs are whole cache lines.  (The first halves of a row's eights lie
-// before the second ones, 16 bytes moved by the row, so that neither side meets a bank twice.)  The residuals of the next 32 rows are on
-// their way while these are finished.
-template <int DT, int MB, int NB>
-static __device__ __forceinline__ void finish_tile(const ProductArgs &a, const f16_t (&acc)[NB][MB], long long m, long long n, const float *bias,
-                                                   unsigned char *stage) {
-    constexpr int kAcross = NB * 4, kDown = 64 / kAcross, kTurns = 32 / kDown;     // lanes of a row, rows at a time
-    const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5, down = lane / kAcross, c = lane % kAcross * 8;
-    auto place = [&](int row, int eight, int half) {
-        return reinterpret_cast<float4 *>(stage + row * NB * 128 + ((half * kAcross + eight) ^ (row & 15)) * 16);
-    };
-    const float4 lo = *reinterpret_cast<const float4 *>(bias + c), hi = *reinterpret_cast<const float4 *>(bias + c + 4);
-    const float add[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    auto finish = [&](auto act) {
-        typename Eight<DT>::vec_t res[2][kTurns];
-        auto ask = [&](int i) {
-#pragma unroll
-            for (int s = 0; s < kTurns; ++s) res[i & 1][s] = residual8<DT>(a, m + i * 32 + s * kDown + down, n + c);
-        };
-        ask(0);
-#pragma unroll
-        for (int i = 0; i < MB; ++i) {
-#pragma unroll
-            for (int k = 0; k < 2 * NB; ++k)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int e = 8 * (k % 2) + 4 * h;
-                    const f16_t &v = acc[k / 2][i];
-                    *place(r, k * 2 + q, h) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                }
-            if (i + 1 < MB) ask(i + 1);
-            asm volatile("" ::: "memory");      // (a wave's own LDS operations come in order)
-#pragma unroll
-            for (int s = 0; s < kTurns; ++s) {
-                const int row = s * kDown + down;
-                const float4 u = *place(row, c / 8, 0), w = *place(row, c / 8, 1);
-                const float v[8] = {u.x + add[0], u.y + add[1], u.z + add[2], u.w + add[3], w.x + add[4], w.y + add[5], w.z + add[6], w.w + add[7]};
-                if (m + i * 32 + row < a.M && n + c < a.N) finish8<DT, decltype(act)::value>(a, m + i * 32 + row, n + c, v, res[i & 1][s]);
-            }
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    if (a.act == TDC_ACT_RELU) finish(std::integral_constant<int, TDC_ACT_RELU>{});
-    else if (a.act == TDC_ACT_SILU) finish(std::integral_constant<int, TDC_ACT_SILU>{});
-    else finish(std::integral_constant<int, TDC_ACT_NONE>{});
-}
-
 template <int DT, int MB, int NB>
 __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile_kernel(const ProductArgs a, int tiles_m, int tiles_n) {
     using L = Tile<MB, NB>;
@@ -504,17 +389,6 @@ __global__ void __launch_bounds__(1024) tdc_mx4_product_few_kernel(const Product
         v = a.act == TDC_ACT_RELU ? act_of<TDC_ACT_RELU>(v) : a.act == TDC_ACT_SILU ? act_of<TDC_ACT_SILU>(v) : v;
         reinterpret_cast<T *>(a.y)[(m0 + m) * a.y_stride + n0 + n] = Num<DT>::down(v);
     }
-}
-
-// Lets a kernel have more than 64 KiB of LDS; once per kernel and device.
-static int allow_lds(const void *fn, int bytes, unsigned long long &done) {
-    int device = 0;
-    if (hipError_t e = hipGetDevice(&device)) return (int)e;
-    const unsigned long long bit = 1ull << (device & 63);
-    if (__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit) return 0;
-    if (hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return (int)e;
-    __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
-    return 0;
 }
 
 template <int DT, int MB, int NB>

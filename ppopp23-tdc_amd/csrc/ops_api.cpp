@@ -2,21 +2,11 @@
 #include <algorithm>
 #include <cmath>
 #include <numeric>
-#include <string>
 
-#include "ops_internal.hpp"
-#include "tdc_internal.hpp"
+#include "ops_checks.hpp"
 
 namespace tdc {
 namespace {
-
-int invalid(const std::string &what) { return api_fail(TDC_ERR_INVALID, what); }
-int launched(const char *what, int err) {
-    return err ? api_fail(TDC_ERR_HIP, std::string(what) + ": " + hipGetErrorString((hipError_t)err)) : (int)TDC_OK;
-}
-bool number(int dtype) { return dtype == TDC_F32 || dtype == TDC_F16 || dtype == TDC_BF16; }
-constexpr long long kMostItems = (1ll << 32) - 1;      // of a launch
-bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (unsigned)(bytes - 1)) == 0; }
 
 // ---- group norm ----
 
@@ -152,30 +142,6 @@ NormArgs norm_args(const tdc_group_norm_desc &d, const void *x, const void *gamm
     a.eps = d.eps;
     return a;
 }
-int ws_check(const char *what, const void *ws, size_t have, size_t need) {
-    if (!need) return TDC_OK;
-    if (!ws || have < need)
-        return invalid(std::string(what) + ": the workspace has " + std::to_string(ws ? have : 0) + " bytes, needs " + std::to_string(need));
-    if (!aligned(ws, 16)) return invalid(std::string(what) + ": the workspace is not 16-byte aligned");
-    return TDC_OK;
-}
-
-// ---- 4-bit numbers ----
-
-int mx4_range(const char *what, long long rows, long long K) {
-    if (rows < 0 || K < 1) return invalid(std::string(what) + ": rows has to be 0 and K 1 at least");
-    if (K > (1ll << 30) || rows > (1ll << 35) / mx4_padded(K) * 32) return invalid(std::string(what) + ": more numbers than 2^40");
-    if (mx4_work_items(rows, K) > kMostItems) return invalid(std::string(what) + ": too many rows, a launch has fewer than 2^32 work items");
-    return TDC_OK;
-}
-int mx4_check(const char *what, long long rows, long long K, const void *codes, const void *scales) {
-    if (int st = mx4_range(what, rows, K)) return st;
-    if (rows && (!codes || !scales)) return invalid(std::string(what) + ": null codes or scales");
-    if (rows && (!aligned(codes, 16) || !aligned(scales, 16)))
-        return invalid(std::string(what) + ": codes and scales have to be 16-byte aligned");
-    return TDC_OK;
-}
-
 // ---- product ----
 
 int linear_check(const tdc_mx4_linear_desc *desc, tdc_mx4_linear_desc &d) {
@@ -208,13 +174,6 @@ size_t linear_ws(const tdc_mx4_linear_desc &d) {
 }  // namespace tdc
 
 using namespace tdc;
-
-// (an error message is the only thing here that allocates: no exception leaves a C entry)
-#define TDC_ENTRY try
-#define TDC_ENTRY_END                 \
-    catch (...) {                     \
-        return (int)TDC_ERR_NOMEM;    \
-    }
 
 extern "C" {
 
@@ -271,7 +230,7 @@ int tdc_group_norm_forward_mx4(const tdc_group_norm_desc *desc, const void *x, c
     if (!x) return invalid("group norm: null x");
     const NormPlan plan = norm_plan(d, true, false);
     if (int st = plan_check(d, plan, false)) return st;
-    if (int st = mx4_check("group norm", d.batch * d.pixels, d.C, codes, scales)) return st;
+    if (int st = mx_check("group norm", d.batch * d.pixels, d.C, codes, scales)) return st;
     if (int st = ws_check("group norm", ws, ws_bytes, forward_ws(d, plan))) return st;
     NormArgs a = norm_args(d, x, gamma, beta);
     a.codes = (unsigned char *)codes;
@@ -321,7 +280,7 @@ int tdc_group_norm_backward(const tdc_group_norm_desc *desc, const void *x, cons
 TDC_ENTRY_END
 
 int tdc_mx4_sizes(int64_t rows, int64_t K, size_t *code_bytes, size_t *scale_bytes) TDC_ENTRY {
-    if (int st = mx4_range("4-bit numbers", rows, K)) return st;
+    if (int st = mx_range("4-bit numbers", rows, K)) return st;
     if (code_bytes) *code_bytes = (size_t)mx4_code_bytes(rows, K);
     if (scale_bytes) *scale_bytes = (size_t)(rows * mx4_scale_bytes(K));
     return TDC_OK;
@@ -330,7 +289,7 @@ TDC_ENTRY_END
 
 int tdc_mx4_quantize(const void *x, int32_t dtype, int64_t rows, int64_t K, int64_t row_stride, void *codes, void *scales, void *stream) TDC_ENTRY {
     if (!number(dtype)) return invalid("4-bit numbers: dtype has to be TDC_F32, TDC_F16 or TDC_BF16");
-    if (int st = mx4_check("4-bit numbers", rows, K, codes, scales)) return st;
+    if (int st = mx_check("4-bit numbers", rows, K, codes, scales)) return st;
     if (!rows) return TDC_OK;
     if (!x) return invalid("4-bit numbers: null x");
     if (!row_stride) row_stride = K;
@@ -342,7 +301,7 @@ TDC_ENTRY_END
 int tdc_mx4_dequantize(const void *codes, const void *scales, int64_t rows, int64_t K, void *y, int32_t dtype, int64_t row_stride,
                        void *stream) TDC_ENTRY {
     if (!number(dtype)) return invalid("4-bit numbers: dtype has to be TDC_F32, TDC_F16 or TDC_BF16");
-    if (int st = mx4_check("4-bit numbers", rows, K, codes, scales)) return st;
+    if (int st = mx_check("4-bit numbers", rows, K, codes, scales)) return st;
     if (!rows) return TDC_OK;
     if (!y) return invalid("4-bit numbers: null y");
     if (!row_stride) row_stride = K;
@@ -366,10 +325,10 @@ int tdc_mx4_linear(const tdc_mx4_linear_desc *desc, const void *x, const void *x
     if (int st = linear_check(desc, d)) return st;
     if (!d.M || !d.N) return TDC_OK;
     if (!x || !y) return invalid("4-bit product: null x or y");
-    if (int st = mx4_check("4-bit product", d.N, d.K, w_codes, w_scales)) return st;
+    if (int st = mx_check("4-bit product", d.N, d.K, w_codes, w_scales)) return st;
     ProductArgs a{};
     if (d.x_dtype == TDC_MX4) {
-        if (int st = mx4_check("4-bit product", d.M, d.K, x, x_scales)) return st;
+        if (int st = mx_check("4-bit product", d.M, d.K, x, x_scales)) return st;
         a.x_codes = (const unsigned char *)x;
         a.x_scales = (const unsigned char *)x_scales;
     } else if (product_takes_numbers(d.M, d.N, d.K)) {

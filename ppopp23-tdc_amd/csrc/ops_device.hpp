@@ -130,6 +130,34 @@ __device__ __forceinline__ float quad_larger(float top) {
     return larger(top, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, top), 0x4E, 0xf, 0xf, true)));
 }
 
+// ---- blocks of 32 numbers in 8 bits (E4M3; scales as above) ----
+
+__device__ __forceinline__ int mx8_scale_byte(float top) {
+    const int e = (int)(__float_as_uint(top) >> 23);
+    return e == 255 ? 255 : max(e - 8, 0);
+}
+// Eight codes.  (The instruction rounds to nearest even, but makes NaNs of what rounds past 448: those saturate before.)
+__device__ __forceinline__ uint2 mx8_codes(const float *v, float divisor) {
+    typedef short s2_t __attribute__((ext_vector_type(2)));
+    const float most = 448.0f * divisor;
+    float c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = __builtin_amdgcn_fmed3f(v[i], -most, most);
+    s2_t lo = {0, 0}, hi = {0, 0};
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, c[0], c[1], divisor, false);
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, c[2], c[3], divisor, true);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, c[4], c[5], divisor, false);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(hi, c[6], c[7], divisor, true);
+    return make_uint2(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi));
+}
+// What eight codes stand for.
+__device__ __forceinline__ void mx8_values(uint2 codes, float scale, float (&v)[8]) {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes.x, true);
+    const auto c = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes.y, true);
+    v[0] = a[0] * scale, v[1] = a[1] * scale, v[2] = b[0] * scale, v[3] = b[1] * scale;
+    v[4] = c[0] * scale, v[5] = c[1] * scale, v[6] = d[0] * scale, v[7] = d[1] * scale;
+}
+
 // The quotient of two numbers below 2^20: an approximate reciprocal is near enough for those.
 static __device__ __forceinline__ int small_quotient(int n, int d) { return (int)((n + 0.5f) * __builtin_amdgcn_rcpf((float)d)); }
 

@@ -84,17 +84,95 @@ int launch_mx4_quantize(const void *x, int dtype, long long rows, long long K, l
 int launch_mx4_dequantize(const void *codes, const void *scales, long long rows, long long K, void *y, int dtype, long long stride,
                           void *stream);
 
-struct ProductArgs {
+// Where a product's sums go: y = act(sums + bias + residual).
+struct ProductOut {
+    const void *bias, *residual;
+    void *y, *z;                    // (z: what the activation is taken of, where a gradient will want it)
+    long long M, N, y_stride, r_stride, z_stride;
+    int bias_dtype, act;
+};
+
+struct ProductArgs : ProductOut {
     const unsigned char *x_codes, *x_scales, *w_codes, *w_scales;
     const void *x;                  // numbers in place of codes (see product_takes_numbers), or null
     long long K, x_stride;
     int x_dtype;
-    const void *bias, *residual;
-    void *y;
-    long long M, N, y_stride, r_stride;
     int ksteps;                     // padded K / 128
-    int bias_dtype, act;
 };
+// A product in 16 or 8 bits (see product_tile.hpp).  The sum runs over `steps` steps of 64 bytes.
+struct TileArgs : ProductOut {
+    const unsigned char *x, *w, *x_scales, *w_scales;
+    long long x_stride, w_stride;   // bytes between the rows in memory: along the sum, or (an operand across it) its places
+    long long x_outer, w_outer;     // rows in memory along the sum, else numbers of one row (a multiple of 8)
+    long long x_limit, w_limit;     // numbers of the sum that are there
+    int steps, split_steps, splits; // of the sum, of one part of it, parts
+    int tiles_m, tiles_n;
+    unsigned blocks;                // workgroups of a part
+    float *part;                    // sums of the parts: [splits][M][part_stride]
+    long long part_stride;
+};
+enum { kTile256, kTile128, kTile32 };
+// How a product is dealt out.
+struct TilePlan {
+    int kernel;                     // which tile
+    int tm, tn, splits, split_steps, steps;
+    long long blocks, part_stride;
+    long long part_bytes;
+    long long items;                // work items of its largest launch
+};
+enum { kAlong, kWAcross, kAcross };     // how x and w lie: both along the sum, w across it, both across it
+TilePlan tile_plan(long long M, long long N, long long K, int in_dtype);
+// `a` with everything but what the plan says; y_dtype is TDC_F16 or TDC_BF16.
+int launch_product_bf16(TileArgs a, const TilePlan &p, int layout, void *stream);
+int launch_product_f16(TileArgs a, const TilePlan &p, int layout, void *stream);
+int launch_product_mx8(TileArgs a, const TilePlan &p, int y_dtype, void *stream);
+int launch_join(const TileArgs &a, int y_dtype, void *stream);
+
+// dz = dy act'(z) in rows of `pitch` numbers (zeros past the N-th), its sums over the rows besides; also a copy of rows (no activation).
+struct ActGradArgs {
+    const void *dy, *kept;          // kept: z, or for ReLU its result; rows of N
+    void *dz;                       // or null
+    void *sums;                     // [N], or null
+    float *part;                    // [chunks][N]
+    long long M, N, dy_stride, pitch;
+    int act, chunks, sums_dtype;
+    long long chunk_rows;
+    int tiles;                      // workgroups across the columns
+    int across;                     // vectors of eight columns of a workgroup (a power of two)
+};
+void act_grad_plan(ActGradArgs &a);      // pitch and the last five
+long long act_grad_items(const ActGradArgs &a);
+int launch_act_grad(const ActGradArgs &a, int dtype, void *stream);
+int launch_column_sums(const float *part, void *out, long long N, int chunks, int out_dtype, void *stream);
+
+// Numbers in 8 bits.
+inline long long mx8_pitch(long long K) { return round_up(K, 128); }
+long long mx8_work_items(long long rows, long long K);
+int launch_mx8_quantize(const void *x, int dtype, long long rows, long long K, long long stride, void *codes, void *scales, void *stream);
+int launch_mx8_dequantize(const void *codes, const void *scales, long long rows, long long K, void *y, int dtype, long long stride,
+                          void *stream);
+
+// RMS norm.
+struct RmsArgs {
+    const void *x, *residual, *weight, *dy, *dh;
+    void *y, *h;                    // h: x + residual, or null
+    void *dx;
+    float *rstd;
+    unsigned char *codes, *scales;  // of y or of h
+    float *part;                    // gradient: [workgroups][C]
+    void *dweight;
+    long long rows, x_stride, r_stride, dy_stride, dh_stride;
+    int C, weight_dtype;
+    float eps;
+    int team, held;                 // lanes of a row, vectors of eight that each keeps
+    int blocks;                     // workgroups
+};
+enum { kRmsPlain, kRmsOutputMx8, kRmsKeptMx8 };      // 8 bits: none, y, what the gradient needs of h
+bool rms_plan(RmsArgs &a, bool grad);                // the last three; false if C is too large
+long long rms_items(const RmsArgs &a, bool grad);
+int launch_rms_forward(const RmsArgs &a, int dtype, int mode, void *stream);
+int launch_rms_backward(const RmsArgs &a, int dtype, bool kept_mx8, void *stream);
+
 bool product_takes_numbers(long long M, long long N, long long K);
 long long product_work_items(long long M, long long N, long long K, bool numbers);
 int launch_mx4_product(const ProductArgs &a, int y_dtype, void *stream);

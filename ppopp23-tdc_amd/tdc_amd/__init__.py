@@ -5,7 +5,8 @@ from ._lib import (LIB_PATH, ConvDesc, TdcError, Tile, TileInfo, conv_desc, lib,
 __all__ = ["LIB_PATH", "ConvDesc", "TdcError", "Tile", "TileInfo", "conv_desc", "lib", "model_enumerate",
            "model_evaluate", "model_select", "set_autotune", "Conv2dPlan", "TKConvOp", "TKConv2dC", "ranks_dict", "partial_tucker2",
            "group_norm_act", "group_norm_act_mx4", "mx4_quantize", "mx4_linear", "mx4_conv1x1", "Mx4Tensor",
-           "GroupNormAct", "TuckerBlockMx4"]
+           "GroupNormAct", "TuckerBlockMx4",
+           "linear_act", "conv1x1_act", "rms_norm", "rms_norm_mx8", "mx8_quantize", "mx8_linear", "mx8_conv1x1", "Mx8Tensor"]
 
 
 def __getattr__(name):
@@ -16,6 +17,8 @@ def __getattr__(name):
         from . import TKConv as module
     elif name in ("group_norm_act", "group_norm_act_mx4", "mx4_quantize", "mx4_linear", "mx4_conv1x1", "Mx4Tensor"):
         from . import channels_last as module
+    elif name in ("linear_act", "conv1x1_act", "rms_norm", "rms_norm_mx8", "mx8_quantize", "mx8_linear", "mx8_conv1x1", "Mx8Tensor"):
+        from . import pointwise as module
     elif name in ("GroupNormAct", "TuckerBlockMx4"):
         from . import mx4_block as module
     else:

@@ -32,7 +32,9 @@ EXPORTS = (
     "tdc_net_read_tensor", "tdc_net_destroy",
     "tdc_group_norm_workspace", "tdc_group_norm_forward", "tdc_group_norm_backward", "tdc_group_norm_forward_mx4",
     "tdc_group_norm_mx4_workspace", "tdc_mx4_sizes", "tdc_mx4_quantize", "tdc_mx4_dequantize", "tdc_mx4_linear_workspace",
-    "tdc_mx4_linear",
+    "tdc_mx4_linear", "tdc_mx8_sizes", "tdc_mx8_quantize", "tdc_mx8_dequantize", "tdc_mx8_linear_workspace", "tdc_mx8_linear",
+    "tdc_linear_workspace", "tdc_linear_forward", "tdc_linear_backward", "tdc_rms_norm_workspace", "tdc_rms_norm_forward",
+    "tdc_rms_norm_forward_mx8", "tdc_rms_norm_backward",
 )
 
 
@@ -94,6 +96,17 @@ class GroupNormDesc(Structure):
 class Mx4LinearDesc(Structure):
     _fields_ = [(n, ctypes.c_int64) for n in ("M", "N", "K")] + [(n, c_int32) for n in (
         "x_dtype", "y_dtype", "bias_dtype", "act")] + [(n, ctypes.c_int64) for n in ("x_stride", "y_stride", "residual_stride")]
+
+
+class LinearDesc(Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("M", "N", "K")] + [(n, c_int32) for n in (
+        "dtype", "bias_dtype", "act", "kept_dtype")] + [(n, ctypes.c_int64) for n in (
+            "x_stride", "w_stride", "y_stride", "residual_stride")]
+
+
+class RmsNormDesc(Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("C", c_int32), ("dtype", c_int32), ("weight_dtype", c_int32), ("eps", ctypes.c_float)] + [
+        (n, ctypes.c_int64) for n in ("x_stride", "residual_stride", "dy_stride", "dh_stride")]
 
 
 _lib = None
@@ -175,6 +188,19 @@ def lib():
     L.tdc_mx4_dequantize.argtypes = [c_void_p, c_void_p, i64, i64, c_void_p, i32, i64, c_void_p]
     L.tdc_mx4_linear_workspace.argtypes = [linear, szp]
     L.tdc_mx4_linear.argtypes = [linear] + [c_void_p] * 8 + [sz, c_void_p]
+    row, rms = POINTER(LinearDesc), POINTER(RmsNormDesc)
+    L.tdc_mx8_sizes.argtypes = [i64, i64, szp, szp]
+    L.tdc_mx8_quantize.argtypes = [c_void_p, i32, i64, i64, i64, c_void_p, c_void_p, c_void_p]
+    L.tdc_mx8_dequantize.argtypes = [c_void_p, c_void_p, i64, i64, c_void_p, i32, i64, c_void_p]
+    L.tdc_mx8_linear_workspace.argtypes = [linear, szp]
+    L.tdc_mx8_linear.argtypes = [linear] + [c_void_p] * 8 + [sz, c_void_p]
+    L.tdc_linear_workspace.argtypes = [row, szp, szp]
+    L.tdc_linear_forward.argtypes = [row] + [c_void_p] * 7 + [sz, c_void_p]
+    L.tdc_linear_backward.argtypes = [row] + [c_void_p] * 10 + [sz, c_void_p]
+    L.tdc_rms_norm_workspace.argtypes = [rms, szp]
+    L.tdc_rms_norm_forward.argtypes = [rms] + [c_void_p] * 9
+    L.tdc_rms_norm_forward_mx8.argtypes = [rms] + [c_void_p] * 7
+    L.tdc_rms_norm_backward.argtypes = [rms] + [c_void_p] * 9 + [sz, c_void_p]
     for name in EXPORTS:
         fn = getattr(L, name)
         if fn.restype is c_int:  # default restype: status code

@@ -1,0 +1,510 @@
+"""The 16- and 8-bit products, RMS norm, their gradients and checkpoints, against plain 64-bit forms.
+
+Tolerances, from the arithmetic.  u is the unit roundoff of the output's type (2^-24, 2^-11, 2^-8), e = 2^-24, S the sum of the
+magnitudes of a sum's terms.
+16-bit product: an instruction adds 16 exact products to a sum and rounds within 2 e of the magnitudes met, bias, residual and
+activation are a few operations more: (16 + K / 8) e S, then u |y|.
+8-bit product: an instruction keeps of each of its 64 products what lies above 2^-14 of the largest: 64 2^-14 times that for each 64
+numbers, besides the above.
+Its gradient: dz = dy act'(z) is rounded (u |dz|), z for "silu" too, and |act''| is at most 1/2: u |dz| + |dy| (u |z| + the product's error) / 2;
+"relu" has either slope where z is within its error of 0.  That error goes through dx = dz w and dw = dz^T x term by term, which add their own.
+dbias adds in chains of at most 256: 512 e S.
+RMS norm: a row's squares add in chains of at most 32 and trees, 1 / sqrt is good to 2 e: 64 e |y|, then u |y|; its gradient the same of the
+magnitudes of its terms; the weight's gradient adds in chains of at most 256: 512 e S.
+Half precision has 2^-25 more wherever it rounds."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import tdc_amd
+from oracle import pointwise_ref as ref
+from oracle.channels_last_ref import act as ref_act
+from util import seeded
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+U = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
+LEAST = {F32: 2.0 ** -149, F16: 2.0 ** -25, BF16: 2.0 ** -134}
+
+
+def host(t):
+    return t.detach().double().cpu().numpy()
+
+
+def close(got, want, bound, what=""):
+    got = host(got) if isinstance(got, torch.Tensor) else got
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~((np.abs(got - want) <= bound) | (np.isnan(got) & np.isnan(want)) | (got == want))
+    if bad.any():
+        i = np.unravel_index(np.argmax(np.where(bad, np.nan_to_num(np.abs(got - want), nan=1e300), 0)), got.shape)
+        raise AssertionError(f"{what}: {bad.sum()} of {bad.size} outside; at {i} got {got[i]!r} want {want[i]!r} bound {np.broadcast_to(bound, got.shape)[i]:.3g}")
+
+
+def rounded(want, dtype):
+    return U[dtype] * np.abs(want) + LEAST[dtype]
+
+
+def numbers(seed, shape, dtype, by=1.0):
+    return (torch.randn(shape, generator=seeded(seed)) * by).to(dtype).cuda()
+
+
+def case(seed, M, N, K, dtype, bias=True, residual=True, bias_dtype=None):
+    x, w = numbers(seed, (M, K), dtype), numbers(seed + 1, (N, K), dtype, K ** -0.5)
+    b = numbers(seed + 2, (N,), bias_dtype or dtype) if bias else None
+    return x, w, b, numbers(seed + 3, (M, N), dtype) if residual else None
+
+
+def opt(t):
+    return None if t is None else host(t)
+
+
+def check_linear(y, x, w, b, r, act, dtype, what=""):
+    """(z, bound of its error)"""
+    z, want = ref.linear(host(x), host(w), opt(b), opt(r), act)
+    S = np.abs(host(x)) @ np.abs(host(w)).T + (0 if b is None else np.abs(host(b))) + (0 if r is None else np.abs(host(r)))
+    off = (16 + x.shape[1] / 8) * E * S
+    close(y, want, 1.1 * off + rounded(want, dtype) * (1 + 1e-3), what)      # (the slope of "silu" is at most 1.1)
+    return z, off
+
+
+PRODUCTS = [(1, 1, 1), (1, 16, 32), (1, 1000, 2048), (2, 17, 33), (5, 100, 130), (15, 64, 128), (16, 33, 512), (31, 129, 72), (33, 256, 96),
+            (64, 40, 1000), (100, 300, 31), (129, 127, 257), (130, 258, 640), (257, 128, 4100), (300, 1001, 203), (1000, 24, 64)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+def test_linear(M, N, K, dtype):
+    for i, act in enumerate(("none", "relu", "silu")):
+        x, w, b, r = case(10 * i, M, N, K, dtype, bias=i != 1, residual=i != 2, bias_dtype=F32 if i == 2 else dtype)
+        y = tdc_amd.linear_act(x, w, b, r, act=act)
+        assert y.dtype == dtype and y.shape == (M, N)
+        check_linear(y, x, w, b, r, act, dtype, f"{M} {N} {K} {act}")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N,K", [(3400, 3500, 2200), (4096, 3336, 2048), (3333, 3850, 128), (40, 40, 40000), (20000, 64, 256)])
+def test_linear_of_whole_numbers_is_exact(M, N, K, dtype):
+    """Of many tiles, and of sums in parts: sums below 2^8 in magnitude are exact in either type."""
+    g = seeded(5)
+    x = torch.zeros(M, K)
+    x.scatter_(1, torch.randint(0, K, (M, 20), generator=g), torch.randint(-3, 4, (M, 20), generator=g).float())
+    w = torch.randint(-4, 5, (N, K), generator=g).float()
+    r = torch.randint(-8, 9, (M, N), generator=g).float()
+    y = tdc_amd.linear_act(x.to(dtype).cuda(), w.to(dtype).cuda(), None, r.to(dtype).cuda())
+    want = x.cuda() @ w.t().contiguous().cuda() + r.cuda()      # (whole numbers: exact in fp32)
+    assert torch.equal(y.float(), want)
+
+
+def grads(out, wrt, dout):
+    return torch.autograd.grad(out, wrt, dout)
+
+
+def check_grads(M, N, K, dtype, act, checkpoint=None, bias_dtype=None, seed=50, residual=True):
+    x, w, b, r = case(seed, M, N, K, dtype, residual=residual, bias_dtype=bias_dtype)
+    dy = numbers(seed + 9, (M, N), dtype)
+    wrt = [t.requires_grad_() for t in (x, w, b, r) if t is not None]
+    y = tdc_amd.linear_act(x, w, b, r, act=act, checkpoint=checkpoint)
+    got = grads(y, wrt, dy)
+    what = f"{M} {N} {K} {act} {checkpoint}"
+    z, off = check_linear(y, x, w, b, r, act, dtype, what)
+    kept = ref.quantize8(host(x))[0] if checkpoint else host(x)
+    dz, dx, dw, db = ref.linear_grads(host(x), host(w), z, host(dy), act, kept)
+    a = np.abs(host(dy))
+    slope = 0 if act == "none" else np.where(np.abs(z) <= off, a, 0) if act == "relu" else a * (rounded(z, dtype) + off) / 2 * 1.01 + 32 * E * a
+    if act == "relu" and dtype == F16:
+        slope = np.where(np.abs(z) <= off + LEAST[F16], a, 0)      # (what is kept is the rounded result)
+    # (dz's rounding is of what the kernel has before it; its own gradient may come as dy itself)
+    ez = np.broadcast_to(slope + (0 if act == "none" else rounded(np.abs(dz) + slope, dtype)), dz.shape)
+    own = lambda L, S: (16 + L / 8) * E * S  # noqa: E731
+    adz = np.abs(dz) + ez
+    close(got[0], dx, ez @ np.abs(host(w)) + own(N, adz @ np.abs(host(w))) + rounded(np.abs(dx) + ez @ np.abs(host(w)), dtype), what + " dx")
+    S = ez.T @ np.abs(kept)
+    close(got[1], dw, S + own(M, adz.T @ np.abs(kept)) + rounded(np.abs(dw) + S, dtype), what + " dw")
+    S = np.broadcast_to(slope, dz.shape).sum(0)
+    close(got[2], db, S + 512 * E * adz.sum(0) + rounded(np.abs(db) + S, b.dtype), what + " dbias")
+    if residual:
+        close(got[3], dz, ez, what + " dresidual")
+    for t, g in zip(wrt, got):
+        assert g.shape == t.shape and g.dtype == t.dtype
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+def test_linear_gradients(M, N, K, dtype):
+    check_grads(M, N, K, dtype, "silu")
+    check_grads(M, N, K, dtype, "none", checkpoint="mx8", bias_dtype=F32)
+    check_grads(M, N, K, dtype, "relu", residual=False)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N,K", [(5000, 96, 160), (2100, 1030, 1100), (9000, 33, 40)])
+def test_linear_gradients_of_many_rows(M, N, K, dtype):
+    check_grads(M, N, K, dtype, "silu", checkpoint="mx8")
+    check_grads(M, N, K, dtype, "none")
+
+
+def test_linear_gradients_by_differences():
+    """The gradient against differences of the forward pass along a direction (in 64 bits of the sums that the outputs make)."""
+    M, N, K = 40, 24, 56
+    x, w, b, r = case(70, M, N, K, BF16)
+    dy = numbers(71, (M, N), BF16)
+    wrt = [t.requires_grad_() for t in (x, w, b, r)]
+    got = grads(tdc_amd.linear_act(x, w, b, r, act="silu"), wrt, dy)
+    f = lambda *v: float((ref.linear(*v, "silu")[1] * host(dy)).sum())  # noqa: E731
+    at = [host(t) for t in wrt]
+    for i, g in enumerate(got):
+        d = np.random.default_rng(i).standard_normal(at[i].shape)
+        step = [a + (1e-5 * d if j == i else 0) for j, a in enumerate(at)]
+        back = [a - (1e-5 * d if j == i else 0) for j, a in enumerate(at)]
+        slope = (f(*step) - f(*back)) / 2e-5
+        # every number of a gradient carries some 2 u of its terms' magnitudes, in random directions
+        assert abs((host(g) * d).sum() - slope) <= 8 * U[BF16] * np.sqrt(((np.abs(host(g)) + 1) ** 2 * d ** 2).sum()) + 1e-6 * abs(slope)
+
+
+def test_linear_strides_axes_and_specials():
+    wide = numbers(80, (6, 9, 200), BF16)
+    w = numbers(81, (50, 96), BF16)
+    for x in (wide[..., 8:104], wide[..., 3:99], wide[:, ::2, 40:136], wide[:, :, 10:106].transpose(0, 1), wide[:1, :1, 1:97].expand(4, 3, 96)):
+        y = tdc_amd.linear_act(x, w)
+        assert torch.equal(y, tdc_amd.linear_act(x.clone(memory_format=torch.contiguous_format), w)) and y.shape == (*x.shape[:-1], 50)
+    big = numbers(82, (50, 300), BF16)
+    for v in (big[:, 5:101], big[:, 16:112], big[::2, 8:104]):
+        assert torch.equal(tdc_amd.linear_act(wide[0, :, 8:104], v), tdc_amd.linear_act(wide[0, :, 8:104], v.contiguous()))
+    r = numbers(83, (6, 9, 51), BF16)
+    assert torch.equal(tdc_amd.linear_act(wide[..., :96], w, None, r[..., 1:]), tdc_amd.linear_act(wide[..., :96], w, None, r[..., 1:].contiguous()))
+    # what is beside an operand does not come in, what is in it stays in its row and column
+    hot = torch.full((20, 300), float("nan"), dtype=BF16, device="cuda")
+    hot[:, 100:140] = 1
+    assert torch.equal(tdc_amd.linear_act(hot[:, 100:140], torch.ones(9, 40, dtype=BF16, device="cuda")), torch.full((20, 9), 40.0, dtype=BF16, device="cuda"))
+    x = numbers(84, (70, 40), BF16)
+    want = tdc_amd.linear_act(x, w[:, :40].contiguous())
+    for v in (float("nan"), float("inf")):
+        y = x.clone()
+        y[33, 7] = v
+        y = tdc_amd.linear_act(y, w[:, :40].contiguous())
+        assert torch.equal(y[:33], want[:33]) and torch.equal(y[34:], want[34:]) and not torch.isfinite(y[33]).any()
+
+
+def test_conv1x1_is_the_product_over_pixels():
+    x = numbers(90, (3, 48, 5, 7), BF16).contiguous(memory_format=torch.channels_last)
+    w, r = numbers(91, (20, 48, 1, 1), BF16), numbers(92, (3, 20, 5, 7), BF16).contiguous(memory_format=torch.channels_last)
+    y = tdc_amd.conv1x1_act(x, w, None, r, act="relu")
+    flat = tdc_amd.linear_act(x.permute(0, 2, 3, 1), w.flatten(1), None, r.permute(0, 2, 3, 1), act="relu")
+    assert y.is_contiguous(memory_format=torch.channels_last) and torch.equal(y.permute(0, 2, 3, 1), flat)
+    wrt = [t.requires_grad_() for t in (x, w, r)]
+    dy = numbers(93, (3, 20, 5, 7), BF16).contiguous(memory_format=torch.channels_last)
+    got = grads(tdc_amd.conv1x1_act(x, w, None, r, act="silu"), wrt, dy)
+    want = grads(tdc_amd.linear_act(x.permute(0, 2, 3, 1), w.flatten(1), None, r.permute(0, 2, 3, 1), act="silu"), wrt, dy.permute(0, 2, 3, 1))
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[1].shape == w.shape
+    h = tdc_amd.mx8_conv1x1(x.detach(), tdc_amd.mx8_quantize(w.detach().flatten(1)))
+    assert torch.equal(h.permute(0, 2, 3, 1), tdc_amd.mx8_linear(x.detach().permute(0, 2, 3, 1), tdc_amd.mx8_quantize(w.detach().flatten(1))))
+
+
+def test_linear_of_nothing():
+    x, w, b, r = case(95, 0, 10, 24, BF16)
+    wrt = [t.requires_grad_() for t in (x, w, b, r)]
+    for checkpoint in (None, "mx8"):
+        y = tdc_amd.linear_act(x, w, b, r, act="silu", checkpoint=checkpoint)
+        dx, dw, db, dr = grads(y, wrt, torch.empty_like(y))
+        assert y.shape == (0, 10) and dx.shape == x.shape and not dw.any() and not db.any() and dr.shape == r.shape
+    x, w, _, _ = case(96, 7, 1, 24, BF16)
+    x, w = x.requires_grad_(), w[:0].detach().requires_grad_()
+    y = tdc_amd.linear_act(x, w)
+    dx, dw = grads(y, (x, w), torch.empty_like(y))
+    assert y.shape == (7, 0) and not dx.any() and dw.shape == (0, 24)
+    q = tdc_amd.mx8_quantize(torch.empty(0, 40, device="cuda"))
+    assert tdc_amd.mx8_linear(q, tdc_amd.mx8_quantize(torch.ones(3, 40, device="cuda"))).shape == (0, 3) and q.dequantize().shape == (0, 40)
+    assert tdc_amd.rms_norm(torch.empty(0, 40, device="cuda")).shape == (0, 40)
+
+
+# ---- 8 bits ----
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,K", [(1, 1), (3, 31), (5, 32), (17, 100), (33, 512), (40, 1001), (2, 4097)])
+def test_mx8_quantize(rows, K, dtype):
+    x = numbers(100, (rows, K), dtype) * torch.exp2(torch.randint(-9, 9, (rows, K), generator=seeded(101))).cuda().to(dtype)
+    if rows > 2:
+        x[1] = 0
+        x[2, K // 2] = float("inf")
+        x[rows - 1, 0] = float("nan")
+    q = tdc_amd.mx8_quantize(x)
+    want, byte = ref.quantize8(host(x))
+    got = host(q.dequantize())
+    assert np.array_equal(got, want, equal_nan=True)
+    assert np.array_equal(host(q.dequantize(BF16)), want, equal_nan=True)
+    codes, scales = q.codes.cpu().numpy(), q.scales.cpu().numpy()
+    assert not codes[:, K:].any()
+    blocks = (K + 31) // 32
+    flat = np.stack([scales[b // 16, :, 4 * (b % 4) + b % 16 // 4] for b in range((K + 511) // 512 * 16)], 1)
+    assert np.array_equal(flat[:, :blocks], byte) and not flat[:, blocks:].any()
+
+
+def test_mx8_rounding_at_every_border():
+    """Every halfway point of the grid, its neighbours, saturation, the smallest and the largest scales."""
+    half = (ref.GRID8[1:] + ref.GRID8[:-1]) / 2
+    v = np.concatenate([half, np.nextafter(half.astype(np.float32), 0).astype(np.float64), np.nextafter(half.astype(np.float32), 1e9).astype(np.float64),
+                        ref.GRID8, [449, 463.9, 464, 465, 480, 496, 511.9]])
+    v = v[: len(v) // 31 * 31].reshape(-1, 31)
+    for power in (0, -60, 100):
+        x = np.concatenate([np.full((len(v), 1), 300.0), v * np.where(np.arange(31) % 2, -1, 1)], 1).astype(np.float32).astype(np.float64) * 2.0 ** power
+        got = host(tdc_amd.mx8_quantize(torch.from_numpy(x).float().cuda()).dequantize())
+        assert np.array_equal(got, ref.quantize8(x)[0])
+    x = torch.full((1, 32), 65504.0, device="cuda")
+    # 65504 = 511.75 2^7 saturates at 448 2^7: half precision's numbers stay finite in 8 bits and back
+    assert tdc_amd.mx8_quantize(x).dequantize()[0, 0] == 57344 and tdc_amd.mx8_quantize(x.half()).dequantize(F16)[0, 0] == 57344
+    tiny = torch.full((1, 32), 2.0 ** -140, device="cuda")
+    assert torch.equal(tdc_amd.mx8_quantize(tiny).dequantize(), torch.zeros_like(tiny))
+
+
+def check_mx8(y, x, w, b, r, act, dtype, what=""):
+    """x, w: the values that the 8 bits stand for."""
+    _, want = ref.linear(x, w, opt(b), opt(r), act)
+    S = np.abs(x) @ np.abs(w).T + (0 if b is None else np.abs(host(b))) + (0 if r is None else np.abs(host(r)))
+    K = x.shape[1]
+    top = lambda v: np.abs(np.pad(v, ((0, 0), (0, -K % 64)))).reshape(len(v), -1, 64).max(2)  # noqa: E731
+    off = (16 + K / 8) * E * S + 64 * 2.0 ** -14 * (top(x) @ top(w).T)
+    close(y, want, 1.1 * off + rounded(want, dtype) * (1 + 1e-2), what)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N,K", PRODUCTS + [(40, 200, 5000), (600, 520, 8200)])
+def test_mx8_linear(M, N, K, dtype):
+    for i, act in enumerate(("none", "relu", "silu")):
+        x, w, b, r = case(110 + 10 * i, M, N, K, dtype, bias=i != 1, residual=i != 2, bias_dtype=F32 if i == 2 else dtype)
+        q, qw = tdc_amd.mx8_quantize(x), tdc_amd.mx8_quantize(w)
+        y = tdc_amd.mx8_linear(x, qw, b, r, act=act)
+        assert y.dtype == dtype and torch.equal(y, tdc_amd.mx8_linear(q, qw, b, r, act=act, out_dtype=dtype))
+        check_mx8(y, host(q.dequantize()), host(qw.dequantize()), b, r, act, dtype, f"{M} {N} {K} {act}")
+
+
+@pytest.mark.parametrize("M,N,K", [(3400, 3500, 4200), (3333, 3850, 128), (30, 40, 40000)])
+def test_mx8_linear_of_whole_numbers_is_exact(M, N, K):
+    """Whole numbers of up to 8 in magnitude are E4M3 values at the scales of blocks that hold an 8 (2^-5), and so are their products above what
+    an instruction keeps."""
+    g = seeded(6)
+    x = torch.zeros(M, K)
+    x.scatter_(1, torch.randint(0, K, (M, 20), generator=g), torch.randint(-3, 4, (M, 20), generator=g).float())
+    w = torch.randint(-4, 5, (N, K), generator=g).float()
+    y = tdc_amd.mx8_linear(x.cuda(), tdc_amd.mx8_quantize(w.cuda()), out_dtype=BF16)
+    assert torch.equal(y.float(), x.cuda() @ w.t().contiguous().cuda())
+
+
+def test_mx8_linear_keeps_nans_to_their_rows():
+    x, w = numbers(130, (70, 700), BF16), numbers(131, (90, 700), BF16)
+    qw = tdc_amd.mx8_quantize(w)
+    want = tdc_amd.mx8_linear(x, qw)
+    x[40, 699] = float("inf")
+    got = tdc_amd.mx8_linear(x, qw)
+    assert torch.equal(got[:40], want[:40]) and torch.equal(got[41:], want[41:]) and got[40].isnan().all()
+    w[7, 300] = float("nan")
+    got = tdc_amd.mx8_linear(x[:40], tdc_amd.mx8_quantize(w))
+    assert got[:, 7].isnan().all() and torch.equal(got[:, :7], want[:40, :7]) and torch.equal(got[:, 8:], want[:40, 8:])
+
+
+# ---- RMS norm ----
+
+ROWS = [(1, 1), (1, 4096), (2, 7), (3, 128), (5, 129), (17, 256), (100, 300), (33, 512), (300, 513), (7, 1001), (40, 2048), (9, 2050), (6, 8192), (3, 5000)]
+
+
+def rms_case(seed, M, C, dtype, residual, weight_dtype=None):
+    x = numbers(seed, (M, C), dtype, 2.0) + 0.5
+    return x, (numbers(seed + 1, (C,), F32) * 0.3 + 1).to(weight_dtype or F32), numbers(seed + 2, (M, C), dtype) if residual else None
+
+
+def summed(x, r):
+    return x if r is None else (x.float() + r.float()).to(x.dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M,C", ROWS)
+def test_rms_norm(M, C, dtype):
+    for residual in (False, True):
+        x, w, r = rms_case(140, M, C, dtype, residual, dtype if residual else F32)
+        out = tdc_amd.rms_norm(x, w, r, eps=1e-3)
+        y, h = out if residual else (out, x)
+        assert torch.equal(h, summed(x, r))
+        _, want, _ = ref.rms(host(h), host(w), float(np.float32(1e-3)))
+        close(y, want, 64 * E * np.abs(want) + rounded(want, dtype) * (1 + 1e-3), f"{M} {C}")
+        close(tdc_amd.rms_norm(x, None, r, eps=1e-3)[0] if residual else tdc_amd.rms_norm(x, eps=1e-3), ref.rms(host(h), 1.0, float(np.float32(1e-3)))[1],
+              (64 * E + U[dtype]) * 1.001 * np.abs(ref.rms(host(h), 1.0, float(np.float32(1e-3)))[1]) + LEAST[dtype])
+        out = tdc_amd.rms_norm_mx8(x, w, r, eps=1e-3)
+        q, h8 = out if residual else (out, x)
+        assert torch.equal(h8, h)
+        # the nearest values, but for numbers within the norm's own error of a border between two
+        low, _ = ref.quantize8(want)
+        got = host(q.dequantize())
+        step = np.maximum(np.abs(want), 0)
+        near = np.abs(got - low) <= 2.0 ** -3 * np.maximum(step, np.abs(want).max() * 2.0 ** -14)
+        assert near.all() and (got != low).mean() <= 0.001 + 2.0 / got.size
+
+
+def check_rms_grads(M, C, dtype, residual, checkpoint, with_dh=True, weight_dtype=None):
+    x, w, r = rms_case(150, M, C, dtype, residual, weight_dtype)
+    dy, dh = numbers(153, (M, C), dtype), numbers(154, (M, C), dtype)
+    wrt = [t.requires_grad_() for t in (x, w, r) if t is not None]
+    out = tdc_amd.rms_norm(x, w, r, eps=1e-3, checkpoint=checkpoint)
+    if residual:
+        got = grads(out, wrt, (dy, dh)) if with_dh else grads(out[0], wrt, dy)
+    else:
+        got = grads(out, wrt, dy)
+    h = host(summed(x.detach(), None if r is None else r.detach()))
+    u, _, rstd = ref.rms(h, host(w), float(np.float32(1e-3)))
+    u = ref.quantize8(h)[0] * rstd if checkpoint else u
+    extra = host(dh) if residual and with_dh else 0.0
+    dx, dw = ref.rms_grads(u, rstd, host(w), host(dy), extra)
+    g = np.abs(host(dy) * host(w))
+    size = rstd * (g + np.abs(u) * (g * np.abs(u)).mean(-1, keepdims=True)) + np.abs(extra)
+    what = f"{M} {C} {residual} {checkpoint}"
+    close(got[0], dx, 64 * E * size + rounded(np.abs(dx) + 64 * E * size, dtype), what + " dx")
+    S = (np.abs(host(dy) * u)).sum(0)
+    close(got[1], dw, 512 * E * S + rounded(np.abs(dw) + 512 * E * S, w.dtype), what + " dweight")
+    if residual:
+        assert torch.equal(got[2], got[0])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M,C", ROWS + [(20000, 24), (3000, 700)])
+def test_rms_norm_gradients(M, C, dtype):
+    check_rms_grads(M, C, dtype, False, None)
+    check_rms_grads(M, C, dtype, True, "mx8", weight_dtype=dtype)
+    check_rms_grads(M, C, dtype, True, None, with_dh=False)
+
+
+def test_rms_norm_where_only_the_sum_is_used():
+    x, w, r = rms_case(160, 5, 40, BF16, True)
+    wrt = [t.requires_grad_() for t in (x, w, r)]
+    y, h = tdc_amd.rms_norm(x, w, r)
+    dh = numbers(161, (5, 40), BF16)
+    got = grads(h, wrt, dh)
+    assert torch.equal(got[0], dh) and torch.equal(got[2], dh) and not got[1].any()
+
+
+def test_rms_norm_strides_specials_and_zeros():
+    wide = numbers(170, (4, 6, 100), BF16)
+    for x in (wide[..., 3:67], wide[:, ::2, 8:72], wide[..., 0:64].transpose(0, 1), wide[:1, :1, :64].expand(3, 2, 64)):
+        assert torch.equal(tdc_amd.rms_norm(x), tdc_amd.rms_norm(x.contiguous()))
+        r = wide[:x.shape[0], :x.shape[1], 33:97].expand(x.shape) if x.shape[1] <= 6 and x.shape[0] <= 4 else None
+        if r is not None:
+            a, b = tdc_amd.rms_norm(x, None, r), tdc_amd.rms_norm(x.contiguous(), None, r.contiguous())
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    x = numbers(171, (9, 333), F32)
+    want = tdc_amd.rms_norm(x)
+    for v in (float("nan"), float("inf")):
+        y = x.clone()
+        y[4, 10] = v
+        y = tdc_amd.rms_norm(y)
+        assert torch.equal(y[:4], want[:4]) and torch.equal(y[5:], want[5:]) and y[4, 10].isnan()
+    assert not tdc_amd.rms_norm(torch.zeros(3, 50, device="cuda")).any()
+
+
+# ---- together ----
+
+def test_block_in_training_and_in_8_bits():
+    """residual -> norm -> factor with an activation -> factor with the residual, as a network's block runs: gradients through all of it against
+    64 bits, and the same block served in 8 bits near the 16-bit one."""
+    M, C, R = 300, 192, 96
+    x, r = numbers(180, (M, C), BF16), numbers(181, (M, C), BF16)
+    gamma = (numbers(182, (C,), F32) * 0.2 + 1)
+    w1, w2, b1 = numbers(183, (R, C), BF16, C ** -0.5), numbers(184, (C, R), BF16, R ** -0.5), numbers(185, (R,), BF16, 0.1)
+    dy = numbers(186, (M, C), BF16)
+    wrt = [t.requires_grad_() for t in (x, r, gamma, w1, w2, b1)]
+
+    def block(checkpoint):
+        n, h = tdc_amd.rms_norm(x, gamma, r, checkpoint=checkpoint)
+        return tdc_amd.linear_act(tdc_amd.linear_act(n, w1, b1, act="silu", checkpoint=checkpoint), w2, None, h, checkpoint=checkpoint)
+    y = block(None)
+    got = grads(y, wrt, dy)
+    d = [t.detach().double().cpu().requires_grad_() for t in wrt]
+    h = d[0] + d[1]
+    n = h / torch.sqrt((h ** 2).mean(-1, keepdim=True) + 1e-6) * d[2]
+    t = n @ d[3].t() + d[5]
+    want_y = t * torch.sigmoid(t) @ d[4].t() + h
+    want = torch.autograd.grad(want_y, d, dy.double().cpu())
+    # some eight roundings to 16 bits one after the other, each u / sqrt(3) of its tensor in the mean
+    for a, b in zip((y, *got), (want_y, *want)):
+        assert (a.detach().double().cpu() - b).norm() <= 8 * U[BF16] * b.norm()
+    # 8 bits: two products of numbers rounded to 4 bits of significand, each 2^-4 / sqrt(3) at most
+    for a, b in zip(grads(block("mx8"), wrt, dy), want):
+        assert (a.double().cpu() - b).norm() <= 2 * 2.0 ** -4 * b.norm()
+    with torch.no_grad():
+        q, h = tdc_amd.rms_norm_mx8(x, gamma, r)
+        z = tdc_amd.mx8_linear(tdc_amd.mx8_linear(q, tdc_amd.mx8_quantize(w1), b1, act="silu"), tdc_amd.mx8_quantize(w2), None, h)
+    assert (z.double().cpu() - want_y).norm() <= 4 * 2.0 ** -4 * want_y.norm()
+
+
+def test_streams_graphs_and_repeats():
+    """Replays with new inputs and the program's own work between them, on a stream that is not the default one, against eager results."""
+    M, N, K = 70, 120, 520
+    x, w, b, r = case(190, M, N, K, BF16)
+    dy = numbers(191, (M, N), BF16)
+    gamma = numbers(192, (K,), F32)
+    qw = tdc_amd.mx8_quantize(w)
+    wrt = [t.requires_grad_() for t in (x, w, b)]
+
+    def step():
+        n, h = tdc_amd.rms_norm(x, gamma, x.detach(), checkpoint="mx8")
+        y = tdc_amd.linear_act(n, w, b, r, act="silu", checkpoint="mx8")
+        g = grads((y, h), wrt, (dy, n.detach()))
+        with torch.no_grad():
+            return (y.detach(), *g, tdc_amd.mx8_linear(x, qw), tdc_amd.mx8_linear(tdc_amd.rms_norm_mx8(x, gamma), qw))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(numbers(200 + k, (M, K), BF16))
+            dy.copy_(numbers(210 + k, (M, N), BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        held = [t.clone() for t in out]
+        want = step()
+        assert all(torch.equal(a, c) for a, c in zip(held, want)), k
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            again = step()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, c) for a, c in zip(again, want)), k
+
+
+def test_refusals():
+    x, w, b, r = case(220, 4, 8, 32, BF16)
+    f = tdc_amd.linear_act
+    for bad in (lambda: f(x.float(), w.float()), lambda: f(x, w.half()), lambda: f(x[:, :31], w), lambda: f(x, w, b[:7]), lambda: f(x, w, b.half()),
+                lambda: f(x, w, None, r[:, :7]), lambda: f(x, w, None, r.float()), lambda: f(x, w, act="gelu"), lambda: f(x, w, checkpoint="mx4"),
+                lambda: f(x.cpu(), w), lambda: f(x, w.cpu()), lambda: f(x, w[0]), lambda: tdc_amd.conv1x1_act(x, w),
+                lambda: tdc_amd.mx8_linear(x, w), lambda: tdc_amd.mx8_linear(x.float(), tdc_amd.mx8_quantize(w)),
+                lambda: tdc_amd.mx8_linear(x, tdc_amd.mx4_quantize(w)), lambda: tdc_amd.mx8_linear(x, tdc_amd.mx8_quantize(w), out_dtype=F32),
+                lambda: tdc_amd.rms_norm(x, b), lambda: tdc_amd.rms_norm(x, None, x.float()), lambda: tdc_amd.rms_norm(torch.zeros(2, 8193, device="cuda")),
+                lambda: tdc_amd.rms_norm(x, eps=-1.0), lambda: tdc_amd.rms_norm(x, checkpoint="mx4"), lambda: tdc_amd.rms_norm(x.int())):
+        with pytest.raises((TypeError, ValueError, tdc_amd.TdcError)):
+            bad()
+    q = tdc_amd.mx8_quantize(w)
+    g = x.clone().requires_grad_()
+    for bad in (lambda: tdc_amd.mx8_quantize(g), lambda: tdc_amd.mx8_linear(g, q), lambda: tdc_amd.mx8_linear(x, q, b.clone().requires_grad_()),
+                lambda: tdc_amd.rms_norm_mx8(g), lambda: tdc_amd.rms_norm_mx8(x, None, g)):
+        with pytest.raises(RuntimeError, match="gradient"):
+            bad()
+    with torch.no_grad():
+        assert tdc_amd.mx8_linear(g, q).shape == (4, 8)
+    y = f(g, w)
+    (d,) = torch.autograd.grad(y, g, torch.ones_like(y), create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
+
+
+def test_copies_of_an_8_bit_tensor():
+    import copy
+    import pickle
+    q = tdc_amd.mx8_quantize(numbers(230, (5, 70), BF16))
+    for c in (copy.deepcopy(q), pickle.loads(pickle.dumps(q)), tdc_amd.Mx8Tensor(q.codes.clone(), q.scales.clone(), q.shape)):
+        assert c._codes_at != q._codes_at and torch.equal(c.dequantize(), q.dequantize())
