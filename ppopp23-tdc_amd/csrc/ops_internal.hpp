@@ -111,7 +111,7 @@ struct TileArgs : ProductOut {
     float *part;                    // sums of the parts: [splits][M][part_stride]
     long long part_stride;
 };
-enum { kTile256, kTile128, kTile32 };
+enum { kTile256, kTile256x128, kTile128Deep, kTile128, kTile64, kTile32 };
 // How a product is dealt out.
 struct TilePlan {
     int kernel;                     // which tile
@@ -142,7 +142,7 @@ struct ActGradArgs {
 };
 void act_grad_plan(ActGradArgs &a);      // pitch and the last five
 long long act_grad_items(const ActGradArgs &a);
-int launch_act_grad(const ActGradArgs &a, int dtype, void *stream);
+int launch_act_grad(const ActGradArgs *jobs, int n, int dtype, void *stream);      // up to three of them
 int launch_column_sums(const float *part, void *out, long long N, int chunks, int out_dtype, void *stream);
 
 // Numbers in 8 bits.

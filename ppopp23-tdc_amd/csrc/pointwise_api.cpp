@@ -56,10 +56,12 @@ ActGradArgs copy_args(const void *from, long long rows, long long n, long long s
     act_grad_plan(a);
     return a;
 }
-int copy_fits(long long rows, long long n) {
-    if (act_grad_items(copy_args(nullptr, rows, n, n, nullptr)) > kMostItems) return invalid("product: too large, a launch has fewer than 2^32 work items");
-    return TDC_OK;
-}
+// Copies and the gradient's first pass are one launch.
+struct Copies {
+    long long items = 0;
+    void add(long long rows, long long n) { items += act_grad_items(copy_args(nullptr, rows, n, n, nullptr)); }
+    int fit() const { return items > kMostItems ? invalid("product: too large, a launch has fewer than 2^32 work items") : (int)TDC_OK; }
+};
 
 // What a pass does, and where its scratch lies.
 struct Forward {
@@ -70,10 +72,10 @@ struct Forward {
 int forward_plan(const tdc_linear_desc &d, Forward &f) {
     f.plan = tile_plan(d.M, d.N, d.K, d.dtype);
     if (int st = plan_fits("product", f.plan)) return st;
-    if ((f.pack_x = must_pack(d.M, d.K, d.x_stride)))
-        if (int st = copy_fits(d.M, d.K)) return st;
-    if ((f.pack_w = must_pack(d.N, d.K, d.w_stride)))
-        if (int st = copy_fits(d.N, d.K)) return st;
+    Copies copies;
+    if ((f.pack_x = must_pack(d.M, d.K, d.x_stride))) copies.add(d.M, d.K);
+    if ((f.pack_w = must_pack(d.N, d.K, d.w_stride))) copies.add(d.N, d.K);
+    if (int st = copies.fit()) return st;
     f.w = f.x + (f.pack_x ? padded(packed_bytes(d.M, d.K)) : 0);
     f.part = f.w + (f.pack_w ? padded(packed_bytes(d.N, d.K)) : 0);
     f.all = f.part + (size_t)f.plan.part_bytes;
@@ -90,14 +92,14 @@ int backward_plan(const tdc_linear_desc &d, Backward &b) {
     b.dw = tile_plan(d.N, d.K, d.M, d.dtype);
     if (int st = plan_fits("product's gradient", b.dx)) return st;
     if (int st = plan_fits("product's gradient", b.dw)) return st;
-    if (int st = copy_fits(d.M, d.N)) return st;
     b.make_dz = d.act != TDC_ACT_NONE || must_pack(d.M, d.N, d.y_stride);
     b.pack_x = d.kept_dtype == TDC_MX8 || must_pack(d.M, d.K, d.x_stride);
     b.pack_w = must_pack(d.N, d.K, d.w_stride);
-    if (b.pack_x && d.kept_dtype != TDC_MX8)
-        if (int st = copy_fits(d.M, d.K)) return st;
-    if (b.pack_w)
-        if (int st = copy_fits(d.N, d.K)) return st;
+    Copies copies;
+    copies.add(d.M, d.N);
+    if (b.pack_x && d.kept_dtype != TDC_MX8) copies.add(d.M, d.K);
+    if (b.pack_w) copies.add(d.N, d.K);
+    if (int st = copies.fit()) return st;
     b.grad = copy_args(nullptr, d.M, d.N, d.y_stride, nullptr);
     b.sums = b.dz + (b.make_dz ? padded(packed_bytes(d.M, d.N)) : 0);
     b.x = b.sums + padded((size_t)b.grad.chunks * d.N * 4);
@@ -212,14 +214,17 @@ int tdc_linear_forward(const tdc_linear_desc *desc, const void *x, const void *w
     if (int st = forward_plan(d, f)) return st;
     if (int st = ws_check("product", ws, ws_bytes, f.all)) return st;
     char *const scratch = (char *)ws;
+    ActGradArgs jobs[2];
+    int n = 0;
     if (f.pack_x) {
-        if (int e = launch_act_grad(copy_args(x, d.M, d.K, d.x_stride, scratch + f.x), d.dtype, stream)) return launched("product", e);
+        jobs[n++] = copy_args(x, d.M, d.K, d.x_stride, scratch + f.x);
         x = scratch + f.x;
     }
     if (f.pack_w) {
-        if (int e = launch_act_grad(copy_args(w, d.N, d.K, d.w_stride, scratch + f.w), d.dtype, stream)) return launched("product", e);
+        jobs[n++] = copy_args(w, d.N, d.K, d.w_stride, scratch + f.w);
         w = scratch + f.w;
     }
+    if (int e = launch_act_grad(jobs, n, d.dtype, stream)) return launched("product", e);
     const Lying lx = lying(x, d.M, d.K, d.x_stride, f.pack_x), lw = lying(w, d.N, d.K, d.w_stride, f.pack_w);
     TileArgs a{};
     a.x = lx.at;
@@ -273,8 +278,10 @@ int tdc_linear_backward(const tdc_linear_desc *desc, const void *x, const void *
     char *const scratch = (char *)ws;
     // dz, and its sums
     void *made = dz ? dz : b.make_dz && (dx || dw) ? scratch + b.dz : nullptr;
+    ActGradArgs jobs[3];
+    int n = 0;
     if (made || dbias) {
-        ActGradArgs g = b.grad;
+        ActGradArgs &g = jobs[n++] = b.grad;
         g.dy = dy;
         g.kept = kept;
         g.dz = made;
@@ -282,8 +289,17 @@ int tdc_linear_backward(const tdc_linear_desc *desc, const void *x, const void *
         g.part = (float *)(scratch + b.sums);
         g.act = d.act;
         g.sums_dtype = d.bias_dtype;
-        if (int e = launch_act_grad(g, d.dtype, stream)) return launched(what, e);
     }
+    // (and what no tile can take as it lies)
+    if (dx && b.pack_w) {
+        jobs[n++] = copy_args(w, d.N, d.K, d.w_stride, scratch + b.w);
+        w = scratch + b.w;
+    }
+    if (dw && b.pack_x && d.kept_dtype != TDC_MX8) {
+        jobs[n++] = copy_args(x, d.M, d.K, d.x_stride, scratch + b.x);
+        x = scratch + b.x;
+    }
+    if (int e = launch_act_grad(jobs, n, d.dtype, stream)) return launched(what, e);
     const Lying lz = made ? lying(made, d.M, d.N, 0, true) : lying(dy, d.M, d.N, d.y_stride, false);
     TileArgs a{};
     a.x = lz.at;
@@ -291,10 +307,6 @@ int tdc_linear_backward(const tdc_linear_desc *desc, const void *x, const void *
     a.part = (float *)(scratch + b.part);
     a.act = TDC_ACT_NONE;
     if (dx) {
-        if (b.pack_w) {
-            if (int e = launch_act_grad(copy_args(w, d.N, d.K, d.w_stride, scratch + b.w), d.dtype, stream)) return launched(what, e);
-            w = scratch + b.w;
-        }
         const Lying lw = lying(w, d.N, d.K, d.w_stride, b.pack_w);
         a.w = lw.at;
         a.w_stride = lw.stride;
@@ -310,9 +322,6 @@ int tdc_linear_backward(const tdc_linear_desc *desc, const void *x, const void *
     if (dw) {
         if (d.kept_dtype == TDC_MX8) {
             if (int e = launch_mx8_dequantize(x, x_scales, d.M, d.K, scratch + b.x, d.dtype, round_up(d.K, 8), stream)) return launched(what, e);
-            x = scratch + b.x;
-        } else if (b.pack_x) {
-            if (int e = launch_act_grad(copy_args(x, d.M, d.K, d.x_stride, scratch + b.x), d.dtype, stream)) return launched(what, e);
             x = scratch + b.x;
         }
         const Lying lx = lying(x, d.M, d.K, d.x_stride, b.pack_x);

@@ -1,6 +1,7 @@
 // What surrounds the products in 16 and 8 bits: how one is dealt out, the join of a sum's parts, and what the gradients need
 // before their products: dz = dy act'(z), its sums over the rows, copies of rows that no request could take as they lie.
 #include <algorithm>
+#include <cmath>
 
 #include "ops_device.hpp"
 
@@ -8,45 +9,85 @@ namespace tdc {
 
 // ---- how a product is dealt out ----
 
+// Tiles, the time of a step and what a tile takes besides (us), as timed with one workgroup a compute unit (M x N x K in bf16, kernel
+// by kernel; a compute unit that holds several gives each its share): 32 x 128 256 x 4096 x 4096 22.9, 64 x 128 512 x 4096 x 4096 28.1,
+// 128 x 128 1024 x 4096 x 4096 40.3, 256 x 128 8192 x 1024 x 4096 74.7, 256 x 256 4096 x 4096 x 4096 124 (0.6 a step where few compute units
+// work: their clock).  Larger tiles do more a step, smaller ones leave fewer compute units without work, and so do parts of the sum, which
+// cost a launch and their bytes: 1024 x 1024 x 1024 8.0 in tiles of 32 rows, 12.6 of 128, 31.9 of 256; 128 x 512 x 25088 19.3 in 14 parts
+// of 32 rows, 106 whole; 8192 x 8192 x 1024 158 in tiles of 256, 166 in 128 x 128 three a compute unit, 195 one by one; 25088 x 512 x 128 15.5
+// three a compute unit, 20.4 in tiles of 256.
+struct Timing {
+    int m, n;
+    double step, besides;
+    int together;      // workgroups of a compute unit that hide each other's `besides`
+};
+static const Timing kTimings[] = {{256, 256, 0.85, 11.0, 1}, {256, 128, 0.53, 5.0, 1}, {128, 128, 0.28, 2.5, 1}, {128, 128, 0.31, 2.1, 3}, {64, 128, 0.18, 1.0, 1}, {32, 128, 0.145, 1.0, 1}};
+
 TilePlan tile_plan(long long M, long long N, long long K, int in_dtype) {
-    TilePlan p{};
-    const long long step = in_dtype == TDC_MX8 ? 64 : 32;
-    p.steps = (int)((K + step - 1) / step);
-    auto tiles = [&](long long m, long long n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
-    p.kernel = M <= 32 ? kTile32 : p.steps >= 64 && tiles(256, 256) >= 192 ? kTile256 : kTile128;
-    const long long m = p.kernel == kTile256 ? 256 : p.kernel == kTile128 ? 128 : 32, n = p.kernel == kTile256 ? 256 : 128;
-    p.tm = (int)((M + m - 1) / m);
-    p.tn = (int)((N + n - 1) / n);
-    const long long all = (long long)p.tm * p.tn;
-    p.blocks = round_up(all, 8);
-    p.splits = 1;
-    p.split_steps = p.steps;
-    if (all < 256 && p.steps >= 16) {
-        const long long splits = std::min<long long>(p.steps / 8, (512 + all - 1) / all);
-        p.split_steps = (int)round_up((p.steps + splits - 1) / splits, 8);
-        p.splits = (p.steps + p.split_steps - 1) / p.split_steps;
+    const long long step = in_dtype == TDC_MX8 ? 64 : 32, steps = (K + step - 1) / step;
+    TilePlan best{};
+    double best_time = 0;
+    for (int kernel = kTile256; kernel <= kTile32; ++kernel) {
+        const Timing &t = kTimings[kernel];
+        const long long tm = (M + t.m - 1) / t.m, tn = (N + t.n - 1) / t.n, all = tm * tn;
+        // Parts as they fill the compute units, or half of that; eight steps each at least.
+        const long long most = std::min(256 / all, steps / 8);
+        for (const long long want : {1ll, most / 2, most}) {
+            if (want < 1) continue;
+            const long long split_steps = want == 1 ? steps : round_up((steps + want - 1) / want, 8), splits = (steps + split_steps - 1) / split_steps;
+            const double each = (double)(all * splits) / 256, rounds = t.together == 1 ? std::ceil(each) : std::max(each, 1.0);
+            double time = 4.0 + rounds * ((double)split_steps * t.step + t.besides / t.together) + (t.together > 1 ? t.besides : 0.0);
+            if (splits > 1) time += 4.0 + (double)splits * M * N * 8 / 4e6;
+            if (best.steps && time >= best_time) continue;
+            best_time = time;
+            best.kernel = kernel;
+            best.steps = (int)steps;
+            best.tm = (int)tm;
+            best.tn = (int)tn;
+            best.splits = (int)splits;
+            best.split_steps = (int)split_steps;
+            best.blocks = round_up(all, 8);
+        }
     }
-    p.part_stride = round_up(N, 4);
-    p.part_bytes = p.splits > 1 ? p.splits * M * p.part_stride * 4 : 0;
-    p.items = std::max(p.blocks * p.splits * 256, p.splits > 1 ? (M * (p.part_stride / 4) + 255) / 256 * 256 : 0);
-    return p;
+    best.part_stride = round_up(N, 4);
+    best.part_bytes = best.splits > 1 ? best.splits * M * best.part_stride * 4 : 0;
+    best.items = std::max(best.blocks * best.splits * 256, best.splits > 1 ? (M * (best.part_stride / 4) + 31) / 32 * 256 : 0);
+    return best;
 }
 
 // ---- the join ----
 
-// Four neighbouring outputs a thread: the parts in their order, then what a tile does with its sums.
-template <int DT, int ACT>
+// Four neighbouring outputs a thread: the parts in their order, then what a tile does with its sums.  GROUPS: so many threads share the
+// outputs, a run of the parts each, and meet in LDS (98 parts of 128 x 512: 25 us with one, a chain of loads).
+template <int DT, int ACT, int GROUPS>
 __global__ void __launch_bounds__(256) tdc_product_join_kernel(const TileArgs a, int across) {
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x, m = id / across, n = (id - m * across) * 4;
-    if (m >= a.M) return;
+    constexpr int kThreads = 256 / GROUPS;
+    __shared__ float4 lds[GROUPS > 1 ? 256 : 1];
+    const int t = threadIdx.x % kThreads, g = threadIdx.x / kThreads;
+    const long long id = (long long)blockIdx.x * kThreads + t, m = id / across, n = (id - m * across) * 4;
     using T = typename Num<DT>::type;
-    const float *const from = a.part + m * a.part_stride + n;
     const long long part = a.M * a.part_stride;
-    float4 v = *reinterpret_cast<const float4 *>(from);
-    for (int s = 1; s < a.splits; ++s) {
-        const float4 w = *reinterpret_cast<const float4 *>(from + s * part);
-        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+    const int each = (a.splits + GROUPS - 1) / GROUPS, end = min(a.splits, (g + 1) * each);
+    float4 v = make_float4(0, 0, 0, 0);
+    if (m < a.M) {
+        const float *const from = a.part + m * a.part_stride + n;
+#pragma unroll 8
+        for (int s = g * each; s < end; ++s) {
+            const float4 w = *reinterpret_cast<const float4 *>(from + s * part);
+            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        }
     }
+    if constexpr (GROUPS > 1) {
+        lds[threadIdx.x] = v;
+        __syncthreads();
+        if (g) return;
+#pragma unroll
+        for (int k = 1; k < GROUPS; ++k) {
+            const float4 w = lds[k * kThreads + t];
+            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        }
+    }
+    if (m >= a.M) return;
     const float sums[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -58,14 +99,18 @@ __global__ void __launch_bounds__(256) tdc_product_join_kernel(const TileArgs a,
         reinterpret_cast<T *>(a.y)[m * a.y_stride + n + i] = Num<DT>::down(act_of<ACT>(z));
     }
 }
+template <int DT, int ACT>
+static int launch_join_act(const TileArgs &a, hipStream_t s) {
+    const int across = (int)(a.part_stride / 4);
+    const long long threads = a.M * across;
+    if (a.splits > 16) tdc_product_join_kernel<DT, ACT, 8><<<(unsigned)((threads + 31) / 32), 256, 0, s>>>(a, across);
+    else tdc_product_join_kernel<DT, ACT, 1><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(a, across);
+    return (int)hipGetLastError();
+}
 template <int DT>
 static int launch_join_of(const TileArgs &a, hipStream_t s) {
-    const int across = (int)(a.part_stride / 4);
-    const unsigned blocks = (unsigned)((a.M * across + 255) / 256);
-    if (a.act == TDC_ACT_RELU) tdc_product_join_kernel<DT, TDC_ACT_RELU><<<blocks, 256, 0, s>>>(a, across);
-    else if (a.act == TDC_ACT_SILU) tdc_product_join_kernel<DT, TDC_ACT_SILU><<<blocks, 256, 0, s>>>(a, across);
-    else tdc_product_join_kernel<DT, TDC_ACT_NONE><<<blocks, 256, 0, s>>>(a, across);
-    return (int)hipGetLastError();
+    if (a.act == TDC_ACT_RELU) return launch_join_act<DT, TDC_ACT_RELU>(a, s);
+    return a.act == TDC_ACT_SILU ? launch_join_act<DT, TDC_ACT_SILU>(a, s) : launch_join_act<DT, TDC_ACT_NONE>(a, s);
 }
 int launch_join(const TileArgs &a, int y_dtype, void *stream) {
     return y_dtype == TDC_F16 ? launch_join_of<TDC_F16>(a, (hipStream_t)stream) : launch_join_of<TDC_BF16>(a, (hipStream_t)stream);
@@ -76,11 +121,10 @@ int launch_join(const TileArgs &a, int y_dtype, void *stream) {
 // A workgroup of 256 owns `across` vectors of eight columns and `chunk_rows` rows.  Sums over the rows: a thread's own rows in fp32 (those of
 // a chunk: see act_grad_plan), then over threads and chunks in 64 bits, in a fixed order.  (Sums are of dz before its rounding.)
 template <int DT, int ACT>
-__global__ void __launch_bounds__(256) tdc_act_grad_kernel(const ActGradArgs a) {
+static __device__ __forceinline__ void act_grad(const ActGradArgs &a, unsigned block, float (&lds)[256][9]) {
     using P = Pack<DT, 8>;
     using T = typename Num<DT>::type;
-    __shared__ float lds[256][9];
-    const unsigned chunk = blockIdx.x / (unsigned)a.tiles, tile = blockIdx.x - chunk * a.tiles;
+    const unsigned chunk = block / (unsigned)a.tiles, tile = block - chunk * a.tiles;
     const int down = 256 / a.across, c = threadIdx.x % a.across, r = threadIdx.x / a.across;
     const long long n = ((long long)tile * a.across + c) * 8, row0 = chunk * a.chunk_rows, rows = min(a.chunk_rows, a.M - row0);
     float sum[8] = {};
@@ -93,6 +137,7 @@ __global__ void __launch_bounds__(256) tdc_act_grad_kernel(const ActGradArgs a) 
         return v;
     };
     if (n < a.N) {
+#pragma unroll 4
         for (long long i = r; i < rows; i += down) {
             const long long m = row0 + i;
             float v[8], z[8];
@@ -117,8 +162,25 @@ __global__ void __launch_bounds__(256) tdc_act_grad_kernel(const ActGradArgs a) 
         if (at >= a.N) continue;
         double s = 0;
         for (int i = 0; i < down; ++i) s += lds[i * a.across + k / 8][k % 8];
-        a.part[chunk * a.N + at] = (float)s;
+        if (a.chunks > 1) a.part[chunk * a.N + at] = (float)s;
+        else if (a.sums_dtype == TDC_F32) reinterpret_cast<float *>(a.sums)[at] = (float)s;
+        else reinterpret_cast<T *>(a.sums)[at] = Num<DT>::down((float)s);
     }
+}
+// Up to three such jobs side by side.
+struct ActGradJobs {
+    ActGradArgs job[3];
+    unsigned end[3];      // workgroups up to a job's last
+};
+template <int DT>
+__global__ void __launch_bounds__(256) tdc_act_grad_kernel(const ActGradJobs jobs) {
+    __shared__ float lds[256][9];
+    const int k = (blockIdx.x >= jobs.end[0]) + (blockIdx.x >= jobs.end[1]);
+    const ActGradArgs &a = jobs.job[k];
+    const unsigned block = blockIdx.x - (k ? jobs.end[k - 1] : 0);
+    if (a.act == TDC_ACT_RELU) act_grad<DT, TDC_ACT_RELU>(a, block, lds);
+    else if (a.act == TDC_ACT_SILU) act_grad<DT, TDC_ACT_SILU>(a, block, lds);
+    else act_grad<DT, TDC_ACT_NONE>(a, block, lds);
 }
 // The chunks' sums, 64 columns a workgroup, sixteen threads a column.
 template <int OUT>
@@ -127,8 +189,10 @@ __global__ void __launch_bounds__(1024) tdc_column_sums_kernel(const float *part
     const long long n = (long long)blockIdx.x * 64 + (threadIdx.x & 63);
     const int k = threadIdx.x >> 6;
     double s = 0;
-    if (n < N)
+    if (n < N) {
+#pragma unroll 8
         for (int i = k; i < chunks; i += 16) s += part[i * N + n];
+    }
     lds[k][threadIdx.x & 63] = s;
     __syncthreads();
     if (k || n >= N) return;
@@ -150,25 +214,35 @@ void act_grad_plan(ActGradArgs &a) {
     a.across = 1;
     while (a.across < 32 && a.across < vectors) a.across *= 2;
     a.tiles = (int)((vectors + a.across - 1) / a.across);
-    // Some 2048 workgroups, of four rows a thread at least and 256 at most (a sum in fp32 is no longer than that).
+    // Some 2048 workgroups, of four rows a thread at least and 256 at most (a sum in fp32 is no longer than that); sixteen rows a thread
+    // make one chunk, whose sums need no second launch.
     const long long down = 256 / a.across, want = std::max(1ll, 2048ll / a.tiles);
     a.chunk_rows = round_up(std::clamp((a.M + want - 1) / want, 4 * down, 256 * down), down);
+    if (a.M <= 16 * down) a.chunk_rows = 16 * down;
     a.chunks = (int)((a.M + a.chunk_rows - 1) / a.chunk_rows);
 }
 long long act_grad_items(const ActGradArgs &a) {
     return std::max((long long)a.chunks * a.tiles * 256, (a.N + 63) / 64 * 1024);
 }
-template <int DT>
-static int launch_act_grad_of(const ActGradArgs &a, hipStream_t s) {
-    const unsigned blocks = (unsigned)a.chunks * (unsigned)a.tiles;
-    if (a.act == TDC_ACT_RELU) tdc_act_grad_kernel<DT, TDC_ACT_RELU><<<blocks, 256, 0, s>>>(a);
-    else if (a.act == TDC_ACT_SILU) tdc_act_grad_kernel<DT, TDC_ACT_SILU><<<blocks, 256, 0, s>>>(a);
-    else tdc_act_grad_kernel<DT, TDC_ACT_NONE><<<blocks, 256, 0, s>>>(a);
+int launch_act_grad(const ActGradArgs *jobs, int n, int dtype, void *stream) {
+    if (!n) return 0;
+    ActGradJobs all{};
+    unsigned blocks = 0;
+    for (int k = 0; k < 3; ++k) {
+        if (k < n) {
+            all.job[k] = jobs[k];
+            blocks += (unsigned)jobs[k].chunks * (unsigned)jobs[k].tiles;
+        }
+        all.end[k] = blocks;
+    }
+    const hipStream_t s = (hipStream_t)stream;
+    if (dtype == TDC_F16) tdc_act_grad_kernel<TDC_F16><<<blocks, 256, 0, s>>>(all);
+    else tdc_act_grad_kernel<TDC_BF16><<<blocks, 256, 0, s>>>(all);
     if (hipError_t e = hipGetLastError()) return (int)e;
-    return a.sums ? launch_column_sums(a.part, a.sums, a.N, a.chunks, a.sums_dtype, s) : 0;
-}
-int launch_act_grad(const ActGradArgs &a, int dtype, void *stream) {
-    return dtype == TDC_F16 ? launch_act_grad_of<TDC_F16>(a, (hipStream_t)stream) : launch_act_grad_of<TDC_BF16>(a, (hipStream_t)stream);
+    for (int k = 0; k < n; ++k)
+        if (jobs[k].sums && jobs[k].chunks > 1)
+            if (int e = launch_column_sums(jobs[k].part, jobs[k].sums, jobs[k].N, jobs[k].chunks, jobs[k].sums_dtype, stream)) return e;
+    return 0;
 }
 
 }  // namespace tdc

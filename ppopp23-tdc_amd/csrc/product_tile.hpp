@@ -11,16 +11,18 @@ typedef short s4_t __attribute__((ext_vector_type(4)));
 
 // A workgroup of four waves, WM x WN of them, owns 32 MB WM rows of x and 32 NB WN of w (below: outputs), a wave MB x NB blocks
 // of 32 x 32.  A step is 64 bytes of each: 32 numbers of 16 bits, 64 of 8.
-template <int WM, int WN, int MB, int NB>
+// LDS holds B steps.
+template <int WM, int WN, int MB, int NB, int B>
 struct Shape {
-    static constexpr int M = 32 * MB * WM, N = 32 * NB * WN;
+    static constexpr int M = 32 * MB * WM, N = 32 * NB * WN, kBuffers = B;
+    static constexpr int kPerUnit = MB * NB <= 2 ? 2 : MB * NB <= 4 && B <= 3 ? 3 : 1;      // workgroups of a compute unit that the registers are for
     static constexpr int kBuffer = (M + N) * 64;                     // bytes of a step: x, then w
     static constexpr int kRequests = (M + N) / 16, kChunks = (kRequests + 3) / 4;   // of a step, of 1 KiB each: in all, of a wave
     static constexpr int kScaleX = (M + 63) / 64 * 64;               // (8 bits: rows of x among those whose scales are requested)
     static constexpr int kScales = (kScaleX + N) * 16;               // bytes of the scales of 512 numbers
     static constexpr int kScaleRequests = (kScaleX + N) / 64, kScaleChunks = (kScaleRequests + 3) / 4;
-    static constexpr int kStage = 4 * NB * 4096;                     // what the outputs pass through
-    static constexpr int kLds16 = 4 * kBuffer + N * 4, kLds8 = 4 * kBuffer + 2 * kScales + N * 4;
+    static constexpr int kLds16 = kBuffers * kBuffer + N * 4, kLds8 = kBuffers * kBuffer + 2 * kScales + N * 4;
+    static_assert(kBuffers * kBuffer >= 4 * NB * 4096, "what the outputs pass through");
 };
 
 // Which tile a workgroup has, if any: neighbouring workgroups of a die take tiles of eight rows by as many columns as run at once, which
@@ -68,6 +70,12 @@ struct Source {
     static __device__ __forceinline__ long long advance(long long stride) { return T ? kStep * stride : 64; }
 };
 
+// Eight bytes a lane from LDS, transposed among sixteen lanes: of the four places of the sum that they point at, 32 bytes each, a lane gets
+// its number of each.  (`__restrict` says nothing about so short a life that is not so, but gives the read a name for the compiler, which
+// else waits for all requests into LDS before it: 1046 us for 8192 x 8192 x 8192 with both operands across the sum, 845 without that wait.)
+typedef __attribute__((address_space(3))) s4_t lds_s4_t;
+static __device__ __forceinline__ s4_t read_transposed(lds_s4_t *__restrict from) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(from); }
+
 // A wave's reads of one operand from LDS: block i (32 rows from `first` on, a multiple of 32), its two halves.
 template <bool T, int R, bool W, int BLOCKS>
 struct Fragments {
@@ -93,9 +101,8 @@ struct Fragments {
     // Read `part` (below kReads) of half `h` of block i, from the buffer's start for this operand on.
     __device__ __forceinline__ void read(const unsigned char *lds, int buffer, int i, int h, int part, i4_t &to) const {
         if constexpr (T) {
-            typedef __attribute__((address_space(3))) s4_t *lds_t;
             const unsigned char *const from = lds + (buffer + at[i & 1]) + (i >> 1) * 128 + (h * 16 + part * 4) * R * 2;
-            const s4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(from));
+            const s4_t v = read_transposed((lds_s4_t *)(from));
             typedef int i2_t __attribute__((ext_vector_type(2)));
             const i2_t w = __builtin_bit_cast(i2_t, v);
             to[2 * part] = w[0];
@@ -121,12 +128,13 @@ static __device__ __forceinline__ f16_t mfma8(const i4_t (&a)[2], const i4_t (&b
 
 // IN: type of the operands (TDC_F16, TDC_BF16, TDC_MX8).  XT, WT: x or w lies across the sum.  OUT: type of y, or TDC_F32 for the sums of one of
 // `splits` parts of the axis, which a launch of its own joins.
-template <int IN, bool XT, bool WT, int OUT, bool Z, int WM, int WN, int MB, int NB>
-__global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_product_tile_kernel(const TileArgs a) {
-    using L = Shape<WM, WN, MB, NB>;
+template <int IN, bool XT, bool WT, int OUT, bool Z, int WM, int WN, int MB, int NB, int B>
+__global__ void __launch_bounds__(256, (Shape<WM, WN, MB, NB, B>::kPerUnit)) tdc_product_tile_kernel(const TileArgs a) {
+    using L = Shape<WM, WN, MB, NB, B>;
     using SX = Source<IN, XT, L::M, false>;
     using SW = Source<IN, WT, L::N, true>;
     constexpr bool kPart = OUT == TDC_F32, k8 = IN == TDC_MX8;
+    constexpr int kLeft = (L::kBuffers - 2) * L::kChunks;       // requests that may be on their way when a step's numbers but one have to be there
     constexpr int kRX = L::M / 16;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), q = lane >> 5;
@@ -167,7 +175,7 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_product_tile_ker
         w_there -= SW::kStep;
     };
     // 8 bits: the scales of 512 numbers, a row a lane.
-    unsigned char *const lds_scales = lds + 4 * L::kBuffer;
+    unsigned char *const lds_scales = lds + L::kBuffers * L::kBuffer;
     const int groups = (a.steps + 7) / 8;
     auto fetch_scales = [&](int g) {
         const long long at = min(first_step / 8 + g, groups - 1);
@@ -217,38 +225,40 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_product_tile_ker
     int sx[MB][2], sw[NB][2];
     if constexpr (k8) fetch_scales(0);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < L::kBuffers; ++s) {
 #pragma unroll
         for (int i = 0; i < L::kChunks; ++i) fetch(i, s * L::kBuffer);
         fetched();
     }
     if (t < L::N) bias[t] = b;
-    meet<2 * L::kChunks>();
+    meet<kLeft>();
 #pragma unroll
     for (int n = 0; n < kReads; ++n) read(std::integral_constant<int, 0>{}, n, 0);
     if constexpr (k8) read_scales(0, sx, sw);
-    meet<2 * L::kChunks>();      // (the first step's requests go where these reads come from)
+    meet<kLeft>();      // (the first step's requests go where these reads come from)
 
-    // Step `step` of this workgroup, of which S = step mod 2: its numbers are in register set S.  Between its matrix instructions stand the
-    // LDS reads of the next step and the requests of the step four on, one at a time, so that none of them keeps the matrix unit waiting.
-    auto run = [&](auto parity, int step) {
-        constexpr int S = decltype(parity)::value, kOps = kReads + L::kChunks;
-        constexpr int kMfma = (k8 ? 1 : 2) * MB * NB;
-        const int next = (step + 1 & 3) * L::kBuffer, now = (step & 3) * L::kBuffer;
+    // A step, the S-th of two: its numbers are in register set S.  Between its matrix instructions stand the
+    // LDS reads of the next step and the requests of the step `kBuffers` on, one at a time, so that none of them keeps the matrix unit waiting.
+    int now = 0, next = L::kBuffer;
+    auto run = [&](auto parity) {
+        constexpr int S = decltype(parity)::value, kMfma = (k8 ? 1 : 2) * MB * NB, kEarly = (kMfma * 3 + 3) / 4;
         const std::integral_constant<int, S ^ 1> other;
 #pragma unroll
         for (int n = 0; n < kMfma; ++n) {
             const int h = n / (MB * NB), j = n % (MB * NB) / MB, i = n % MB;
             if constexpr (k8) acc[j][i] = mfma8(w[S][j], x[S][i], acc[j][i], sw[j][S], sx[i][S]);
             else acc[j][i] = mfma16<IN>(w[S][j][h], x[S][i][h], acc[j][i]);
+            // (the requests evenly: four waves that ask at once would wait for the address unit, and the matrix unit with them.  The
+            // reads in the first three quarters, so that none is out when the waves meet)
 #pragma unroll
-            for (int o = n * kOps / kMfma; o < (n + 1) * kOps / kMfma; ++o) {
-                if (o < kReads) read(other, o, next);
-                else fetch(o - kReads, now);
-            }
+            for (int o = min(n * kReads / kEarly, kReads); o < min((n + 1) * kReads / kEarly, kReads); ++o) read(other, o, next);
+#pragma unroll
+            for (int o = n * L::kChunks / kMfma; o < (n + 1) * L::kChunks / kMfma; ++o) fetch(o, now);
             __builtin_amdgcn_sched_barrier(0);
         }
         fetched();
+        now = next;
+        next = next == (L::kBuffers - 1) * L::kBuffer ? 0 : next + L::kBuffer;
         if constexpr (k8 && S == 1) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -258,7 +268,7 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_product_tile_ker
                 for (int j = 0; j < NB; ++j) sw[j][h] = (int)((unsigned)sw[j][h] >> 8);
             }
         }
-        meet<2 * L::kChunks>();
+        meet<kLeft>();
     };
     // (an odd number of steps is rounded up: what lies past the last number is zeros)
     const int steps = (steps_here + 1) / 2 * 2;
@@ -267,15 +277,15 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_product_tile_ker
         for (int g = 0; step < steps; ++g) {
             fetch_scales(g + 1);
             for (const int end = min(step + 8, steps); step < end; step += 2) {
-                run(std::integral_constant<int, 0>{}, step);
-                run(std::integral_constant<int, 1>{}, step + 1);
+                run(std::integral_constant<int, 0>{});
+                run(std::integral_constant<int, 1>{});
             }
             read_scales(g + 1, sx, sw);
         }
     } else {
         for (; step < steps; step += 2) {
-            run(std::integral_constant<int, 0>{}, step);
-            run(std::integral_constant<int, 1>{}, step + 1);
+            run(std::integral_constant<int, 0>{});
+            run(std::integral_constant<int, 1>{});
         }
     }
     meet<0>();       // (nothing may still be on its way into LDS when the outputs pass through it, or the workgroup ends)
@@ -292,12 +302,12 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_product_tile_ker
     } else finish_tile<OUT, MB, NB, Z>(a, acc, m, n, bias + wn * 32 * NB, stage);
 }
 
-template <int IN, bool XT, bool WT, int OUT, bool Z, int WM, int WN, int MB, int NB>
+template <int IN, bool XT, bool WT, int OUT, bool Z, int WM, int WN, int MB, int NB, int B>
 static int launch_tile(TileArgs &a, const TilePlan &p, hipStream_t s) {
-    using L = Shape<WM, WN, MB, NB>;
+    using L = Shape<WM, WN, MB, NB, B>;
     constexpr int kLds = IN == TDC_MX8 ? L::kLds8 : L::kLds16;
     static unsigned long long done = 0;
-    auto *const fn = &tdc_product_tile_kernel<IN, XT, WT, OUT, Z, WM, WN, MB, NB>;
+    auto *const fn = &tdc_product_tile_kernel<IN, XT, WT, OUT, Z, WM, WN, MB, NB, B>;
     if (int e = allow_lds((const void *)fn, kLds, done)) return e;
     fn<<<(unsigned)(p.blocks * p.splits), 256, kLds, s>>>(a);
     return (int)hipGetLastError();
@@ -305,9 +315,12 @@ static int launch_tile(TileArgs &a, const TilePlan &p, hipStream_t s) {
 template <int IN, bool XT, bool WT, int OUT, bool Z>
 static int launch_shape(TileArgs &a, const TilePlan &p, hipStream_t s) {
     switch (p.kernel) {
-        case kTile256: return launch_tile<IN, XT, WT, OUT, Z, 2, 2, 4, 4>(a, p, s);
-        case kTile128: return launch_tile<IN, XT, WT, OUT, Z, 2, 2, 2, 2>(a, p, s);
-        default: return launch_tile<IN, XT, WT, OUT, Z, 1, 4, 1, 1>(a, p, s);
+        case kTile256: return launch_tile<IN, XT, WT, OUT, Z, 2, 2, 4, 4, 4>(a, p, s);
+        case kTile256x128: return launch_tile<IN, XT, WT, OUT, Z, 2, 2, 4, 2, 6>(a, p, s);
+        case kTile128Deep: return launch_tile<IN, XT, WT, OUT, Z, 2, 2, 2, 2, 8>(a, p, s);
+        case kTile128: return launch_tile<IN, XT, WT, OUT, Z, 2, 2, 2, 2, 3>(a, p, s);
+        case kTile64: return launch_tile<IN, XT, WT, OUT, Z, 2, 2, 1, 2, 6>(a, p, s);
+        default: return launch_tile<IN, XT, WT, OUT, Z, 1, 4, 1, 1, 7>(a, p, s);
     }
 }
 // One launch, or one for the parts of the sum and one that joins them.

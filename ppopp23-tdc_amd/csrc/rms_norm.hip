@@ -63,6 +63,11 @@ static __device__ __forceinline__ void again(T &v) {
 // Eight weights from column c on.
 template <int DT>
 static __device__ __forceinline__ void weights(const RmsArgs &a, int c, float (&w)[8]) {
+    if (a.weight && c + 8 <= a.C) {
+        if (DT == TDC_F32 || a.weight_dtype == TDC_F32) Pack<TDC_F32, 8>::up(Pack<TDC_F32, 8>::load(a.weight, c), w);
+        else Pack<DT, 8>::up(Pack<DT, 8>::load(a.weight, c), w);
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = c + j >= a.C ? 0.0f : a.weight ? param<DT>(a.weight, c + j, a.weight_dtype) : 1.0f;
 }
@@ -78,18 +83,22 @@ __global__ void __launch_bounds__(kThreads) tdc_rms_forward_kernel(const RmsArgs
     constexpr int kRows = kThreads / TEAM;
     __shared__ float lds[TEAM > 64 ? TEAM / 64 : 1];
     const int l = threadIdx.x % TEAM;
-    float w[NV][8];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) weights<DT>(a, (l + TEAM * i) * 8, w[i]);
     const float by_C = 1.0f / (float)a.C;
-    for (long long row = (long long)blockIdx.x * kRows + threadIdx.x / TEAM; row < a.rows; row += (long long)gridDim.x * kRows) {
-        typename P::type px[NV], pr[NV];
+    typename P::type px[NV], pr[NV];
+    auto ask = [&](long long row) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) px[i] = load8<DT>(a.x, row * a.x_stride, (l + TEAM * i) * 8, a.C);
         if (a.residual) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) pr[i] = load8<DT>(a.residual, row * a.r_stride, (l + TEAM * i) * 8, a.C);
         }
+    };
+    long long row = (long long)blockIdx.x * kRows + threadIdx.x / TEAM;
+    if (row < a.rows) ask(row);
+    float w[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) weights<DT>(a, (l + TEAM * i) * 8, w[i]);
+    for (const long long on = (long long)gridDim.x * kRows; row < a.rows; row += on) {
         float h[NV][8], sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -104,6 +113,7 @@ __global__ void __launch_bounds__(kThreads) tdc_rms_forward_kernel(const RmsArgs
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
         }
+        if (row + on < a.rows) ask(row + on);      // (the next row is on its way while this one is finished)
         const float r = rsqrtf(fmaf(team_sum<TEAM>(sum, lds), by_C, a.eps));
         if (a.rstd && l == 0) a.rstd[row] = r;
         const long long pitch = (a.C + 127) & ~127;
@@ -239,8 +249,8 @@ bool rms_plan(RmsArgs &a, bool grad) {
     if (a.team > 16 && a.held == 1) a.held = 2;
     const int rows = kThreads / a.team;
     const long long groups = (a.rows + rows - 1) / rows;
-    // Forward: eight workgroups of 256 to a compute unit, that load their weights once.  Gradient: 256 rows a thread at most.
-    const long long most = grad ? 1024 : 2048;
+    // Forward: eight workgroups to a compute unit.  Gradient: two, as many as its registers leave room for; 256 rows a thread at most.
+    const long long most = grad ? 512 : 2048;
     a.blocks = (int)std::max(std::min(groups, most), grad ? (groups + 255) / 256 : 1);
     return true;
 }

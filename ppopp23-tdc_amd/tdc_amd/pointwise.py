@@ -24,7 +24,7 @@ from .channels_last import (_act, _Cache, _call, _DTYPES, _no_gradient, _no_tang
 from .conv import _device, _raw_stream
 
 _MX8 = 4
-_empty, _u8, _f32 = torch.empty, torch.uint8, torch.float32
+_empty, _empty_like, _u8, _f32 = torch.empty, torch.empty_like, torch.uint8, torch.float32
 
 
 def _checkpoint(how):
@@ -33,13 +33,36 @@ def _checkpoint(how):
     return how is not None
 
 
-def _tile_rows(t):
-    """`_rows` at an address that 16-byte requests can start from."""
+def _flat(t):
+    """t as evenly spaced rows of neighbouring numbers: (what holds them, rows, distance between rows)."""
+    K = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // K if K else _product(t.shape[:-1]), K
     t, step = _rows(t)
+    return t, t.shape[0], step
+
+
+def _like(t):
+    """A dense tensor like t."""
+    return _empty_like(t) if t.is_contiguous() else _empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _tile_rows(t):
+    """`_flat` at an address that 16-byte requests can start from."""
+    t, rows, step = _flat(t)
     if t.data_ptr() & 15:
+        step = t.shape[-1]
         t = t.clone(memory_format=torch.contiguous_format)
-        step = t.shape[1]
-    return t, step
+    return t, rows, step
+
+
+def _once(body):
+    """A backward that refuses to be differentiated itself.  (The wrapper that does costs some microseconds: not where no graph is made.)"""
+    refusing = once_differentiable(body)
+
+    def backward(ctx, *grads):
+        return refusing(ctx, *grads) if torch.is_grad_enabled() else body(ctx, *grads)
+    return backward
 
 
 # ---- 8-bit numbers --------------------------------------------------------------------------------------------------------
@@ -127,9 +150,9 @@ def _mx8_again(codes, scales, shape):
 
 
 def _quantize(x):
-    flat, step = _rows(x)
+    flat, rows, step = _flat(x)
     index = x.get_device()
-    q = Mx8Tensor._new(flat.shape[0], flat.shape[1], tuple(x.shape), x.device, index)
+    q = Mx8Tensor._new(rows, x.shape[-1], tuple(x.shape), x.device, index)
     status = _call("tdc_mx8_quantize")(flat.data_ptr(), _DTYPES[x.dtype], q.rows, q.K, step, q._codes_at, q._scales_at, _raw_stream(index))
     if status:
         check(status)
@@ -192,15 +215,15 @@ def _mx8_linear(x, weight, bias, residual, act, out_dtype, pixels):
         M, dtype, x_type, x_step = x.rows, out_dtype or torch.bfloat16, _MX8, 0
         x_at, x_scales = x._codes_at, x._scales_at
     else:
-        flat, x_step = _rows(x)
-        M, dtype, x_type = flat.shape[0], out_dtype or x.dtype, _DTYPES[x.dtype]
+        flat, M, x_step = _flat(x)
+        dtype, x_type = out_dtype or x.dtype, _DTYPES[x.dtype]
         x_at, x_scales = flat.data_ptr(), None
     if dtype != torch.float16 and dtype != torch.bfloat16:
         raise TypeError(f"the 8-bit product's result is float16 or bfloat16 (out_dtype): got {dtype}")
     r_step, r_at, bias_type, b_at = 0, None, _f32, None
     if residual is not None:
         _residual(residual, (*shape[:-1], N), dtype, dev)
-        residual, r_step = _rows(residual)
+        residual, _, r_step = _flat(residual)
         r_at = residual.data_ptr()
     if bias is not None:
         _vector(bias, N, dtype, dev, "bias")
@@ -271,12 +294,11 @@ def _linear_plan(M, N, K, dtype, bias_dtype, act, kept8, x_step, w_step, y_step,
 def _linear_forward(x, weight, bias, residual, act, want_z):
     """(y, z): rows [M, K] and so on, on the current device."""
     dev, dtype, N = x.device, x.dtype, weight.shape[0]
-    flat, x_step = _tile_rows(x)
-    w, w_step = _tile_rows(weight)
-    M, K = flat.shape
-    r_step, r_at = 0, None
+    flat, M, x_step = _tile_rows(x)
+    w, _, w_step = _tile_rows(weight)
+    K, r_step, r_at = weight.shape[1], 0, None
     if residual is not None:
-        r, r_step = _rows(residual)
+        r, _, r_step = _flat(residual)
         r_at = r.data_ptr()
     ref, need = _linear_plan(M, N, K, dtype, _f32 if bias is None else bias.dtype, act, False, x_step, w_step, 0, r_step, False)
     y = _empty((*x.shape[:-1], N), dtype=dtype, device=dev)
@@ -304,7 +326,7 @@ class _LinearAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         held, weight, kept = ctx.saved_tensors
         _no_tangent("the gradient of linear_act", dy)
@@ -314,8 +336,7 @@ class _LinearAct(torch.autograd.Function):
         dx = _empty(shape, dtype=dtype, device=dev) if need_x else None
         dw = _empty((N, K), dtype=dtype, device=dev) if need_w else None
         db = _empty(N, dtype=bias_dtype, device=dev) if need_b else None
-        flat, y_step = _tile_rows(dy)
-        M = flat.shape[0]
+        flat, M, y_step = _tile_rows(dy)
         dz, dr = None, None
         if need_r:
             if act == "none":
@@ -330,9 +351,9 @@ class _LinearAct(torch.autograd.Function):
                 q = Mx8Tensor._of(held, M, K, shape, dev, index)
                 x_at, x_scales = q._codes_at, q._scales_at
             elif need_w:
-                x, x_step = _tile_rows(held)
+                x, _, x_step = _tile_rows(held)
                 x_at = x.data_ptr()
-            w, w_step = _tile_rows(weight) if need_x else (None, 0)
+            w, _, w_step = _tile_rows(weight) if need_x else (None, 0, 0)
             ref, need = _linear_plan(M, N, K, dtype, bias_dtype, act, kept8, x_step, w_step, y_step, 0, True)
             ws = _empty(need, dtype=_u8, device=dev) if need else None
             status = _call("tdc_linear_backward")(ref, x_at, x_scales, _ptr(w), _ptr(kept), flat.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
@@ -414,12 +435,12 @@ def _rms_plan(rows, C, dtype, weight_dtype, eps, x_step, r_step, dy_step, dh_ste
 def _rms_forward(x, weight, residual, eps, output8, grad, kept8):
     """(y or an Mx8Tensor, h or None, rstd or None, h in 8 bits or None), on the current device."""
     dev, dtype, C, index = x.device, x.dtype, x.shape[-1], x.get_device()
-    flat, x_step = _rows(x)
-    M, r_step, r_at, h = flat.shape[0], 0, None, None
+    flat, M, x_step = _flat(x)
+    r_step, r_at, h = 0, None, None
     if residual is not None:
-        r, r_step = _rows(residual)
+        r, _, r_step = _flat(residual)
         r_at = r.data_ptr()
-        h = _empty(x.shape, dtype=dtype, device=dev)
+        h = _like(x)
     ref, _ = _rms_plan(M, C, dtype, _f32 if weight is None else weight.dtype, eps, x_step, r_step, 0, 0, False)
     if output8:
         q = Mx8Tensor._new(M, C, tuple(x.shape), dev, index)
@@ -428,7 +449,7 @@ def _rms_forward(x, weight, residual, eps, output8, grad, kept8):
         if status:
             check(status)
         return q, h, None, None
-    y = _empty(x.shape, dtype=dtype, device=dev)
+    y = _like(x)
     rstd = _empty(M, dtype=_f32, device=dev) if grad else None
     kept = Mx8Tensor._new(M, C, tuple(x.shape), dev, index) if kept8 else None
     status = _call("tdc_rms_norm_forward")(ref, flat.data_ptr(), r_at, _ptr(weight), y.data_ptr(), _ptr(h), _ptr(rstd),
@@ -448,7 +469,7 @@ class _RmsNorm(torch.autograd.Function):
         return y if residual is None else (y, h)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dh=None):
         held, weight, rstd = ctx.saved_tensors
         _no_tangent("the gradient of rms_norm", dy, dh)
@@ -457,19 +478,19 @@ class _RmsNorm(torch.autograd.Function):
         if dy is None:      # (only h was used)
             return dh if need_x else None, torch.zeros_like(weight) if need_w and dh is not None else None, dh if need_r else None, None, None
         dev, C, index = dy.device, shape[-1], dy.get_device()
-        g, dy_step = _rows(dy)
-        M, h_step, dh_step, e = g.shape[0], 0, 0, None
+        g, M, dy_step = _flat(dy)
+        h_step, dh_step, e = 0, 0, None
         if kept8:
             q = Mx8Tensor._of(held, M, C, shape, dev, index)
             h_at, h_scales = q._codes_at, q._scales_at
         else:
-            flat, h_step = _rows(held)
+            flat, _, h_step = _flat(held)
             h_at, h_scales = flat.data_ptr(), None
         if dh is not None:
-            e, dh_step = _rows(dh)
+            e, _, dh_step = _flat(dh)
         ref, need = _rms_plan(M, C, dtype, _f32 if weight is None else weight.dtype, eps, h_step, 0, dy_step, dh_step, True)
-        dx = _empty(shape, dtype=dtype, device=dev) if need_x or need_r else None
-        dw = _empty(C, dtype=weight.dtype, device=dev) if need_w else None
+        dx = _like(dy) if need_x or need_r else None
+        dw = _empty_like(weight) if need_w else None
         need = need if need_w else 0
         ws = _empty(need, dtype=_u8, device=dev) if need else None
         status = _call("tdc_rms_norm_backward")(ref, h_at, h_scales, _ptr(weight), g.data_ptr(), _ptr(e), rstd.data_ptr(), _ptr(dx),
