@@ -18,46 +18,37 @@ struct Eight {
     typedef T vec_t __attribute__((ext_vector_type(8)));
     typedef T mem_t __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
-// The residual of eight neighbouring outputs of a row: zeros where there is none (rows from M on, outputs from N on).
-template <int DT>
-static __device__ __forceinline__ typename Eight<DT>::vec_t residual8(const ProductOut &a, long long m, long long n) {
+// Eight neighbouring numbers of a row of which `left` (at least 1) are there: whole, or by fours, twos and one.  WHOLE: all eight are.
+template <int DT, bool WHOLE>
+static __device__ __forceinline__ typename Eight<DT>::vec_t load8(const void *base, long long at, long long left) {
     using T = typename Num<DT>::type;
+    const T *from = reinterpret_cast<const T *>(base) + at;
+    if (WHOLE || left >= 8) return *reinterpret_cast<const typename Eight<DT>::mem_t *>(from);
+    typename Pack<DT, 4>::type four = {};
+    typename Pack<DT, 2>::type two = {};
+    T one = {};
+    const int l = (int)left;
+    if (l & 4) four = Pack<DT, 4>::load(from, 0);
+    if (l & 2) two = Pack<DT, 2>::load(from, l & 4);
+    if (l & 1) one = from[l & 6];
     typename Eight<DT>::vec_t r = {};
-    if (a.residual && m < a.M) {
-        const T *const from = reinterpret_cast<const T *>(a.residual) + m * a.r_stride + n;
-        if (n + 8 <= a.N) r = *reinterpret_cast<const typename Eight<DT>::mem_t *>(from);
-        else {
-#pragma unroll
-            for (int i = 0; i < 7; ++i)
-                if (n + i < a.N) r[i] = from[i];
-        }
-    }
+    if (l & 4) r = typename Eight<DT>::vec_t{four[0], four[1], four[2], four[3], l & 2 ? two[0] : one, two[1], l & 2 ? one : T{}, T{}};
+    else r = typename Eight<DT>::vec_t{l & 2 ? two[0] : one, two[1], l & 2 ? one : T{}, T{}, T{}, T{}, T{}, T{}};
     return r;
 }
-template <int DT>
+template <int DT, bool WHOLE>
 static __device__ __forceinline__ void store8(void *base, long long at, long long left, const typename Eight<DT>::vec_t &v) {
     using T = typename Num<DT>::type;
     T *const to = reinterpret_cast<T *>(base) + at;
-    if (left >= 8) *reinterpret_cast<typename Eight<DT>::mem_t *>(to) = v;
-    else {
-#pragma unroll
-        for (int i = 0; i < 7; ++i)
-            if (i < left) to[i] = v[i];
+    if (WHOLE || left >= 8) {
+        *reinterpret_cast<typename Eight<DT>::mem_t *>(to) = v;
+        return;
     }
-}
-// Eight neighbouring outputs of a row (those before N): residual on sums with the bias, activation, store; what the activation
-// was taken of besides if Z.
-template <int DT, int ACT, bool Z>
-static __device__ __forceinline__ void finish8(const ProductOut &a, long long m, long long n, const float (&v)[8], typename Eight<DT>::vec_t r) {
-    typename Eight<DT>::vec_t out, sum;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float z = v[i] + Num<DT>::up(r[i]);
-        out[i] = Num<DT>::down(act_of<ACT>(z));
-        sum[i] = Num<DT>::down(z);
-    }
-    store8<DT>(a.y, m * a.y_stride + n, a.N - n, out);
-    if constexpr (Z) store8<DT>(a.z, m * a.z_stride + n, a.N - n, sum);
+    const int l = (int)left;
+    if (l & 4) Pack<DT, 4>::store(to, 0, typename Pack<DT, 4>::type{v[0], v[1], v[2], v[3]});
+    const typename Pack<DT, 4>::type rest = {l & 4 ? v[4] : v[0], l & 4 ? v[5] : v[1], l & 4 ? v[6] : v[2], T{}};
+    if (l & 2) Pack<DT, 2>::store(to, l & 4, typename Pack<DT, 2>::type{rest[0], rest[1]});
+    if (l & 1) to[l & 6] = l & 2 ? rest[2] : rest[0];
 }
 // The row of w that is row r of a block: bits 2 and 3 change places, which makes a lane's outputs 8 i .. 8 i + 7 neighbours.
 static __device__ __forceinline__ int weight_row(int r) { return (r & 19) | (r & 4) << 1 | (r & 8) >> 1; }
@@ -81,28 +72,48 @@ static __device__ __forceinline__ float bias_of(const ProductOut &a, long long n
     return wanted && a.bias && n < a.N ? param<DT>(a.bias, n, a.bias_dtype) : 0.0f;
 }
 
-// A wave's outputs from row m on and from column n on; `bias` is that of its columns, `stage` its own 4 KiB NB of LDS (PART: sums that others join, without an activation).  Of a block a lane
+// A wave's outputs from row m on and from column n on; `bias` is that of its columns, `stage` its own 4 KiB NB of LDS.  Z: what the activation
+// is taken of leaves too; PART: sums that others join, and nothing with them.  Of a block a lane
 // has row r of x, and of w 16 u + 8 q .. 16 u + 8 q + 7, u = 0, 1.  32 rows at a time go through LDS, where a lane takes eight outputs of a
 // row and its neighbours those beside them: residuals and outputs are whole cache lines.  (The first halves of a row's eights lie
-// before the second ones, 16 bytes moved by the row, so that neither side meets a bank twice.)  The residuals of the next 32 rows are on
+// before the second ones, 16 bytes moved by the row, so that neither side meets a bank twice.)  The residuals of the next rows are on
 // their way while these are finished.
+// A tile runs this once, with one wave a vector unit where tiles are large: instructions count, and so does the code itself, which comes from
+// memory.  The rows loop, one copy serves all activations, whole tiles have no bounds to check (64 tiles of 256 x 256 with a sum of 32:
+// 17.3 us unrolled, with a copy for each activation; 11.7 now).
 template <int DT, int MB, int NB, bool Z = false, bool PART = false>
 static __device__ __forceinline__ void finish_tile(const ProductOut &a, const f16_t (&acc)[NB][MB], long long m, long long n, const float *bias,
                                                    unsigned char *stage) {
     constexpr int kAcross = NB * 4, kDown = 64 / kAcross, kTurns = 32 / kDown;     // lanes of a row, rows at a time
+    constexpr int kAtOnce = kTurns < 4 ? kTurns : 4, kGroups = kTurns / kAtOnce;
+    using V = typename Eight<DT>::vec_t;
     const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5, down = lane / kAcross, c = lane % kAcross * 8;
     auto place = [&](int row, int eight, int half) {
         return reinterpret_cast<float4 *>(stage + row * NB * 128 + ((half * kAcross + eight) ^ (row & 15 & (NB * 8 - 1))) * 16);
     };
     const float4 lo = *reinterpret_cast<const float4 *>(bias + c), hi = *reinterpret_cast<const float4 *>(bias + c + 4);
     const float add[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    auto finish = [&](auto act) {
-        typename Eight<DT>::vec_t res[2][kTurns];
-        auto ask = [&](int i) {
+    const long long left = a.N - n - c;
+    auto finish = [&](auto whole, auto with_residual) {
+        constexpr bool kWhole = decltype(whole)::value, kResidual = decltype(with_residual)::value;
+        // (this lane's places, from row to row; a row past the last is not touched)
+        long long y_at = (m + down) * a.y_stride + n + c, z_at = (m + down) * a.z_stride + n + c, r_at = (m + down) * a.r_stride + n + c;
+        int rows = kWhole || left > 0 ? (int)min((long long)32 * MB, a.M - m) - down : 0;      // of this lane, from `down` on
+        V now[kAtOnce], next[kAtOnce];
+        int asked = rows;
+        auto ask = [&] {
 #pragma unroll
-            for (int s = 0; s < kTurns; ++s) res[i & 1][s] = residual8<DT>(a, m + i * 32 + s * kDown + down, n + c);
+            for (int s = 0; s < kAtOnce; ++s) {
+                if constexpr (kWhole) next[s] = load8<DT, true>(a.residual, r_at, left);
+                else {
+                    next[s] = V{};
+                    if (asked > 0) next[s] = load8<DT, false>(a.residual, r_at, left);
+                }
+                r_at += kDown * a.r_stride;
+                asked -= kDown;
+            }
         };
-        ask(0);
+        if constexpr (kResidual) ask();
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
 #pragma unroll
@@ -113,23 +124,61 @@ static __device__ __forceinline__ void finish_tile(const ProductOut &a, const f1
                     const f16_t &v = acc[k / 2][i];
                     *place(r, k * 2 + q, h) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                 }
-            if (i + 1 < MB) ask(i + 1);
             asm volatile("" ::: "memory");      // (a wave's own LDS operations come in order)
+#pragma unroll 1
+            for (int g = 0; g < kGroups; ++g) {
+                if constexpr (kResidual) {
 #pragma unroll
-            for (int s = 0; s < kTurns; ++s) {
-                const int row = s * kDown + down;
-                const float4 u = *place(row, c / 8, 0), w = *place(row, c / 8, 1);
-                const float v[8] = {u.x + add[0], u.y + add[1], u.z + add[2], u.w + add[3], w.x + add[4], w.y + add[5], w.z + add[6], w.w + add[7]};
-                if (m + i * 32 + row < a.M && n + c < a.N) finish8<DT, decltype(act)::value, Z>(a, m + i * 32 + row, n + c, v, res[i & 1][s]);
+                    for (int s = 0; s < kAtOnce; ++s) now[s] = next[s];
+                    if (i * kGroups + g + 1 < MB * kGroups) ask();
+                }
+#pragma unroll
+                for (int s = 0; s < kAtOnce; ++s) {
+                    const int row = (g * kAtOnce + s) * kDown + down;
+                    const float4 u = *place(row, c / 8, 0), w = *place(row, c / 8, 1);
+                    float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+                    V out, sum;
+                    if constexpr (!PART) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            v[j] += add[j];
+                            if constexpr (kResidual) v[j] += Num<DT>::up(now[s][j]);
+                            if constexpr (Z) sum[j] = Num<DT>::down(v[j]);
+                        }
+                        if (a.act == TDC_ACT_RELU) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[j] = act_of<TDC_ACT_RELU>(v[j]);
+                        } else if (a.act == TDC_ACT_SILU) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[j] = act_of<TDC_ACT_SILU>(v[j]);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) out[j] = Num<DT>::down(v[j]);
+                    if (kWhole || rows > 0) {
+                        store8<DT, kWhole>(a.y, y_at, left, out);
+                        if constexpr (Z) store8<DT, kWhole>(a.z, z_at, left, sum);
+                    }
+                    rows -= kDown;
+                    y_at += kDown * a.y_stride;
+                    if constexpr (Z) z_at += kDown * a.z_stride;
+                }
             }
             asm volatile("" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    if constexpr (PART) finish(std::integral_constant<int, TDC_ACT_NONE>{});
-    else if (a.act == TDC_ACT_RELU) finish(std::integral_constant<int, TDC_ACT_RELU>{});
-    else if (a.act == TDC_ACT_SILU) finish(std::integral_constant<int, TDC_ACT_SILU>{});
-    else finish(std::integral_constant<int, TDC_ACT_NONE>{});
+    const std::true_type yes;
+    const std::false_type no;
+    const bool whole = m + 32 * MB <= a.M && n + 32 * NB <= a.N;
+    if constexpr (PART) {
+        if (whole) finish(yes, no);
+        else finish(no, no);
+    } else if (a.residual) {
+        if (whole) finish(yes, yes);
+        else finish(no, yes);
+    } else if (whole) finish(yes, no);
+    else finish(no, no);
 }
 
 // Lets a kernel have more than 64 KiB of LDS; once per kernel and device.

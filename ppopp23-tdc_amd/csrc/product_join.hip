@@ -11,17 +11,17 @@ namespace tdc {
 
 // Tiles, the time of a step and what a tile takes besides (us), as timed with one workgroup a compute unit (M x N x K in bf16, kernel
 // by kernel; a compute unit that holds several gives each its share): 32 x 128 256 x 4096 x 4096 22.9, 64 x 128 512 x 4096 x 4096 28.1,
-// 128 x 128 1024 x 4096 x 4096 40.3, 256 x 128 8192 x 1024 x 4096 74.7, 256 x 256 4096 x 4096 x 4096 124 (0.6 a step where few compute units
+// 128 x 128 1024 x 4096 x 4096 40.3, 256 x 128 8192 x 1024 x 4096 71, 256 x 256 4096 x 4096 x 4096 115 (0.6 a step where few compute units
 // work: their clock).  Larger tiles do more a step, smaller ones leave fewer compute units without work, and so do parts of the sum, which
-// cost a launch and their bytes: 1024 x 1024 x 1024 8.0 in tiles of 32 rows, 12.6 of 128, 31.9 of 256; 128 x 512 x 25088 19.3 in 14 parts
-// of 32 rows, 106 whole; 8192 x 8192 x 1024 158 in tiles of 256, 166 in 128 x 128 three a compute unit, 195 one by one; 25088 x 512 x 128 15.5
-// three a compute unit, 20.4 in tiles of 256.
+// cost a launch and their bytes: 1024 x 1024 x 1024 7.7 in tiles of 32 rows, 11.7 of 128, 26.6 of 256; 128 x 512 x 25088 19.3 in 14 parts
+// of 32 rows, 106 whole; 8192 x 8192 x 1024 140 in tiles of 256, 167 in 128 x 128 three a compute unit, 192 one by one; 25088 x 512 x 128 13.6
+// three a compute unit, 15.6 in tiles of 256.
 struct Timing {
     int m, n;
     double step, besides;
     int together;      // workgroups of a compute unit that hide each other's `besides`
 };
-static const Timing kTimings[] = {{256, 256, 0.85, 11.0, 1}, {256, 128, 0.53, 5.0, 1}, {128, 128, 0.28, 2.5, 1}, {128, 128, 0.31, 2.1, 3}, {64, 128, 0.18, 1.0, 1}, {32, 128, 0.145, 1.0, 1}};
+static const Timing kTimings[] = {{256, 256, 0.82, 7.0, 1}, {256, 128, 0.51, 4.0, 1}, {128, 128, 0.28, 2.0, 1}, {128, 128, 0.31, 1.5, 3}, {64, 128, 0.175, 0.8, 1}, {32, 128, 0.14, 0.8, 1}};
 
 TilePlan tile_plan(long long M, long long N, long long K, int in_dtype) {
     const long long step = in_dtype == TDC_MX8 ? 64 : 32, steps = (K + step - 1) / step;
