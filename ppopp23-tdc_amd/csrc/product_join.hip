@@ -15,13 +15,17 @@ namespace tdc {
 // work: their clock).  Larger tiles do more a step, smaller ones leave fewer compute units without work, and so do parts of the sum, which
 // cost a launch and their bytes: 1024 x 1024 x 1024 7.7 in tiles of 32 rows, 11.7 of 128, 26.6 of 256; 128 x 512 x 25088 19.3 in 14 parts
 // of 32 rows, 106 whole; 8192 x 8192 x 1024 140 in tiles of 256, 167 in 128 x 128 three a compute unit, 192 one by one; 25088 x 512 x 128 13.6
-// three a compute unit, 15.6 in tiles of 256.
+// three a compute unit, 15.6 in tiles of 256.  Small tiles wait for memory alone: one row by 16384 x 4096 weights that no cache holds 36.4
+// with a workgroup a compute unit, 30.0 with two, 34.5 with four.
 struct Timing {
     int m, n;
     double step, besides;
     int together;      // workgroups of a compute unit that hide each other's `besides`
+    double alone;      // a step of a workgroup by itself
+    int parts;         // a sum's parts fill the compute units so many times
 };
-static const Timing kTimings[] = {{256, 256, 0.82, 7.0, 1}, {256, 128, 0.51, 4.0, 1}, {128, 128, 0.28, 2.0, 1}, {128, 128, 0.31, 1.5, 3}, {64, 128, 0.175, 0.8, 1}, {32, 128, 0.14, 0.8, 1}};
+static const Timing kTimings[] = {{256, 256, 0.82, 7.0, 1, 0.82, 1},   {256, 128, 0.51, 4.0, 1, 0.51, 1},  {128, 128, 0.28, 2.0, 1, 0.28, 1},
+                                   {128, 128, 0.31, 1.5, 3, 0.31, 1}, {64, 128, 0.175, 0.8, 1, 0.24, 2}, {32, 128, 0.14, 0.8, 1, 0.22, 2}};
 
 TilePlan tile_plan(long long M, long long N, long long K, int in_dtype) {
     const long long step = in_dtype == TDC_MX8 ? 64 : 32, steps = (K + step - 1) / step;
@@ -31,12 +35,12 @@ TilePlan tile_plan(long long M, long long N, long long K, int in_dtype) {
         const Timing &t = kTimings[kernel];
         const long long tm = (M + t.m - 1) / t.m, tn = (N + t.n - 1) / t.n, all = tm * tn;
         // Parts as they fill the compute units, or half of that; eight steps each at least.
-        const long long most = std::min(256 / all, steps / 8);
+        const long long most = std::min(256 * t.parts / all, steps / 8);
         for (const long long want : {1ll, most / 2, most}) {
             if (want < 1) continue;
             const long long split_steps = want == 1 ? steps : round_up((steps + want - 1) / want, 8), splits = (steps + split_steps - 1) / split_steps;
             const double each = (double)(all * splits) / 256, rounds = t.together == 1 ? std::ceil(each) : std::max(each, 1.0);
-            double time = 4.0 + rounds * ((double)split_steps * t.step + t.besides / t.together) + (t.together > 1 ? t.besides : 0.0);
+            double time = 4.0 + std::max(rounds * t.step, t.alone) * (double)split_steps + rounds * t.besides / t.together + (t.together > 1 ? t.besides : 0.0);
             if (splits > 1) time += 4.0 + (double)splits * M * N * 8 / 4e6;
             if (best.steps && time >= best_time) continue;
             best_time = time;
