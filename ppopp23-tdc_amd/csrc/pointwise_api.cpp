@@ -100,6 +100,8 @@ int backward_plan(const tdc_linear_desc &d, Backward &b) {
     if (b.pack_x && d.kept_dtype != TDC_MX8) copies.add(d.M, d.K);
     if (b.pack_w) copies.add(d.N, d.K);
     if (int st = copies.fit()) return st;
+    if (d.kept_dtype == TDC_MX8)
+        if (int st = mx_range("product's gradient", d.M, d.K)) return st;
     b.grad = copy_args(nullptr, d.M, d.N, d.y_stride, nullptr);
     b.sums = b.dz + (b.make_dz ? padded(packed_bytes(d.M, d.N)) : 0);
     b.x = b.sums + padded((size_t)b.grad.chunks * d.N * 4);

@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "ops_device.hpp"
+#include "product_device.hpp"
 
 namespace tdc {
 
@@ -132,30 +132,35 @@ static __device__ __forceinline__ void act_grad(const ActGradArgs &a, unsigned b
     const int down = 256 / a.across, c = threadIdx.x % a.across, r = threadIdx.x / a.across;
     const long long n = ((long long)tile * a.across + c) * 8, row0 = chunk * a.chunk_rows, rows = min(a.chunk_rows, a.M - row0);
     float sum[8] = {};
-    auto load = [&](const void *base, long long at) {
-        if (n + 8 <= a.N) return P::load(base, at);
-        typename P::type v = {};
+    // Four rows are on their way at a time.
+    auto rows_of = [&](auto load) {
+        for (long long i = r; i < rows; i += 4 * down) {
+            typename P::type dy[4], kept[4];
 #pragma unroll
-        for (int i = 0; i < 7; ++i)
-            if (n + i < a.N) v[i] = reinterpret_cast<const T *>(base)[at + i];
-        return v;
-    };
-    if (n < a.N) {
-#pragma unroll 4
-        for (long long i = r; i < rows; i += down) {
-            const long long m = row0 + i;
-            float v[8], z[8];
-            P::up(load(a.dy, m * a.dy_stride + n), v);
-            if constexpr (ACT != TDC_ACT_NONE) {
-                P::up(load(a.kept, m * a.N + n), z);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] *= act_slope<ACT>(z[j]);
+            for (int k = 0; k < 4; ++k) {
+                const long long m = row0 + min(i + k * down, rows - 1);      // (a repeated one is not used)
+                dy[k] = load(a.dy, m * a.dy_stride + n);
+                if constexpr (ACT != TDC_ACT_NONE) kept[k] = load(a.kept, m * a.N + n);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum[j] += v[j];
-            if (a.dz) P::store(a.dz, m * a.pitch + n, P::down(v));
+            for (int k = 0; k < 4; ++k) {
+                if (i + k * down >= rows) break;
+                float v[8];
+                P::up(dy[k], v);
+                if constexpr (ACT != TDC_ACT_NONE) {
+                    float z[8];
+                    P::up(kept[k], z);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] *= act_slope<ACT>(z[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j] += v[j];
+                if (a.dz) P::store(a.dz, (row0 + i + k * down) * a.pitch + n, P::down(v));
+            }
         }
-    }
+    };
+    if (n + 8 <= a.N) rows_of([](const void *base, long long at) { return P::load(base, at); });
+    else if (n < a.N) rows_of([&](const void *base, long long at) { return load8<DT, false>(base, at, a.N - n); });
     if (!a.sums) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j) lds[threadIdx.x][j] = sum[j];

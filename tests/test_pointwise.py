@@ -103,6 +103,14 @@ def test_products_of_more_tiles_than_a_launch_has(d):
     assert L.tdc_linear_workspace(ctypes.byref(linear(**d)), ctypes.byref(n), None) == INVALID and "work items" in error()
 
 
+def test_gradients_of_more_rows_than_a_launch_has():
+    L, n = tdc_amd.lib(), ctypes.c_size_t()
+    d = linear(M=(1 << 31) - 1, N=8, K=512, kept_dtype=4)
+    assert L.tdc_linear_workspace(ctypes.byref(d), None, ctypes.byref(n)) == INVALID and "work items" in error()
+    d = linear(M=(1 << 24), N=8, K=512, kept_dtype=4)
+    assert L.tdc_linear_workspace(ctypes.byref(d), None, ctypes.byref(n)) == 0 and n.value >= (1 << 24) * 512 * 2
+
+
 @pytest.mark.parametrize("bad", [dict(M=-1), dict(N=-1), dict(K=0), dict(K=1 << 22), dict(x_dtype=3), dict(x_dtype=5), dict(y_dtype=0), dict(y_dtype=4), dict(bias_dtype=1),
                                  dict(act=3), dict(x_dtype=0, x_stride=39), dict(y_stride=4), dict(residual_stride=-5)])
 def test_8_bit_product_descriptors_are_refused(bad):

@@ -508,3 +508,124 @@ def test_copies_of_an_8_bit_tensor():
     q = tdc_amd.mx8_quantize(numbers(230, (5, 70), BF16))
     for c in (copy.deepcopy(q), pickle.loads(pickle.dumps(q)), tdc_amd.Mx8Tensor(q.codes.clone(), q.scales.clone(), q.shape)):
         assert c._codes_at != q._codes_at and torch.equal(c.dequantize(), q.dequantize())
+
+
+def test_rows_of_other_forms():
+    """One row without a leading axis, a transposed weight, a gradient that is one number everywhere, a graph that is walked twice."""
+    x, w, b, r = case(240, 6, 40, 64, BF16)
+    one = tdc_amd.linear_act(x[0], w, b, r[0], act="silu")
+    assert one.shape == (40,) and torch.equal(one, tdc_amd.linear_act(x[:1], w, b, r[:1], act="silu")[0])
+    t = numbers(241, (64, 40), BF16).t()
+    assert torch.equal(tdc_amd.linear_act(x, t), tdc_amd.linear_act(x, t.contiguous()))
+    wrt = [v.requires_grad_() for v in (x, w, b, r)]
+    for act in ("none", "silu"):
+        y = tdc_amd.linear_act(x, w, b, r, act=act)
+        first = torch.autograd.grad(y.sum(), wrt, retain_graph=True)
+        again = torch.autograd.grad(y.sum(), wrt)
+        want = torch.autograd.grad(tdc_amd.linear_act(x, w, b, r, act=act), wrt, torch.ones_like(y))
+        assert all(torch.equal(p, q) and torch.equal(p, s) for p, q, s in zip(first, again, want))
+    x1 = x.detach()[0].clone().requires_grad_()
+    (d,) = torch.autograd.grad(tdc_amd.linear_act(x1, w.detach(), act="silu"), x1, torch.ones(40, dtype=BF16, device="cuda"))
+    assert d.shape == (64,)
+    y, h = tdc_amd.rms_norm(x.detach()[0], None, x.detach()[1])
+    assert y.shape == h.shape == (64,)
+    # a residual for all rows at once, whose gradient is summed over them
+    shared = numbers(242, (40,), BF16).requires_grad_()
+    (g,) = torch.autograd.grad(tdc_amd.linear_act(x.detach(), w.detach(), None, shared.expand(6, 40)), shared, torch.ones(6, 40, dtype=BF16, device="cuda"))
+    assert torch.equal(g, torch.full_like(g, 6))
+
+
+@pytest.mark.parametrize("needs", [(1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (1, 0, 1, 0), (0, 1, 0, 1)])
+@pytest.mark.parametrize("N,K", [(40, 64), (41, 67)])
+def test_gradients_that_are_wanted_alone(needs, N, K):
+    x, w, b, r = case(250, 9, N, K, F16)
+    dy = numbers(251, (9, N), F16)
+    for act in ("none", "relu", "silu"):
+        for checkpoint in (None, "mx8"):
+            full = [t.detach().clone().requires_grad_() for t in (x, w, b, r)]
+            want = grads(tdc_amd.linear_act(*full, act=act, checkpoint=checkpoint), full, dy)
+            some = [t.detach().clone().requires_grad_(bool(n)) for t, n in zip((x, w, b, r), needs)]
+            got = grads(tdc_amd.linear_act(*some, act=act, checkpoint=checkpoint), [t for t in some if t.requires_grad], dy)
+            assert all(torch.equal(p, q) for p, q in zip(got, [v for v, n in zip(want, needs) if n]))
+
+
+def test_recomputed_layers_and_accumulated_gradients():
+    """torch's recomputing checkpoints around the operators, and .grad of leaves that two terms share."""
+    from torch.utils.checkpoint import checkpoint
+    x, w, _, r = case(260, 30, 64, 64, BF16)
+    gamma = numbers(261, (64,), F32)
+    leaves = [t.requires_grad_() for t in (x, w, gamma, r)]
+
+    def layer(x, w, gamma, r):
+        n, h = tdc_amd.rms_norm(x, gamma, r)
+        return tdc_amd.linear_act(n, w, None, h, act="silu", checkpoint="mx8")
+    plain = grads(layer(*leaves), leaves, torch.ones(30, 64, dtype=BF16, device="cuda"))
+    again = grads(checkpoint(layer, *leaves, use_reentrant=False), leaves, torch.ones(30, 64, dtype=BF16, device="cuda"))
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
+    layer(*leaves).backward(torch.ones(30, 64, dtype=BF16, device="cuda"))
+    assert all(torch.equal(t.grad, g) for t, g in zip(leaves, plain))
+    assert x.grad.data_ptr() != r.grad.data_ptr()
+    x.grad.zero_()
+    assert torch.equal(r.grad, plain[3])
+
+
+def test_calls_on_two_streams_at_once():
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    x, w, _, _ = case(270, 500, 300, 2000, BF16)
+    y, v, _, _ = case(280, 40, 700, 3300, BF16)
+    q, qv = tdc_amd.mx8_quantize(w), tdc_amd.mx8_quantize(v)
+    want = [(tdc_amd.linear_act(x, w), tdc_amd.mx8_linear(x, q)), (tdc_amd.linear_act(y, v), tdc_amd.mx8_linear(y, qv))]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for k, (s, args) in enumerate(((a, (x, w, q)), (b, (y, v, qv)))):
+            with torch.cuda.stream(s):
+                got[k].append((tdc_amd.linear_act(args[0], args[1]), tdc_amd.mx8_linear(args[0], args[2])))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(p, want[k][0]) and torch.equal(r, want[k][1]) for p, r in got[k])
+
+
+def test_offsets_beyond_32_bits():
+    """Operands of more than 4 GiB: the last rows of each, against the same rows by themselves."""
+    M, K, N = 300000, 8200, 24
+    x = torch.empty((M, K), dtype=BF16, device="cuda")
+    x[:1000] = 0
+    x[1000:] = numbers(290, (1, K), BF16)
+    x[-100:] = numbers(291, (100, K), BF16)
+    w = numbers(292, (N, K), BF16, K ** -0.5)
+    small = x[-100:].clone()
+    y = tdc_amd.linear_act(x, w)
+    assert torch.equal(y[:1000], torch.zeros_like(y[:1000]))
+    want = tdc_amd.linear_act(small, w)
+    assert (y[-100:].double() - want.double()).abs().max() <= 2 * U[BF16] * want.double().abs().max()      # (summed in other parts)
+    n = tdc_amd.rms_norm(x[:, :8192])
+    assert torch.equal(n[-100:], tdc_amd.rms_norm(small[:, :8192]))
+    del n
+    q = tdc_amd.mx8_quantize(x)
+    assert torch.equal(q.codes[-100:], tdc_amd.mx8_quantize(small).codes)
+    del q
+    # the weight's gradient: rows of zeros but for the last hundred
+    dy = torch.zeros((M, N), dtype=BF16, device="cuda")
+    dy[-100:] = numbers(293, (100, N), BF16)
+    w.requires_grad_()
+    (dw,) = grads(tdc_amd.linear_act(x, w), (w,), dy)
+    want = dy[-100:].double().cpu().t() @ small.double().cpu()
+    assert (dw.double().cpu() - want).abs().max() <= 2 * U[BF16] * want.abs().max()
+
+
+def test_long_rows():
+    K = 1 << 21
+    x, w = torch.zeros(2, K, dtype=BF16, device="cuda"), torch.zeros(3, K, dtype=BF16, device="cuda")
+    x[:, ::4096] = 1
+    w[:, ::2048] = torch.tensor([[1.0], [2.0], [-1.0]], dtype=BF16, device="cuda")
+    want = torch.tensor([512.0, 1024.0, -512.0], device="cuda").expand(2, 3)
+    assert torch.equal(tdc_amd.linear_act(x, w).float(), want)
+    assert torch.equal(tdc_amd.mx8_linear(x, tdc_amd.mx8_quantize(w)).float(), want)
+    with pytest.raises(tdc_amd.TdcError):
+        tdc_amd.linear_act(torch.zeros(1, K + 1, dtype=BF16, device="cuda"), torch.zeros(1, K + 1, dtype=BF16, device="cuda"))
+    # rows further apart than a request's offset reaches are copied first
+    far = torch.zeros(3 * (1 << 22) + 64, dtype=BF16, device="cuda").as_strided((3, 64), (1 << 22, 1))
+    far.copy_(numbers(295, (3, 64), BF16))
+    v = numbers(296, (10, 64), BF16)
+    assert torch.equal(tdc_amd.linear_act(far, v), tdc_amd.linear_act(far.contiguous(), v))
