@@ -111,7 +111,7 @@ struct TileArgs : ProductOut {
     float *part;                    // sums of the parts: [splits][M][part_stride]
     long long part_stride;
 };
-enum { kTile256, kTile256x128, kTile128Deep, kTile128, kTile64, kTile32 };
+enum { kTile256, kTile256x128, kTile128Deep, kTile128, kTile64, kTile32, kFewRows };
 // How a product is dealt out.
 struct TilePlan {
     int kernel;                     // which tile
@@ -121,12 +121,15 @@ struct TilePlan {
     long long items;                // work items of its largest launch
 };
 enum { kAlong, kWAcross, kAcross };     // how x and w lie: both along the sum, w across it, both across it
-TilePlan tile_plan(long long M, long long N, long long K, int in_dtype);
+TilePlan tile_plan(long long M, long long N, long long K, int in_dtype, int layout);
 // `a` with everything but what the plan says; y_dtype is TDC_F16 or TDC_BF16.
 int launch_product_bf16(TileArgs a, const TilePlan &p, int layout, void *stream);
 int launch_product_f16(TileArgs a, const TilePlan &p, int layout, void *stream);
 int launch_product_mx8(TileArgs a, const TilePlan &p, int y_dtype, void *stream);
 int launch_join(const TileArgs &a, int y_dtype, void *stream);
+double few_time(long long N, long long bytes);       // estimated, us
+long long few_items(long long N);
+int launch_product_few(const TileArgs &a, int in_dtype, int y_dtype, void *stream);      // both along the sum
 
 // dz = dy act'(z) in rows of `pitch` numbers (zeros past the N-th), its sums over the rows besides; also a copy of rows (no activation).
 struct ActGradArgs {

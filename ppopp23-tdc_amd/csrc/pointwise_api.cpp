@@ -70,7 +70,7 @@ struct Forward {
     bool pack_x, pack_w;
 };
 int forward_plan(const tdc_linear_desc &d, Forward &f) {
-    f.plan = tile_plan(d.M, d.N, d.K, d.dtype);
+    f.plan = tile_plan(d.M, d.N, d.K, d.dtype, kAlong);
     if (int st = plan_fits("product", f.plan)) return st;
     Copies copies;
     if ((f.pack_x = must_pack(d.M, d.K, d.x_stride))) copies.add(d.M, d.K);
@@ -88,8 +88,8 @@ struct Backward {
     ActGradArgs grad;
 };
 int backward_plan(const tdc_linear_desc &d, Backward &b) {
-    b.dx = tile_plan(d.M, d.K, d.N, d.dtype);
-    b.dw = tile_plan(d.N, d.K, d.M, d.dtype);
+    b.dx = tile_plan(d.M, d.K, d.N, d.dtype, kWAcross);
+    b.dw = tile_plan(d.N, d.K, d.M, d.dtype, kAcross);
     if (int st = plan_fits("product's gradient", b.dx)) return st;
     if (int st = plan_fits("product's gradient", b.dw)) return st;
     b.make_dz = d.act != TDC_ACT_NONE || must_pack(d.M, d.N, d.y_stride);
@@ -138,7 +138,7 @@ int linear8_check(const tdc_mx4_linear_desc *desc, tdc_mx4_linear_desc &d, TileP
     if (!d.residual_stride) d.residual_stride = d.N;
     if (d.x_dtype != TDC_MX8 && d.M > 1 && d.x_stride < d.K) return invalid("8-bit product: a row stride of x below K");
     if (d.M > 1 && (d.y_stride < d.N || d.residual_stride < d.N)) return invalid("8-bit product: a row stride below N");
-    p = tile_plan(std::max<long long>(d.M, 1), std::max<long long>(d.N, 1), d.K, TDC_MX8);
+    p = tile_plan(std::max<long long>(d.M, 1), std::max<long long>(d.N, 1), d.K, TDC_MX8, kAlong);
     if (int st = plan_fits("8-bit product", p)) return st;
     return d.x_dtype == TDC_MX8 ? (int)TDC_OK : mx_range("8-bit product", d.M, d.K);
 }

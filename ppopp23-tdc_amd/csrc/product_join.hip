@@ -27,7 +27,7 @@ struct Timing {
 static const Timing kTimings[] = {{256, 256, 0.82, 7.0, 1, 0.82, 1},   {256, 128, 0.51, 4.0, 1, 0.51, 1},  {128, 128, 0.28, 2.0, 1, 0.28, 1},
                                    {128, 128, 0.31, 1.5, 3, 0.31, 1}, {64, 128, 0.175, 0.8, 1, 0.24, 2}, {32, 128, 0.14, 0.8, 1, 0.22, 2}};
 
-TilePlan tile_plan(long long M, long long N, long long K, int in_dtype) {
+TilePlan tile_plan(long long M, long long N, long long K, int in_dtype, int layout) {
     const long long step = in_dtype == TDC_MX8 ? 64 : 32, steps = (K + step - 1) / step;
     TilePlan best{};
     double best_time = 0;
@@ -41,7 +41,7 @@ TilePlan tile_plan(long long M, long long N, long long K, int in_dtype) {
             const long long split_steps = want == 1 ? steps : round_up((steps + want - 1) / want, 8), splits = (steps + split_steps - 1) / split_steps;
             const double each = (double)(all * splits) / 256, rounds = t.together == 1 ? std::ceil(each) : std::max(each, 1.0);
             double time = 4.0 + std::max(rounds * t.step, t.alone) * (double)split_steps + rounds * t.besides / t.together + (t.together > 1 ? t.besides : 0.0);
-            if (splits > 1) time += 4.0 + (double)splits * M * N * 8 / 4e6;
+            if (splits > 1) time += 5.5 + (double)splits * M * N * 8 / 4e6;
             if (best.steps && time >= best_time) continue;
             best_time = time;
             best.kernel = kernel;
@@ -52,6 +52,13 @@ TilePlan tile_plan(long long M, long long N, long long K, int in_dtype) {
             best.split_steps = (int)split_steps;
             best.blocks = round_up(all, 8);
         }
+    }
+    if (layout == kAlong && M <= 16 && few_time(N, K * (in_dtype == TDC_MX8 ? 1 : 2)) < best_time) {
+        best = TilePlan{};
+        best.kernel = kFewRows;
+        best.splits = 1;
+        best.items = few_items(N);
+        return best;
     }
     best.part_stride = round_up(N, 4);
     best.part_bytes = best.splits > 1 ? best.splits * M * best.part_stride * 4 : 0;

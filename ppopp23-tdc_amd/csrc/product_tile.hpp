@@ -326,6 +326,8 @@ static int launch_shape(TileArgs &a, const TilePlan &p, hipStream_t s) {
 // One launch, or one for the parts of the sum and one that joins them.
 template <int IN, bool XT, bool WT, int OUT>
 static int launch_product_of(TileArgs &a, const TilePlan &p, hipStream_t s) {
+    if constexpr (!XT && !WT)
+        if (p.kernel == kFewRows) return launch_product_few(a, IN, OUT, s);
     a.steps = p.steps;
     a.split_steps = p.split_steps;
     a.splits = p.splits;
