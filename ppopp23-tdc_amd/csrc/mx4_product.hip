@@ -25,7 +25,7 @@ static __device__ __forceinline__ f16_t mfma4(i4_t a, i4_t b, f16_t c, int sa, i
 // that one wave to a SIMD keeps the matrix unit fed across its one barrier a step.  LDS holds the codes as they lie in
 // memory: a block's read is 1 KiB in a row, which meets no bank twice.
 //
-// Measured, tiles of 256, 8192 x 8192 x 8192 in random codes: 316 us, 3.5 PFLOP/s; 237 on zeros, 4.7, so that a quarter of it is the clock that
+// Measured, tiles of 256, 8192 x 8192 x 8192: 252 to 260 us on a layer's numbers.  While outputs took 10 to 15 us more, in random codes: 316 us, 3.5 PFLOP/s; 237 on zeros, 4.7, so that a quarter of it is the clock that
 // the power leaves.  Without the outputs 294 and 202, without new codes besides 233 and 181 (registers only: 172 and 124).  On zeros, where
 // power does not bind, half of the matrix unit's time is idle all the same; on random codes matrix instructions take half of the busy
 // cycles and LDS 28 %: one wave a SIMD with a barrier every step keeps neither full.  The same workgroups going from tile to tile, the next one's codes on their way while this one's outputs
@@ -205,7 +205,8 @@ __global__ void __launch_bounds__(256, MB * NB > 8 ? 1 : 2) tdc_mx4_product_tile
 // one can store while others load.  (Making x into 4 bits here as well, once for every tile across, took longer than a launch of its
 // own that leaves codes: 25088 rows of 128 by 512 18.5 us against 17.6, 4096 of 512 by 4096 41 against 22.)
 //
-// Measured: 25088 rows of 128 by 512, outputs in bf16: 12.6 us, 16.4 with a residual (51 MB and 3.2 TB/s of it, two and a half us the launch);
+// Measured: 25088 rows of 128 by 512, outputs in bf16, with a residual: 12.9 us (51 MB and 5 TB/s of it, two and a half us the launch).  Without one,
+// while outputs took longer: 12.6;
 // 5.2 of the 12.6 are the stores, 3 the way of the sums through LDS.
 template <int DT>
 __global__ void __launch_bounds__(256, (DT == TDC_F32 ? 2 : 3)) tdc_mx4_product_short_kernel(const ProductArgs a, int tiles_m, int tiles_n) {
