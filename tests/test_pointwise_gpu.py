@@ -524,6 +524,9 @@ def test_rows_of_other_forms():
         again = torch.autograd.grad(y.sum(), wrt)
         want = torch.autograd.grad(tdc_amd.linear_act(x, w, b, r, act=act), wrt, torch.ones_like(y))
         assert all(torch.equal(p, q) and torch.equal(p, s) for p, q, s in zip(first, again, want))
+        with torch.autograd.set_multithreading_enabled(False):
+            here = torch.autograd.grad(tdc_amd.linear_act(x, w, b, r, act=act), wrt, torch.ones_like(y))
+        assert all(torch.equal(p, q) for p, q in zip(here, want))
     x1 = x.detach()[0].clone().requires_grad_()
     (d,) = torch.autograd.grad(tdc_amd.linear_act(x1, w.detach(), act="silu"), x1, torch.ones(40, dtype=BF16, device="cuda"))
     assert d.shape == (64,)
@@ -629,3 +632,36 @@ def test_long_rows():
     far.copy_(numbers(295, (3, 64), BF16))
     v = numbers(296, (10, 64), BF16)
     assert torch.equal(tdc_amd.linear_act(far, v), tdc_amd.linear_act(far.contiguous(), v))
+
+
+@pytest.mark.parametrize("needs", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (0, 1, 1)])
+@pytest.mark.parametrize("C", [64, 301, 4100])
+def test_norm_gradients_that_are_wanted_alone(needs, C):
+    x, w, r = rms_case(300, 40, C, BF16, True)
+    dy, dh = numbers(303, (40, C), BF16), numbers(304, (40, C), BF16)
+    for checkpoint in (None, "mx8"):
+        full = [t.detach().clone().requires_grad_() for t in (x, w, r)]
+        want = grads(tdc_amd.rms_norm(*full, checkpoint=checkpoint), full, (dy, dh))
+        some = [t.detach().clone().requires_grad_(bool(n)) for t, n in zip((x, w, r), needs)]
+        got = grads(tdc_amd.rms_norm(*some, checkpoint=checkpoint), [t for t in some if t.requires_grad], (dy, dh))
+        assert all(torch.equal(p, q) for p, q in zip(got, [v for v, n in zip(want, needs) if n]))
+
+
+def test_what_is_kept_may_wait_on_the_host():
+    """What a gradient needs goes to the host and comes back elsewhere; how much it is."""
+    x, w, b, _ = case(310, 50, 70, 96, BF16)
+    gamma = numbers(311, (96,), F32)
+    leaves = [t.requires_grad_() for t in (x, w, b, gamma)]
+    dy = numbers(312, (50, 70), BF16)
+    for checkpoint in (None, "mx8"):
+        layer = lambda: tdc_amd.linear_act(tdc_amd.rms_norm(x, gamma, checkpoint=checkpoint), w, b, act="silu", checkpoint=checkpoint)  # noqa: E731, B023
+        want = grads(layer(), leaves, dy)
+        with torch.autograd.graph.save_on_cpu():
+            y = layer()
+        assert all(torch.equal(p, q) for p, q in zip(grads(y, leaves, dy), want))
+        kept = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.numel() * t.element_size()) or t, lambda t: t):
+            layer()
+        rows = 50 * 128 + 50 * 16 if checkpoint else 50 * 96 * 2
+        # x twice (of the norm, of the product), z, and the parameters and 1 / root mean square
+        assert sum(kept) <= 2 * rows + 50 * 70 * 2 + 70 * 96 * 2 + 96 * 4 + 50 * 4
