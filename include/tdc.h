@@ -522,7 +522,8 @@ int tdc_linear_backward(const tdc_linear_desc *desc, const void *x, const void *
                         const void *dy, void *dx, void *dw, void *dbias, void *dz, void *ws, size_t ws_bytes, void *stream);
 
 /* h = x + residual (rounded to dtype; x itself without one), y[m,c] = weight[c] * h[m,c] * rstd[m],
- * rstd[m] = 1 / sqrt(mean over c of h[m,c]^2 + eps), and its gradient. */
+ * rstd[m] = 1 / sqrt(mean over c of h[m,c]^2 + eps), and its gradient.  Everything between is fp32: a row whose squares' sum
+ * passes 3.4e38 has an rstd of 0. */
 typedef struct tdc_rms_norm_desc {
     int64_t rows;
     int32_t C;               /* up to 8192                                                   */

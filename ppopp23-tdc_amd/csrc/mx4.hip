@@ -107,8 +107,6 @@ static long long workgroups(long long rows, int runs) { return (rows + kRows - 1
 static int runs_of(long long K) { return (int)((mx4_padded(K) / 128 + kSteps - 1) / kSteps); }
 long long mx4_work_items(long long rows, long long K) { return workgroups(rows, runs_of(K)) * 256; }
 
-long long mx8_work_items(long long rows, long long K) { return mx4_work_items(rows, K); }
-
 template <bool E8>
 static int quantize(const void *x, int dtype, long long rows, long long K, long long stride, void *codes, void *scales, void *stream) {
     const int groups = (int)(mx4_padded(K) / 128), runs = runs_of(K);

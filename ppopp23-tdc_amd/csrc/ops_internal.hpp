@@ -147,10 +147,10 @@ void act_grad_plan(ActGradArgs &a);      // pitch and the last five
 long long act_grad_items(const ActGradArgs &a);
 int launch_act_grad(const ActGradArgs *jobs, int n, int dtype, void *stream);      // up to three of them
 int launch_column_sums(const float *part, void *out, long long N, int chunks, int out_dtype, void *stream);
+int launch_zeros(void *out, long long N, int dtype, void *stream);      // N numbers
 
 // Numbers in 8 bits.
 inline long long mx8_pitch(long long K) { return round_up(K, 128); }
-long long mx8_work_items(long long rows, long long K);
 int launch_mx8_quantize(const void *x, int dtype, long long rows, long long K, long long stride, void *codes, void *scales, void *stream);
 int launch_mx8_dequantize(const void *codes, const void *scales, long long rows, long long K, void *y, int dtype, long long stride,
                           void *stream);
@@ -171,7 +171,7 @@ struct RmsArgs {
     int blocks;                     // workgroups
 };
 enum { kRmsPlain, kRmsOutputMx8, kRmsKeptMx8 };      // 8 bits: none, y, what the gradient needs of h
-bool rms_plan(RmsArgs &a, bool grad);                // the last three; false if C is too large
+void rms_plan(RmsArgs &a, bool grad);                // the last three
 long long rms_items(const RmsArgs &a, bool grad);
 int launch_rms_forward(const RmsArgs &a, int dtype, int mode, void *stream);
 int launch_rms_backward(const RmsArgs &a, int dtype, bool kept_mx8, void *stream);

@@ -262,11 +262,11 @@ int tdc_linear_backward(const tdc_linear_desc *desc, const void *x, const void *
     if (!d.M || !d.N) {
         // sums of nothing
         if (dw && d.N)
-            if (int e = launch_column_sums(nullptr, dw, d.N * d.K, 0, d.dtype, stream)) return launched(what, e);
+            if (int e = launch_zeros(dw, d.N * d.K, d.dtype, stream)) return launched(what, e);
         if (dbias && d.N)
-            if (int e = launch_column_sums(nullptr, dbias, d.N, 0, d.bias_dtype, stream)) return launched(what, e);
+            if (int e = launch_zeros(dbias, d.N, d.bias_dtype, stream)) return launched(what, e);
         if (dx && d.M)
-            if (int e = launch_column_sums(nullptr, dx, d.M * d.K, 0, d.dtype, stream)) return launched(what, e);
+            if (int e = launch_zeros(dx, d.M * d.K, d.dtype, stream)) return launched(what, e);
         return TDC_OK;
     }
     Backward b;
@@ -480,7 +480,7 @@ int tdc_rms_norm_backward(const tdc_rms_norm_desc *desc, const void *h, const vo
     if (!dx && !dweight) return TDC_OK;
     if (!d.rows) {
         if (!dweight) return TDC_OK;      // (a sum of nothing)
-        return launched("RMS norm's gradient", launch_column_sums(nullptr, dweight, d.C, 0, d.weight_dtype, stream));
+        return launched("RMS norm's gradient", launch_zeros(dweight, d.C, d.weight_dtype, stream));
     }
     if (!h || !dy || !rstd) return invalid("RMS norm's gradient: null h, dy or rstd");
     if (h_scales)

@@ -224,6 +224,17 @@ int launch_column_sums(const float *part, void *out, long long N, int chunks, in
     return (int)hipGetLastError();
 }
 
+// Zeros of every type are the same bits.  (A fill, not a sum of no chunks: its 1024 threads for 64 numbers could not be launched for
+// 2^28 of them.)
+static __global__ void __launch_bounds__(256) tdc_zeros_kernel(unsigned short *out, long long n) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) out[i] = 0;
+}
+int launch_zeros(void *out, long long N, int dtype, void *stream) {
+    const long long n = dtype == TDC_F32 ? 2 * N : N;
+    tdc_zeros_kernel<<<(unsigned)std::min((n + 255) / 256, 16384ll), 256, 0, (hipStream_t)stream>>>((unsigned short *)out, n);
+    return (int)hipGetLastError();
+}
+
 void act_grad_plan(ActGradArgs &a) {
     a.pitch = round_up(a.N, 8);
     const long long vectors = (a.N + 7) / 8;

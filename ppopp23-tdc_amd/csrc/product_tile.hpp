@@ -47,8 +47,8 @@ static __device__ __forceinline__ int turn_along(int row) { return row >> 2 & 3;
 template <int R>
 static __device__ __forceinline__ int turn_across(int k) { return R >= 128 ? (k & 3) * 4 : R == 64 ? (k & 2) * 2 : 0; }
 
-// How a wave brings one operand.  `rows` and `stride` (bytes) are those in memory; `limit`: numbers of the sum that are there, zeros
-// from there on.
+// How a wave brings one operand: rows `stride` bytes apart in memory; `outer` runs over what is not summed, and `outer_left` of that are there
+// from the tile's first on (what lies past them repeats the last: its outputs go nowhere).
 template <int IN, bool T, int R>
 struct Source {
     static constexpr int kBytes = IN == TDC_MX8 ? 1 : 2, kStep = 64 / kBytes, kSlots = R * 2 / 16;

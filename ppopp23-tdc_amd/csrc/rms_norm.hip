@@ -249,9 +249,8 @@ __global__ void __launch_bounds__(kThreads) tdc_rms_backward_kernel(const RmsArg
     }
 }
 
-bool rms_plan(RmsArgs &a, bool grad) {
-    const int vectors = (a.C + 7) / 8;
-    if (vectors > 1024) return false;
+void rms_plan(RmsArgs &a, bool grad) {
+    const int vectors = (a.C + 7) / 8;      // (1024 at most)
     // (100352 x 512 in bf16, gradient from 8 bits: 65 us with 32 lanes and two requests each, 70 with 16 and four, 71 with 64 and one; 25088 x 512
     // into 8 bits 14.5, 16.6, 15.8; 100352 x 256 the same with 16 lanes and two as with 32 and one)
     a.team = vectors <= 32 ? 16 : vectors <= 64 ? 32 : vectors <= 256 ? 64 : 256;
@@ -261,7 +260,6 @@ bool rms_plan(RmsArgs &a, bool grad) {
     // Forward: eight workgroups to a compute unit.  Gradient: two, as many as its registers leave room for; 256 rows a thread at most.
     const long long most = grad ? 512 : 2048;
     a.blocks = (int)std::max(std::min(groups, most), grad ? (groups + 255) / 256 : 1);
-    return true;
 }
 long long rms_items(const RmsArgs &a, bool grad) {
     return std::max((long long)a.blocks * kThreads, grad ? ((long long)a.C + 63) / 64 * 1024 : 0);

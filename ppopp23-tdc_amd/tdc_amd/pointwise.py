@@ -520,7 +520,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, checkpoint=None):
 
     ``x`` and ``residual`` [..., C] (C up to 8192) are float32, float16 or bfloat16; ``weight`` [C] is of that type or float32.  Without
     a residual h is x and the result is returned; with one ``(result, h)``, h rounded to x's type, which is what is normalised.
-    Differentiable once, backwards, in all three.  ``checkpoint="mx8"`` keeps h for the gradient in microscaled 8 bits in place of h
+    Sums are in 32 bits (a row whose squares' sum passes 3.4e38 comes out as zeros).  Differentiable once, backwards, in all three.
+    ``checkpoint="mx8"`` keeps h for the gradient in microscaled 8 bits in place of h
     (33/32 byte a number): the gradients are then those at the rounded h, with the unrounded one's root mean square."""
     eps = _rms_check("rms_norm", x, weight, residual, eps)
     kept8 = _checkpoint(checkpoint)

@@ -221,6 +221,29 @@ def test_linear_of_nothing():
     assert tdc_amd.rms_norm(torch.empty(0, 40, device="cuda")).shape == (0, 40)
 
 
+def test_gradients_of_nothing_are_zeros_at_any_size():
+    """2^28 of them and some: more than a launch of sixteen threads a number could take."""
+    w = torch.ones(32769, 8192, device="cuda", dtype=BF16, requires_grad=True)
+    x = torch.ones(0, 8192, device="cuda", dtype=BF16)
+    dw, = grads(tdc_amd.linear_act(x, w), (w,), torch.ones(0, 32769, device="cuda", dtype=BF16))
+    assert dw.shape == w.shape and not dw.view(torch.int16).any()
+    x = torch.ones(1 << 20, 264, device="cuda", dtype=F16, requires_grad=True)
+    w = torch.ones(0, 264, device="cuda", dtype=F16)
+    dx, = grads(tdc_amd.linear_act(x, w), (x,), torch.ones(1 << 20, 0, device="cuda", dtype=F16))
+    assert dx.shape == x.shape and not dx.view(torch.int16).any()
+    for dtype in (F32, BF16):
+        w = torch.ones(1001, device="cuda", dtype=dtype, requires_grad=True)
+        dw, = grads(tdc_amd.rms_norm(torch.ones(0, 1001, device="cuda", dtype=BF16), w), (w,), torch.ones(0, 1001, device="cuda", dtype=BF16))
+        assert dw.dtype == dtype and dw.shape == (1001,) and not dw.any()
+
+
+def test_rms_norm_of_squares_past_32_bits_is_zeros():
+    x = torch.full((3, 100), 3.0, device="cuda")
+    x[1] = 3e19
+    y = tdc_amd.rms_norm(x)
+    assert not y[1].any() and (y[[0, 2]] - 1).abs().max() < 1e-5
+
+
 # ---- 8 bits ----
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
