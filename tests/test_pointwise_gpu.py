@@ -688,3 +688,25 @@ def test_what_is_kept_may_wait_on_the_host():
         rows = 50 * 128 + 50 * 16 if checkpoint else 50 * 96 * 2
         # x twice (of the norm, of the product), z, and the parameters and 1 / root mean square
         assert sum(kept) <= 2 * rows + 50 * 70 * 2 + 70 * 96 * 2 + 96 * 4 + 50 * 4
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 24, 40), (70, 120, 520), (33, 1001, 2001), (300, 96, 64)])
+@pytest.mark.parametrize("dtype,far", [(F16, 1e5), (BF16, 3.4e38)])
+def test_silu_gradient_where_what_it_is_taken_of_leaves_the_type(M, N, K, dtype, far):
+    """Sums that are finite in 32 bits and infinite in 16: the slope there is 0 or 1, as it is in 32 bits 50 from the origin."""
+    x, w, _, r = case(320, M, N, K, dtype)
+    dy = numbers(321, (M, N), dtype)
+
+    def at(distance):
+        b = torch.zeros(N, device="cuda")
+        b[3], b[5] = -distance, distance
+        wrt = [t.detach().clone().requires_grad_() for t in (x, w, b, r)]
+        y = tdc_amd.linear_act(*wrt, act="silu")
+        return y.detach(), grads(y, wrt, dy)
+    y, got = at(far)
+    _, want = at(50.0)
+    assert not y[:, 3].any() and (y[:, 5] > 6e4).all()
+    for g, v in zip(got, want):
+        # (50 from the origin it is 2^-66 off, and so is what is summed of it)
+        assert torch.isfinite(g).all() and (g.double() - v.double()).abs().max() <= M * 16 * 2.0 ** -60
+    assert not got[3][:, 3].any() and torch.equal(got[3][:, 5], dy[:, 5])
