@@ -516,7 +516,7 @@ int tdc_linear_workspace(const tdc_linear_desc *desc, size_t *forward_bytes, siz
 int tdc_linear_forward(const tdc_linear_desc *desc, const void *x, const void *w, const void *bias, const void *residual, void *y,
                        void *z, void *ws, size_t ws_bytes, void *stream);
 /* x: its numbers (x_scales NULL), or codes and scales; needed for dw only.  w: for dx only.  kept [M][N]: z for TDC_ACT_SILU, z or y for
- * TDC_ACT_RELU (whose gradient at 0 is 0), else ignored.  x, w and dy 16-byte aligned.  dx [M][K], dw [N][K], dbias [N] and
+ * TDC_ACT_RELU (whose gradient is 0 at 0 and dy at a NaN), else ignored.  x, w and dy 16-byte aligned.  dx [M][K], dw [N][K], dbias [N] and
  * dz [M][N rounded up to 8] (16-byte aligned; what the residual's gradient is), each or NULL. */
 int tdc_linear_backward(const tdc_linear_desc *desc, const void *x, const void *x_scales, const void *w, const void *kept,
                         const void *dy, void *dx, void *dw, void *dbias, void *dz, void *ws, size_t ws_bytes, void *stream);

@@ -32,7 +32,7 @@ static __device__ __forceinline__ void slopes(const typename Pack<DT, V>::type &
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         xh[j] = (xh[j] - mean[j]) * rstd[j];
-        dz[j] *= act_slope<ACT>(fmaf(xh[j], gamma[j], beta[j]));
+        dz[j] = act_back<ACT>(dz[j], fmaf(xh[j], gamma[j], beta[j]));
     }
 }
 

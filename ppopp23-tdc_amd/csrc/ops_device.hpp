@@ -81,16 +81,17 @@ __device__ __forceinline__ float act_of(float z) {
     if constexpr (ACT == TDC_ACT_SILU) return z * sigmoid(z);
     return z;
 }
-// The derivative at z.  ("silu": from 128 on s is 0 or 1 to the last bit, and so is the derivative.  A z kept in 16 bits may have become
-// infinite there, which times 0 would be a NaN; where z is one, s is.)
+// dy times the derivative at z.  "relu" chooses: a NaN passes dy on, and an infinite dy where nothing passes is 0.
+// "silu": from 128 on s is 0 or 1 to the last bit, and so is the derivative.  A z kept in 16 bits may have become infinite there,
+// which times 0 would be a NaN; where z is one, s is.
 template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-    if constexpr (ACT == TDC_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+__device__ __forceinline__ float act_back(float dy, float z) {
+    if constexpr (ACT == TDC_ACT_RELU) return z <= 0.0f ? 0.0f : dy;
     if constexpr (ACT == TDC_ACT_SILU) {
         const float s = sigmoid(z);
-        return s * (1.0f + __builtin_amdgcn_fmed3f(z, -128.0f, 128.0f) * (1.0f - s));
+        return dy * (s * (1.0f + __builtin_amdgcn_fmed3f(z, -128.0f, 128.0f) * (1.0f - s)));
     }
-    return 1.0f;
+    return dy;
 }
 
 // ---- blocks of 32 numbers in 4 bits ----

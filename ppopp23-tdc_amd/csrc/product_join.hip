@@ -158,7 +158,7 @@ static __device__ __forceinline__ void act_grad(const ActGradArgs &a, unsigned b
                     float z[8];
                     P::up(kept[k], z);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] *= act_slope<ACT>(z[j]);
+                    for (int j = 0; j < 8; ++j) v[j] = act_back<ACT>(v[j], z[j]);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) sum[j] += v[j];

@@ -710,3 +710,36 @@ def test_silu_gradient_where_what_it_is_taken_of_leaves_the_type(M, N, K, dtype,
         # (50 from the origin it is 2^-66 off, and so is what is summed of it)
         assert torch.isfinite(g).all() and (g.double() - v.double()).abs().max() <= M * 16 * 2.0 ** -60
     assert not got[3][:, 3].any() and torch.equal(got[3][:, 5], dy[:, 5])
+
+
+def test_relu_gradient_at_nans_and_of_infinities():
+    """What is not a number passes its gradient on; where the result is 0 an infinite gradient is as none."""
+    M, N, K = 40, 24, 64
+    x, w, b, _ = case(330, M, N, K, BF16, residual=False)
+    dy = numbers(331, (M, N), BF16)
+    bad = x.clone()
+    bad[7, 3] = float("nan")
+    for rows in (slice(0, M), slice(0, 9)):
+        wrt = [t.detach().clone().requires_grad_() for t in (bad[rows], w, b)]
+        y = tdc_amd.linear_act(*wrt, act="relu")
+        assert y[7].isnan().all()
+        dx, _, db = grads(y, wrt, dy[rows])
+        passed = torch.where(y.isnan() | (y > 0), dy[rows], torch.zeros_like(y)).double().cpu()
+        close(dx, (passed @ w.double().cpu()).numpy(), host(rounded_products(passed, w)), "dx")
+        S = passed.abs().sum(0).numpy()
+        close(db, passed.sum(0).numpy(), 512 * E * S + rounded(S, BF16), "dbias")
+        wrt = [t.detach().clone().requires_grad_() for t in (x[rows], w, b)]
+        y = tdc_amd.linear_act(*wrt, act="relu")
+        off = (y == 0) & (torch.arange(N, device="cuda") % 5 == 0)
+        assert off.any()
+        far = dy[rows].clone()
+        far[off] = float("inf")
+        got = grads(y, wrt, far)
+        far[off] = 1
+        assert all(torch.equal(g, v) for g, v in zip(got, grads(tdc_amd.linear_act(*wrt, act="relu"), wrt, far)))
+
+
+def rounded_products(a, w):
+    """The bound on a row of products a w: their sums in fp32, rounded to 16 bits once."""
+    S = a.abs() @ w.double().cpu().abs()
+    return ((16 + a.shape[1] / 8) * E + U[BF16] * 1.001) * S + LEAST[BF16]
