@@ -132,6 +132,12 @@ __global__ void __launch_bounds__(kThreads) tdc_rms_forward_kernel(const RmsArgs
             float y[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = h[i][j] * r * w[i][j];
+            if (MODE == kRmsOutputMx8 && c + 8 > a.C) {
+                // (what lies past the last number is zeros, also where r is none or infinite)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (c + j >= a.C) y[j] = 0.0f;
+            }
             if constexpr (MODE != kRmsOutputMx8) keep8<DT>(a.y, row * a.C, c, a.C, y);
             if constexpr (MODE != kRmsPlain) {
                 const float *const v = MODE == kRmsOutputMx8 ? y : h[i];

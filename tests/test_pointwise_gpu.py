@@ -743,3 +743,23 @@ def rounded_products(a, w):
     """The bound on a row of products a w: their sums in fp32, rounded to 16 bits once."""
     S = a.abs() @ w.double().cpu().abs()
     return ((16 + a.shape[1] / 8) * E + U[BF16] * 1.001) * S + LEAST[BF16]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("C", [1, 40, 100, 300, 1001, 2100, 5000])
+def test_rms_norm_mx8_leaves_zeros_behind_a_row_of_nans(C, dtype):
+    """Codes and scales past the last number are zeros, also in rows whose root mean square is a NaN or, of zeros without eps, 0."""
+    x = numbers(340, (5, C), dtype)
+    x[1, C // 2] = float("nan")
+    x[2, 0] = float("inf")
+    x[3] = 0
+    for eps in (1e-6, 0.0):
+        for r in (None, torch.zeros_like(x)):
+            out = tdc_amd.rms_norm_mx8(x, None, r, eps=eps)
+            q = out if r is None else out[0]
+            got = q.dequantize()
+            assert got[1].isnan().all() and got[2, 0].isnan() and torch.isfinite(got[[0, 4]]).all()
+            assert got[3].isnan().all() if eps == 0 else not got[3].any()
+            assert not q.codes[:, C:].any()
+            scales = torch.stack([q.scales[b // 16, :, 4 * (b % 4) + b % 16 // 4] for b in range((C + 511) // 512 * 16)], 1)
+            assert not scales[:, (C + 31) // 32:].any()
