@@ -512,6 +512,8 @@ typedef struct tdc_linear_desc {
 } tdc_linear_desc;
 
 int tdc_linear_workspace(const tdc_linear_desc *desc, size_t *forward_bytes, size_t *backward_bytes);
+/* The backward pass by itself: for calls that are given dz (not 0), which need no dz in the workspace, or for all. */
+int tdc_linear_backward_workspace(const tdc_linear_desc *desc, int32_t dz_given, size_t *bytes);
 /* x, w: 16-byte aligned.  bias, residual: or NULL.  z: [M][N], what the activation is taken of, or NULL. */
 int tdc_linear_forward(const tdc_linear_desc *desc, const void *x, const void *w, const void *bias, const void *residual, void *y,
                        void *z, void *ws, size_t ws_bytes, void *stream);

@@ -87,7 +87,8 @@ struct Backward {
     bool make_dz, pack_x, pack_w;       // (make_dz: dy is not dz as it lies)
     ActGradArgs grad;
 };
-int backward_plan(const tdc_linear_desc &d, Backward &b) {
+// (dz_given: the caller takes dz as a result, and there it lies)
+int backward_plan(const tdc_linear_desc &d, bool dz_given, Backward &b) {
     b.dx = tile_plan(d.M, d.K, d.N, d.dtype, kWAcross);
     b.dw = tile_plan(d.N, d.K, d.M, d.dtype, kAcross);
     if (int st = plan_fits("product's gradient", b.dx)) return st;
@@ -103,7 +104,7 @@ int backward_plan(const tdc_linear_desc &d, Backward &b) {
     if (d.kept_dtype == TDC_MX8)
         if (int st = mx_range("product's gradient", d.M, d.K)) return st;
     b.grad = copy_args(nullptr, d.M, d.N, d.y_stride, nullptr);
-    b.sums = b.dz + (b.make_dz ? padded(packed_bytes(d.M, d.N)) : 0);
+    b.sums = b.dz + (b.make_dz && !dz_given ? padded(packed_bytes(d.M, d.N)) : 0);
     b.x = b.sums + padded((size_t)b.grad.chunks * d.N * 4);
     b.w = b.x + (b.pack_x ? padded(packed_bytes(d.M, d.K)) : 0);
     b.part = b.w + (b.pack_w ? padded(packed_bytes(d.N, d.K)) : 0);
@@ -198,9 +199,20 @@ int tdc_linear_workspace(const tdc_linear_desc *desc, size_t *forward_bytes, siz
         *forward_bytes = f.all;
     }
     if (backward_bytes) {
-        if (int st = some ? backward_plan(d, b) : TDC_OK) return st;
+        if (int st = some ? backward_plan(d, false, b) : TDC_OK) return st;
         *backward_bytes = b.all;
     }
+    return TDC_OK;
+}
+TDC_ENTRY_END
+
+int tdc_linear_backward_workspace(const tdc_linear_desc *desc, int32_t dz_given, size_t *bytes) TDC_ENTRY {
+    tdc_linear_desc d;
+    if (int st = linear_check(desc, d)) return st;
+    if (!bytes) return invalid("product's gradient: null argument");
+    Backward b;
+    if (int st = d.M && d.N ? backward_plan(d, dz_given != 0, b) : TDC_OK) return st;
+    *bytes = b.all;
     return TDC_OK;
 }
 TDC_ENTRY_END
@@ -270,7 +282,7 @@ int tdc_linear_backward(const tdc_linear_desc *desc, const void *x, const void *
         return TDC_OK;
     }
     Backward b;
-    if (int st = backward_plan(d, b)) return st;
+    if (int st = backward_plan(d, dz != nullptr, b)) return st;
     if (!dy || (dw && !x) || (dx && !w)) return invalid("product's gradient: null x, w or dy");
     if (dw && (d.kept_dtype == TDC_MX8) != (x_scales != nullptr)) return invalid("product's gradient: scales go with x in 8 bits");
     if (d.act != TDC_ACT_NONE && !kept) return invalid("product's gradient: an activation's gradient needs what it was taken of");

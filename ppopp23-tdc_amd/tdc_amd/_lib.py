@@ -33,8 +33,8 @@ EXPORTS = (
     "tdc_group_norm_workspace", "tdc_group_norm_forward", "tdc_group_norm_backward", "tdc_group_norm_forward_mx4",
     "tdc_group_norm_mx4_workspace", "tdc_mx4_sizes", "tdc_mx4_quantize", "tdc_mx4_dequantize", "tdc_mx4_linear_workspace",
     "tdc_mx4_linear", "tdc_mx8_sizes", "tdc_mx8_quantize", "tdc_mx8_dequantize", "tdc_mx8_linear_workspace", "tdc_mx8_linear",
-    "tdc_linear_workspace", "tdc_linear_forward", "tdc_linear_backward", "tdc_rms_norm_workspace", "tdc_rms_norm_forward",
-    "tdc_rms_norm_forward_mx8", "tdc_rms_norm_backward",
+    "tdc_linear_workspace", "tdc_linear_backward_workspace", "tdc_linear_forward", "tdc_linear_backward", "tdc_rms_norm_workspace",
+    "tdc_rms_norm_forward", "tdc_rms_norm_forward_mx8", "tdc_rms_norm_backward",
 )
 
 
@@ -195,6 +195,7 @@ def lib():
     L.tdc_mx8_linear_workspace.argtypes = [linear, szp]
     L.tdc_mx8_linear.argtypes = [linear] + [c_void_p] * 8 + [sz, c_void_p]
     L.tdc_linear_workspace.argtypes = [row, szp, szp]
+    L.tdc_linear_backward_workspace.argtypes = [row, i32, szp]
     L.tdc_linear_forward.argtypes = [row] + [c_void_p] * 7 + [sz, c_void_p]
     L.tdc_linear_backward.argtypes = [row] + [c_void_p] * 10 + [sz, c_void_p]
     L.tdc_rms_norm_workspace.argtypes = [rms, szp]

@@ -283,14 +283,17 @@ def mx8_conv1x1(x, weight, bias=None, residual=None, act="none", out_dtype=None)
 _plans = _Cache()
 
 
-def _linear_plan(M, N, K, dtype, bias_dtype, act, kept8, x_step, w_step, y_step, r_step, backward):
-    key = (M, N, K, dtype, bias_dtype, act, kept8, x_step, w_step, y_step, r_step, backward)
+def _linear_plan(M, N, K, dtype, bias_dtype, act, kept8, x_step, w_step, y_step, r_step, backward, dz_given=False):
+    key = (M, N, K, dtype, bias_dtype, act, kept8, x_step, w_step, y_step, r_step, backward, dz_given)
     plan = _plans.get(key)
     if plan is None:
         kind = _DTYPES[dtype]
         desc = _lib.LinearDesc(M, N, K, kind, _DTYPES[bias_dtype], _act(act), _MX8 if kept8 else kind, x_step, w_step, y_step, r_step)
         need = ctypes.c_size_t()
-        check(lib().tdc_linear_workspace(byref(desc), None if backward else byref(need), byref(need) if backward else None))
+        if backward:
+            check(lib().tdc_linear_backward_workspace(byref(desc), dz_given, byref(need)))
+        else:
+            check(lib().tdc_linear_workspace(byref(desc), byref(need), None))
         plan = _plans.keep(key, (byref(desc), need.value))
     return plan
 
@@ -358,7 +361,7 @@ class _LinearAct(torch.autograd.Function):
                 x, _, x_step = _tile_rows(held)
                 x_at = x.data_ptr()
             w, _, w_step = _tile_rows(weight) if need_x else (None, 0, 0)
-            ref, need = _linear_plan(M, N, K, dtype, bias_dtype, act, kept8, x_step, w_step, y_step, 0, True)
+            ref, need = _linear_plan(M, N, K, dtype, bias_dtype, act, kept8, x_step, w_step, y_step, 0, True, dz is not None)
             ws = _empty(need, dtype=_u8, device=dev) if need else None
             status = _call("tdc_linear_backward")(ref, x_at, x_scales, _ptr(w), _ptr(kept), flat.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
                                                   _ptr(dz), _ptr(ws), need, _raw_stream(index))

@@ -208,3 +208,17 @@ def test_oracle_gradients_by_differences():
                         (dz, lambda v: f(x, w, b, v), r), (dn, lambda v: n(v, wt), h), (dwt, lambda v: n(h, v), wt)):
         d = g.standard_normal(at.shape)
         assert abs((got * d).sum() - slope(fn, at, d)) < 1e-7
+
+
+@pytest.mark.parametrize("act,N,second", [(2, 300, 300 * 304 * 2), (1, 304, 300 * 304 * 2), (0, 300, 300 * 304 * 2), (0, 304, 0)])
+def test_the_workspace_of_a_gradient_that_is_given_dz_holds_no_other(act, N, second):
+    L, need, given = tdc_amd.lib(), ctypes.c_size_t(), ctypes.c_size_t()
+    d = ctypes.byref(linear(M=300, N=N, K=41, act=act))
+    assert L.tdc_linear_backward_workspace(d, 0, ctypes.byref(need)) == 0 and need.value == sizes(linear(M=300, N=N, K=41, act=act))[1]
+    assert L.tdc_linear_backward_workspace(d, 1, ctypes.byref(given)) == 0
+    assert given.value == need.value - (second + 255) // 256 * 256 and given.value > 0
+    g = L.tdc_linear_backward
+    assert g(d, 16, None, 16, 16, 16, 16, 16, None, 16, 16, given.value - 1, None) == INVALID and "workspace" in error()
+    assert g(d, 16, None, 16, 16, 16, 16, 16, None, None, 16, need.value - 1, None) == INVALID and "workspace" in error()
+    assert L.tdc_linear_backward_workspace(None, 0, ctypes.byref(need)) == INVALID and L.tdc_linear_backward_workspace(d, 0, None) == INVALID
+    assert L.tdc_linear_backward_workspace(ctypes.byref(linear(M=0)), 1, ctypes.byref(need)) == 0 and need.value == 0
