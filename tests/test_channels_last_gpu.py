@@ -797,3 +797,16 @@ def test_norm_into_a_slice_and_its_statistics(shape, groups, dtype):
     rstd = 1 / np.sqrt(var + 1e-5)
     assert (np.abs(got[0] - mean) <= E * np.abs(mean) + 1e-12 * np.abs(v).max()).all()
     assert (np.abs(got[1] / rstd - 1) <= 10 * E).all()
+
+
+def test_relu_gradient_of_infinities():
+    """An infinite gradient where the result is 0 is as any other there."""
+    x = torch.randn(2, 24, 5, 7, generator=seeded(900)).cuda().contiguous(memory_format=torch.channels_last)
+    dy = torch.randn(2, 24, 5, 7, generator=seeded(901)).cuda().contiguous(memory_format=torch.channels_last)
+    w, b = torch.rand(24, generator=seeded(902)).cuda() + 0.5, torch.randn(24, generator=seeded(903)).cuda()
+    wrt = [t.requires_grad_() for t in (x, w, b)]
+    y = tdc_amd.group_norm_act(x, 4, w, b, act="relu")
+    off = (y == 0) & (torch.arange(7, device="cuda") % 2 == 0)
+    assert off.any()
+    got = [torch.autograd.grad(tdc_amd.group_norm_act(x, 4, w, b, act="relu"), wrt, dy.masked_fill(off, v)) for v in (float("inf"), 1.0)]
+    assert all(torch.isfinite(g).all() and torch.equal(g, v) for g, v in zip(*got))
