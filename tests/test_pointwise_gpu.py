@@ -780,3 +780,59 @@ def test_the_residuals_gradient_is_made_once():
     made = torch.cuda.max_memory_allocated() - held
     # dresidual, dx and dw, and what else the workspace is for: a tenth of a second one is more than enough
     assert sum(t.numel() * 2 for t in got) <= made <= sum(t.numel() * 2 for t in got) + M * N * 2 * 0.6, made
+
+
+# Sizes at which the product, w's gradient and x's take each of the six tiles, whole and in parts of the sum: 20 to 145 rows take tiles of 32 and 64
+# rows and the deep one of 128, 2022 x 6488 x 1031 and 14328 x 456 x 2072 those of 256 x 256 and 256 x 128 in every layout.
+TILES = [(20, 9, 42), (8506, 11, 40), (21, 1483, 1280), (2801, 33, 1428), (19193, 195, 50), (250, 8720, 176), (69, 2544, 4744), (2022, 6488, 1031),
+         (14328, 456, 2072), (430, 924, 15735), (8559, 8896, 152), (2796, 10, 11494), (145, 8299, 8858)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_every_tile_and_layout_on_whole_numbers(M, N, K, dtype):
+    """Sums of small whole numbers are exact in fp32 in any order, and rounded once: results are those, to the bit.  With "silu" what the
+    activation is taken of is a whole number too, so that its gradient in each place is known to its own rounding."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    whole = lambda *shape: torch.randint(-4, 5, shape, generator=g, device="cuda").to(dtype)  # noqa: E731
+    x, w, r, dy = whole(M, K), whole(N, K), whole(M, N), whole(M, N)
+    f = lambda t: t.detach().float()  # noqa: E731
+    z = f(x) @ f(w).t().contiguous() + f(r)
+    assert z.abs().max() < 2 ** 24
+    x, w, r = (t.requires_grad_() for t in (x, w, r))
+    y = tdc_amd.linear_act(x, w, None, r)
+    assert torch.equal(y, z.to(dtype))
+    dx, dw, dr = grads(y, (x, w, r), dy)
+    assert torch.equal(dx, (f(dy) @ f(w)).to(dtype)) and torch.equal(dw, (f(dy).t().contiguous() @ f(x)).to(dtype)) and torch.equal(dr, dy)
+    del dx, dw, dr, y
+    # an eighth of the product: numbers at which "silu" bends
+    x8 = (x.detach() / 8).requires_grad_()
+    y = tdc_amd.linear_act(x8, w, None, r, act="silu")
+    z = ((z - f(r)) / 8 + f(r)).double()
+    s = torch.sigmoid(z)
+    u, least = U[dtype], LEAST[dtype]
+    # (the hardware's sigmoid is good to 2^-22 and |z| 2^-24 of itself, and to 2^-126 where e^-z passes 32 bits)
+    assert ((y.double() - z * s).abs() <= (u + 2.0 ** -20 + z.abs() * 2.0 ** -22) * (z * s).abs() + z.abs() * 2.0 ** -125 + 2 * least).all()
+    _, _, dr = grads(y, (x8, w, r), dy)
+    z = z.to(dtype).double()      # (what is kept)
+    s = torch.sigmoid(z)
+    slope, d = s * (1 + z * (1 - s)), dy.double()
+    # (1 + z (1 - s) may cancel)
+    off = d.abs() * (1 + z.abs()) * (s * (2.0 ** -20 + z.abs() * 2.0 ** -22) + 2.0 ** -125)
+    assert ((dr.double() - d * slope).abs() <= off + u * 1.001 * (d * slope).abs() + 2 * least).all()
+
+
+TILES8 = [(17, 10, 42), (17, 9, 2994), (9828, 9, 47), (266, 9, 17403), (19659, 9, 352), (1593, 9, 6595), (16794, 136, 46), (8356, 9, 6438),
+          (1926, 4040, 960), (8069, 1995, 533), (9161, 156, 14045), (25088, 128, 512)]
+
+
+@pytest.mark.parametrize("M,N,K", TILES8)
+def test_every_tile_of_the_8_bit_product_on_whole_numbers(M, N, K):
+    """The six tiles in 8 bits, whole and in parts of the sum, on numbers that 8 bits hold and sums that an instruction keeps whole."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.zeros(M, K, device="cuda")
+    x.scatter_(1, torch.randint(0, K, (M, 20), generator=g, device="cuda"), torch.randint(-3, 4, (M, 20), generator=g, device="cuda").float())
+    w = torch.randint(-4, 5, (N, K), generator=g, device="cuda").float()
+    r = torch.randint(-8, 9, (M, N), generator=g, device="cuda").to(BF16)
+    y = tdc_amd.mx8_linear(x, tdc_amd.mx8_quantize(w), None, r, act="relu", out_dtype=BF16)
+    assert torch.equal(y.float(), (x @ w.t().contiguous() + r.float()).clamp(min=0).to(BF16).float())
