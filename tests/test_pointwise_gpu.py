@@ -836,3 +836,39 @@ def test_every_tile_of_the_8_bit_product_on_whole_numbers(M, N, K):
     r = torch.randint(-8, 9, (M, N), generator=g, device="cuda").to(BF16)
     y = tdc_amd.mx8_linear(x, tdc_amd.mx8_quantize(w), None, r, act="relu", out_dtype=BF16)
     assert torch.equal(y.float(), (x @ w.t().contiguous() + r.float()).clamp(min=0).to(BF16).float())
+
+
+@pytest.mark.parametrize("M,C", [(40000, 256), (20000, 512), (36000, 100), (9000, 1001), (2600, 2100), (2100, 5000)])
+def test_rms_norm_of_more_rows_than_run_at_once(M, C):
+    """Every team of lanes goes on to further rows, whose numbers are on their way meanwhile: all rows, in every form of the result."""
+    test_rms_norm(M, C, BF16)
+    for residual in (False, True):
+        check_rms_grads(M, C, BF16, residual, "mx8")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("M,C", [(1300, 2100), (700, 8192), (2300, 900), (9000, 200)])
+def test_rms_norm_gradients_of_more_rows_than_run_at_once(M, C, dtype):
+    for checkpoint in (None, "mx8"):
+        check_rms_grads(M, C, dtype, True, checkpoint)
+        check_rms_grads(M, C, dtype, False, checkpoint, weight_dtype=dtype)
+
+
+def test_mx8_at_the_smallest_and_largest_scales():
+    """Blocks whose largest magnitudes lie on either side of where the scale byte stops at 0, and those of the largest numbers there are."""
+    top = np.array([2.0 ** -119, 1.9 * 2.0 ** -119, 2.0 ** -120, 1.3 * 2.0 ** -122, 2.0 ** -125, 1.7 * 2.0 ** -126, 2.0 ** -127, 2.0 ** -130, 2.0 ** -135, 2.0 ** -136,
+                    2.0 ** 126, 2.0 ** 127, 1.5 * 2.0 ** 127, 1.75 * 2.0 ** 127, float(np.finfo(np.float32).max)])
+    share = np.random.default_rng(9).uniform(-1, 1, (len(top), 32))
+    share[:, 5] = 1
+    x = (share * top[:, None]).astype(np.float32)
+    want, byte = ref.quantize8(x.astype(np.float64))
+    assert byte[:, 0].tolist() == [0] * 10 + [245] + [246] * 4 and (want[:10] != 0).any(1).all()
+    q = tdc_amd.mx8_quantize(torch.from_numpy(x).cuda())
+    assert np.array_equal(q.scales[0, :, 0].cpu().numpy(), byte[:, 0]) and np.array_equal(host(q.dequantize()), want)
+    # and in the products, small ones with large ones
+    for M, N, K in ((5, 24, 96), (70, 40, 200), (300, 200, 700)):
+        a, b = torch.randint(-4, 5, (M, K), generator=seeded(350)).float(), torch.randint(-4, 5, (N, K), generator=seeded(351)).float()
+        a[:, 20:] *= (torch.arange(K - 20) % 16 == 0).float()      # (sums below 2^8: whole in 16 bits)
+        for small in (2.0 ** -122, 2.0 ** -124, 2.0 ** -126):
+            y = tdc_amd.mx8_linear(a.cuda() * small, tdc_amd.mx8_quantize(b.cuda() * 2.0 ** 120), out_dtype=BF16)
+            assert torch.equal(y.float(), (a.cuda() @ b.t().contiguous().cuda() * (small * 2.0 ** 120)).to(BF16).float())
