@@ -872,3 +872,25 @@ def test_mx8_at_the_smallest_and_largest_scales():
         for small in (2.0 ** -122, 2.0 ** -124, 2.0 ** -126):
             y = tdc_amd.mx8_linear(a.cuda() * small, tdc_amd.mx8_quantize(b.cuda() * 2.0 ** 120), out_dtype=BF16)
             assert torch.equal(y.float(), (a.cuda() @ b.t().contiguous().cuda() * (small * 2.0 ** 120)).to(BF16).float())
+
+
+@pytest.mark.parametrize("dtype,small,large", [(F16, 2.0 ** -22, 2.0 ** 12), (BF16, 2.0 ** -131, 2.0 ** 121)])
+@pytest.mark.parametrize("M,N,K", [(3, 40, 96), (70, 40, 96), (300, 130, 203)])
+def test_numbers_below_the_normal_ones_take_part(M, N, K, dtype, small, large):
+    """Subnormal numbers of either type, as operands (each of x, w and dy in turn) and as results."""
+    g = seeded(370)
+    x, w, dy = (torch.randint(-3, 4, s, generator=g).float().cuda() for s in ((M, K), (N, K), (M, N)))
+    # (a sum whose terms' magnitudes stay below 2^127 passes nothing on the way, and 64 bits hold it: the others are left out)
+    def same(got, p, q, by):
+        whole = (p.abs() @ q.abs()).double() * by < 2.0 ** 127
+        assert torch.equal(got[whole], ((p @ q).double() * by).to(dtype)[whole]) and (whole.all() or by == large)
+    for a, b, c in ((small, large, 1.0), (large, small, 1.0), (1.0, large, small), (large, 1.0, small)):
+        p, q = ((t * s).to(dtype).requires_grad_() for t, s in ((x, a), (w, b)))
+        y = tdc_amd.linear_act(p, q)
+        dx, dw = grads(y, (p, q), (dy * c).to(dtype))
+        same(y, x, w.t().contiguous(), a * b)
+        same(dx, dy, w, c * b)
+        same(dw, dy.t().contiguous(), x, c * a)
+    tiny = (x * small).to(dtype)
+    gamma = torch.ones(K, device="cuda")
+    assert torch.equal(tdc_amd.rms_norm(tiny, gamma, torch.zeros_like(tiny))[1], tiny)
