@@ -894,3 +894,119 @@ def test_numbers_below_the_normal_ones_take_part(M, N, K, dtype, small, large):
     tiny = (x * small).to(dtype)
     gamma = torch.ones(K, device="cuda")
     assert torch.equal(tdc_amd.rms_norm(tiny, gamma, torch.zeros_like(tiny))[1], tiny)
+
+
+# ---- the C entries, with strides that Python does not pass ----
+
+class Guarded:
+    """A tensor with numbers of its own before and behind it, which have to stay."""
+
+    def __init__(self, shape, dtype):
+        n, self.pad = int(np.prod(shape)), 64 // torch.empty((), dtype=dtype).element_size()
+        self.held = torch.full((n + 2 * self.pad,), 77, dtype=dtype, device="cuda")
+        self.t = self.held[self.pad:self.pad + n].view(shape)
+
+    def kept(self):
+        return bool((self.held[:self.pad] == 77).all() and (self.held[len(self.held) - self.pad:] == 77).all())
+
+
+def entry(name, *args):
+    at = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    assert getattr(tdc_amd.lib(), name)(*at, torch.cuda.current_stream().cuda_stream) == 0, tdc_amd.lib().tdc_last_error_string()
+
+
+def workspace(name, *args):
+    need = ctypes.c_size_t()
+    assert getattr(tdc_amd.lib(), name)(*args, ctypes.byref(need)) == 0
+    return Guarded((need.value,), torch.uint8)
+
+
+ENTRY_CASES = [(1, 1, 1), (5, 24, 40), (16, 100, 1000), (33, 1001, 2001), (70, 2544, 744), (129, 127, 257), (300, 96, 64), (1000, 24, 64), (2100, 1030, 1100), (9000, 33, 40)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N,K", ENTRY_CASES)
+def test_entries_of_the_product_write_what_is_theirs(M, N, K, dtype):
+    """Results in slices of wider tensors and workspaces of just the size that is asked for: nothing beside them is touched."""
+    from tdc_amd import _lib
+    x, w, b, r = case(380, M, N, K, dtype)
+    dy = numbers(381, (M, N), dtype)
+    wrt = [t.requires_grad_() for t in (x, w, b, r)]
+    want_y = tdc_amd.linear_act(*wrt, act="silu")
+    want = grads(want_y, wrt, dy)
+    kind = 1 if dtype == F16 else 2
+    wide, wide_r = Guarded((M, N + 9), dtype), torch.full((M, N + 5), float("nan"), dtype=dtype, device="cuda")
+    y = wide.t[:, 3:3 + N]
+    wide_r[:, 1:1 + N] = r.detach()
+    z, residual = Guarded((M, N), dtype), wide_r[:, 1:1 + N]
+    desc = _lib.LinearDesc(M, N, K, kind, kind, 2, kind, 0, 0, N + 9, N + 5)
+    need = ctypes.c_size_t()
+    assert tdc_amd.lib().tdc_linear_workspace(ctypes.byref(desc), ctypes.byref(need), None) == 0
+    ws = Guarded((need.value,), torch.uint8)
+    entry("tdc_linear_forward", ctypes.byref(desc), x, w, b, residual, y, z.t, ws.t, need.value)
+    assert torch.equal(y, want_y) and wide.kept() and z.kept() and ws.kept()
+    assert (wide.t[:, :3] == 77).all() and (wide.t[:, 3 + N:] == 77).all()
+    # z is what the activation is taken of: the result without one
+    assert torch.equal(z.t, tdc_amd.linear_act(x.detach(), w.detach(), b.detach(), r.detach()))
+    for step in ((N + 7) // 8 * 8 + 24, N + 13):
+        wide_dy = torch.full((M, step), float("nan"), dtype=dtype, device="cuda")
+        wide_dy[:, 8:8 + N] = dy
+        desc = _lib.LinearDesc(M, N, K, kind, kind, 2, kind, 0, 0, step, 0)
+        dx, dw, db, dz = (Guarded(s, dtype) for s in ((M, K), (N, K), (N,), (M, (N + 7) // 8 * 8)))
+        for given in (1, 0):
+            ws = workspace("tdc_linear_backward_workspace", ctypes.byref(desc), given)
+            entry("tdc_linear_backward", ctypes.byref(desc), x, None, w, z.t, wide_dy[:, 8:], dx.t, dw.t, db.t, dz.t if given else None, ws.t, ws.t.numel())
+            assert all(g.kept() for g in (dx, dw, db, dz, ws))
+            assert torch.equal(dx.t, want[0]) and torch.equal(dw.t, want[1]) and torch.equal(db.t, want[2]) and torch.equal(dz.t[:, :N], want[3])
+            assert not dz.t[:, N:].any()
+            for g in (dx, dw, db):
+                g.t.fill_(77)
+
+
+@pytest.mark.parametrize("M,N,K", ENTRY_CASES + [(40, 33, 513)])
+def test_entries_in_8_bits_write_what_is_theirs(M, N, K):
+    from tdc_amd import _lib
+    x, w, b, r = case(390, M, N, K, BF16)
+    want_q, qw = tdc_amd.mx8_quantize(x), tdc_amd.mx8_quantize(w)
+    codes, scales = Guarded(tuple(want_q.codes.shape), torch.uint8), Guarded(tuple(want_q.scales.shape), torch.uint8)
+    wide_x = torch.full((M, K + 3), float("nan"), dtype=BF16, device="cuda")
+    wide_x[:, 1:1 + K] = x
+    entry("tdc_mx8_quantize", wide_x[:, 1:], 2, M, K, K + 3, codes.t, scales.t)
+    assert codes.kept() and scales.kept() and torch.equal(codes.t, want_q.codes) and torch.equal(scales.t, want_q.scales)
+    back = Guarded((M, K + 7), BF16)
+    entry("tdc_mx8_dequantize", codes.t, scales.t, M, K, back.t[:, 2:], 2, K + 7)
+    assert back.kept() and torch.equal(back.t[:, 2:2 + K], want_q.dequantize(BF16)) and (back.t[:, :2] == 77).all() and (back.t[:, 2 + K:] == 77).all()
+    want = tdc_amd.mx8_linear(x, qw, b, r, act="relu")
+    for kind in (2, 4):
+        wide = Guarded((M, N + 9), BF16)
+        desc = _lib.Mx4LinearDesc(M, N, K, kind, 2, 2, 1, K + 3 if kind == 2 else 0, N + 9, 0)
+        ws = workspace("tdc_mx8_linear_workspace", ctypes.byref(desc))
+        entry("tdc_mx8_linear", ctypes.byref(desc), wide_x[:, 1:] if kind == 2 else codes.t, None if kind == 2 else scales.t, qw.codes, qw.scales, b, r, wide.t[:, 3:],
+              ws.t, ws.t.numel())
+        assert wide.kept() and ws.kept() and torch.equal(wide.t[:, 3:3 + N], want) and (wide.t[:, :3] == 77).all() and (wide.t[:, 3 + N:] == 77).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,C", [(1, 1), (3, 129), (40, 513), (9, 2050), (3000, 700), (20000, 24), (5, 8191)])
+def test_entries_of_rms_norm_write_what_is_theirs(M, C, dtype):
+    from tdc_amd import _lib
+    x, w, r = rms_case(400, M, C, dtype, True, dtype)
+    dy, dh = numbers(403, (M, C), dtype), numbers(404, (M, C), dtype)
+    wrt = [t.requires_grad_() for t in (x, w, r)]
+    out = tdc_amd.rms_norm(x, w, r, checkpoint="mx8")
+    want = grads(out, wrt, (dy, dh))
+    kind = {F32: 0, BF16: 2}[dtype]
+    p = ctypes.byref(_lib.RmsNormDesc(M, C, kind, kind, 1e-6, 0, 0, 0, 0))
+    y, h, rstd = Guarded((M, C), dtype), Guarded((M, C), dtype), Guarded((M,), F32)
+    codes, scales = Guarded((M, (C + 127) // 128 * 128), torch.uint8), Guarded(((C + 511) // 512, M, 16), torch.uint8)
+    entry("tdc_rms_norm_forward", p, x, r, w, y.t, h.t, rstd.t, codes.t, scales.t)
+    assert all(g.kept() for g in (y, h, rstd, codes, scales)) and torch.equal(y.t, out[0]) and torch.equal(h.t, out[1])
+    q = tdc_amd.mx8_quantize(h.t)
+    assert torch.equal(codes.t, q.codes) and torch.equal(scales.t, q.scales)
+    dx, dw = Guarded((M, C), dtype), Guarded((C,), dtype)
+    ws = workspace("tdc_rms_norm_workspace", p)
+    entry("tdc_rms_norm_backward", p, codes.t, scales.t, w, dy, dh, rstd.t, dx.t, dw.t, ws.t, ws.t.numel())
+    assert all(g.kept() for g in (dx, dw, ws)) and torch.equal(dx.t, want[0]) and torch.equal(dw.t, want[1])
+    want = tdc_amd.rms_norm_mx8(x.detach(), w.detach(), r.detach())
+    entry("tdc_rms_norm_forward_mx8", p, x, r, w, codes.t, scales.t, h.t)
+    assert all(g.kept() for g in (codes, scales, h)) and torch.equal(codes.t, want[0].codes) and torch.equal(scales.t, want[0].scales) and torch.equal(h.t, want[1])
