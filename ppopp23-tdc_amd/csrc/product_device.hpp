@@ -73,7 +73,7 @@ static __device__ __forceinline__ float bias_of(const ProductOut &a, long long n
 }
 
 // A wave's outputs from row m on and from column n on; `bias` is that of its columns, `stage` its own 4 KiB NB of LDS.  Z: what the activation
-// is taken of leaves too; PART: sums that others join, and nothing with them.  Of a block a lane
+// is taken of leaves too, in y's 16 bits (the slope is taken there; in 32 it would cost twice y's bytes); PART: sums that others join, and nothing with them.  Of a block a lane
 // has row r of x, and of w 16 u + 8 q .. 16 u + 8 q + 7, u = 0, 1.  32 rows at a time go through LDS, where a lane takes eight outputs of a
 // row and its neighbours those beside them: residuals and outputs are whole cache lines.  (The first halves of a row's eights lie
 // before the second ones, 16 bytes moved by the row, so that neither side meets a bank twice.)  The residuals of the next rows are on

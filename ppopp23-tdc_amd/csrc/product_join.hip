@@ -131,6 +131,7 @@ int launch_join(const TileArgs &a, int y_dtype, void *stream) {
 
 // A workgroup of 256 owns `across` vectors of eight columns and `chunk_rows` rows.  Sums over the rows: a thread's own rows in fp32 (those of
 // a chunk: see act_grad_plan), then over threads and chunks in 64 bits, in a fixed order.  (Sums are of dz before its rounding.)
+// dz itself is rounded: the matrix instructions that multiply it take 16 bits.
 template <int DT, int ACT>
 static __device__ __forceinline__ void act_grad(const ActGradArgs &a, unsigned block, float (&lds)[256][9]) {
     using P = Pack<DT, 8>;

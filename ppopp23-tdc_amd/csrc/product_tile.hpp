@@ -131,10 +131,12 @@ static __device__ __forceinline__ f16_t mfma8(const i4_t (&a)[2], const i4_t (&b
 // second set of registers while the last step's are multiplied: one barrier a step, at which nothing is waited for but the requests of the
 // step after the next.
 //
-// Measured, tiles of 256, 8192 x 8192 x 8192: on random numbers 860 us in bf16 (1.28 PFLOP/s; w across the sum 852, both across it 840) and
-// 400 in 8 bits (2.75), on zeros, where power does not bind, 688 (641 both across) and 329.  Without new requests 693 and 510 on zeros, from
-// registers alone 610 and 503: on numbers that are not all alike the power that these bytes take on their way costs as much as the
-// stalls.  LDS is busy for 275000 of 1.5 million cycles, without conflicts; 0.8 GB come from beyond the L2.
+// Measured, tiles of 256, 8192 x 8192 x 8192, in runs of a hundred: on random numbers 856 us in bf16 (1.28 PFLOP/s; w across the sum 847, both
+// across it 837) and 420 to 440 in 8 bits (2.5 to 2.6), on zeros, which leave the clock up, 692 and 331; the first twenty launches behind other work take up
+// to 930 and 480.  Without new requests 693 and 510 on zeros, when every tile asks for the same bytes 587 on zeros, from registers
+// alone 610 and 503: a fifth of the time is operands on their way, and on numbers that are not all alike the power that these bytes take costs as much
+// again.  That is not the card's limit: the library's product takes 670, 487 on zeros.  LDS is busy for 275000 of 1.5 million cycles, without conflicts; 0.8 GB come from
+// beyond the L2.
 //
 // IN: type of the operands (TDC_F16, TDC_BF16, TDC_MX8).  XT, WT: x or w lies across the sum.  OUT: type of y, or TDC_F32 for the sums of one of
 // `splits` parts of the axis, which a launch of its own joins.

@@ -3,8 +3,10 @@
 //   h = x + residual (rounded to their type: what is handed on is what is normalised),  y = w h r,  r = 1 / sqrt(mean h^2 + eps)
 //   g = w dy,  u = h r:  dx = dresidual = r (g - u mean(g u)) + dh,  dw = sum over the rows of dy u
 //
-// Bound by memory: every number is read once and written once.  In bf16: 100352 x 256 with its residual 30 us (6.8 TB/s), 100352 x 512 with h
-// in 8 bits besides 85 (5.5 TB/s), its gradient from that 65 (5.6 TB/s) or from h 75 (5.5 TB/s), 25088 x 512 into 8 bits 14.5 (6.2 TB/s).
+// Bound by memory: every number is read once and written once.  In bf16: 100352 x 256 with its residual 30 us (6.8 TB/s), 25088 x 512 with its
+// residual into 8 bits 14.8 (6.1 TB/s).  100352 x 512 in a training step, forward and backward in turn: with the residual and h in 8 bits besides 76 (6.1 TB/s), the gradient
+// from that 79 (4.6 TB/s: what the forward pass left in the caches goes to memory meanwhile).  The same over and over by themselves: 86 (5.4 TB/s) and 65
+// (5.6 TB/s), from h 76 (5.4 TB/s).
 // A team of lanes keeps a row in registers, eight numbers a lane and
 // request; small teams with several requests in flight where rows are short, a whole workgroup where they are long.  Everything
 // between loads and stores is fp32; sums over rows are fp32 along a thread's own rows (256 at most) and 64 bits from there on.
